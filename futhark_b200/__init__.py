@@ -41,12 +41,16 @@ ARRAY_TYPES = {
     "f32_3d": (np.float32, 3, ctypes.c_float),
     "i32_3d": (np.int32, 3, ctypes.c_int32),
     "f16_3d": (np.uint16, 3, ctypes.c_uint16),
+    "f16_2d": (np.uint16, 2, ctypes.c_uint16),
 }
 
 PAIR = "opaque_tup2_arr1d_u32_arr1d_u32"
 TRIPLE = "opaque_tup3_arr1d_i32_arr1d_i32_arr1d_i32"
 PAIR_I32 = "opaque_tup2_arr1d_i32_arr1d_i32"
 SEXTUPLE = "opaque_tup6" + "_arr1d_i32" * 6
+LOSSES = "opaque_tup2_arr1d_f32_arr1d_f32"
+GRADS_F16 = "opaque_tup2_arr2d_f16_arr2d_f16"
+BALANCE = "opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32"
 
 _lib = None
 
@@ -230,6 +234,18 @@ def load():
         getattr(L, "futhark_project_%s_%d" % (SEXTUPLE, i)).argtypes = [vp, pvp, vp]
     getattr(L, "futhark_free_" + SEXTUPLE).argtypes = [vp, vp]
     getattr(L, "futhark_new_" + SEXTUPLE).argtypes = [vp, pvp] + [vp] * 6
+    for name, k in ((LOSSES, 2), (GRADS_F16, 2), (BALANCE, 3)):
+        for i in range(k):
+            getattr(L, "futhark_project_%s_%d" % (name, i)).argtypes = [vp, pvp, vp]
+        getattr(L, "futhark_free_" + name).argtypes = [vp, vp]
+        getattr(L, "futhark_new_" + name).argtypes = [vp, pvp] + [vp] * k
+    L.futhark_entry_vocab_xent_f16.argtypes = [vp, pvp] + [vp] * 3
+    L.futhark_entry_vocab_xent_grad_f16.argtypes = [vp, pvp] + [vp] * 6
+    for t in ("f32", "f16"):
+        getattr(L, "futhark_entry_topk_distill_" + t).argtypes = [vp, pvp, ctypes.c_float] + [vp] * 3
+        getattr(L, "futhark_entry_topk_distill_grad_" + t).argtypes = [vp, pvp, ctypes.c_float] + [vp] * 5
+        getattr(L, "futhark_entry_router_balance_" + t).argtypes = [vp, pvp] + [vp] * 3
+        getattr(L, "futhark_entry_router_balance_grad_" + t).argtypes = [vp, pvp] + [vp] * 5
     L.futhark_b200_value_error.restype = ctypes.c_char_p
     L.futhark_b200_value_read_mem.argtypes = [vp, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t), ctypes.c_char_p, ci, ctypes.POINTER(HostValue)]
     L.futhark_b200_value_write_mem.argtypes = [ctypes.POINTER(HostValue), ci, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
@@ -616,6 +632,43 @@ class Context:
         self._check(getattr(self.lib, "futhark_free_" + SEXTUPLE)(self.ptr, obj))
         return parts
 
+    def _fields(self, rec, types, obj):
+        """The fields of an opaque record as arrays; the record is freed."""
+        parts = []
+        for i, t in enumerate(types):
+            out = ctypes.c_void_p()
+            self._check(getattr(self.lib, "futhark_project_%s_%d" % (rec, i))(self.ptr, ctypes.byref(out), obj))
+            parts.append(Array(self, t, out.value))
+        self._check(getattr(self.lib, "futhark_free_" + rec)(self.ptr, obj))
+        return tuple(parts)
+
+    def _entry_rec(self, name, rec, types, *args):
+        obj = ctypes.c_void_p()
+        self._check(getattr(self.lib, "futhark_entry_" + name)(self.ptr, ctypes.byref(obj), *args))
+        return self._fields(rec, types, obj)
+
+    def entry_vocab_xent_f16(self, X, W, ts):
+        """Cross entropy of hidden states X against the vocabulary W: (losses, lses)."""
+        return self._entry_rec("vocab_xent_f16", LOSSES, ("f32_1d", "f32_1d"), X.ptr, W.ptr, ts.ptr)
+
+    def entry_vocab_xent_grad_f16(self, X, W, ts, losses, lses, dls):
+        """Its gradients (dX, dW); losses and lses as entry_vocab_xent_f16 returned them."""
+        return self._entry_rec("vocab_xent_grad_f16", GRADS_F16, ("f16_2d", "f16_2d"), X.ptr, W.ptr, ts.ptr, losses.ptr, lses.ptr, dls.ptr)
+
+    def entry_topk_distill(self, t, tau, S, iss, T):
+        """Distillation of a student's logits S (t: "f32" or "f16") from a teacher's top logits T at words iss: (losses, lses)."""
+        return self._entry_rec("topk_distill_" + t, LOSSES, ("f32_1d", "f32_1d"), tau, S.ptr, iss.ptr, T.ptr)
+
+    def entry_topk_distill_grad(self, t, tau, S, iss, T, lses, dls):
+        return self._entry_arr("topk_distill_grad_" + t, t + "_2d", tau, S.ptr, iss.ptr, T.ptr, lses.ptr, dls.ptr)
+
+    def entry_router_balance(self, t, R, keep, iss):
+        """The balance loss of a router's logits R (t: "f32" or "f16"): (loss, counts, norm)."""
+        return self._entry_rec("router_balance_" + t, BALANCE, ("f32_1d", "i32_1d", "f32_1d"), R.ptr, keep.ptr, iss.ptr)
+
+    def entry_router_balance_grad(self, t, R, keep, counts, norm, dl):
+        return self._entry_arr("router_balance_grad_" + t, t + "_2d", R.ptr, keep.ptr, counts.ptr, norm.ptr, dl.ptr)
+
     def entry_mss_i32(self, xs):
         out = ctypes.c_int32()
         self._check(self.lib.futhark_entry_mss_i32(self.ptr, ctypes.byref(out), xs.ptr))
@@ -923,3 +976,51 @@ def scan_i64(ctx, xs):
 
 def linrec_f32(ctx, as_, bs):
     return _run(ctx, [("f32_1d", as_), ("f32_1d", bs)], ctx.entry_linrec_f32)
+
+
+def _run_multi(ctx, ins, fn):
+    arrs = [ctx.new(t, d) for t, d in ins]
+    try:
+        outs = fn(*arrs)
+        try:
+            return tuple(o.values() for o in outs)
+        finally:
+            for o in outs:
+                o.free()
+    finally:
+        for a in arrs:
+            a.free()
+
+
+def _bits(x):
+    """Binary16 values as the bit patterns the API takes."""
+    x = np.asarray(x)
+    return x.view(np.uint16) if x.dtype == np.float16 else x
+
+
+def vocab_xent_f16(ctx, X, W, ts):
+    return _run_multi(ctx, [("f16_2d", _bits(X)), ("f16_2d", _bits(W)), ("i32_1d", ts)], ctx.entry_vocab_xent_f16)
+
+
+def vocab_xent_grad_f16(ctx, X, W, ts, losses, lses, dls):
+    """Gradients as uint16 bit patterns."""
+    return _run_multi(ctx, [("f16_2d", _bits(X)), ("f16_2d", _bits(W)), ("i32_1d", ts), ("f32_1d", losses), ("f32_1d", lses), ("f32_1d", dls)],
+                      ctx.entry_vocab_xent_grad_f16)
+
+
+def topk_distill(ctx, t, tau, S, iss, T):
+    return _run_multi(ctx, [(t + "_2d", _bits(S)), ("i32_2d", iss), ("f32_2d", T)], lambda s, i, q: ctx.entry_topk_distill(t, tau, s, i, q))
+
+
+def topk_distill_grad(ctx, t, tau, S, iss, T, lses, dls):
+    return _run(ctx, [(t + "_2d", _bits(S)), ("i32_2d", iss), ("f32_2d", T), ("f32_1d", lses), ("f32_1d", dls)],
+                lambda s, i, q, l, d: ctx.entry_topk_distill_grad(t, tau, s, i, q, l, d))
+
+
+def router_balance(ctx, t, R, keep, iss):
+    return _run_multi(ctx, [(t + "_2d", _bits(R)), ("bool_1d", keep), ("i32_2d", iss)], lambda r, k, i: ctx.entry_router_balance(t, r, k, i))
+
+
+def router_balance_grad(ctx, t, R, keep, counts, norm, dl):
+    return _run(ctx, [(t + "_2d", _bits(R)), ("bool_1d", keep), ("i32_1d", counts), ("f32_1d", norm), ("f32_1d", dl)],
+                lambda r, k, c, m, d: ctx.entry_router_balance_grad(t, r, k, c, m, d))

@@ -58,7 +58,7 @@ static const ArrayType ARRAYS[] = {
     FE_ARRAY(bool, bool, 2, "[][]bool", "bool"), FE_ARRAY(i8, int8_t, 1, "[]i8", "i8"), FE_ARRAY(i16, int16_t, 1, "[]i16", "i16"),
     FE_ARRAY(f16, uint16_t, 1, "[]f16", "f16"), FE_ARRAY(i32, int32_t, 3, "[][][]i32", "i32"),
     FE_ARRAY(u8, uint8_t, 1, "[]u8", "u8"), FE_ARRAY(u16, uint16_t, 1, "[]u16", "u16"),
-    FE_ARRAY(f64, double, 2, "[][]f64", "f64"),
+    FE_ARRAY(f64, double, 2, "[][]f64", "f64"),  FE_ARRAY(f16, uint16_t, 2, "[][]f16", "f16"),
 };
 inline const ArrayType *array_type(const std::string &name) {
   for (const ArrayType &a : ARRAYS)
@@ -111,6 +111,19 @@ inline T scalar_of(const Value &v) {
   return x;
 }
 
+// a record of two arrays of the same type
+#define FE_PAIR(NAME, REC, T, ELEM)                                                                                 \
+  {NAME, {ELEM, ELEM}, [](futhark_context *c, void *o) { return futhark_free_##REC(c, (futhark_##REC *)o); },         \
+   [](futhark_context *c, const void *o, int k, Value &out) {                                                        \
+     futhark_##T *a = nullptr;                                                                                       \
+     const auto *obj = (const futhark_##REC *)o;                                                                     \
+     const int rc = k == 0 ? futhark_project_##REC##_0(c, &a, obj) : futhark_project_##REC##_1(c, &a, obj);            \
+     if (!rc) set_array(out, ELEM, a);                                                                               \
+     return rc;                                                                                                      \
+   },                                                                                                                \
+   [](futhark_context *c, const std::vector<const Value *> &f, void **obj) {                                         \
+     return futhark_new_##REC(c, (futhark_##REC **)obj, (const futhark_##T *)f[0]->arr, (const futhark_##T *)f[1]->arr); \
+   }}
 static const RecordType RECORDS[] = {
     {"([]u32, []u32)", {"[]u32", "[]u32"},
      [](futhark_context *c, void *o) { return futhark_free_opaque_tup2_arr1d_u32_arr1d_u32(c, (futhark_opaque_tup2_arr1d_u32_arr1d_u32 *)o); },
@@ -141,6 +154,27 @@ static const RecordType RECORDS[] = {
      },
      [](futhark_context *c, const std::vector<const Value *> &f, void **obj) {
        return futhark_new_opaque_tup2_arr1d_i64_arr2d_f64(c, (futhark_opaque_tup2_arr1d_i64_arr2d_f64 **)obj, (const futhark_i64_1d *)f[0]->arr, (const futhark_f64_2d *)f[1]->arr);
+     }},
+    FE_PAIR("([]f32, []f32)", opaque_tup2_arr1d_f32_arr1d_f32, f32_1d, "[]f32"),
+    FE_PAIR("([][]f16, [][]f16)", opaque_tup2_arr2d_f16_arr2d_f16, f16_2d, "[][]f16"),
+    {"([]f32, []i32, []f32)", {"[]f32", "[]i32", "[]f32"},
+     [](futhark_context *c, void *o) { return futhark_free_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32(c, (futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *)o); },
+     [](futhark_context *c, const void *o, int k, Value &out) {
+       const auto *obj = (const futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *)o;
+       if (k == 1) {
+         futhark_i32_1d *a = nullptr;
+         const int rc = futhark_project_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32_1(c, &a, obj);
+         if (!rc) set_array(out, "[]i32", a);
+         return rc;
+       }
+       futhark_f32_1d *a = nullptr;
+       const int rc = k == 0 ? futhark_project_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32_0(c, &a, obj) : futhark_project_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32_2(c, &a, obj);
+       if (!rc) set_array(out, "[]f32", a);
+       return rc;
+     },
+     [](futhark_context *c, const std::vector<const Value *> &f, void **obj) {
+       return futhark_new_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32(c, (futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 **)obj, (const futhark_f32_1d *)f[0]->arr,
+                                                                    (const futhark_i32_1d *)f[1]->arr, (const futhark_f32_1d *)f[2]->arr);
      }},
     {"([]i32, []i32)", {"[]i32", "[]i32"},
      [](futhark_context *c, void *o) { return futhark_free_opaque_tup2_arr1d_i32_arr1d_i32(c, (futhark_opaque_tup2_arr1d_i32_arr1d_i32 *)o); },
@@ -274,6 +308,13 @@ struct EntryPoint {
 #define FE_EH(NAME, T1, S1, T2, S2, TO, SO) \
   {#NAME, {"i64", S1, S2}, SO, [](C *c, In in, Value &o) { futhark_##TO *r = nullptr; int rc = futhark_entry_##NAME(c, &r, scalar_of<int64_t>(*in[0]), FE_IN(1, T1), FE_IN(2, T2)); if (!rc) set_array(o, SO, r); return rc; }}
 
+// the losses on logits of one element type
+#define FE_LOSSES(T) \
+  {"topk_distill_" #T, {"f32", "[][]" #T, "[][]i32", "[][]f32"}, "([]f32, []f32)", [](C *c, In in, Value &o) { futhark_opaque_tup2_arr1d_f32_arr1d_f32 *r = nullptr; int rc = futhark_entry_topk_distill_##T(c, &r, scalar_of<float>(*in[0]), FE_IN(1, T##_2d), FE_IN(2, i32_2d), FE_IN(3, f32_2d)); if (!rc) set_record(o, "([]f32, []f32)", r); return rc; }}, \
+  {"topk_distill_grad_" #T, {"f32", "[][]" #T, "[][]i32", "[][]f32", "[]f32", "[]f32"}, "[][]" #T, [](C *c, In in, Value &o) { futhark_##T##_2d *r = nullptr; int rc = futhark_entry_topk_distill_grad_##T(c, &r, scalar_of<float>(*in[0]), FE_IN(1, T##_2d), FE_IN(2, i32_2d), FE_IN(3, f32_2d), FE_IN(4, f32_1d), FE_IN(5, f32_1d)); if (!rc) set_array(o, "[][]" #T, r); return rc; }}, \
+  {"router_balance_" #T, {"[][]" #T, "[]bool", "[][]i32"}, "([]f32, []i32, []f32)", [](C *c, In in, Value &o) { futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *r = nullptr; int rc = futhark_entry_router_balance_##T(c, &r, FE_IN(0, T##_2d), FE_IN(1, bool_1d), FE_IN(2, i32_2d)); if (!rc) set_record(o, "([]f32, []i32, []f32)", r); return rc; }}, \
+  {"router_balance_grad_" #T, {"[][]" #T, "[]bool", "[]i32", "[]f32", "[]f32"}, "[][]" #T, [](C *c, In in, Value &o) { futhark_##T##_2d *r = nullptr; int rc = futhark_entry_router_balance_grad_##T(c, &r, FE_IN(0, T##_2d), FE_IN(1, bool_1d), FE_IN(2, i32_1d), FE_IN(3, f32_1d), FE_IN(4, f32_1d)); if (!rc) set_array(o, "[][]" #T, r); return rc; }}
+
 inline const std::vector<EntryPoint> &entry_points() {
   typedef futhark_context C;
   typedef const std::vector<const Value *> &In;
@@ -351,6 +392,10 @@ inline const std::vector<EntryPoint> &entry_points() {
       {"hist_rows_vec_add_i32", {"i64", "[][]i32", "[][][]i32"}, "[][][]i32", [](C *c, In in, Value &o) { futhark_i32_3d *r = nullptr; int rc = futhark_entry_hist_rows_vec_add_i32(c, &r, scalar_of<int64_t>(*in[0]), FE_IN(1, i32_2d), FE_IN(2, i32_3d)); if (!rc) set_array(o, "[][][]i32", r); return rc; }},
       {"reduce_by_index_minpair_i32", {"i64", "[]i32", "[]i32", "[]i32"}, "([]i32, []i32)", [](C *c, In in, Value &o) { futhark_opaque_tup2_arr1d_i32_arr1d_i32 *r = nullptr; int rc = futhark_entry_reduce_by_index_minpair_i32(c, &r, scalar_of<int64_t>(*in[0]), FE_IN(1, i32_1d), FE_IN(2, i32_1d), FE_IN(3, i32_1d)); if (!rc) set_record(o, "([]i32, []i32)", r); return rc; }},
       {"partition2_pairs_i32", {"[]i32", "[]i32"}, "([]i32, []i32, []i32, []i32, []i32, []i32)", [](C *c, In in, Value &o) { futhark_opaque_tup6_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32 *r = nullptr; int rc = futhark_entry_partition2_pairs_i32(c, &r, FE_IN(0, i32_1d), FE_IN(1, i32_1d)); if (!rc) set_record(o, "([]i32, []i32, []i32, []i32, []i32, []i32)", r); return rc; }},
+      {"vocab_xent_f16", {"[][]f16", "[][]f16", "[]i32"}, "([]f32, []f32)", [](C *c, In in, Value &o) { futhark_opaque_tup2_arr1d_f32_arr1d_f32 *r = nullptr; int rc = futhark_entry_vocab_xent_f16(c, &r, FE_IN(0, f16_2d), FE_IN(1, f16_2d), FE_IN(2, i32_1d)); if (!rc) set_record(o, "([]f32, []f32)", r); return rc; }},
+      {"vocab_xent_grad_f16", {"[][]f16", "[][]f16", "[]i32", "[]f32", "[]f32", "[]f32"}, "([][]f16, [][]f16)", [](C *c, In in, Value &o) { futhark_opaque_tup2_arr2d_f16_arr2d_f16 *r = nullptr; int rc = futhark_entry_vocab_xent_grad_f16(c, &r, FE_IN(0, f16_2d), FE_IN(1, f16_2d), FE_IN(2, i32_1d), FE_IN(3, f32_1d), FE_IN(4, f32_1d), FE_IN(5, f32_1d)); if (!rc) set_record(o, "([][]f16, [][]f16)", r); return rc; }},
+      FE_LOSSES(f32),
+      FE_LOSSES(f16),
       {"replicate_i32", {"i64", "i32"}, "[]i32", [](C *c, In in, Value &o) { futhark_i32_1d *r = nullptr; int rc = futhark_entry_replicate_i32(c, &r, scalar_of<int64_t>(*in[0]), scalar_of<int32_t>(*in[1])); if (!rc) set_array(o, "[]i32", r); return rc; }},
       {"iota_i64", {"i64"}, "[]i64", [](C *c, In in, Value &o) { futhark_i64_1d *r = nullptr; int rc = futhark_entry_iota_i64(c, &r, scalar_of<int64_t>(*in[0])); if (!rc) set_array(o, "[]i64", r); return rc; }},
   };

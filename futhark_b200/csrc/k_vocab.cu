@@ -1,0 +1,641 @@
+// Cross entropy over a vocabulary without the logits, and its gradient.
+//
+//   z = X W^T             X [n][d] f16 hidden states, W [v][d] f16 vocabulary weights
+//   lse_i  = log sum_v exp z_iv
+//   loss_i = lse_i - z_{i,t_i}                        0 where t_i is outside [0, v)
+//   g_iv   = dl_i (exp(z_iv - lse_i) - [v = t_i]);    dX = g W,  dW = g^T X
+//
+// A map-map-reduce contraction whose result is consumed by a (maximum, sum) reduction.  The logits stay in
+// tensor memory: the contraction's epilogue folds each 256 x 256 tile to one (maximum, sum) pair per
+// row, and a small kernel folds the v/256 pairs of a row.  The gradient works the vocabulary off in pieces: a
+// piece's logits are computed again (the same instructions in the same order, so the same bits), turned into g in
+// binary16 in the epilogue, and that piece of g meets W (summed over the pieces in f32) and X.
+//
+// Rounding of g to 11 bits.  With q_i = 1 - exp(-loss_i) the row is kept as
+//   G_iv = 2^13 (exp(z_iv - lse_i) - [v = t_i]) / q_i,  G_{i,t_i} = -2^13 exactly,  and  w_i = dl_i q_i  aside:
+//   dX_i = 2^-13 w_i sum_v G_iv W_v                 w_i in f32, after the sum
+//   dW_v = 2^(E+1-13) sum_i G_iv (X_i w_i 2^-(E+1))   E the largest exponent of the w_i
+// The target's term, the largest of its row by far, is thus exact in dX; the others round relative to
+// themselves (2^13 keeps probabilities down to 2^-27 out of binary16's subnormals, and the sum over the others is q_i,
+// so |G| <= 2^13 up to the rounding of the losses).  In dW the scaled X is rounded once more to binary16: half
+// a unit in the last place of each element, independent of the others, of the size of the result's own rounding.
+// Both products accumulate in f32.
+//
+// All four products run on one kernel (vocab_mma_kernel): pairs of CTAs on 256 x 256 tiles with
+// tcgen05.mma.cta_group::2, operands by bulk tensor copies through a six-stage ring, two accumulators in tensor
+// memory so that the epilogue of a tile runs under the next tile's instructions.  The operands are taken
+// as they lie in memory, contiguous along the summed axis or across it: no transposition.
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "kernels.h"
+#include "tcgen.cuh"
+
+namespace fb {
+
+constexpr int VT = 256;                                // tile edge of a CTA pair
+constexpr int VK = 64;                                 // summed elements per stage
+constexpr int V_STAGES = 6;
+constexpr int V_OPERAND = 128 * VK * 2;                // a CTA's half of one operand in one stage: 16 KiB
+constexpr int V_STAGE = 2 * V_OPERAND;
+constexpr int V_SLAB = VK * 64 * 2;                    // 64 x 64 block of an operand that is contiguous across the sum
+constexpr int V_EPI_BUF = 32 * 128;                    // 32 rows of 128 bytes
+constexpr int V_EPI = 4 * 2 * V_EPI_BUF;               // two per epilogue warp
+constexpr int V_SMEM = V_STAGES * V_STAGE + 1024 /*alignment*/ + 1024 /*barriers*/ + V_EPI;
+constexpr int V_THREADS = 192;
+constexpr int V_GROUP = 16;                            // row tiles that share the columns' operand before it moves on
+constexpr float V_LOG2E = 1.4426950408889634f;
+constexpr float V_GSCALE = 8192.f;                     // 2^13, see above
+
+enum VocabEpilogue : int {
+  VE_SOFTMAX = 0,      // (maximum, sum) of the tile's columns per row, and the target's logit
+  VE_GRAD = 1,         // G in binary16
+  VE_SLAB = 2,         // f32 partial products, one slab per part of the summed axis
+  VE_HALF = 3,         // binary16, times a factor from device memory
+};
+
+struct VocabArgs {
+  int M, N, kblocks;            // extents; the summed axis in blocks of VK
+  int splits, kps;              // parts of the summed axis and the blocks of each
+  int tiles_m, tiles_n;
+  const int32_t *targets;       // VE_SOFTMAX, VE_GRAD
+  int64_t v, v0;                // size of the vocabulary, first word of the piece
+  float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum in units of log 2, sum)
+  float *ztarget;
+  const float *cexp;            // VE_GRAD: per row the exponent's constant term
+  const float *factor;          // VE_HALF
+  int add;                      // VE_SLAB: add to the slab instead of writing it
+  int *failure;
+};
+
+__device__ __forceinline__ float ex2(float x) {        // 2^x: at most 2 units in the last place off, 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct VocabBarriers {
+  uint64_t full[V_STAGES];       // used in the pair's first CTA only
+  uint64_t empty[V_STAGES];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];        // used in the pair's first CTA only
+  uint32_t tmem_base;
+};
+
+// Tiles in the order the pairs take them: V_GROUP row tiles by all column tiles, the rows first.  74 pairs then
+// work on about 16 x 5 tiles at a time, whose operands come from HBM once and from L2 for every further tile.
+__device__ __forceinline__ void vocab_tile(const VocabArgs &a, int64_t t, int &split, int &tm, int &tn) {
+  const int64_t per = (int64_t)a.tiles_m * a.tiles_n;
+  split = (int)(t / per);
+  const int64_t r = t - split * per;
+  const int64_t gsize = (int64_t)V_GROUP * a.tiles_n;
+  const int g = (int)(r / gsize);
+  const int in = (int)(r - g * gsize);
+  const int rows = min(V_GROUP, a.tiles_m - g * V_GROUP);
+  tn = in / rows;
+  tm = g * V_GROUP + in - tn * rows;
+}
+
+// A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
+template <bool A_MN, bool B_MN, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
+vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmC, const VocabArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  VocabBarriers *bars = reinterpret_cast<VocabBarriers *>(smem + V_STAGES * V_STAGE);
+  uint8_t *epi = smem + V_STAGES * V_STAGE + 1024;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int64_t num_tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+
+  if (tid == 0) {
+    for (int s = 0; s < V_STAGES; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], 256); }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                  // both CTAs' barriers exist before either signals the other's
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  const bool poisoned = ld_failure(a.failure) != FAIL_NONE;
+
+  if (!poisoned) {
+    if (warp == 0) {
+      // ---------------- producer: this CTA's half of each operand ----------------
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int64_t t = pair; t < num_tiles && ok; t += npairs) {
+          int split, tm, tn;
+          vocab_tile(a, t, split, tm, tn);
+          const int m0 = tm * VT + (int)rank * 128, n0 = tn * VT + (int)rank * 128;
+          const int kb1 = min(a.kblocks, (split + 1) * a.kps);
+          for (int kb = split * a.kps; kb < kb1; kb++, it++) {
+            const int s = it % V_STAGES;
+            const uint32_t ph = (it / V_STAGES) & 1;
+            if (!mbar_wait_bounded(&bars->empty[s], ph ^ 1)) { ok = false; break; }
+            uint8_t *sa = smem + s * V_STAGE;
+            uint8_t *sb = sa + V_OPERAND;
+            const uint32_t full0 = map_to_cta(smem_u32(&bars->full[s]), 0);
+            if (rank == 0) mbar_expect_tx(&bars->full[s], 2 * V_STAGE);          // both CTAs' bytes
+            if (A_MN) {
+              tma_load_3d_pair(sa, &tmA, m0, kb * VK, 0, full0);
+              tma_load_3d_pair(sa + V_SLAB, &tmA, m0 + 64, kb * VK, 0, full0);
+            } else {
+              tma_load_3d_pair(sa, &tmA, kb * VK, m0, 0, full0);
+            }
+            if (B_MN) {
+              tma_load_3d_pair(sb, &tmB, n0, kb * VK, 0, full0);
+              tma_load_3d_pair(sb + V_SLAB, &tmB, n0 + 64, kb * VK, 0, full0);
+            } else {
+              tma_load_3d_pair(sb, &tmB, kb * VK, n0, 0, full0);
+            }
+          }
+        }
+        if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
+      }
+    } else if (warp == 1) {
+      // ---------------- MMA issuer: one thread of the first CTA ----------------
+      if (lane == 0 && rank == 0) {
+        // D = f32, A = B = f16, N = 256, M = 256 over the pair
+        constexpr uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(VT >> 3) << 17) | ((uint32_t)(VT >> 4) << 24);
+        uint32_t it = 0, tile_it = 0;
+        bool ok = true;
+        for (int64_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
+          int split, tm, tn;
+          vocab_tile(a, t, split, tm, tn);
+          const uint32_t acc = tile_it & 1, acc_ph = (tile_it >> 1) & 1;
+          if (!mbar_wait_bounded(&bars->tmem_empty[acc], acc_ph ^ 1)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d_tmem = tmem_base + acc * VT;
+          const int kb0 = split * a.kps, kb1 = min(a.kblocks, kb0 + a.kps);
+          for (int kb = kb0; kb < kb1; kb++, it++) {
+            const int s = it % V_STAGES;
+            const uint32_t ph = (it / V_STAGES) & 1;
+            if (!mbar_wait_bounded(&bars->full[s], ph)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + s * V_STAGE);
+            const uint32_t sb = sa + V_OPERAND;
+            // along the sum: rows of 128 bytes, 8-row groups 1024 bytes apart, a step of 16 is 32 bytes inside the
+            // swizzled row; across it: 64-wide slabs (leading), 8-row groups 1024 bytes apart, a step is 16 rows
+            const uint64_t adesc = A_MN ? make_smem_desc(sa, V_SLAB, 1024) : make_smem_desc(sa, 16, 1024);
+            const uint64_t bdesc = B_MN ? make_smem_desc(sb, V_SLAB, 1024) : make_smem_desc(sb, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < VK / 16; k++)
+              tc2_mma_f16(d_tmem, adesc + (uint64_t)(k * (A_MN ? 128 : 2)), bdesc + (uint64_t)(k * (B_MN ? 128 : 2)), idesc,
+                          (kb > kb0 || k > 0) ? 1u : 0u);
+            tc2_commit_both(&bars->empty[s]);
+          }
+          if (ok) tc2_commit_both(&bars->tmem_full[acc]);
+        }
+        if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
+      }
+    } else {
+      // ---------------- epilogue (warps 2..5): this CTA's 128 rows of the tile, one row per thread ----------------
+      const int quarter = warp & 3;
+      uint32_t tile_it = 0;
+      bool ok = true;
+      uint8_t *stg = epi + (warp - 2) * (2 * V_EPI_BUF);
+      int buf = 0;
+      const float factor = EPI == VE_HALF ? *a.factor : 1.f;
+      for (int64_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
+        int split, tm, tn;
+        vocab_tile(a, t, split, tm, tn);
+        const int row0 = tm * VT + (int)rank * 128 + quarter * 32, n0 = tn * VT;
+        const int row = row0 + lane;
+        const uint32_t acc = tile_it & 1, acc_ph = (tile_it >> 1) & 1;
+        const int ncols = min(VT, a.N - n0);
+        int tcol = -1;                                     // the target's column in this tile, if it has it
+        float c = 0.f;
+        bool counts = false;
+        if ((EPI == VE_SOFTMAX || EPI == VE_GRAD) && row < a.M) {
+          const int64_t tg = a.targets[row];
+          counts = tg >= 0 && tg < a.v;
+          const int64_t tl = tg - a.v0 - n0;
+          if (counts && tl >= 0 && tl < ncols) tcol = (int)tl;
+          if (EPI == VE_GRAD) c = a.cexp[row];
+        }
+        if (!__all_sync(kFull, mbar_wait_bounded(&bars->tmem_full[acc], acc_ph))) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * VT;
+        float m2 = -INFINITY, sum = 0.f;
+
+        // 32 columns of a row: running maximum (in units of log 2, so that it is exactly what was subtracted) and sum
+        auto fold = [&](uint32_t (&v)[32], int c0) {
+          if (c0 >= ncols) return;
+          if (c0 + 32 > ncols) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) if (c0 + j >= ncols) v[j] = 0xff800000u;     // columns that do not exist
+          }
+          float mx[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) mx[j] = __uint_as_float(v[j]);
+#pragma unroll
+          for (int j = 4; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
+          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * V_LOG2E;
+          const float mn = fmaxf(m2, cm);
+          const float ref = mn == -INFINITY ? 0.f : mn;    // a row of -inf so far: the sum stays 0
+          float s4[4] = {sum * ex2(m2 - ref), 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; j++) s4[j & 3] += ex2(fmaf(__uint_as_float(v[j]), V_LOG2E, -ref));
+          sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          m2 = mn;
+          const int tj = tcol - c0;
+          if (tj >= 0 && tj < 32) {
+            float zt = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j++) if (j == tj) zt = __uint_as_float(v[j]);
+            a.ztarget[row] = zt;
+          }
+        };
+        // 32 columns of G (or of the scaled product) as 16 pairs of binary16
+        auto to_half = [&](const uint32_t (&v)[32], int c0, uint32_t (&h)[16]) {
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; j++) {
+            if (EPI == VE_GRAD) {
+              const float e = ex2(fmaf(__uint_as_float(v[j]), V_LOG2E, c));
+              f[j] = e > 65504.f ? 65504.f : e;            // NaN stays
+            } else {
+              f[j] = __uint_as_float(v[j]) * factor;
+            }
+          }
+          if (EPI == VE_GRAD) {
+            const int tj = tcol - c0;
+            if (tj >= 0 && tj < 32) {
+#pragma unroll
+              for (int j = 0; j < 32; j++) if (j == tj) f[j] = -V_GSCALE;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const __half2 p = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+            h[j] = (EPI == VE_GRAD && !counts) ? 0u : *reinterpret_cast<const uint32_t *>(&p);
+          }
+        };
+        // Chunks are staged as the 128-byte swizzle wants them (16-byte piece q of row r at q ^ (r & 7)) and leave
+        // by one bulk tensor store; of two buffers the one written is the one whose store has been read.
+        auto half_pieces = [&](const uint32_t (&h)[16], int q0) {
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            *reinterpret_cast<uint4 *>(stg + buf * V_EPI_BUF + lane * 128 + (((q0 + q) ^ (lane & 7)) << 4)) =
+                make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+        };
+        auto acquire = [&] {
+          if (lane == 0) bulk_wait_read1();
+          __syncwarp();
+        };
+        auto release = [&](int c0) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < a.M && n0 + c0 < a.N) {
+              if (EPI == VE_SLAB && a.add) tma_add_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, split);
+              else tma_store_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, split);
+            }
+            bulk_commit();
+          }
+          buf ^= 1;
+        };
+        auto slab = [&](const uint32_t (&v)[32], int c0) {
+          acquire();
+#pragma unroll
+          for (int q = 0; q < 8; q++)
+            *reinterpret_cast<uint4 *>(stg + buf * V_EPI_BUF + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          release(c0);
+        };
+
+        uint32_t va[32], vb[32];
+        tmem_ld_32x32(taddr0, va);
+#pragma unroll 1
+        for (int cc = 0; cc < VT; cc += 64) {
+          tmem_ld_wait();
+          tmem_ld_32x32(taddr0 + cc + 32, vb);
+          if (EPI == VE_SOFTMAX) fold(va, cc);
+          else if (EPI == VE_SLAB) slab(va, cc);
+          else { uint32_t h[16]; to_half(va, cc, h); acquire(); half_pieces(h, 0); }
+          tmem_ld_wait();
+          if (cc + 64 < VT) tmem_ld_32x32(taddr0 + cc + 64, va);
+          if (EPI == VE_SOFTMAX) fold(vb, cc + 32);
+          else if (EPI == VE_SLAB) slab(vb, cc + 32);
+          else { uint32_t h[16]; to_half(vb, cc + 32, h); half_pieces(h, 4); release(cc); }
+        }
+        tc_fence_before();
+        mbar_arrive_cluster(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
+        if (EPI == VE_SOFTMAX && row < a.M) a.part[(int64_t)row * a.tiles_n + tn] = make_float2(m2, sum);
+      }
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
+    }
+  }
+  // ---------------- teardown: every thread of both CTAs arrives here, whatever happened ----------------
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                  // nobody signals into a partner that has left
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+  }
+}
+
+// ---- the small kernels around it ------------------------------------------------------------------
+// One warp per row: fold of the row's (maximum, sum) pairs; the last step in f64, where a loss near 0 is a difference.
+__global__ void __launch_bounds__(256)
+vocab_loss_kernel(const float2 *__restrict__ part, int tiles, const float *__restrict__ ztarget, const int32_t *__restrict__ targets,
+                  float *__restrict__ loss, float *__restrict__ lse, int64_t n, int64_t v) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= n) return;
+  float m = -INFINITY, s = 0.f;
+  for (int t = lane; t < tiles; t += 32) {
+    const float2 p = part[row * tiles + t];
+    const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.f : mn;
+    s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
+    m = mn;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, s, o);
+    const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.f : mn;
+    s = s * exp2f(m - ref) + ps * exp2f(pm - ref);
+    m = mn;
+  }
+  if (lane == 0) {
+    const double l = ((double)m + log2((double)s)) * 0.69314718055994530942;
+    const int64_t t = targets[row];
+    lse[row] = (float)l;
+    loss[row] = t >= 0 && t < v ? (float)(l - (double)ztarget[row]) : 0.f;
+  }
+}
+
+// One CTA: per row w_i = dl_i q_i and the constant term of G's exponent, and over the rows the largest exponent E.
+// factors[0] = 2^-(E+1) as an exponent for ldexp, factors[1] = 2^(E+1-13) as a float.
+__global__ void __launch_bounds__(1024)
+vocab_prep_kernel(const int32_t *__restrict__ targets, const float *__restrict__ loss, const float *__restrict__ lse,
+                  const float *__restrict__ dl, float *__restrict__ w, float *__restrict__ cexp, int *__restrict__ exponent,
+                  float *__restrict__ factor, int64_t n, int64_t v) {
+  __shared__ int top;
+  if (threadIdx.x == 0) top = -200;
+  __syncthreads();
+  int mine = -200;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const int64_t t = targets[i];
+    float wi = 0.f, ci = 0.f;
+    if (t >= 0 && t < v) {
+      const float l = lse[i];
+      // losses are off by a few units in the last place of lse: q below that is as good as that
+      const float least = 0x1p-22f * fmaxf(1.f, fabsf(l)), q0 = -expm1f(-loss[i]), q = q0 < least ? least : q0;
+      wi = dl[i] * q;
+      ci = 13.f - log2f(q) - l * V_LOG2E;
+      if (wi != 0.f && isfinite(wi)) mine = max(mine, ilogbf(wi));
+    }
+    w[i] = wi;
+    cexp[i] = ci;
+  }
+  atomicMax(&top, mine);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int e = top == -200 ? 0 : top;
+    *exponent = -(e + 1);
+    *factor = ldexpf(1.f, e + 1 - 13);
+  }
+}
+
+// X_i w_i 2^-(E+1) in binary16, rows without a target 0.
+__global__ void __launch_bounds__(256)
+vocab_scale_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const int32_t *__restrict__ targets, int64_t v, const float *__restrict__ w, const int *__restrict__ exponent, __half *__restrict__ out) {
+  const int64_t per = dp / 8, total = n * per;
+  const int ex = *exponent;
+  for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
+    const int64_t i = o / per, c = (o - i * per) * 8;
+    const int64_t t = targets[i];
+    __align__(16) __half h[8] = {};
+    if (t >= 0 && t < v) {
+      const float f = ldexpf(w[i], ex);
+      *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(x + i * dp + c);
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
+    }
+    *reinterpret_cast<uint4 *>(out + i * dp + c) = *reinterpret_cast<const uint4 *>(h);
+  }
+}
+
+// Rows of another pitch, what is behind the narrower of the two 0 or left out.
+__global__ void __launch_bounds__(256)
+vocab_pitch_kernel(const __half *__restrict__ in, int64_t rows, int64_t in_cols, __half *__restrict__ out, int64_t out_cols) {
+  const int64_t total = rows * out_cols;
+  for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
+    const int64_t i = o / out_cols, c = o - i * out_cols;
+    out[o] = c < in_cols ? in[i * in_cols + c] : __half(0.f);
+  }
+}
+
+// dX_i = 2^-13 w_i times the sum of the slabs, in f32, rounded once.
+__global__ void __launch_bounds__(256)
+vocab_dx_kernel(const float *__restrict__ slabs, int splits, int64_t n, int64_t d, int64_t dp, const int32_t *__restrict__ targets, int64_t v,
+                const float *__restrict__ w, __half *__restrict__ dx) {
+  const int64_t per = dp / 4, total = n * per;
+  for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
+    const int64_t i = o / per, c = (o - i * per) * 4;
+    const int64_t t = targets[i];
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (t >= 0 && t < v) {
+      for (int k = 0; k < splits; k++) {
+        const float4 p = *reinterpret_cast<const float4 *>(slabs + ((int64_t)k * n + i) * dp + c);
+        s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+      }
+      const float f = w[i];
+      constexpr float g = 1.f / V_GSCALE;
+      s.x *= g; s.y *= g; s.z *= g; s.w *= g;
+      s.x *= f; s.y *= f; s.z *= f; s.w *= f;
+    }
+    const __half2 lo = __floats2half2_rn(s.x, s.y), hi = __floats2half2_rn(s.z, s.w);
+    if (d == dp) {
+      uint2 r;
+      r.x = *reinterpret_cast<const uint32_t *>(&lo); r.y = *reinterpret_cast<const uint32_t *>(&hi);
+      *reinterpret_cast<uint2 *>(dx + i * d + c) = r;
+    } else {
+      if (c + 0 < d) dx[i * d + c + 0] = __low2half(lo);
+      if (c + 1 < d) dx[i * d + c + 1] = __high2half(lo);
+      if (c + 2 < d) dx[i * d + c + 2] = __low2half(hi);
+      if (c + 3 < d) dx[i * d + c + 3] = __high2half(hi);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256)
+vocab_fill_kernel(float *__restrict__ loss, float *__restrict__ lse, int64_t n, float l) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) { loss[i] = 0.f; lse[i] = l; }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------
+static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static inline size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+static inline int elementwise_grid(int64_t items, int num_sms) {
+  const int64_t g = ceil_div(items, 256);
+  return (int)(g < 1 ? 1 : g < (int64_t)num_sms * 16 ? g : (int64_t)num_sms * 16);
+}
+
+// Parts of the summed axis of dX = G W.  A small batch has fewer tiles than there are pairs of SMs, while its sum
+// runs over the vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks: 512 per
+// block of 64 and tile at the tensor cores' rate, 3000 per tile for its epilogue where nothing hides it, 3600 bytes of HBM per clock.
+static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int pairs) {
+  const int64_t tiles = ceil_div(n, VT) * ceil_div(dp, VT);
+  int best = 1;
+  double best_cost = 0;
+  for (int s = 1; s <= 64 && s <= kblocks; s++) {
+    const int64_t kps = ceil_div(kblocks, s);
+    if (ceil_div(kblocks, kps) != s) continue;
+    const double cost = (double)ceil_div(tiles * s, pairs) * (kps * 512.0 + 3000.0) + (double)s * n * dp * 8 / 3600.0;
+    if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
+  }
+  return best;
+}
+
+VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_aligned, bool grad, int num_sms) {
+  VocabPlan p = {};
+  if (n <= 0 || v <= 0 || (grad && d <= 0)) return p;           // nothing will run
+  p.dp = d <= 0 ? 8 : (d + 7) & ~(int64_t)7;
+  const bool padded = p.dp != d;
+  size_t off = 0;
+  auto take = [&](size_t bytes) { const size_t at = off; off += align256(bytes); return at; };
+  p.copy_x = padded || !x_aligned;
+  p.copy_w = padded || !w_aligned;
+  p.xp = p.copy_x ? take((size_t)(n * p.dp) * 2) : 0;
+  p.wp = p.copy_w ? take((size_t)(v * p.dp) * 2) : 0;
+  if (!grad) {
+    p.part = take((size_t)(n * ceil_div(v, VT)) * sizeof(float2));
+    p.zt = take((size_t)n * 4);
+  } else {
+    // pieces of the vocabulary whose part of G is at most 1 GiB: 65536 words for 8192 tokens
+    const int64_t most = (int64_t)1 << 29;
+    const int64_t want = ceil_div(v, VT) * VT;
+    int64_t words = most / (n > 0 ? n : 1) / VT * VT;
+    if (words < VT) words = VT;
+    if (words > want) words = want;
+    p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
+    const int pairs = num_sms / 2 > 0 ? num_sms / 2 : 1;
+    p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), pairs);
+    p.w = take((size_t)n * 4);
+    p.cexp = take((size_t)n * 4);
+    p.scalars = take(256);
+    p.xs = take((size_t)(n * p.dp) * 2);
+    p.g = take((size_t)(n * p.piece) * 2);
+    p.slabs = take((size_t)p.splits * (size_t)(n * p.dp) * 4);
+    p.dwp = padded ? take((size_t)((p.piece < v ? p.piece : v) * p.dp) * 2) : 0;
+  }
+  p.bytes = off;
+  return p;
+}
+
+template <bool A_MN, bool B_MN, int EPI>
+static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
+  auto kernel = vocab_mma_kernel<A_MN, B_MN, EPI>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, V_SMEM);
+  if (err != cudaSuccess) return err;
+  a.tiles_m = (int)ceil_div(a.M, VT);
+  a.tiles_n = (int)ceil_div(a.N, VT);
+  a.kps = (int)ceil_div(a.kblocks, a.splits);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+  int pairs = num_sms / 2;
+  if (tiles < pairs) pairs = (int)tiles;
+  kernel<<<2 * pairs, V_THREADS, V_SMEM, stream>>>(tmA, tmB, tmC, a);
+  return cudaGetLastError();
+}
+
+// an operand [rows][cols] of row pitch `pitch`: boxes of 128 rows where it is read along the sum, of 64 where across it
+static bool operand_map(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, int64_t pitch, bool across) {
+  return make_tensor_map(tm, base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)pitch, (uint64_t)pitch * rows, 64, across ? 64 : 128);
+}
+
+static cudaError_t repitch(const uint16_t *in, int64_t rows, int64_t in_cols, uint16_t *out, int64_t out_cols, int num_sms, cudaStream_t stream) {
+  vocab_pitch_kernel<<<elementwise_grid(rows * out_cols, num_sms), 256, 0, stream>>>(reinterpret_cast<const __half *>(in), rows, in_cols,
+                                                                                     reinterpret_cast<__half *>(out), out_cols);
+  return cudaGetLastError();
+}
+
+#define FB_TRY(e) do { const cudaError_t fb_err = (e); if (fb_err != cudaSuccess) return fb_err; } while (0)
+
+cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
+                              float *lse, int64_t n, int64_t v, int64_t d, int *failure, int num_sms, cudaStream_t stream) {
+  if (n <= 0) return cudaSuccess;
+  if (v <= 0) {                                   // the sum of nothing
+    vocab_fill_kernel<<<elementwise_grid(n, num_sms), 256, 0, stream>>>(loss, lse, n, -INFINITY);
+    return cudaGetLastError();
+  }
+  uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
+  if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
+  if (p.copy_w) { FB_TRY(repitch(w, v, d, reinterpret_cast<uint16_t *>(ws + p.wp), p.dp, num_sms, stream)); w = reinterpret_cast<uint16_t *>(ws + p.wp); }
+  CUtensorMap tmX, tmW;
+  if (!operand_map(&tmX, x, n, p.dp, p.dp, false) || !operand_map(&tmW, w, v, p.dp, p.dp, false)) return cudaErrorInvalidValue;
+  VocabArgs a = {};
+  a.M = (int)n; a.N = (int)v; a.kblocks = (int)ceil_div(p.dp, VK); a.splits = 1;
+  a.targets = targets; a.v = v; a.v0 = 0;
+  a.part = reinterpret_cast<float2 *>(ws + p.part);
+  a.ztarget = reinterpret_cast<float *>(ws + p.zt);
+  a.failure = failure;
+  FB_TRY((launch_mma<false, false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
+  vocab_loss_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, stream>>>(a.part, (int)ceil_div(v, VT), a.ztarget, targets, loss, lse, n, v);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets,
+                                   const float *loss, const float *lse, const float *dl, uint16_t *dx, uint16_t *dw, int64_t n, int64_t v,
+                                   int64_t d, int *failure, int num_sms, cudaStream_t stream) {
+  if (n <= 0 || v <= 0 || d <= 0) {               // what there is of the results is a sum of nothing
+    if (n > 0 && d > 0) FB_TRY(cudaMemsetAsync(dx, 0, (size_t)(n * d) * 2, stream));
+    if (v > 0 && d > 0) FB_TRY(cudaMemsetAsync(dw, 0, (size_t)(v * d) * 2, stream));
+    return cudaSuccess;
+  }
+  uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
+  float *rw = reinterpret_cast<float *>(ws + p.w), *cexp = reinterpret_cast<float *>(ws + p.cexp), *slabs = reinterpret_cast<float *>(ws + p.slabs);
+  int *exponent = reinterpret_cast<int *>(ws + p.scalars);
+  float *factor = reinterpret_cast<float *>(ws + p.scalars) + 1;
+  uint16_t *xs = reinterpret_cast<uint16_t *>(ws + p.xs), *g = reinterpret_cast<uint16_t *>(ws + p.g);
+  vocab_prep_kernel<<<1, 1024, 0, stream>>>(targets, loss, lse, dl, rw, cexp, exponent, factor, n, v);
+  FB_TRY(cudaGetLastError());
+  if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
+  if (p.copy_w) { FB_TRY(repitch(w, v, d, reinterpret_cast<uint16_t *>(ws + p.wp), p.dp, num_sms, stream)); w = reinterpret_cast<uint16_t *>(ws + p.wp); }
+  vocab_scale_kernel<<<elementwise_grid(n * p.dp / 8, num_sms), 256, 0, stream>>>(reinterpret_cast<const __half *>(x), n, p.dp, targets, v, rw,
+                                                                                  exponent, reinterpret_cast<__half *>(xs));
+  FB_TRY(cudaGetLastError());
+  for (int64_t v0 = 0; v0 < v; v0 += p.piece) {
+    const int64_t vw = v - v0 < p.piece ? v - v0 : p.piece;
+    CUtensorMap tmX, tmW, tmG, tmGk, tmWn, tmS, tmGm, tmXn, tmD;
+    uint16_t *dwo = p.dp == d ? dw + v0 * d : reinterpret_cast<uint16_t *>(ws + p.dwp);
+    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, false) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, false) &&
+                    make_tensor_map(&tmG, g, (uint64_t)vw, (uint64_t)n, 1, (uint64_t)p.piece, (uint64_t)p.piece * n, 64, 32) &&
+                    operand_map(&tmGk, g, n, vw, p.piece, false) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, true) &&
+                    make_tensor_map(&tmS, slabs, (uint64_t)p.dp, (uint64_t)n, (uint64_t)p.splits, (uint64_t)p.dp, (uint64_t)(p.dp * n), 32, 32, true) &&
+                    operand_map(&tmGm, g, n, vw, p.piece, true) && operand_map(&tmXn, xs, n, p.dp, p.dp, true) &&
+                    make_tensor_map(&tmD, dwo, (uint64_t)p.dp, (uint64_t)vw, 1, (uint64_t)p.dp, (uint64_t)(p.dp * vw), 64, 32);
+    if (!ok) return cudaErrorInvalidValue;
+    VocabArgs a = {};
+    a.failure = failure;
+    a.targets = targets; a.v = v; a.v0 = v0; a.cexp = cexp; a.factor = factor;
+    a.splits = 1;
+    a.M = (int)n; a.N = (int)vw; a.kblocks = (int)ceil_div(p.dp, VK);
+    FB_TRY((launch_mma<false, false, VE_GRAD>(tmX, tmW, tmG, a, num_sms, stream)));
+    // every part has its blocks in every piece: the last one may be shorter, and then some slabs get nothing more
+    a.M = (int)n; a.N = (int)p.dp; a.kblocks = (int)ceil_div(vw, VK);
+    a.splits = (int)ceil_div(a.kblocks, ceil_div(a.kblocks, p.splits < a.kblocks ? p.splits : a.kblocks));
+    a.add = v0 > 0;
+    FB_TRY((launch_mma<false, true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
+    a.M = (int)vw; a.N = (int)p.dp; a.kblocks = (int)ceil_div(n, VK); a.splits = 1; a.add = 0;
+    FB_TRY((launch_mma<true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
+    if (p.dp != d) FB_TRY(repitch(dwo, vw, p.dp, dw + v0 * d, d, num_sms, stream));
+  }
+  vocab_dx_kernel<<<elementwise_grid(n * p.dp / 4, num_sms), 256, 0, stream>>>(slabs, p.splits, n, d, p.dp, targets, v, rw, reinterpret_cast<__half *>(dx));
+  return cudaGetLastError();
+}
+
+}  // namespace fb

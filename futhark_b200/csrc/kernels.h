@@ -181,4 +181,33 @@ cudaError_t launch_lmad_copy(int elem_size, int r, void *dst, int64_t dst_offset
 cudaError_t launch_bmm_f16(const uint16_t *A, const uint16_t *B, float *C, int64_t nb, int64_t m, int64_t k,
                            int64_t n, int *failure, cudaStream_t stream);
 
+// ---- cross entropy over a vocabulary (k_vocab.cu) ---------------------------------------
+// What a call needs of device memory: byte offsets into one workspace of `bytes`, and the shape of the work.
+struct VocabPlan {
+  int64_t dp;                  // width of the rows the tensor cores see: d rounded up to 8
+  bool copy_x, copy_w;         // operands that are copied: another width, or a base that is no multiple of 16 bytes
+  int64_t piece;               // gradient: words per piece of the vocabulary
+  int splits;                  // gradient: parts of the sum over a piece's words
+  size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dwp, bytes;
+};
+VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_aligned, bool grad, int num_sms);
+cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
+                              float *lse, int64_t n, int64_t v, int64_t d, int *failure, int num_sms, cudaStream_t stream);
+cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets,
+                                   const float *loss, const float *lse, const float *dl, uint16_t *dx, uint16_t *dw, int64_t n, int64_t v,
+                                   int64_t d, int *failure, int num_sms, cudaStream_t stream);
+
+// ---- losses on logits (k_losses.cu); elem is the size of a logit: 2 (binary16) or 4 ---------------
+constexpr int DISTILL_MAX_K = 1024, ROUTER_MAX_E = 1024;
+size_t distill_workspace_bytes(int64_t n, int64_t v, int64_t k, int elem, bool grad);
+cudaError_t launch_topk_distill(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
+                                float *loss, float *lse, cudaStream_t stream);
+cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,
+                                     const float *dl, int64_t n, int64_t v, int64_t k, void *ds, cudaStream_t stream);
+size_t router_workspace_bytes(int64_t n, int64_t e, int num_sms);
+cudaError_t launch_router_balance(void *workspace, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k,
+                                  float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream);
+cudaError_t launch_router_balance_grad(int elem, const void *r, const uint8_t *keep, const int32_t *counts, const float *norm, const float *dl, int64_t n,
+                                       int64_t e, void *dr, int num_sms, cudaStream_t stream);
+
 }  // namespace fb

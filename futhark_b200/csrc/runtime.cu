@@ -633,6 +633,7 @@ FB_ARRAY_1D(u16_1d, uint16_t)
 FB_ARRAY_3D(f32_3d, float)
 FB_ARRAY_3D(i32_3d, int32_t)
 FB_ARRAY_3D(f16_3d, uint16_t)
+FB_ARRAY_2D(f16_2d, uint16_t)
 
 // ---- the opaque pair returned by partition (docs/c-api.rst:317-438) --------------------------------
 typedef struct futhark_opaque_tup2_arr1d_u32_arr1d_u32 pair_t;

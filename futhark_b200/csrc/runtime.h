@@ -152,6 +152,7 @@ FB_DEFINE_ARRAY_STRUCT(u16_1d, 1)
 FB_DEFINE_ARRAY_STRUCT(f32_3d, 3)
 FB_DEFINE_ARRAY_STRUCT(i32_3d, 3)
 FB_DEFINE_ARRAY_STRUCT(f16_3d, 3)
+FB_DEFINE_ARRAY_STRUCT(f16_2d, 2)
 
 struct futhark_opaque_tup2_arr1d_u32_arr1d_u32 {
   futhark_u32_1d *v0;
@@ -173,6 +174,20 @@ struct futhark_opaque_tup2_arr1d_i32_arr1d_i32 {
 
 struct futhark_opaque_tup6_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32 {
   futhark_i32_1d *v[6];
+};
+
+struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 {
+  futhark_f32_1d *v0, *v1;
+};
+
+struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 {
+  futhark_f16_2d *v0, *v1;
+};
+
+struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 {
+  futhark_f32_1d *v0;
+  futhark_i32_1d *v1;
+  futhark_f32_1d *v2;
 };
 
 struct futhark_opaque_tup2_i32_f32 {

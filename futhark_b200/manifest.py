@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PATH = os.path.join(HERE, "futhark_b200.json")
 
 ELEM = {"i32": "int32_t", "i64": "int64_t", "u32": "uint32_t", "f32": "float", "f64": "double", "bool": "bool", "f16": "uint16_t"}
-ARRAYS = ["i32_1d", "i64_1d", "u32_1d", "f32_1d", "f64_1d", "i8_1d", "i16_1d", "f16_1d", "u8_1d", "u16_1d", "bool_1d", "f32_2d", "i32_2d", "i64_2d", "f64_2d", "bool_2d", "f32_3d", "i32_3d", "f16_3d"]
+ARRAYS = ["i32_1d", "i64_1d", "u32_1d", "f32_1d", "f64_1d", "i8_1d", "i16_1d", "f16_1d", "u8_1d", "u16_1d", "bool_1d", "f32_2d", "i32_2d", "i64_2d", "f64_2d", "bool_2d", "f32_3d", "i32_3d", "f16_3d", "f16_2d"]
 
 PAIR = "opaque_tup2_arr1d_u32_arr1d_u32"
 TRIPLE = "opaque_tup3_arr1d_i32_arr1d_i32_arr1d_i32"
@@ -92,6 +92,15 @@ ENTRIES = {
     "prod_of_sums_i32": ([("xs", "[]i32"), ("ys", "[]i32")], "i32", []),
     "dotprod_i32": ([("xs", "[]i32"), ("ys", "[]i32")], "i32", []),
     "product_i32": ([("xs", "[]i32")], "i32", []),
+    "vocab_xent_f16": ([("X", "[][]f16"), ("W", "[][]f16"), ("ts", "[]i32")], "([]f32, []f32)", []),
+    "vocab_xent_grad_f16": ([("X", "[][]f16"), ("W", "[][]f16"), ("ts", "[]i32"), ("losses", "[]f32"), ("lses", "[]f32"), ("dls", "[]f32")],
+                            "([][]f16, [][]f16)", []),
+    **{"topk_distill_" + t: ([("tau", "f32"), ("S", "[][]" + t), ("iss", "[][]i32"), ("T", "[][]f32")], "([]f32, []f32)", []) for t in ("f32", "f16")},
+    **{"topk_distill_grad_" + t: ([("tau", "f32"), ("S", "[][]" + t), ("iss", "[][]i32"), ("T", "[][]f32"), ("lses", "[]f32"), ("dls", "[]f32")],
+                                  "[][]" + t, []) for t in ("f32", "f16")},
+    **{"router_balance_" + t: ([("R", "[][]" + t), ("keep", "[]bool"), ("iss", "[][]i32")], "([]f32, []i32, []f32)", []) for t in ("f32", "f16")},
+    **{"router_balance_grad_" + t: ([("R", "[][]" + t), ("keep", "[]bool"), ("counts", "[]i32"), ("norm", "[]f32"), ("dl", "[]f32")], "[][]" + t, [])
+       for t in ("f32", "f16")},
     "linrec_last_f32": ([("as", "[]f32"), ("bs", "[]f32")], "f32", []),
 }
 
@@ -142,6 +151,13 @@ def build():
                    "fields": [{"name": "0", "type": "[]i64", "project": "futhark_project_opaque_tup2_arr1d_i64_arr2d_f64_0"},
                               {"name": "1", "type": "[][]f64", "project": "futhark_project_opaque_tup2_arr1d_i64_arr2d_f64_1"}]},
     }
+    for name, fields in (("opaque_tup2_arr1d_f32_arr1d_f32", ("[]f32", "[]f32")), ("opaque_tup2_arr2d_f16_arr2d_f16", ("[][]f16", "[][]f16")),
+                         ("opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32", ("[]f32", "[]i32", "[]f32"))):
+        types["(%s)" % ", ".join(fields)] = {
+            "kind": "opaque", "ctype": "struct futhark_%s *" % name, "ops": {"free": "futhark_free_" + name},
+            "record": {"new": "futhark_new_" + name,
+                       "fields": [{"name": str(i), "type": t, "project": "futhark_project_%s_%d" % (name, i)} for i, t in enumerate(fields)]},
+        }
     entries = {}
     for name, (ins, out, tuning) in ENTRIES.items():
         entries[name] = {

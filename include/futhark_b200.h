@@ -147,6 +147,7 @@ FUTHARK_B200_ARRAY_1D(u16_1d, uint16_t)
 FUTHARK_B200_ARRAY_3D(f32_3d, float)
 FUTHARK_B200_ARRAY_3D(i32_3d, int32_t)
 FUTHARK_B200_ARRAY_3D(f16_3d, uint16_t)
+FUTHARK_B200_ARRAY_2D(f16_2d, uint16_t)
 
 /* ---- opaque tuple returned by partition: naming per
  *      src/Futhark/CodeGen/Backends/SimpleRep.hs:152-158; functions per
@@ -232,6 +233,36 @@ int futhark_project_opaque_tup6_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i3
     struct futhark_context *ctx, struct futhark_i32_1d **out, const struct futhark_opaque_tup6_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32 *obj);
 int futhark_project_opaque_tup6_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_5(
     struct futhark_context *ctx, struct futhark_i32_1d **out, const struct futhark_opaque_tup6_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32_arr1d_i32 *obj);
+
+/* ---- opaque tuples of the training losses: ([]f32, []f32) of vocab_xent_f16 and topk_distill_*, ([][]f16, [][]f16) of
+ *      vocab_xent_grad_f16, ([]f32, []i32, []f32) of router_balance_* (same naming rule and functions as the pairs above) ---------- */
+struct futhark_opaque_tup2_arr1d_f32_arr1d_f32;
+int futhark_free_opaque_tup2_arr1d_f32_arr1d_f32(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 *obj);
+int futhark_new_opaque_tup2_arr1d_f32_arr1d_f32(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out,
+                                                const struct futhark_f32_1d *v0, const struct futhark_f32_1d *v1);
+int futhark_project_opaque_tup2_arr1d_f32_arr1d_f32_0(struct futhark_context *ctx, struct futhark_f32_1d **out,
+                                                      const struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 *obj);
+int futhark_project_opaque_tup2_arr1d_f32_arr1d_f32_1(struct futhark_context *ctx, struct futhark_f32_1d **out,
+                                                      const struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 *obj);
+struct futhark_opaque_tup2_arr2d_f16_arr2d_f16;
+int futhark_free_opaque_tup2_arr2d_f16_arr2d_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 *obj);
+int futhark_new_opaque_tup2_arr2d_f16_arr2d_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 **out,
+                                                const struct futhark_f16_2d *v0, const struct futhark_f16_2d *v1);
+int futhark_project_opaque_tup2_arr2d_f16_arr2d_f16_0(struct futhark_context *ctx, struct futhark_f16_2d **out,
+                                                      const struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 *obj);
+int futhark_project_opaque_tup2_arr2d_f16_arr2d_f16_1(struct futhark_context *ctx, struct futhark_f16_2d **out,
+                                                      const struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 *obj);
+struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32;
+int futhark_free_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32(struct futhark_context *ctx, struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *obj);
+int futhark_new_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32(struct futhark_context *ctx, struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 **out,
+                                                          const struct futhark_f32_1d *v0, const struct futhark_i32_1d *v1,
+                                                          const struct futhark_f32_1d *v2);
+int futhark_project_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32_0(struct futhark_context *ctx, struct futhark_f32_1d **out,
+                                                                const struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *obj);
+int futhark_project_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32_1(struct futhark_context *ctx, struct futhark_i32_1d **out,
+                                                                const struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *obj);
+int futhark_project_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32_2(struct futhark_context *ctx, struct futhark_f32_1d **out,
+                                                                const struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 *obj);
 
 /* ---- opaque tuple (i32, f32) returned by sum_i32_f32: same naming and functions; its
  *      fields are scalars, so `new` takes and the projections return them by value ---------- */
@@ -465,6 +496,63 @@ int futhark_entry_partition_u32(struct futhark_context *ctx,
  * segmap_intrablock of src/Futhark/Optimise/BlkRegTiling.hs:68-140. */
 int futhark_entry_bmm_f16(struct futhark_context *ctx, struct futhark_f32_3d **out0,
                           const struct futhark_f16_3d *in0, const struct futhark_f16_3d *in1);
+
+/* ---- the losses of a training step and their vector-Jacobian products.  Results are enqueued like any others; none is read back.
+ *
+ * entry vocab_xent_f16 [n][v][d] (X: [n][d]f16) (W: [v][d]f16) (ts: [n]i32): ([n]f32, [n]f32) =
+ *   unzip (map2 (\x t -> let zs = map (\w -> f32.sum (map2 (\a b -> f32.f16 a * f32.f16 b) x w)) W
+ *                        let lse = f32.log (f32.sum (map f32.exp zs))
+ *                        in (if 0 <= t && t < i32.i64 v then lse - zs[t] else 0, lse)) X ts)
+ *   Softmax cross entropy of hidden states against a vocabulary, without the [n][v] logits in memory: the losses, and the
+ *   logarithms of the sums.  The sums are taken relative to the largest logit.  A target outside [0, v) is a token without one.
+ * entry vocab_xent_grad_f16 [n][v][d] (X: [n][d]f16) (W: [v][d]f16) (ts: [n]i32) (losses: [n]f32) (lses: [n]f32) (dls: [n]f32):
+ *     ([n][d]f16, [v][d]f16)
+ *   The gradients with respect to X and W of sum_i dls[i] losses[i]; losses and lses are what vocab_xent_f16 returned for the
+ *   same X, W and ts.  The logits are computed again in pieces of the vocabulary (at most 1 GiB of workspace for them); gradients
+ *   are rounded to binary16 once, so dls carries the scale that keeps them in its range.  Rows without a target have gradient 0. */
+int futhark_entry_vocab_xent_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0,
+                                 const struct futhark_f16_2d *in0, const struct futhark_f16_2d *in1, const struct futhark_i32_1d *in2);
+int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 **out0,
+                                      const struct futhark_f16_2d *in0, const struct futhark_f16_2d *in1, const struct futhark_i32_1d *in2,
+                                      const struct futhark_f32_1d *in3, const struct futhark_f32_1d *in4, const struct futhark_f32_1d *in5);
+
+/* entry topk_distill_f32 [n][v][k] (tau: f32) (S: [n][v]f32) (iss: [n][k]i32) (T: [n][k]f32): ([n]f32, [n]f32)
+ * entry topk_distill_f16 [n][v][k] (tau: f32) (S: [n][v]f16) (iss: [n][k]i32) (T: [n][k]f32): ([n]f32, [n]f32)
+ *   Distillation from a teacher of which every row's top k logits T and their words iss are kept.  With q = softmax (T/tau) over
+ *   the row's words, lse = log (sum (exp (S/tau))): the losses tau^2 sum_j q_j (log q_j - S[iss_j]/tau + lse), and the lse.  A word
+ *   outside [0, v), or whose logit is -inf, is padding; a row without words has loss 0; a word may stand in a row more than once.
+ *   tau is in [2^-60, 2^60], k at most 1024.
+ * entry topk_distill_grad_{f32,f16} (tau) (S) (iss) (T) (lses: [n]f32) (dls: [n]f32): [n][v]{f32,f16}
+ *   The gradient with respect to S of sum_i dls[i] losses[i]; rows without words have gradient 0. */
+int futhark_entry_topk_distill_f32(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0, const float in0,
+                                   const struct futhark_f32_2d *in1, const struct futhark_i32_2d *in2, const struct futhark_f32_2d *in3);
+int futhark_entry_topk_distill_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0, const float in0,
+                                   const struct futhark_f16_2d *in1, const struct futhark_i32_2d *in2, const struct futhark_f32_2d *in3);
+int futhark_entry_topk_distill_grad_f32(struct futhark_context *ctx, struct futhark_f32_2d **out0, const float in0,
+                                        const struct futhark_f32_2d *in1, const struct futhark_i32_2d *in2, const struct futhark_f32_2d *in3,
+                                        const struct futhark_f32_1d *in4, const struct futhark_f32_1d *in5);
+int futhark_entry_topk_distill_grad_f16(struct futhark_context *ctx, struct futhark_f16_2d **out0, const float in0,
+                                        const struct futhark_f16_2d *in1, const struct futhark_i32_2d *in2, const struct futhark_f32_2d *in3,
+                                        const struct futhark_f32_1d *in4, const struct futhark_f32_1d *in5);
+
+/* entry router_balance_f32 [n][e][k] (R: [n][e]f32) (keep: [n]bool) (iss: [n][k]i32): ([1]f32, [e]i32, [1]f32)
+ * entry router_balance_f16 [n][e][k] (R: [n][e]f16) (keep: [n]bool) (iss: [n][k]i32): ([1]f32, [e]i32, [1]f32)
+ *   The balance loss of a router and its per-expert counts.  counts = hist (+) 0 e of the experts iss of the kept rows (those
+ *   outside [0, e) are dropped), norm = e / (sum counts * number of kept rows), loss = norm * sum_e counts[e] * sum over the
+ *   kept rows of softmax(R)[e]: (loss, counts, norm).  Without a kept row or without an expert in range loss and norm are 0; a
+ *   row whose logits are all -inf has softmax 0.  e is at most 1024, n k below 2^31.
+ * entry router_balance_grad_{f32,f16} (R) (keep) (counts: [e]i32) (norm: [1]f32) (dl: [1]f32): [n][e]{f32,f16}
+ *   The gradient with respect to R of dl[0] * loss (the counts are constants); rows that are not kept have gradient 0. */
+int futhark_entry_router_balance_f32(struct futhark_context *ctx, struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 **out0,
+                                     const struct futhark_f32_2d *in0, const struct futhark_bool_1d *in1, const struct futhark_i32_2d *in2);
+int futhark_entry_router_balance_f16(struct futhark_context *ctx, struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 **out0,
+                                     const struct futhark_f16_2d *in0, const struct futhark_bool_1d *in1, const struct futhark_i32_2d *in2);
+int futhark_entry_router_balance_grad_f32(struct futhark_context *ctx, struct futhark_f32_2d **out0, const struct futhark_f32_2d *in0,
+                                          const struct futhark_bool_1d *in1, const struct futhark_i32_1d *in2,
+                                          const struct futhark_f32_1d *in3, const struct futhark_f32_1d *in4);
+int futhark_entry_router_balance_grad_f16(struct futhark_context *ctx, struct futhark_f16_2d **out0, const struct futhark_f16_2d *in0,
+                                          const struct futhark_bool_1d *in1, const struct futhark_i32_1d *in2,
+                                          const struct futhark_f32_1d *in3, const struct futhark_f32_1d *in4);
 
 /* entry transpose_f32 (xss: [][]f32): [][]f32 = transpose xss
  * entry transpose_f32_3d (xsss: [][][]f32): [][][]f32 = map transpose xsss

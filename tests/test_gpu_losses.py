@@ -1,0 +1,419 @@
+"""The training losses and their gradients through the C ABI against their definitions in 64 bits."""
+import numpy as np
+import pytest
+
+import futhark_b200 as fb
+import loss_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def half(bits):
+    return np.asarray(bits).view(np.float16).astype(np.float64)
+
+
+def within(got, want, err, what):
+    got = np.asarray(got, np.float64)
+    bad = ~(np.abs(got - want) <= err)
+    assert not bad.any(), "%s: %d of %d off, worst %.3g of what is allowed, first at %s: %r for %r" % (
+        what, bad.sum(), bad.size, float((np.abs(got - want) / err)[bad].max()), np.argwhere(bad)[0].tolist(), got[bad][0], want[bad][0])
+
+
+# ---- cross entropy over a vocabulary --------------------------------------------------------------------------
+def xent_inputs(n, v, d, seed, scale=2.0):
+    r = np.random.default_rng(seed)
+    X = r.normal(size=(n, d)).astype(np.float16)
+    W = (r.normal(size=(v, d)) * scale / max(1, d) ** 0.5).astype(np.float16)
+    ts = r.integers(0, max(1, v), n).astype(np.int32)
+    ts[r.random(n) < 0.1] = -1
+    dl = ((r.random(n) + 0.5) * 1024 / max(1, n)).astype(np.float32)
+    return X, W, ts, dl
+
+
+def check_xent(ctx, X, W, ts, dl):
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    want, wantl = ref.vocab_xent(X, W, ts)
+    err = ref.vocab_xent_error(X, W, ts)
+    within(lse, wantl, err, "lse")
+    within(loss, want, 2 * err, "loss")
+    dx, dw = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    wx, ww = ref.vocab_xent_grad(X, W, ts, dl)
+    ex, ew = ref.vocab_xent_grad_error(X, W, ts, dl)
+    within(half(dx), wx, ex, "dX")
+    within(half(dw), ww, ew, "dW")
+    assert np.all(dx[(ts < 0) | (ts >= len(W))] & 0x7fff == 0)
+
+
+@pytest.mark.parametrize("n,v,d", [
+    (1, 256, 64), (256, 256, 64), (1, 1, 1), (2, 3, 5), (1, 1000, 64), (31, 257, 8), (129, 255, 72), (128, 513, 136), (257, 1000, 100),
+    (300, 700, 129), (5, 4097, 64), (1000, 300, 512), (64, 3001, 1000), (7, 20001, 64), (700, 1234, 63)])
+def test_vocab_xent_and_gradient(ctx, n, v, d):
+    check_xent(ctx, *xent_inputs(n, v, d, n * 7 + v + d))
+
+
+def test_vocab_xent_many_row_and_column_tiles(ctx):
+    # more row tiles than share the columns' operand (16), and a ragged last one
+    check_xent(ctx, *xent_inputs(4500, 1500, 96, 5))
+
+
+def test_vocab_xent_in_pieces_of_the_vocabulary(ctx):
+    # more logits than 2^29: the vocabulary is worked off in two pieces, the second one shorter
+    n, v, d = 33000, 16500, 8
+    X, W, ts, dl = xent_inputs(n, v, d, 6)
+    rows = np.random.default_rng(7).permutation(n)[:400]          # dW sums over all rows: all but these weigh nothing
+    dl[np.delete(np.arange(n), rows)] = 0
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    dx, dw = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    X, ts, dl = X[rows], ts[rows], dl[rows]
+    want, wantl = ref.vocab_xent(X, W, ts)
+    err = ref.vocab_xent_error(X, W, ts)
+    within(lse[rows], wantl, err, "lse")
+    within(loss[rows], want, 2 * err, "loss")
+    wx, ww = ref.vocab_xent_grad(X, W, ts, dl)
+    ex, ew = ref.vocab_xent_grad_error(X, W, ts, dl)
+    within(half(dx)[rows], wx, ex, "dX")
+    within(half(dw), ww, ew, "dW")
+    assert not half(np.delete(dx, rows, axis=0)).any()
+
+
+@pytest.mark.parametrize("scale", [0.0, 30.0, 200.0])
+def test_vocab_xent_flat_and_peaked(ctx, scale):
+    # all logits equal; logits of which one is nearly all of the sum, with the target on it in every other row
+    X, W, ts, dl = xent_inputs(150, 400, 64, 11, scale)
+    ts[::2] = ref.vocab_xent(X, W, ts)[1].shape and (X.astype(np.float64) @ W.astype(np.float64).T).argmax(axis=1)[::2]
+    check_xent(ctx, X, W, ts, dl)
+
+
+def test_vocab_xent_weights_of_very_different_size(ctx):
+    X, W, ts, dl = xent_inputs(200, 300, 64, 12)
+    dl *= np.float32(2.0) ** np.random.default_rng(1).integers(-12, 3, 200).astype(np.float32)
+    dl[::7] *= -1
+    dl[5] = 0
+    check_xent(ctx, X, W, ts, dl)
+
+
+def test_vocab_xent_tokens_without_a_target(ctx):
+    X, W, ts, dl = xent_inputs(100, 300, 64, 13)
+    ts[:] = [-1, 300, -2**31, 2**31 - 1] * 25
+    X[3], X[4], dl[5], dl[6] = np.nan, np.inf, np.nan, np.inf      # of tokens that do not count
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    assert np.all(loss == 0)
+    dx, dw = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    assert np.all(half(dx) == 0) and np.all(half(dw) == 0)
+    # among others
+    X, W, ts, dl = xent_inputs(300, 300, 64, 14)
+    ts[10:20] = -1
+    clean = X.copy()
+    X[10:15], X[15:20] = np.nan, np.inf
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    got = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    loss, lse = fb.vocab_xent_f16(ctx, clean, W, ts)
+    want = fb.vocab_xent_grad_f16(ctx, clean, W, ts, loss, lse, dl)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+def test_vocab_xent_nan_and_infinity_stay(ctx):
+    X, W, ts, dl = xent_inputs(40, 300, 64, 15)
+    ts[:] = 1
+    X[7] = np.nan
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    assert np.isnan(loss[7]) and np.isnan(lse[7]) and np.isfinite(np.delete(loss, 7)).all()
+    dx, dw = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    assert np.isnan(half(dx)[7]).all() and np.isfinite(np.delete(half(dx), 7, axis=0)).all() and np.isnan(half(dw)).all()
+
+
+@pytest.mark.parametrize("n,v,d", [(0, 5, 8), (5, 0, 8), (5, 7, 0), (0, 0, 0)])
+def test_vocab_xent_of_nothing(ctx, n, v, d):
+    X, W, ts, dl = xent_inputs(n, v, d, 1)
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    if v == 0:
+        assert np.all(loss == 0) and np.all(lse == -np.inf)
+    else:
+        ok = (ts >= 0) & (ts < v)
+        assert np.allclose(lse, np.log(v)) and np.allclose(loss, np.where(ok, np.log(v), 0))
+    dx, dw = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    assert dx.shape == (n, d) and dw.shape == (v, d) and not dx.any() and not dw.any()
+
+
+def test_vocab_xent_operands_at_any_address(ctx):
+    X, W, ts, dl = xent_inputs(70, 300, 64, 16)
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    dx, dw = fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+    bx = ctx.new("f16_1d", np.concatenate([np.zeros(3, np.uint16), X.view(np.uint16).ravel()]))
+    bw = ctx.new("f16_1d", np.concatenate([np.zeros(1, np.uint16), W.view(np.uint16).ravel()]))
+    x, w = ctx.new_raw("f16_2d", bx.raw + 6, 70, 64), ctx.new_raw("f16_2d", bw.raw + 2, 300, 64)
+    t, g = ctx.new("i32_1d", ts), ctx.new("f32_1d", dl)
+    l, s = ctx.entry_vocab_xent_f16(x, w, t)
+    assert np.array_equal(l.values(), loss) and np.array_equal(s.values(), lse)
+    gx, gw = ctx.entry_vocab_xent_grad_f16(x, w, t, l, s, g)
+    assert np.array_equal(gx.values(), dx) and np.array_equal(gw.values(), dw)
+    for a in (gx, gw, l, s, t, g, x, w, bx, bw):
+        a.free()
+
+
+def test_vocab_xent_is_the_same_every_time(ctx):
+    X, W, ts, dl = xent_inputs(500, 5000, 256, 17)
+    first = None
+    for _ in range(3):
+        loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+        now = (loss, lse) + fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)
+        first = first or now
+        assert all(np.array_equal(a, b) for a, b in zip(first, now))
+
+
+# ---- distillation -----------------------------------------------------------------------------------------------
+def distill_inputs(t, n, v, k, seed, scale=3.0):
+    r = np.random.default_rng(seed)
+    S = (r.normal(size=(n, v)) * scale).astype(np.float16 if t == "f16" else np.float32)
+    iss = r.integers(0, max(1, v), (n, k)).astype(np.int32)
+    iss[r.random((n, k)) < 0.1] = -1
+    T = np.sort(r.normal(size=(n, k)) * 2 + 5, axis=1)[:, ::-1].astype(np.float32)
+    dl = (r.random(n) + 0.5).astype(np.float32) * (64 if t == "f16" else 1)
+    return S, iss, T, dl
+
+
+def check_distill(ctx, t, tau, S, iss, T, dl):
+    loss, lse = fb.topk_distill(ctx, t, tau, S, iss, T)
+    want, wantl, mag = ref.topk_distill(S, iss, T, tau)
+    big = np.abs(S.astype(np.float64)).max(axis=1, initial=0) / tau
+    # exponents are products with an f32 constant: 2^-23 of their size; exp2, sums and the teacher's softmax 2^-20
+    err = 2.0 ** -22 * big + 2.0 ** -20
+    within(lse, wantl, err + 2.0 ** -23 * np.abs(wantl), "lse")
+    within(loss, want, 2 * tau * tau * err + 2.0 ** -19 * mag, "loss")
+    g = fb.topk_distill_grad(ctx, t, tau, S, iss, T, lse, dl)
+    wg, mag = ref.topk_distill_grad(S, iss, T, tau, dl)
+    got = half(g) if t == "f16" else g
+    out = ref.H * np.abs(wg) + ref.HMIN if t == "f16" else 0
+    within(got, wg, mag * (4 * err + 2.0 ** -20)[:, None] + out + 1e-37, "dS")
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("n,v,k,tau", [
+    (1, 1, 1, 1.0), (3, 5, 2, 2.0), (17, 64, 8, 1.0), (9, 1001, 33, 0.5), (5, 8191, 64, 2.0), (4, 16385, 7, 4.0), (3, 50003, 128, 1.5),
+    (300, 257, 20, 3.0), (2, 70000, 1024, 1.0)])
+def test_topk_distill_and_gradient(ctx, t, n, v, k, tau):
+    check_distill(ctx, t, tau, *distill_inputs(t, n, v, k, n + v + k))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_topk_distill_rows_of_every_kind(ctx, t):
+    S, iss, T, dl = distill_inputs(t, 8, 4099, 6, 3)
+    iss[0] = [7, 7, 7, 7, 7, 7]                        # one word six times
+    iss[1] = [-1, 4099, -5, 2**31 - 1, -2**31, -1]     # none
+    T[2] = -np.inf                                     # none either
+    T[3, 2:] = -np.inf
+    iss[4] = [0, 4098, 0, 4098, 1, 4097]               # both ends, twice
+    S[5, 100:] = -np.inf                               # a student that rules words out
+    iss[5] = [0, 1, 99, 5, 6, -1]
+    S[6] = 0                                           # flat
+    T[7] = [60000, 0, 0, -60000, 1, 2]                 # all of the weight on one word
+    S[7, iss[7, 3]] = -np.inf if iss[7, 3] not in (iss[7, 0], iss[7, 4], iss[7, 5]) else 0
+    check_distill_special(ctx, t, 1.5, S, iss, T, dl)
+
+
+def check_distill_special(ctx, t, tau, S, iss, T, dl):
+    loss, lse = fb.topk_distill(ctx, t, tau, S, iss, T)
+    want, wantl, mag = ref.topk_distill(S, iss, T, tau)
+    within(lse, wantl, np.full(len(S), 1e-5), "lse")
+    within(loss, want, 1e-5 * (1 + mag), "loss")
+    g = fb.topk_distill_grad(ctx, t, tau, S, iss, T, lse, dl)
+    wg, mag = ref.topk_distill_grad(S, iss, T, tau, dl)
+    got = half(g) if t == "f16" else np.asarray(g, np.float64)
+    within(got, wg, 1e-5 * mag + (ref.H * np.abs(wg) + ref.HMIN if t == "f16" else 1e-37), "dS")
+    assert loss[1] == 0 and loss[2] == 0 and not got[1].any() and not got[2].any()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("shift", [1, 2, 3, 5])
+def test_topk_distill_rows_at_any_address(ctx, t, shift):
+    S, iss, T, dl = distill_inputs(t, 5, 2111, 9, shift)
+    loss, lse = fb.topk_distill(ctx, t, 2.0, S, iss, T)
+    want = fb.topk_distill_grad(ctx, t, 2.0, S, iss, T, lse, dl)
+    raw = fb._bits(S).ravel()
+    base = ctx.new(t + "_1d", np.concatenate([np.zeros(shift, raw.dtype), raw]))
+    s = ctx.new_raw(t + "_2d", base.raw + shift * raw.itemsize, 5, 2111)
+    i, q, d = ctx.new("i32_2d", iss), ctx.new("f32_2d", T), ctx.new("f32_1d", dl)
+    l, e = ctx.entry_topk_distill(t, 2.0, s, i, q)
+    g = ctx.entry_topk_distill_grad(t, 2.0, s, i, q, e, d)
+    # groups start elsewhere, so sums associate differently
+    assert np.allclose(l.values(), loss, rtol=1e-5, atol=1e-5) and np.allclose(e.values(), lse, rtol=1e-6)
+    if t == "f32":
+        assert np.allclose(g.values(), want, rtol=1e-5, atol=1e-9)
+    else:
+        assert np.allclose(half(g.values()), half(want), rtol=2.0 ** -9, atol=2.0 ** -24)
+    for a in (g, l, e, i, q, d, s, base):
+        a.free()
+
+
+@pytest.mark.parametrize("n,v,k", [(0, 5, 2), (4, 0, 2), (4, 5, 0)])
+def test_topk_distill_of_nothing(ctx, n, v, k):
+    S, iss, T, dl = distill_inputs("f32", n, v, k, 1)
+    loss, lse = fb.topk_distill(ctx, "f32", 1.0, S, iss, T)
+    assert np.all(loss == 0) and (v > 0 or np.all(lse == -np.inf))
+    g = fb.topk_distill_grad(ctx, "f32", 1.0, S, iss, T, lse, dl)
+    assert g.shape == (n, v) and not g.any()
+
+
+# ---- router balance -----------------------------------------------------------------------------------------------
+def router_inputs(t, n, e, k, seed):
+    r = np.random.default_rng(seed)
+    R = (r.normal(size=(n, e)) * 1.5 + r.normal(size=e)).astype(np.float16 if t == "f16" else np.float32)
+    iss = np.argsort(-R.astype(np.float64), axis=1, kind="stable")[:, :k].astype(np.int32)
+    iss[r.random((n, k)) < 0.05] = -1
+    return R, r.random(n) > 0.1, np.ascontiguousarray(iss)
+
+
+def check_router(ctx, t, R, keep, iss, dl):
+    loss, counts, norm = fb.router_balance(ctx, t, R, keep, iss)
+    wl, wc, wn, _ = ref.router_balance(R, keep, iss)
+    assert np.array_equal(counts, wc)
+    # rounded once from 64 bits; sums of positive terms, each within 2^-20 of its size (exponents up to 2^5)
+    assert loss.shape == norm.shape == (1,)
+    assert abs(float(norm[0]) - wn) <= ref.F * wn and abs(float(loss[0]) - wl) <= 2.0 ** -19 * wl
+    g = fb.router_balance_grad(ctx, t, R, keep, counts, norm, np.array([dl], np.float32))
+    wg, mag = ref.router_balance_grad(R, keep, iss, float(np.float32(dl)))
+    got = half(g) if t == "f16" else g
+    within(got, wg, 2.0 ** -19 * mag + (ref.H * np.abs(wg) + ref.HMIN if t == "f16" else 1e-37), "dR")
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("n,e,k", [
+    (1, 1, 1), (1, 2, 1), (5, 3, 2), (16, 8, 2), (100, 31, 4), (333, 32, 4), (333, 33, 6), (1000, 60, 4), (777, 64, 8), (500, 100, 3),
+    (2000, 256, 8), (300, 300, 16), (100, 513, 8), (64, 1024, 32), (20000, 5, 5), (9000, 160, 6)])
+def test_router_balance_and_gradient(ctx, t, n, e, k):
+    check_router(ctx, t, *router_inputs(t, n, e, k, n + e + k), 100.0 if t == "f16" else 0.01)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_router_balance_rows_of_every_kind(ctx, t):
+    R, keep, iss = router_inputs(t, 40, 20, 3, 9)
+    R[keep.nonzero()[0][0]] = -np.inf                  # every expert ruled out: no probability at all
+    R[5, 3:] = -np.inf
+    R[6] = -60000
+    out = (~keep).nonzero()[0]
+    R[out], iss[out] = np.nan, 1                       # padding does not count, whatever it holds
+    iss[8] = [4, 4, 4]
+    iss[9] = [-1, 20, 2**31 - 1]
+    check_router(ctx, t, R, keep, iss, 3.0)
+
+
+@pytest.mark.parametrize("keep,expert", [(False, 0), (True, -1)])
+def test_router_balance_with_nothing_to_count(ctx, keep, expert):
+    R, _, iss = router_inputs("f32", 30, 7, 2, 4)
+    iss[:] = expert
+    loss, counts, norm = fb.router_balance(ctx, "f32", R, np.full(30, keep), iss)
+    assert loss[0] == 0 and norm[0] == 0 and not counts.any()
+    g = fb.router_balance_grad(ctx, "f32", R, np.full(30, keep), counts, norm, np.ones(1, np.float32))
+    assert not g.any()
+
+
+@pytest.mark.parametrize("n,e,k", [(0, 4, 2), (4, 0, 2), (4, 4, 0)])
+def test_router_balance_of_nothing(ctx, n, e, k):
+    R, keep, iss = np.zeros((n, e), np.float32), np.ones(n, bool), np.zeros((n, k), np.int32)
+    loss, counts, norm = fb.router_balance(ctx, "f32", R, keep, iss)
+    assert loss[0] == 0 and norm[0] == 0 and counts.shape == (e,) and not counts.any()
+    assert fb.router_balance_grad(ctx, "f32", R, keep, counts, norm, np.ones(1, np.float32)).shape == (n, e)
+
+
+def test_router_balance_nearly_equal_counts(ctx):
+    # every token goes everywhere but for a few drops: the gradient is what is left of a difference
+    R, keep, _ = router_inputs("f32", 5000, 16, 16, 21)
+    iss = np.tile(np.arange(16, dtype=np.int32), (5000, 1))
+    iss[::1000, 3] = -1
+    loss, counts, norm = fb.router_balance(ctx, "f32", R, keep, iss)
+    g = fb.router_balance_grad(ctx, "f32", R, keep, counts, norm, np.ones(1, np.float32))
+    want, _ = ref.router_balance_grad(R, keep, iss, 1.0)
+    assert np.linalg.norm(g - want) <= 2.0 ** -18 * np.linalg.norm(want)
+
+
+# ---- together, refusals, streams -------------------------------------------------------------------------------------
+def test_a_step_with_all_three_losses(ctx):
+    """A training step's sum of losses, every gradient taken: results stay on the device between the calls, blocks are reused."""
+    n, v, d, e, k = 96, 1000, 64, 8, 2
+    X, W, ts, dl = xent_inputs(n, v, d, 31)
+    S, si, T, ddl = distill_inputs("f16", n, v, 5, 32)
+    R, keep, ri = router_inputs("f32", n, e, k, 33)
+    want = None
+    for _ in range(3):
+        arrs = [ctx.new(t, a) for t, a in (("f16_2d", X.view(np.uint16)), ("f16_2d", W.view(np.uint16)), ("i32_1d", ts), ("f32_1d", dl),
+                                           ("f16_2d", S.view(np.uint16)), ("i32_2d", si), ("f32_2d", T), ("f32_1d", ddl),
+                                           ("f32_2d", R), ("bool_1d", keep), ("i32_2d", ri), ("f32_1d", np.full(1, 0.01, np.float32)))]
+        x, w, t, g, s, i, q, sg, r, kp, ex, rg = arrs
+        out = ctx.entry_vocab_xent_f16(x, w, t)
+        out += ctx.entry_topk_distill("f16", 2.0, s, i, q)
+        out += ctx.entry_router_balance("f32", r, kp, ex)
+        out += ctx.entry_vocab_xent_grad_f16(x, w, t, out[0], out[1], g)
+        out += (ctx.entry_topk_distill_grad("f16", 2.0, s, i, q, out[3], sg), ctx.entry_router_balance_grad("f32", r, kp, out[5], out[6], rg))
+        vals = [a.values_into(np.empty(a.shape, fb.ARRAY_TYPES[a.tname][0])) for a in out]
+        for a in arrs + list(out):
+            a.free()
+        ctx.sync()
+        want = want or vals
+        assert all(np.array_equal(a, b) for a, b in zip(want, vals))
+    within(want[0], ref.vocab_xent(X, W, ts)[0], 2 * ref.vocab_xent_error(X, W, ts), "loss")
+    assert np.array_equal(want[5], ref.router_balance(R, keep, ri)[1])
+
+
+def test_two_contexts_at_once(ctx):
+    X, W, ts, dl = xent_inputs(600, 3000, 128, 41)
+    want = fb.vocab_xent_f16(ctx, X, W, ts)
+    with fb.Context() as other:
+        a = [[c.new("f16_2d", X.view(np.uint16)), c.new("f16_2d", W.view(np.uint16)), c.new("i32_1d", ts)] for c in (ctx, other)]
+        outs = [c.entry_vocab_xent_f16(*b) for _ in range(4) for c, b in zip((ctx, other), a)]
+        for o in outs:
+            assert np.array_equal(o[0].values(), want[0]) and np.array_equal(o[1].values(), want[1])
+            o[0].free(); o[1].free()
+        for b in a:
+            for x in b:
+                x.free()
+
+
+def refused(ctx, call, text):
+    with pytest.raises(fb.FutharkError) as e:
+        call()
+    assert text in str(e.value)
+
+
+def test_refusals(ctx):
+    X, W, ts, dl = xent_inputs(4, 6, 8, 1)
+    f = np.zeros(4, np.float32)
+    sizes = "invalid sizes"
+    refused(ctx, lambda: fb.vocab_xent_f16(ctx, X, W[:, :7], ts), sizes)
+    refused(ctx, lambda: fb.vocab_xent_f16(ctx, X, W, ts[:3]), sizes)
+    for at in range(3):
+        args = [f, f, f]
+        args[at] = f[:3]
+        refused(ctx, lambda: fb.vocab_xent_grad_f16(ctx, X, W, ts, *args), sizes)
+    S, iss, T, dl = distill_inputs("f32", 4, 9, 2, 1)
+    refused(ctx, lambda: fb.topk_distill(ctx, "f32", 1.0, S, iss[:3], T), sizes)
+    refused(ctx, lambda: fb.topk_distill(ctx, "f32", 1.0, S, iss, T[:, :1]), sizes)
+    refused(ctx, lambda: fb.topk_distill_grad(ctx, "f32", 1.0, S, iss, T, f[:3], f), sizes)
+    refused(ctx, lambda: fb.topk_distill_grad(ctx, "f32", 1.0, S, iss, T, f, f[:3]), sizes)
+    for tau in (0.0, -1.0, float("nan"), float("inf"), 1e-30):
+        refused(ctx, lambda: fb.topk_distill(ctx, "f32", tau, S, iss, T), "temperature")
+        refused(ctx, lambda: fb.topk_distill_grad(ctx, "f32", tau, S, iss, T, f, f), "temperature")
+    wide = np.zeros((4, 1025), np.int32)
+    refused(ctx, lambda: fb.topk_distill(ctx, "f32", 1.0, S, wide, wide.astype(np.float32)), "1024")
+    R, keep, ri = router_inputs("f32", 4, 3, 2, 1)
+    one = np.ones(1, np.float32)
+    refused(ctx, lambda: fb.router_balance(ctx, "f32", R, keep[:3], ri), sizes)
+    refused(ctx, lambda: fb.router_balance(ctx, "f32", R, keep, ri[:3]), sizes)
+    refused(ctx, lambda: fb.router_balance(ctx, "f32", np.zeros((4, 1025), np.float32), keep, ri), "1024")
+    refused(ctx, lambda: fb.router_balance_grad(ctx, "f32", R, keep, np.zeros(2, np.int32), one, one), sizes)
+    refused(ctx, lambda: fb.router_balance_grad(ctx, "f32", R, keep, np.zeros(3, np.int32), one, f), sizes)
+    # and the context goes on
+    assert fb.vocab_xent_f16(ctx, X, W, ts)[0].shape == (4,)
+
+
+@pytest.mark.parametrize("rec,types", [(fb.LOSSES, ("f32_1d", "f32_1d")), (fb.GRADS_F16, ("f16_2d", "f16_2d")), (fb.BALANCE, ("f32_1d", "i32_1d", "f32_1d"))])
+def test_records_share_their_fields(ctx, rec, types):
+    import ctypes
+    data = [np.arange(6, dtype=fb.ARRAY_TYPES[t][0]).reshape((2, 3) if t.endswith("2d") else 6) + i for i, t in enumerate(types)]
+    arrs = [ctx.new(t, x) for t, x in zip(types, data)]
+    obj = ctypes.c_void_p()
+    assert getattr(ctx.lib, "futhark_new_" + rec)(ctx.ptr, ctypes.byref(obj), *[a.ptr for a in arrs]) == 0
+    for a in arrs:
+        a.free()
+    for got, want in zip(ctx._fields(rec, types, obj), data):
+        assert np.array_equal(got.values(), want)
+        got.free()
