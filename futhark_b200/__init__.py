@@ -277,27 +277,49 @@ def _take_string(ptr):
     return s
 
 
+class _TypeFns:
+    """The functions of one array type, looked up once."""
+
+    def __init__(self, L, tname):
+        self.dtype, self.rank, _ = ARRAY_TYPES[tname]
+        self.typestr = np.dtype(self.dtype).str
+        self.new_raw, self.free = getattr(L, "futhark_new_raw_" + tname), getattr(L, "futhark_free_" + tname)
+        self.shape, self.raw = getattr(L, "futhark_shape_" + tname), getattr(L, "futhark_values_raw_" + tname)
+
+
+_type_fns = {}
+
+
+def _fns(tname):
+    f = _type_fns.get(tname)
+    if f is None:
+        f = _type_fns[tname] = _TypeFns(load(), tname)
+    return f
+
+
 class Array:
     """A device array owned by a context (struct futhark_<t>_<n>d *)."""
 
     def __init__(self, ctx, tname, ptr):
         self.ctx, self.tname, self.ptr = ctx, tname, ptr
+        self._interface = None
 
     @property
     def shape(self):
-        rank = ARRAY_TYPES[self.tname][1]
-        p = getattr(self.ctx.lib, "futhark_shape_" + self.tname)(self.ctx.ptr, self.ptr)
-        return tuple(int(p[i]) for i in range(rank))
+        f = _fns(self.tname)
+        return tuple(f.shape(self.ctx.ptr, self.ptr)[:f.rank])
 
     @property
     def raw(self):
         """Device address (futhark_values_raw_*)."""
-        return int(getattr(self.ctx.lib, "futhark_values_raw_" + self.tname)(self.ctx.ptr, self.ptr))
+        return _fns(self.tname).raw(self.ctx.ptr, self.ptr)
 
     @property
     def __cuda_array_interface__(self):
-        dt = np.dtype(ARRAY_TYPES[self.tname][0])
-        return {"shape": self.shape, "typestr": dt.str, "data": (self.raw, False), "version": 2}
+        d = self._interface                  # neither the shape nor the address of an array ever changes
+        if d is None or self.ptr is None:
+            d = self._interface = {"shape": self.shape, "typestr": _fns(self.tname).typestr, "data": (self.raw, False), "version": 2}
+        return d
 
     def values_into(self, out):
         """Asynchronous copy to a host buffer (futhark_values_*); call ctx.sync() before reading."""
@@ -320,8 +342,20 @@ class Array:
 
     def free(self):
         if self.ptr:
-            getattr(self.ctx.lib, "futhark_free_" + self.tname)(self.ctx.ptr, self.ptr)
+            _fns(self.tname).free(self.ctx.ptr, self.ptr)
             self.ptr = None
+
+
+_record_fn_cache = {}
+
+
+def _record_fns(rec, k):
+    """(free, project_0, ...) of an opaque record type, looked up once."""
+    f = _record_fn_cache.get(rec)
+    if f is None:
+        L = load()
+        f = _record_fn_cache[rec] = tuple([getattr(L, "futhark_free_" + rec)] + [getattr(L, "futhark_project_%s_%d" % (rec, i)) for i in range(k)])
+    return f
 
 
 class Pair:
@@ -448,7 +482,7 @@ class Context:
         return arr
 
     def new_raw(self, tname, devptr, *shape):
-        p = getattr(self.lib, "futhark_new_raw_" + tname)(self.ptr, int(devptr), *shape)
+        p = _fns(tname).new_raw(self.ptr, int(devptr), *shape)
         if not p:
             raise FutharkError(1, self.get_error() or "futhark_new_raw_%s failed" % tname)
         return Array(self, tname, p)
@@ -635,11 +669,11 @@ class Context:
     def _fields(self, rec, types, obj):
         """The fields of an opaque record as arrays; the record is freed."""
         parts = []
-        for i, t in enumerate(types):
+        for project, t in zip(_record_fns(rec, len(types))[1:], types):
             out = ctypes.c_void_p()
-            self._check(getattr(self.lib, "futhark_project_%s_%d" % (rec, i))(self.ptr, ctypes.byref(out), obj))
+            self._check(project(self.ptr, ctypes.byref(out), obj))
             parts.append(Array(self, t, out.value))
-        self._check(getattr(self.lib, "futhark_free_" + rec)(self.ptr, obj))
+        self._check(_record_fns(rec, len(types))[0](self.ptr, obj))
         return tuple(parts)
 
     def _entry_rec(self, name, rec, types, *args):

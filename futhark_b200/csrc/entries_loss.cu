@@ -82,6 +82,8 @@ typedef struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 grads_t;
 typedef struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 balance_t;
 
 // ---- cross entropy over a vocabulary ------------------------------------------------------------------
+// sizes that are 32-bit numbers in the kernels, tiles among them
+static bool vocab_fits(int64_t n, int64_t v, int64_t d) { return fits(n) && fits(v) && fits(d + 8) && n / 256 * (v / 128) < ((int64_t)1 << 30); }
 static std::string vocab_details(int64_t n, int64_t v, int64_t d) { return "{" + kv("n", n) + "," + kv("v", v) + "," + kv("d", d) + "}"; }
 
 extern "C" {
@@ -92,7 +94,7 @@ int futhark_entry_vocab_xent_f16(struct futhark_context *ctx, losses_t **out0, c
   CtxGuard g(ctx);
   const int64_t n = in0->shape[0], d = in0->shape[1], v = in1->shape[0];
   if (in1->shape[1] != d || in2->shape[0] != n) return bad_sizes(ctx);
-  if (!fits(n) || !fits(v) || !fits(d + 8)) return refuse(ctx, "Error: vocab_xent_f16: sizes must be below 2^31.\n");
+  if (!vocab_fits(n, v, d)) return refuse(ctx, "Error: vocab_xent_f16: sizes must be below 2^31 and n v below 2^45.\n");
   Call call(ctx);
   auto *loss = call.array<futhark_f32_1d>({n}, 4, "vocab_xent_f16.loss"), *lse = call.array<futhark_f32_1d>({n}, 4, "vocab_xent_f16.lse");
   auto *rec = call.record<losses_t>();
@@ -116,7 +118,7 @@ int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, grads_t **out
   CtxGuard g(ctx);
   const int64_t n = in0->shape[0], d = in0->shape[1], v = in1->shape[0];
   if (in1->shape[1] != d || in2->shape[0] != n || in3->shape[0] != n || in4->shape[0] != n || in5->shape[0] != n) return bad_sizes(ctx);
-  if (!fits(n) || !fits(v) || !fits(d + 8)) return refuse(ctx, "Error: vocab_xent_grad_f16: sizes must be below 2^31.\n");
+  if (!vocab_fits(n, v, d)) return refuse(ctx, "Error: vocab_xent_grad_f16: sizes must be below 2^31 and n v below 2^45.\n");
   Call call(ctx);
   auto *dx = call.array<futhark_f16_2d>({n, d}, 2, "vocab_xent_grad_f16.dx"), *dw = call.array<futhark_f16_2d>({v, d}, 2, "vocab_xent_grad_f16.dw");
   auto *rec = call.record<grads_t>();

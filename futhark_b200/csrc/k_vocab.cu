@@ -35,14 +35,10 @@ namespace fb {
 
 constexpr int VT = 256;                                // tile edge of a CTA pair
 constexpr int VK = 64;                                 // summed elements per stage
-constexpr int V_STAGES = 6;
 constexpr int V_OPERAND = 128 * VK * 2;                // a CTA's half of one operand in one stage: 16 KiB
 constexpr int V_STAGE = 2 * V_OPERAND;
 constexpr int V_SLAB = VK * 64 * 2;                    // 64 x 64 block of an operand that is contiguous across the sum
 constexpr int V_EPI_BUF = 32 * 128;                    // 32 rows of 128 bytes
-constexpr int V_EPI = 4 * 2 * V_EPI_BUF;               // two per epilogue warp
-constexpr int V_SMEM = V_STAGES * V_STAGE + 1024 /*alignment*/ + 1024 /*barriers*/ + V_EPI;
-constexpr int V_THREADS = 192;
 constexpr int V_GROUP = 16;                            // row tiles that share the columns' operand before it moves on
 constexpr float V_LOG2E = 1.4426950408889634f;
 constexpr float V_GSCALE = 8192.f;                     // 2^13, see above
@@ -54,13 +50,28 @@ enum VocabEpilogue : int {
   VE_HALF = 3,         // binary16, times a factor from device memory
 };
 
+// Shared memory and warps by epilogue.  One epilogue warp per SM partition cannot hide its own latencies (an
+// instruction every 4.5 clocks, 7400 clocks for a 256-column tile of which the exponentials need 2048): there are
+// V_SOFT_WARPS / 4 or V_STORE_WARPS / 4, each with its share of the tile's columns.  Folding needs no staging and leaves room for another stage.
+constexpr int V_SOFT_WARPS = 8, V_STORE_WARPS = 8;
+template <int EPI> struct VocabShape {
+  static constexpr int warps = EPI == VE_SOFTMAX ? V_SOFT_WARPS : V_STORE_WARPS;
+  static constexpr int cols = VT / (warps / 4);                      // columns of a warp
+  static constexpr int stages = EPI == VE_SOFTMAX ? 6 : 5;
+  static constexpr int threads = 64 + 32 * warps;
+  static constexpr int staging = EPI == VE_SOFTMAX ? 0 : warps * 2 * V_EPI_BUF;
+  static constexpr int smem = stages * V_STAGE + 1024 /*alignment*/ + 1024 /*barriers*/ + staging;
+};
+
 struct VocabArgs {
   int M, N, kblocks;            // extents; the summed axis in blocks of VK
+  int nt;                       // columns of a tile: a multiple of 32 up to 256
+  int arows0, arows1;           // rows of A that the two CTAs bring per stage: 128 unless there is one row tile
   int splits, kps;              // parts of the summed axis and the blocks of each
   int tiles_m, tiles_n;
   const int32_t *targets;       // VE_SOFTMAX, VE_GRAD
-  int64_t v, v0;                // size of the vocabulary, first word of the piece
-  float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum in units of log 2, sum)
+  int v, v0;                    // size of the vocabulary, first word of the piece
+  float2 *part;                 // VE_SOFTMAX: [M][tiles_n][warps / 4] (maximum in units of log 2, sum)
   float *ztarget;
   const float *cexp;            // VE_GRAD: per row the exponent's constant term
   const float *factor;          // VE_HALF
@@ -74,9 +85,10 @@ __device__ __forceinline__ float ex2(float x) {        // 2^x: at most 2 units i
   return y;
 }
 
+constexpr int V_MAX_STAGES = 8;
 struct VocabBarriers {
-  uint64_t full[V_STAGES];       // used in the pair's first CTA only
-  uint64_t empty[V_STAGES];
+  uint64_t full[V_MAX_STAGES];   // used in the pair's first CTA only
+  uint64_t empty[V_MAX_STAGES];
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];        // used in the pair's first CTA only
   uint32_t tmem_base;
@@ -84,23 +96,23 @@ struct VocabBarriers {
 
 // Tiles in the order the pairs take them: V_GROUP row tiles by all column tiles, the rows first.  74 pairs then
 // work on about 16 x 5 tiles at a time, whose operands come from HBM once and from L2 for every further tile.
-__device__ __forceinline__ void vocab_tile(const VocabArgs &a, int64_t t, int &split, int &tm, int &tn) {
-  const int64_t per = (int64_t)a.tiles_m * a.tiles_n;
-  split = (int)(t / per);
-  const int64_t r = t - split * per;
-  const int64_t gsize = (int64_t)V_GROUP * a.tiles_n;
-  const int g = (int)(r / gsize);
-  const int in = (int)(r - g * gsize);
-  const int rows = min(V_GROUP, a.tiles_m - g * V_GROUP);
-  tn = in / rows;
-  tm = g * V_GROUP + in - tn * rows;
+__device__ __forceinline__ void vocab_tile(const VocabArgs &a, uint32_t t, int &split, int &tm, int &tn) {
+  const uint32_t per = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n, gsize = (uint32_t)V_GROUP * (uint32_t)a.tiles_n;
+  const uint32_t sp = a.splits > 1 ? t / per : 0, r = t - sp * per;
+  const uint32_t g = r / gsize, in = r - g * gsize;
+  const uint32_t rows = min((uint32_t)V_GROUP, (uint32_t)a.tiles_m - g * V_GROUP);
+  const uint32_t n = in / rows;
+  split = (int)sp;
+  tn = (int)n;
+  tm = (int)(g * V_GROUP + in - n * rows);
 }
 
 // A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
 template <bool A_MN, bool B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VocabShape<EPI>::threads, 1)
 vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const VocabArgs a) {
+  constexpr int V_STAGES = VocabShape<EPI>::stages, EPI_WARPS = VocabShape<EPI>::warps, COLS = VocabShape<EPI>::cols;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   VocabBarriers *bars = reinterpret_cast<VocabBarriers *>(smem + V_STAGES * V_STAGE);
@@ -108,12 +120,12 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int64_t num_tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+  const uint32_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const uint32_t num_tiles = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n * (uint32_t)a.splits;     // below 2^31
 
   if (tid == 0) {
     for (int s = 0; s < V_STAGES; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], 256); }
+    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], 2 * EPI_WARPS); }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -133,10 +145,11 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (lane == 0) {
         uint32_t it = 0;
         bool ok = true;
-        for (int64_t t = pair; t < num_tiles && ok; t += npairs) {
+        for (uint32_t t = pair; t < num_tiles && ok; t += npairs) {
           int split, tm, tn;
           vocab_tile(a, t, split, tm, tn);
-          const int m0 = tm * VT + (int)rank * 128, n0 = tn * VT + (int)rank * 128;
+          const int m0 = tm * VT + (int)rank * 128, n0 = tn * a.nt + (int)rank * (a.nt >> 1);
+          const int arows = rank == 0 ? a.arows0 : a.arows1;
           const int kb1 = min(a.kblocks, (split + 1) * a.kps);
           for (int kb = split * a.kps; kb < kb1; kb++, it++) {
             const int s = it % V_STAGES;
@@ -145,16 +158,16 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             uint8_t *sa = smem + s * V_STAGE;
             uint8_t *sb = sa + V_OPERAND;
             const uint32_t full0 = map_to_cta(smem_u32(&bars->full[s]), 0);
-            if (rank == 0) mbar_expect_tx(&bars->full[s], 2 * V_STAGE);          // both CTAs' bytes
+            if (rank == 0) mbar_expect_tx(&bars->full[s], (a.arows0 + a.arows1 + a.nt) * (VK * 2));   // both CTAs' bytes
             if (A_MN) {
               tma_load_3d_pair(sa, &tmA, m0, kb * VK, 0, full0);
               tma_load_3d_pair(sa + V_SLAB, &tmA, m0 + 64, kb * VK, 0, full0);
-            } else {
+            } else if (arows > 0) {
               tma_load_3d_pair(sa, &tmA, kb * VK, m0, 0, full0);
             }
             if (B_MN) {
               tma_load_3d_pair(sb, &tmB, n0, kb * VK, 0, full0);
-              tma_load_3d_pair(sb + V_SLAB, &tmB, n0 + 64, kb * VK, 0, full0);
+              if (a.nt > 128) tma_load_3d_pair(sb + V_SLAB, &tmB, n0 + 64, kb * VK, 0, full0);
             } else {
               tma_load_3d_pair(sb, &tmB, kb * VK, n0, 0, full0);
             }
@@ -165,11 +178,11 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     } else if (warp == 1) {
       // ---------------- MMA issuer: one thread of the first CTA ----------------
       if (lane == 0 && rank == 0) {
-        // D = f32, A = B = f16, N = 256, M = 256 over the pair
-        constexpr uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(VT >> 3) << 17) | ((uint32_t)(VT >> 4) << 24);
+        // D = f32, A = B = f16, M = 256 over the pair, N the tile's columns
+        const uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(a.nt >> 3) << 17) | ((uint32_t)(VT >> 4) << 24);
         uint32_t it = 0, tile_it = 0;
         bool ok = true;
-        for (int64_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
+        for (uint32_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
           int split, tm, tn;
           vocab_tile(a, t, split, tm, tn);
           const uint32_t acc = tile_it & 1, acc_ph = (tile_it >> 1) & 1;
@@ -199,32 +212,42 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
       }
     } else {
-      // ---------------- epilogue (warps 2..5): this CTA's 128 rows of the tile, one row per thread ----------------
-      const int quarter = warp & 3;
+      // ---------------- epilogue: this CTA's 128 rows of the tile, one row and COLS columns per thread ----------------
+      const int quarter = warp & 3, share = (warp - 2) >> 2, cbase = share * COLS;
       uint32_t tile_it = 0;
       bool ok = true;
       uint8_t *stg = epi + (warp - 2) * (2 * V_EPI_BUF);
       int buf = 0;
       const float factor = EPI == VE_HALF ? *a.factor : 1.f;
-      for (int64_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
-        int split, tm, tn;
-        vocab_tile(a, t, split, tm, tn);
-        const int row0 = tm * VT + (int)rank * 128 + quarter * 32, n0 = tn * VT;
+      // what a tile needs of its row is fetched while the tile before it is worked on
+      int tm = 0, tn = 0, split = 0, next_target = -1;
+      float next_c = 0.f;
+      auto fetch = [&](uint32_t t, int &sp, int &m, int &n) {
+        if (t >= num_tiles) return;
+        vocab_tile(a, t, sp, m, n);
+        const int r = m * VT + (int)rank * 128 + quarter * 32 + lane;
+        if ((EPI == VE_SOFTMAX || EPI == VE_GRAD) && r < a.M) {
+          next_target = a.targets[r];
+          if (EPI == VE_GRAD) next_c = a.cexp[r];
+        }
+      };
+      fetch(pair, split, tm, tn);
+      for (uint32_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
+        const int row0 = tm * VT + (int)rank * 128 + quarter * 32, n0 = tn * a.nt;
         const int row = row0 + lane;
         const uint32_t acc = tile_it & 1, acc_ph = (tile_it >> 1) & 1;
-        const int ncols = min(VT, a.N - n0);
+        const int ncols = min(a.nt, a.N - n0);
         int tcol = -1;                                     // the target's column in this tile, if it has it
-        float c = 0.f;
-        bool counts = false;
-        if ((EPI == VE_SOFTMAX || EPI == VE_GRAD) && row < a.M) {
-          const int64_t tg = a.targets[row];
-          counts = tg >= 0 && tg < a.v;
-          const int64_t tl = tg - a.v0 - n0;
-          if (counts && tl >= 0 && tl < ncols) tcol = (int)tl;
-          if (EPI == VE_GRAD) c = a.cexp[row];
+        const float c = next_c;
+        const bool counts = next_target >= 0 && next_target < a.v && row < a.M;
+        if (EPI == VE_SOFTMAX || EPI == VE_GRAD) {
+          const int tl = next_target - a.v0 - n0;
+          if (counts && tl >= 0 && tl < ncols) tcol = tl;
         }
+        const int this_split = split, this_tn = tn;
         if (!__all_sync(kFull, mbar_wait_bounded(&bars->tmem_full[acc], acc_ph))) { ok = false; break; }
         tc_fence_after();
+        fetch(t + npairs, split, tm, tn);
         const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * VT;
         float m2 = -INFINITY, sum = 0.f;
 
@@ -297,9 +320,9 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (row0 < a.M && n0 + c0 < a.N) {
-              if (EPI == VE_SLAB && a.add) tma_add_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, split);
-              else tma_store_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, split);
+            if (c0 < ncols) {                              // the tile's, and not behind the last column
+              if (EPI == VE_SLAB && a.add) tma_add_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, this_split);
+              else tma_store_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, this_split);
             }
             bulk_commit();
           }
@@ -313,24 +336,27 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           release(c0);
         };
 
-        uint32_t va[32], vb[32];
-        tmem_ld_32x32(taddr0, va);
+        if (row0 < a.M && cbase < ncols) {                 // uniform over the warp
+          uint32_t va[32], vb[32];
+          tmem_ld_32x32(taddr0 + cbase, va);
 #pragma unroll 1
-        for (int cc = 0; cc < VT; cc += 64) {
-          tmem_ld_wait();
-          tmem_ld_32x32(taddr0 + cc + 32, vb);
-          if (EPI == VE_SOFTMAX) fold(va, cc);
-          else if (EPI == VE_SLAB) slab(va, cc);
-          else { uint32_t h[16]; to_half(va, cc, h); acquire(); half_pieces(h, 0); }
-          tmem_ld_wait();
-          if (cc + 64 < VT) tmem_ld_32x32(taddr0 + cc + 64, va);
-          if (EPI == VE_SOFTMAX) fold(vb, cc + 32);
-          else if (EPI == VE_SLAB) slab(vb, cc + 32);
-          else { uint32_t h[16]; to_half(vb, cc + 32, h); half_pieces(h, 4); release(cc); }
+          for (int cc = cbase; cc < cbase + COLS; cc += 64) {
+            tmem_ld_wait();
+            tmem_ld_32x32(taddr0 + cc + 32, vb);
+            if (EPI == VE_SOFTMAX) fold(va, cc);
+            else if (EPI == VE_SLAB) slab(va, cc);
+            else { uint32_t h[16]; to_half(va, cc, h); acquire(); half_pieces(h, 0); }
+            tmem_ld_wait();
+            if (cc + 64 < cbase + COLS) tmem_ld_32x32(taddr0 + cc + 64, va);
+            if (EPI == VE_SOFTMAX) fold(vb, cc + 32);
+            else if (EPI == VE_SLAB) slab(vb, cc + 32);
+            else { uint32_t h[16]; to_half(vb, cc + 32, h); half_pieces(h, 4); release(cc); }
+          }
         }
         tc_fence_before();
-        mbar_arrive_cluster(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
-        if (EPI == VE_SOFTMAX && row < a.M) a.part[(int64_t)row * a.tiles_n + tn] = make_float2(m2, sum);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
+        if (EPI == VE_SOFTMAX && row < a.M) a.part[((int64_t)row * a.tiles_n + this_tn) * (EPI_WARPS / 4) + share] = make_float2(m2, sum);
       }
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
@@ -429,13 +455,20 @@ vocab_scale_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const in
   }
 }
 
-// Rows of another pitch, what is behind the narrower of the two 0 or left out.
+// Rows of another pitch, what is behind the narrower of the two 0 or left out; 8 elements of the result per thread.
 __global__ void __launch_bounds__(256)
 vocab_pitch_kernel(const __half *__restrict__ in, int64_t rows, int64_t in_cols, __half *__restrict__ out, int64_t out_cols) {
   const int64_t total = rows * out_cols;
-  for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
-    const int64_t i = o / out_cols, c = o - i * out_cols;
-    out[o] = c < in_cols ? in[i * in_cols + c] : __half(0.f);
+  for (int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; o < total; o += (int64_t)gridDim.x * 2048) {
+    int64_t i = o / out_cols, c = o - i * out_cols;
+    __align__(16) __half h[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      h[j] = c < in_cols && o + j < total ? in[i * in_cols + c] : __half(0.f);
+      if (++c == out_cols) { c = 0; i++; }
+    }
+    if (o + 8 <= total && ((uintptr_t)(out + o) & 15) == 0) *reinterpret_cast<uint4 *>(out + o) = *reinterpret_cast<const uint4 *>(h);
+    else for (int j = 0; j < 8 && o + j < total; j++) out[o + j] = h[j];
   }
 }
 
@@ -485,18 +518,34 @@ static inline int elementwise_grid(int64_t items, int num_sms) {
   return (int)(g < 1 ? 1 : g < (int64_t)num_sms * 16 ? g : (int64_t)num_sms * 16);
 }
 
+// Columns of a tile.  A tile of fewer columns reuses its rows less, but a number of tiles that is just above a multiple of
+// the number of pairs leaves most pairs idle in the last round; the estimate is in clocks, 512 per block of 64
+// summed elements and 256 columns at the tensor cores' rate, a fifth of it for the rows' operand.
+static int tile_columns(int64_t rows, int64_t cols, int64_t parts, int64_t kblocks, int step, int pairs) {
+  int best = VT;
+  double best_cost = 0;
+  for (int nt = VT; nt >= 128; nt -= step) {
+    const int64_t tiles = ceil_div(rows, VT) * ceil_div(cols, nt) * parts;
+    const double cost = (double)ceil_div(tiles, pairs) * (kblocks * (nt + 64) * 1.6 + 1500.0);
+    if (nt == VT || cost < 0.97 * best_cost) { best = nt; best_cost = cost; }
+  }
+  return best;
+}
+
 // Parts of the summed axis of dX = G W.  A small batch has fewer tiles than there are pairs of SMs, while its sum
-// runs over the vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks: 512 per
-// block of 64 and tile at the tensor cores' rate, 3000 per tile for its epilogue where nothing hides it, 3600 bytes of HBM per clock.
-static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int pairs) {
-  const int64_t tiles = ceil_div(n, VT) * ceil_div(dp, VT);
+// runs over the vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks, as above, with
+// 3000 per tile for its epilogue where nothing hides it and 3600 bytes of HBM per clock for the slabs.
+static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int pairs, int *nt) {
   int best = 1;
   double best_cost = 0;
-  for (int s = 1; s <= 64 && s <= kblocks; s++) {
-    const int64_t kps = ceil_div(kblocks, s);
-    if (ceil_div(kblocks, kps) != s) continue;
-    const double cost = (double)ceil_div(tiles * s, pairs) * (kps * 512.0 + 3000.0) + (double)s * n * dp * 8 / 3600.0;
-    if (s == 1 || cost < best_cost) { best = s; best_cost = cost; }
+  for (int w = VT; w >= 128; w -= 128) {
+    const int64_t tiles = ceil_div(n, VT) * ceil_div(dp, w);
+    for (int s = 1; s <= 64 && s <= kblocks; s++) {
+      const int64_t kps = ceil_div(kblocks, s);
+      if (ceil_div(kblocks, kps) != s) continue;
+      const double cost = (double)ceil_div(tiles * s, pairs) * (kps * (w + 64) * 1.6 + 3000.0) + (double)s * n * dp * 8 / 3600.0;
+      if ((s == 1 && w == VT) || cost < best_cost) { best = s; *nt = w; best_cost = cost; }
+    }
   }
   return best;
 }
@@ -506,6 +555,7 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   if (n <= 0 || v <= 0 || (grad && d <= 0)) return p;           // nothing will run
   p.dp = d <= 0 ? 8 : (d + 7) & ~(int64_t)7;
   const bool padded = p.dp != d;
+  const int pairs = num_sms / 2;
   size_t off = 0;
   auto take = [&](size_t bytes) { const size_t at = off; off += align256(bytes); return at; };
   p.copy_x = padded || !x_aligned;
@@ -513,7 +563,8 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   p.xp = p.copy_x ? take((size_t)(n * p.dp) * 2) : 0;
   p.wp = p.copy_w ? take((size_t)(v * p.dp) * 2) : 0;
   if (!grad) {
-    p.part = take((size_t)(n * ceil_div(v, VT)) * sizeof(float2));
+    p.nt = tile_columns(n, v, 1, ceil_div(p.dp, VK), 32, pairs);
+    p.part = take((size_t)(n * ceil_div(v, p.nt) * (V_SOFT_WARPS / 4)) * sizeof(float2));
     p.zt = take((size_t)n * 4);
   } else {
     // pieces of the vocabulary whose part of G is at most 1 GiB: 65536 words for 8192 tokens
@@ -523,8 +574,8 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     if (words < VT) words = VT;
     if (words > want) words = want;
     p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
-    const int pairs = num_sms / 2 > 0 ? num_sms / 2 : 1;
-    p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), pairs);
+    p.nt = tile_columns(n, p.piece < v ? p.piece : v, 1, ceil_div(p.dp, VK), 64, pairs);
+    p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), pairs, &p.ntd);
     p.w = take((size_t)n * 4);
     p.cexp = take((size_t)n * 4);
     p.scalars = take(256);
@@ -539,26 +590,33 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
 
 template <bool A_MN, bool B_MN, int EPI>
 static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
+  using Shape = VocabShape<EPI>;
   auto kernel = vocab_mma_kernel<A_MN, B_MN, EPI>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, V_SMEM);
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem);
   if (err != cudaSuccess) return err;
   a.tiles_m = (int)ceil_div(a.M, VT);
-  a.tiles_n = (int)ceil_div(a.N, VT);
+  a.tiles_n = (int)ceil_div(a.N, a.nt);
   a.kps = (int)ceil_div(a.kblocks, a.splits);
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   int pairs = num_sms / 2;
   if (tiles < pairs) pairs = (int)tiles;
-  kernel<<<2 * pairs, V_THREADS, V_SMEM, stream>>>(tmA, tmB, tmC, a);
+  kernel<<<2 * pairs, Shape::threads, Shape::smem, stream>>>(tmA, tmB, tmC, a);
   return cudaGetLastError();
 }
 
-// an operand [rows][cols] of row pitch `pitch`: boxes of 128 rows where it is read along the sum, of 64 where across it
-static bool operand_map(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, int64_t pitch, bool across) {
-  return make_tensor_map(tm, base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)pitch, (uint64_t)pitch * rows, 64, across ? 64 : 128);
+// an operand [rows][cols] of row pitch `pitch`, in boxes of 64 columns and `box` rows: 64 where it is read across the sum
+static bool operand_map(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, int64_t pitch, int box) {
+  return make_tensor_map(tm, base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)pitch, (uint64_t)pitch * rows, 64, (uint32_t)box);
+}
+// Rows of an operand that the CTAs of a pair bring per stage.  A single row tile brings no more than there are (whole
+// groups of 8, as the swizzle has them): what shared memory holds below is the product of rows that no one reads.
+static void single_tile_rows(VocabArgs &a) {
+  a.arows0 = a.arows1 = 128;
+  if (a.M <= 128) { a.arows0 = (a.M + 7) / 8 * 8; a.arows1 = 0; }
 }
 
 static cudaError_t repitch(const uint16_t *in, int64_t rows, int64_t in_cols, uint16_t *out, int64_t out_cols, int num_sms, cudaStream_t stream) {
-  vocab_pitch_kernel<<<elementwise_grid(rows * out_cols, num_sms), 256, 0, stream>>>(reinterpret_cast<const __half *>(in), rows, in_cols,
+  vocab_pitch_kernel<<<elementwise_grid((rows * out_cols + 7) / 8, num_sms), 256, 0, stream>>>(reinterpret_cast<const __half *>(in), rows, in_cols,
                                                                                      reinterpret_cast<__half *>(out), out_cols);
   return cudaGetLastError();
 }
@@ -576,15 +634,17 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
   if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
   if (p.copy_w) { FB_TRY(repitch(w, v, d, reinterpret_cast<uint16_t *>(ws + p.wp), p.dp, num_sms, stream)); w = reinterpret_cast<uint16_t *>(ws + p.wp); }
   CUtensorMap tmX, tmW;
-  if (!operand_map(&tmX, x, n, p.dp, p.dp, false) || !operand_map(&tmW, w, v, p.dp, p.dp, false)) return cudaErrorInvalidValue;
   VocabArgs a = {};
   a.M = (int)n; a.N = (int)v; a.kblocks = (int)ceil_div(p.dp, VK); a.splits = 1;
-  a.targets = targets; a.v = v; a.v0 = 0;
+  a.nt = p.nt;
+  single_tile_rows(a);
+  if (!operand_map(&tmX, x, n, p.dp, p.dp, a.arows0) || !operand_map(&tmW, w, v, p.dp, p.dp, a.nt / 2)) return cudaErrorInvalidValue;
+  a.targets = targets; a.v = (int)v; a.v0 = 0;
   a.part = reinterpret_cast<float2 *>(ws + p.part);
   a.ztarget = reinterpret_cast<float *>(ws + p.zt);
   a.failure = failure;
   FB_TRY((launch_mma<false, false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
-  vocab_loss_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, stream>>>(a.part, (int)ceil_div(v, VT), a.ztarget, targets, loss, lse, n, v);
+  vocab_loss_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, stream>>>(a.part, (int)ceil_div(v, p.nt) * (V_SOFT_WARPS / 4), a.ztarget, targets, loss, lse, n, v);
   return cudaGetLastError();
 }
 
@@ -612,25 +672,29 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     const int64_t vw = v - v0 < p.piece ? v - v0 : p.piece;
     CUtensorMap tmX, tmW, tmG, tmGk, tmWn, tmS, tmGm, tmXn, tmD;
     uint16_t *dwo = p.dp == d ? dw + v0 * d : reinterpret_cast<uint16_t *>(ws + p.dwp);
-    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, false) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, false) &&
+    VocabArgs a = {};
+    a.M = (int)n;
+    single_tile_rows(a);
+    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, a.arows0) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, p.nt / 2) &&
                     make_tensor_map(&tmG, g, (uint64_t)vw, (uint64_t)n, 1, (uint64_t)p.piece, (uint64_t)p.piece * n, 64, 32) &&
-                    operand_map(&tmGk, g, n, vw, p.piece, false) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, true) &&
+                    operand_map(&tmGk, g, n, vw, p.piece, a.arows0) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, 64) &&
                     make_tensor_map(&tmS, slabs, (uint64_t)p.dp, (uint64_t)n, (uint64_t)p.splits, (uint64_t)p.dp, (uint64_t)(p.dp * n), 32, 32, true) &&
-                    operand_map(&tmGm, g, n, vw, p.piece, true) && operand_map(&tmXn, xs, n, p.dp, p.dp, true) &&
+                    operand_map(&tmGm, g, n, vw, p.piece, 64) && operand_map(&tmXn, xs, n, p.dp, p.dp, 64) &&
                     make_tensor_map(&tmD, dwo, (uint64_t)p.dp, (uint64_t)vw, 1, (uint64_t)p.dp, (uint64_t)(p.dp * vw), 64, 32);
     if (!ok) return cudaErrorInvalidValue;
-    VocabArgs a = {};
     a.failure = failure;
-    a.targets = targets; a.v = v; a.v0 = v0; a.cexp = cexp; a.factor = factor;
+    a.targets = targets; a.v = (int)v; a.v0 = (int)v0; a.cexp = cexp; a.factor = factor;
     a.splits = 1;
-    a.M = (int)n; a.N = (int)vw; a.kblocks = (int)ceil_div(p.dp, VK);
+    a.N = (int)vw; a.kblocks = (int)ceil_div(p.dp, VK); a.nt = p.nt;
     FB_TRY((launch_mma<false, false, VE_GRAD>(tmX, tmW, tmG, a, num_sms, stream)));
     // every part has its blocks in every piece: the last one may be shorter, and then some slabs get nothing more
-    a.M = (int)n; a.N = (int)p.dp; a.kblocks = (int)ceil_div(vw, VK);
+    a.N = (int)p.dp; a.kblocks = (int)ceil_div(vw, VK); a.nt = p.ntd;
     a.splits = (int)ceil_div(a.kblocks, ceil_div(a.kblocks, p.splits < a.kblocks ? p.splits : a.kblocks));
     a.add = v0 > 0;
     FB_TRY((launch_mma<false, true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
     a.M = (int)vw; a.N = (int)p.dp; a.kblocks = (int)ceil_div(n, VK); a.splits = 1; a.add = 0;
+    a.nt = tile_columns(vw, p.dp, 1, a.kblocks, 128, num_sms / 2);
+    a.arows0 = a.arows1 = 128;
     FB_TRY((launch_mma<true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
     if (p.dp != d) FB_TRY(repitch(dwo, vw, p.dp, dw + v0 * d, d, num_sms, stream));
   }

@@ -187,7 +187,8 @@ struct VocabPlan {
   int64_t dp;                  // width of the rows the tensor cores see: d rounded up to 8
   bool copy_x, copy_w;         // operands that are copied: another width, or a base that is no multiple of 16 bytes
   int64_t piece;               // gradient: words per piece of the vocabulary
-  int splits;                  // gradient: parts of the sum over a piece's words
+  int nt;                      // columns of a tile of logits
+  int splits, ntd;             // gradient: parts of the sum over a piece's words, columns of a tile of dX
   size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dwp, bytes;
 };
 VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_aligned, bool grad, int num_sms);
