@@ -50,16 +50,13 @@ enum VocabEpilogue : int {
   VE_HALF = 3,         // binary16, times a factor from device memory
 };
 
-// Shared memory and warps by epilogue.  One epilogue warp per SM partition cannot hide its own latencies (an
-// instruction every 4.5 clocks, 7400 clocks for a 256-column tile of which the exponentials need 2048): there are
-// V_SOFT_WARPS / 4 or V_STORE_WARPS / 4, each with its share of the tile's columns.  Folding needs no staging and leaves room for another stage.
-constexpr int V_SOFT_WARPS = 8, V_STORE_WARPS = 8;
+// Sixteen epilogue warps, four per SM partition, each with a row and 64 of the tile's columns per thread.  One warp
+// per partition cannot hide its own latencies: it issued every 4.5 clocks and took 7400 clocks for a tile of which the
+// exponentials need 2048.  Folding stages nothing and leaves room for another stage of operands.
+constexpr int V_WARPS = 16, V_COLS = VT / (V_WARPS / 4), V_THREADS = 64 + 32 * V_WARPS;
 template <int EPI> struct VocabShape {
-  static constexpr int warps = EPI == VE_SOFTMAX ? V_SOFT_WARPS : V_STORE_WARPS;
-  static constexpr int cols = VT / (warps / 4);                      // columns of a warp
   static constexpr int stages = EPI == VE_SOFTMAX ? 6 : 5;
-  static constexpr int threads = 64 + 32 * warps;
-  static constexpr int staging = EPI == VE_SOFTMAX ? 0 : warps * 2 * V_EPI_BUF;
+  static constexpr int staging = EPI == VE_SOFTMAX ? 2 * (V_WARPS / 4) * 128 * (int)sizeof(float2) : V_WARPS * V_EPI_BUF;
   static constexpr int smem = stages * V_STAGE + 1024 /*alignment*/ + 1024 /*barriers*/ + staging;
 };
 
@@ -71,7 +68,7 @@ struct VocabArgs {
   int tiles_m, tiles_n;
   const int32_t *targets;       // VE_SOFTMAX, VE_GRAD
   int v, v0;                    // size of the vocabulary, first word of the piece
-  float2 *part;                 // VE_SOFTMAX: [M][tiles_n][warps / 4] (maximum in units of log 2, sum)
+  float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum in units of log 2, sum)
   float *ztarget;
   const float *cexp;            // VE_GRAD: per row the exponent's constant term
   const float *factor;          // VE_HALF
@@ -91,6 +88,7 @@ struct VocabBarriers {
   uint64_t empty[V_MAX_STAGES];
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];        // used in the pair's first CTA only
+  uint64_t met[2][4];            // VE_SOFTMAX: three shares of 32 rows are in shared memory
   uint32_t tmem_base;
 };
 
@@ -109,10 +107,10 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs &a, uint32_t t, int &
 
 // A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
 template <bool A_MN, bool B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(VocabShape<EPI>::threads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
 vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const VocabArgs a) {
-  constexpr int V_STAGES = VocabShape<EPI>::stages, EPI_WARPS = VocabShape<EPI>::warps, COLS = VocabShape<EPI>::cols;
+  constexpr int V_STAGES = VocabShape<EPI>::stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   VocabBarriers *bars = reinterpret_cast<VocabBarriers *>(smem + V_STAGES * V_STAGE);
@@ -125,7 +123,8 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   if (tid == 0) {
     for (int s = 0; s < V_STAGES; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], 2 * EPI_WARPS); }
+    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], 2 * V_WARPS); }
+    for (int i = 0; i < 8; i++) mbar_init(&bars->met[i >> 2][i & 3], V_WARPS / 4 - 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -212,12 +211,11 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
       }
     } else {
-      // ---------------- epilogue: this CTA's 128 rows of the tile, one row and COLS columns per thread ----------------
-      const int quarter = warp & 3, share = (warp - 2) >> 2, cbase = share * COLS;
+      // ---------------- epilogue: this CTA's 128 rows of the tile, one row and V_COLS columns per thread ----------------
+      const int quarter = warp & 3, share = (warp - 2) >> 2, cbase = share * V_COLS;
       uint32_t tile_it = 0;
       bool ok = true;
-      uint8_t *stg = epi + (warp - 2) * (2 * V_EPI_BUF);
-      int buf = 0;
+      uint8_t *stg = epi + (warp - 2) * V_EPI_BUF;
       const float factor = EPI == VE_HALF ? *a.factor : 1.f;
       // what a tile needs of its row is fetched while the tile before it is worked on
       int tm = 0, tn = 0, split = 0, next_target = -1;
@@ -304,16 +302,16 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             h[j] = (EPI == VE_GRAD && !counts) ? 0u : *reinterpret_cast<const uint32_t *>(&p);
           }
         };
-        // Chunks are staged as the 128-byte swizzle wants them (16-byte piece q of row r at q ^ (r & 7)) and leave
-        // by one bulk tensor store; of two buffers the one written is the one whose store has been read.
+        // 128 bytes of a row are staged as the 128-byte swizzle wants them (16-byte piece q of row r at q ^ (r & 7))
+        // and leave by one bulk tensor store, which has read the buffer before it is written again.
         auto half_pieces = [&](const uint32_t (&h)[16], int q0) {
 #pragma unroll
           for (int q = 0; q < 4; q++)
-            *reinterpret_cast<uint4 *>(stg + buf * V_EPI_BUF + lane * 128 + (((q0 + q) ^ (lane & 7)) << 4)) =
+            *reinterpret_cast<uint4 *>(stg + lane * 128 + (((q0 + q) ^ (lane & 7)) << 4)) =
                 make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
         };
         auto acquire = [&] {
-          if (lane == 0) bulk_wait_read1();
+          if (lane == 0) bulk_wait_read0();
           __syncwarp();
         };
         auto release = [&](int c0) {
@@ -321,42 +319,56 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           __syncwarp();
           if (lane == 0) {
             if (c0 < ncols) {                              // the tile's, and not behind the last column
-              if (EPI == VE_SLAB && a.add) tma_add_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, this_split);
-              else tma_store_3d(&tmC, stg + buf * V_EPI_BUF, n0 + c0, row0, this_split);
+              if (EPI == VE_SLAB && a.add) tma_add_3d(&tmC, stg, n0 + c0, row0, this_split);
+              else tma_store_3d(&tmC, stg, n0 + c0, row0, this_split);
             }
             bulk_commit();
           }
-          buf ^= 1;
         };
         auto slab = [&](const uint32_t (&v)[32], int c0) {
           acquire();
 #pragma unroll
           for (int q = 0; q < 8; q++)
-            *reinterpret_cast<uint4 *>(stg + buf * V_EPI_BUF + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            *reinterpret_cast<uint4 *>(stg + lane * 128 + ((q ^ (lane & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           release(c0);
         };
 
         if (row0 < a.M && cbase < ncols) {                 // uniform over the warp
           uint32_t va[32], vb[32];
           tmem_ld_32x32(taddr0 + cbase, va);
-#pragma unroll 1
-          for (int cc = cbase; cc < cbase + COLS; cc += 64) {
-            tmem_ld_wait();
-            tmem_ld_32x32(taddr0 + cc + 32, vb);
-            if (EPI == VE_SOFTMAX) fold(va, cc);
-            else if (EPI == VE_SLAB) slab(va, cc);
-            else { uint32_t h[16]; to_half(va, cc, h); acquire(); half_pieces(h, 0); }
-            tmem_ld_wait();
-            if (cc + 64 < cbase + COLS) tmem_ld_32x32(taddr0 + cc + 64, va);
-            if (EPI == VE_SOFTMAX) fold(vb, cc + 32);
-            else if (EPI == VE_SLAB) slab(vb, cc + 32);
-            else { uint32_t h[16]; to_half(vb, cc + 32, h); half_pieces(h, 4); release(cc); }
+          tmem_ld_wait();
+          tmem_ld_32x32(taddr0 + cbase + 32, vb);
+          if (EPI == VE_SOFTMAX) fold(va, cbase);
+          else if (EPI == VE_SLAB) slab(va, cbase);
+          else { uint32_t h[16]; to_half(va, cbase, h); acquire(); half_pieces(h, 0); }
+          tmem_ld_wait();
+          if (EPI == VE_SOFTMAX) fold(vb, cbase + 32);
+          else if (EPI == VE_SLAB) slab(vb, cbase + 32);
+          else { uint32_t h[16]; to_half(vb, cbase + 32, h); half_pieces(h, 4); release(cbase); }
+        }
+        if (EPI == VE_SOFTMAX) {
+          // the four shares of a row meet in shared memory, at the first one's warp; its arrival below is what lets the
+          // tile after the next one, which uses the same places, begin
+          float2 *meet = reinterpret_cast<float2 *>(epi) + (tile_it & 1) * (V_WARPS / 4) * 128 + quarter * 32 + lane;
+          if (share != 0) {
+            meet[share * 128] = make_float2(m2, sum);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->met[tile_it & 1][quarter]);
+          } else {
+            if (!__all_sync(kFull, mbar_wait_bounded(&bars->met[tile_it & 1][quarter], acc_ph))) { ok = false; break; }
+#pragma unroll
+            for (int w = 1; w < V_WARPS / 4; w++) {
+              const float2 o = meet[w * 128];
+              const float mn = fmaxf(m2, o.x), ref = mn == -INFINITY ? 0.f : mn;
+              sum = sum * ex2(m2 - ref) + o.y * ex2(o.x - ref);
+              m2 = mn;
+            }
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
-        if (EPI == VE_SOFTMAX && row < a.M) a.part[((int64_t)row * a.tiles_n + this_tn) * (EPI_WARPS / 4) + share] = make_float2(m2, sum);
+        if (lane == 0) mbar_arrive_pair(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
+        if (EPI == VE_SOFTMAX && share == 0 && row < a.M) a.part[(int64_t)row * a.tiles_n + this_tn] = make_float2(m2, sum);
       }
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
@@ -564,7 +576,7 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   p.wp = p.copy_w ? take((size_t)(v * p.dp) * 2) : 0;
   if (!grad) {
     p.nt = tile_columns(n, v, 1, ceil_div(p.dp, VK), 32, pairs);
-    p.part = take((size_t)(n * ceil_div(v, p.nt) * (V_SOFT_WARPS / 4)) * sizeof(float2));
+    p.part = take((size_t)(n * ceil_div(v, p.nt)) * sizeof(float2));
     p.zt = take((size_t)n * 4);
   } else {
     // pieces of the vocabulary whose part of G is at most 1 GiB: 65536 words for 8192 tokens
@@ -590,9 +602,9 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
 
 template <bool A_MN, bool B_MN, int EPI>
 static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
-  using Shape = VocabShape<EPI>;
+  constexpr int smem = VocabShape<EPI>::smem;
   auto kernel = vocab_mma_kernel<A_MN, B_MN, EPI>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::smem);
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (err != cudaSuccess) return err;
   a.tiles_m = (int)ceil_div(a.M, VT);
   a.tiles_n = (int)ceil_div(a.N, a.nt);
@@ -600,7 +612,7 @@ static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, co
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   int pairs = num_sms / 2;
   if (tiles < pairs) pairs = (int)tiles;
-  kernel<<<2 * pairs, Shape::threads, Shape::smem, stream>>>(tmA, tmB, tmC, a);
+  kernel<<<2 * pairs, V_THREADS, smem, stream>>>(tmA, tmB, tmC, a);
   return cudaGetLastError();
 }
 
@@ -644,7 +656,7 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
   a.ztarget = reinterpret_cast<float *>(ws + p.zt);
   a.failure = failure;
   FB_TRY((launch_mma<false, false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
-  vocab_loss_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, stream>>>(a.part, (int)ceil_div(v, p.nt) * (V_SOFT_WARPS / 4), a.ztarget, targets, loss, lse, n, v);
+  vocab_loss_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, stream>>>(a.part, (int)ceil_div(v, p.nt), a.ztarget, targets, loss, lse, n, v);
   return cudaGetLastError();
 }
 

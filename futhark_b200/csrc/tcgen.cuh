@@ -98,6 +98,10 @@ __device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorM
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
+// The same without a fence of the thread's global stores: for what the thread has only read (tensor memory, after tcgen05.wait::ld).
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
 __device__ __forceinline__ void tc2_commit_both(uint64_t *bar) {     // arrives on `bar` in both CTAs of the pair
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
