@@ -142,7 +142,7 @@ int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, grads_t **out
 static int distill_refusal(futhark_context *ctx, float tau, int64_t n, int64_t v, int64_t k) {
   if (!(tau >= 0x1p-60f && tau <= 0x1p60f)) return refuse(ctx, "Error: topk_distill: the temperature must be in [2^-60, 2^60].\n");
   if (k > fb::DISTILL_MAX_K) return refuse(ctx, "Error: topk_distill: at most 1024 logits per row.\n");
-  if (!fits(n) || !fits(v)) return refuse(ctx, "Error: topk_distill: sizes must be below 2^31.\n");
+  if (!fits(n) || !fits(v + 16384)) return refuse(ctx, "Error: topk_distill: sizes must be below 2^31 - 2^14.\n");
   return 0;
 }
 static std::string distill_details(int64_t n, int64_t v, int64_t k) { return "{" + kv("n", n) + "," + kv("v", v) + "," + kv("k", k) + "}"; }
@@ -227,7 +227,7 @@ static int router_balance(futhark_context *ctx, const char *name, int elem, bala
   auto *counts = call.array<futhark_i32_1d>({e}, 4, "router_balance.counts");
   auto *norm = call.array<futhark_f32_1d>({1}, 4, "router_balance.norm");
   auto *rec = call.record<balance_t>();
-  void *ws = call.workspace(fb::router_workspace_bytes(n, e, ctx->num_sms), "router_balance.workspace");
+  void *ws = call.workspace(fb::router_workspace_bytes(dptr<void>(r->mem), elem, n, e, ctx->num_sms), "router_balance.workspace");
   call.launch(name, "(norm * sum (map2 (*) counts (reduce (map2 (+)) (map softmax R))), hist (+) 0 e is, norm)",
               "{" + kv("n", n) + "," + kv("e", e) + "," + kv("k", k) + "}", [&] {
     return fb::launch_router_balance(ws, elem, dptr<void>(r->mem), dptr<uint8_t>(keep->mem), dptr<int32_t>(is->mem), n, e, k, dptr<float>(loss->mem),

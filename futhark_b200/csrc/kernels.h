@@ -205,7 +205,7 @@ cudaError_t launch_topk_distill(void *workspace, int elem, const void *s, const 
                                 float *loss, float *lse, cudaStream_t stream);
 cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,
                                      const float *dl, int64_t n, int64_t v, int64_t k, void *ds, cudaStream_t stream);
-size_t router_workspace_bytes(int64_t n, int64_t e, int num_sms);
+size_t router_workspace_bytes(const void *r, int elem, int64_t n, int64_t e, int num_sms);
 cudaError_t launch_router_balance(void *workspace, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k,
                                   float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream);
 cudaError_t launch_router_balance_grad(int elem, const void *r, const uint8_t *keep, const int32_t *counts, const float *norm, const float *dl, int64_t n,
