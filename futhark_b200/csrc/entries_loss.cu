@@ -58,10 +58,10 @@ struct Call {
     rc = fb_alloc(ctx, bytes, desc, &ws);
     return dptr<void>(ws);
   }
-  template <typename LAUNCH>
-  void launch(const char *name, const char *prov, const std::string &details, LAUNCH f) {
+  template <typename DETAILS, typename LAUNCH>
+  void launch(const char *name, const char *prov, DETAILS details, LAUNCH f) {       // details are only made where someone reads them
     if (rc != FUTHARK_SUCCESS) return;
-    LaunchScope ls(ctx, name, prov, details);
+    LaunchScope ls(ctx, name, prov, ctx->logging || ctx->profiling ? details() : std::string());
     rc = fb_cuda_check(ctx, f(), name);
   }
   ~Call() {
@@ -100,7 +100,7 @@ int futhark_entry_vocab_xent_f16(struct futhark_context *ctx, losses_t **out0, c
   auto *rec = call.record<losses_t>();
   const fb::VocabPlan plan = fb::vocab_plan(n, v, d, aligned16(in0->mem), aligned16(in1->mem), false, ctx->num_sms);
   void *ws = call.workspace(plan.bytes, "vocab_xent_f16.workspace");
-  call.launch("vocab_xent_f16.segred", "map2 (\\x t -> log (sum (map exp (map (dot x) W))) - dot x W[t]) X ts", vocab_details(n, v, d), [&] {
+  call.launch("vocab_xent_f16.segred", "map2 (\\x t -> log (sum (map exp (map (dot x) W))) - dot x W[t]) X ts", [&] { return vocab_details(n, v, d); }, [&] {
     ctx->failure_is_an_option = true;
     return fb::launch_vocab_xent(plan, ws, dptr<uint16_t>(in0->mem), dptr<uint16_t>(in1->mem), dptr<int32_t>(in2->mem), dptr<float>(loss->mem),
                                  dptr<float>(lse->mem), n, v, d, ctx->d_failure, ctx->num_sms, ctx->stream);
@@ -124,7 +124,7 @@ int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, grads_t **out
   auto *rec = call.record<grads_t>();
   const fb::VocabPlan plan = fb::vocab_plan(n, v, d, aligned16(in0->mem), aligned16(in1->mem), true, ctx->num_sms);
   void *ws = call.workspace(plan.bytes, "vocab_xent_grad_f16.workspace");
-  call.launch("vocab_xent_grad_f16.segmap_segred", "vjp of vocab_xent_f16", vocab_details(n, v, d), [&] {
+  call.launch("vocab_xent_grad_f16.segmap_segred", "vjp of vocab_xent_f16", [&] { return vocab_details(n, v, d); }, [&] {
     ctx->failure_is_an_option = true;
     return fb::launch_vocab_xent_grad(plan, ws, dptr<uint16_t>(in0->mem), dptr<uint16_t>(in1->mem), dptr<int32_t>(in2->mem), dptr<float>(in3->mem),
                                       dptr<float>(in4->mem), dptr<float>(in5->mem), dptr<uint16_t>(dx->mem), dptr<uint16_t>(dw->mem), n, v, d,
@@ -158,10 +158,10 @@ static int topk_distill(futhark_context *ctx, const char *name, int elem, losses
   Call call(ctx);
   auto *loss = call.array<futhark_f32_1d>({n}, 4, "topk_distill.loss"), *lse = call.array<futhark_f32_1d>({n}, 4, "topk_distill.lse");
   auto *rec = call.record<losses_t>();
-  void *ws = call.workspace(fb::distill_workspace_bytes(n, v, k, elem, false), "topk_distill.workspace");
-  call.launch(name, "map3 (\\s is t -> tau**2 * sum (map2 (\\q i -> q * (log q - s[i]/tau + lse s)) (softmax t) is)) S iss T", distill_details(n, v, k), [&] {
+  void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), n, v, k, elem, false), "topk_distill.workspace");
+  call.launch(name, "map3 (\\s is t -> tau**2 * sum (map2 (\\q i -> q * (log q - s[i]/tau + lse s)) (softmax t) is)) S iss T", [&] { return distill_details(n, v, k); }, [&] {
     return fb::launch_topk_distill(ws, elem, dptr<void>(s->mem), dptr<int32_t>(is->mem), dptr<float>(t->mem), tau, n, v, k, dptr<float>(loss->mem),
-                                   dptr<float>(lse->mem), ctx->stream);
+                                   dptr<float>(lse->mem), ctx->num_sms, ctx->stream);
   });
   if (call.rc != FUTHARK_SUCCESS) return call.rc;
   rec->v0 = loss; rec->v1 = lse;
@@ -179,10 +179,10 @@ static int topk_distill_grad(futhark_context *ctx, const char *name, int elem, M
   if (distill_refusal(ctx, tau, n, v, k)) return 1;
   Call call(ctx);
   auto *ds = call.array<MAT>({n, v}, elem, "topk_distill_grad.ds");
-  void *ws = call.workspace(fb::distill_workspace_bytes(n, v, k, elem, true), "topk_distill_grad.workspace");
-  call.launch(name, "vjp of topk_distill", distill_details(n, v, k), [&] {
+  void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), n, v, k, elem, true), "topk_distill_grad.workspace");
+  call.launch(name, "vjp of topk_distill", [&] { return distill_details(n, v, k); }, [&] {
     return fb::launch_topk_distill_grad(ws, elem, dptr<void>(s->mem), dptr<int32_t>(is->mem), dptr<float>(t->mem), tau, dptr<float>(lse->mem),
-                                        dptr<float>(dl->mem), n, v, k, dptr<void>(ds->mem), ctx->stream);
+                                        dptr<float>(dl->mem), n, v, k, dptr<void>(ds->mem), ctx->num_sms, ctx->stream);
   });
   if (call.rc != FUTHARK_SUCCESS) return call.rc;
   *out0 = ds;
@@ -229,7 +229,7 @@ static int router_balance(futhark_context *ctx, const char *name, int elem, bala
   auto *rec = call.record<balance_t>();
   void *ws = call.workspace(fb::router_workspace_bytes(dptr<void>(r->mem), elem, n, e, ctx->num_sms), "router_balance.workspace");
   call.launch(name, "(norm * sum (map2 (*) counts (reduce (map2 (+)) (map softmax R))), hist (+) 0 e is, norm)",
-              "{" + kv("n", n) + "," + kv("e", e) + "," + kv("k", k) + "}", [&] {
+              [&] { return "{" + kv("n", n) + "," + kv("e", e) + "," + kv("k", k) + "}"; }, [&] {
     return fb::launch_router_balance(ws, elem, dptr<void>(r->mem), dptr<uint8_t>(keep->mem), dptr<int32_t>(is->mem), n, e, k, dptr<float>(loss->mem),
                                      dptr<int32_t>(counts->mem), dptr<float>(norm->mem), ctx->num_sms, ctx->stream);
   });
@@ -249,7 +249,7 @@ static int router_balance_grad(futhark_context *ctx, const char *name, int elem,
   if (e > fb::ROUTER_MAX_E) return refuse(ctx, "Error: router_balance: at most 1024 experts.\n");
   Call call(ctx);
   auto *dr = call.array<MAT>({n, e}, elem, "router_balance_grad.dr");
-  call.launch(name, "vjp of router_balance", "{" + kv("n", n) + "," + kv("e", e) + "}", [&] {
+  call.launch(name, "vjp of router_balance", [&] { return "{" + kv("n", n) + "," + kv("e", e) + "}"; }, [&] {
     return fb::launch_router_balance_grad(elem, dptr<void>(r->mem), dptr<uint8_t>(keep->mem), dptr<int32_t>(counts->mem), dptr<float>(norm->mem),
                                           dptr<float>(dl->mem), n, e, dptr<void>(dr->mem), ctx->num_sms, ctx->stream);
   });

@@ -39,23 +39,21 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return
 
 // ---- distillation -----------------------------------------------------------------------------------------
 // A row is read in aligned 16-byte groups; what of the first and last group lies outside the row is not read.  It is cut
-// into parts of at most 2048 groups, each worked on by `tpr` threads (32 to 256; CTAs have 256 and as many rows as
-// fit) with up to 8 groups per thread, all in flight at once.  Rows of any length and start keep every SM busy this way,
-// a single one included.
-constexpr int D_THREADS = 256;
+// into chunks of at most 32 x 4 groups, one for a warp at a time: a lane has up to 4 groups in registers and the 4 of the
+// warp's next chunk in flight.  Nothing is shared between warps, so rows of any length and start keep every SM busy, a
+// single one included.
+constexpr int D_THREADS = 256, D_WARPS = D_THREADS / 32, D_PER = 4, D_CTAS = 4;
 struct DistillShape {
-  int parts, tpr, per;               // parts of a row, threads of a part, groups of a thread (1, 2, 4 or 8)
+  int chunks, groups;                // chunks of a row, groups of a chunk
 };
-static DistillShape distill_shape(int64_t v, int elem) {
-  const int64_t w = 16 / elem, groups = (v + w - 1) / w + 1;          // one more if the row starts inside a group
-  DistillShape s;
-  s.parts = (int)((groups + D_THREADS * 8 - 1) / (D_THREADS * 8));
-  const int64_t g = (groups + s.parts - 1) / s.parts;
-  s.tpr = 32;
-  while (s.tpr < D_THREADS && s.tpr * 8 < g) s.tpr *= 2;
-  s.per = 1;
-  while (s.per < 8 && s.tpr * s.per < g) s.per *= 2;
-  return s;
+static DistillShape distill_shape(const void *s, int64_t v, int elem) {
+  const int64_t w = 16 / elem, slack = ((uintptr_t)s & 15) == 0 && v % w == 0 ? 0 : 1;      // rows may start inside a group
+  const int64_t groups = (v + w - 1) / w + slack;
+  DistillShape d;
+  d.chunks = (int)((groups + 32 * D_PER - 1) / (32 * D_PER));
+  if (d.chunks < 1) d.chunks = 1;
+  d.groups = (int)((groups + d.chunks - 1) / d.chunks);
+  return d;
 }
 
 template <typename T> struct DistillRow {
@@ -98,6 +96,16 @@ __device__ __forceinline__ int4 pack(const float (&x)[8]) {
   return b;
 }
 
+// Its largest element; NaN does not count here, it is seen in the sum.
+__device__ __forceinline__ float group_max(const int4 &b, const float *) {
+  return fmaxf(fmaxf(__int_as_float(b.x), __int_as_float(b.y)), fmaxf(__int_as_float(b.z), __int_as_float(b.w)));
+}
+__device__ __forceinline__ float group_max(const int4 &b, const __half *) {
+  const __half2 *h = reinterpret_cast<const __half2 *>(&b);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
 // (maximum in units of log 2, exactly what was subtracted; sum): the fold of two
 __device__ __forceinline__ void fold_pair(float &m, float &s, float om, float os) {
   const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
@@ -105,84 +113,109 @@ __device__ __forceinline__ void fold_pair(float &m, float &s, float om, float os
   m = mn;
 }
 
-// One part of one row.
-template <typename T, int PER>
-__global__ void __launch_bounds__(D_THREADS, 4)
-distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, int parts, int tpr, float scale, float2 *__restrict__ part) {
+// A warp's chunk: its row, its groups, and their contents.
+template <typename T> struct DistillChunk {
+  int64_t row;
+  int first;                                         // the lane's first group
+  int4 x[D_PER];
+  __device__ __forceinline__ void load(const T *s, int64_t v, int chunks, int groups, int64_t item, bool small, int lane) {
+    row = small ? (int64_t)((uint32_t)item / (uint32_t)chunks) : item / chunks;
+    const int at = (int)(item - row * chunks) * groups, end = at + groups;
+    const DistillRow<T> r(s, row, v);
+    first = at + lane;
+#pragma unroll
+    for (int i = 0; i < D_PER; i++)
+      if (first + 32 * i < end) x[i] = load_group<T>(r, first + 32 * i);
+  }
+};
+
+// (maximum, sum) of every chunk.
+template <typename T>
+__global__ void __launch_bounds__(D_THREADS, D_CTAS)
+distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, int chunks, int groups, float scale, float2 *__restrict__ part) {
   constexpr int W = 16 / (int)sizeof(T);
-  __shared__ float2 sm[D_THREADS / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = threadIdx.x & (tpr - 1), rpc = D_THREADS / tpr;
-  const int64_t items = n * parts;
-  for (int64_t b0 = (int64_t)blockIdx.x * rpc; b0 < items; b0 += (int64_t)gridDim.x * rpc) {
-    const int64_t b = b0 + threadIdx.x / tpr;
-    float m = -INFINITY, sum = 0.f;
-    if (b < items) {                                 // uniform over the warp
-      const int64_t row = b / parts;
-      const DistillRow<T> r(s, row, v);
-      const int g0 = (int)(b - row * parts) * (tpr * PER) + t;
-      int4 x[PER];
+  const int lane = threadIdx.x & 31;
+  const int64_t items = n * chunks, step = (int64_t)gridDim.x * D_WARPS;
+  const bool small = items < (1ll << 31);
+  int64_t b = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
+  if (b >= items) return;
+  DistillChunk<T> next;
+  next.load(s, v, chunks, groups, b, small, lane);
+  for (; b < items; b += step) {
+    const DistillChunk<T> c = next;
+    if (b + step < items) next.load(s, v, chunks, groups, b + step, small, lane);
+    float m = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < PER; i++) x[i] = load_group<T>(r, g0 + i * tpr);
+    for (int i = 0; i < D_PER; i++)
+      if (lane + 32 * i < groups) m = fmaxf(m, group_max(c.x[i], (const T *)nullptr));
 #pragma unroll
-      for (int i = 0; i < PER; i++) {
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+    m *= scale;
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, sum1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < D_PER; i++)
+      if (lane + 32 * i < groups) {
         float f[W];
-        unpack(x[i], f);
+        unpack(c.x[i], f);
 #pragma unroll
-        for (int j = 0; j < W; j++) m = fmaxf(m, f[j]);
+        for (int j = 0; j < W; j += 2) { sum += ex2_approx(fmaf(f[j], scale, -ref)); sum1 += ex2_approx(fmaf(f[j + 1], scale, -ref)); }
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-      m *= scale;
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int i = 0; i < PER; i++) {
-        float f[W], a = 0.f, c = 0.f;
-        unpack(x[i], f);
-#pragma unroll
-        for (int j = 0; j < W; j += 2) { a += ex2_approx(fmaf(f[j], scale, -ref)); c += ex2_approx(fmaf(f[j + 1], scale, -ref)); }
-        sum += a + c;
-      }
-      sum = warp_sum(sum);
-    }
-    if (tpr > 32) {
-      if (lane == 0) sm[warp] = make_float2(m, sum);
-      __syncthreads();
-      if (t == 0)
-        for (int w = 1; w < tpr / 32; w++) fold_pair(m, sum, sm[warp + w].x, sm[warp + w].y);
-      __syncthreads();                               // sm is used again
-    }
-    if (t == 0 && b < items) part[b] = make_float2(m, sum);
+    sum = warp_sum(sum + sum1);
+    if (lane == 0) part[b] = make_float2(m, sum);
   }
 }
 
 __device__ __forceinline__ bool is_word(int32_t c, float t, int64_t v) { return c >= 0 && c < v && t != -INFINITY; }
 
-// The teacher's softmax of a row over its words, one warp: maximum and sum of exp in the lanes' common registers.
-__device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, int k, int64_t v, float inv_tau, int lane, float &m, float &sum) {
-  m = -INFINITY;
+// The teacher's softmax of a row over its words, by one warp in shared memory: its words (-1: padding), and log q or q.  The lanes
+// read what they wrote themselves until the caller's __syncwarp.  False if the row has no word.
+template <bool LOG>
+__device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, int k, int64_t v, float inv_tau, int lane, int *wi, float *wq) {
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int j = lane; j < k; j += 32) {
+    const int c = is[j];
+    const float x = t[j];
+    const bool in = is_word(c, x, v);
+    wi[j] = in ? c : -1;
+    wq[j] = x * inv_tau;
+    if (in) m = fmaxf(m, x * inv_tau);
+  }
   bool some = false;
-  for (int j = lane; j < k; j += 32)
-    if (is_word(is[j], t[j], v)) { some = true; m = fmaxf(m, t[j] * inv_tau); }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-  sum = 0.f;
+  float sum = 0.f;
   for (int j = lane; j < k; j += 32)
-    if (is_word(is[j], t[j], v)) sum += expf(t[j] * inv_tau - m);
+    if (wi[j] >= 0) {
+      some = true;
+      const float x = wq[j] - m, e = expf(x);
+      wq[j] = LOG ? x : e;
+      sum += e;
+    }
   sum = warp_sum(sum);
+  const float c = LOG ? logf(sum) : 1.f / sum;
+  for (int j = lane; j < k; j += 32)
+    if (wi[j] >= 0) wq[j] = LOG ? wq[j] - c : wq[j] * c;
   return __any_sync(kFull, some);
 }
 
-// One warp per row: fold of the parts, and the loss over the teacher's words (in f64: its terms cancel).
+// One warp per row: fold of the chunks, and the loss over the teacher's words (in f64: its terms cancel).
 template <typename T>
 __global__ void __launch_bounds__(256)
-distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, const float *__restrict__ t, const float2 *__restrict__ part, int parts,
+distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, const float *__restrict__ t, const float2 *__restrict__ part, int chunks,
                     int64_t n, int64_t v, int k, float tau, float *__restrict__ loss, float *__restrict__ lse) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  extern __shared__ float sh[];                      // per warp: words [k], log q [k]
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= n) return;
+  int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * k;
+  float *wq = reinterpret_cast<float *>(wi + k);
+  is += row * k; t += row * k; s += row * v;
+  const bool some = teacher_row<true>(is, t, k, v, 1.f / tau, lane, wi, wq);
   float m = -INFINITY, sum = 0.f;
-  for (int p = lane; p < parts; p += 32) {
-    const float2 q = part[row * parts + p];
+  for (int p = lane; p < chunks; p += 32) {
+    const float2 q = part[row * chunks + p];
     fold_pair(m, sum, q.x, q.y);
   }
 #pragma unroll
@@ -190,21 +223,17 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
     const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, sum, o);
     fold_pair(m, sum, pm, ps);
   }
-  const double l = ((double)m + log2((double)sum)) * L_LN2;
-  is += row * k; t += row * k; s += row * v;
-  const float inv_tau = 1.f / tau;
-  float tm, ts;
-  const bool some = teacher_row(is, t, k, v, inv_tau, lane, tm, ts);
-  const float logsum = logf(ts);
+  const double l = ((double)m + log2((double)sum)) * L_LN2, inv_tau = 1.0 / (double)tau;
   double total = 0;
-  if (some)
+  if (some) {
+#pragma unroll 4
     for (int j = lane; j < k; j += 32) {
-      const int64_t c = is[j];
-      if (!is_word(is[j], t[j], v)) continue;
-      const float lq = t[j] * inv_tau - tm - logsum, q = expf(lq);
+      const int c = wi[j];
+      const float lq = wq[j], q = c >= 0 ? expf(lq) : 0.f;
       // a teacher's weight of exactly 0 adds nothing, whatever the student says
-      if (q != 0.f) total += (double)q * ((double)lq - (double)to_f32<T>(s[c]) / (double)tau + l);
+      if (q != 0.f) total += (double)q * ((double)lq - (double)to_f32<T>(s[c]) * inv_tau + l);
     }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
   if (lane == 0) {
@@ -216,28 +245,21 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
 // One warp per row, before the gradient: per word of the teacher its weight, those of a word that stands there
 // more than once added up (in the order of j) at the first place, -1 at the others.  Whether one does is seen by a hash
 // table of the words; only then are they compared with one another.
+// Per row: dl tau, whether there is a word, and exp(S / tau - lse) = 2^(S scale - hi) f, with hi + log f to more than 32 bits.
 __global__ void __launch_bounds__(256)
 distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__ t, int64_t n, int64_t v, int k, int table, float tau,
-                       const float *__restrict__ dl, int32_t *__restrict__ words, float *__restrict__ weights, float2 *__restrict__ rows) {
+                       const float *__restrict__ dl, const float *__restrict__ lse, int32_t *__restrict__ words, float *__restrict__ weights,
+                       float4 *__restrict__ rows) {
   extern __shared__ float sh[];                      // per warp: words [k], weights [k], places [table]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + warp;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
   if (row >= n) return;
   is += row * k; t += row * k;
   int *wi = reinterpret_cast<int *>(sh) + warp * (2 * k + table);
   float *wq = reinterpret_cast<float *>(wi + k);
   int *place = wi + 2 * k;
-  const float inv_tau = 1.f / tau;
-  float tm, ts;
-  const bool some = teacher_row(is, t, k, v, inv_tau, lane, tm, ts);
-  const float inv = 1.f / ts;
   for (int h = lane; h < table; h += 32) place[h] = -1;
-  for (int j = lane; j < k; j += 32) {
-    const int c = is[j];
-    const bool in = is_word(c, t[j], v);
-    wi[j] = in ? c : -1;
-    wq[j] = in ? expf(t[j] * inv_tau - tm) * inv : 0.f;
-  }
+  const bool some = teacher_row<false>(is, t, k, v, 1.f / tau, lane, wi, wq);
   __syncwarp();
   bool twice = false;
   for (int j = lane; j < k; j += 32) {
@@ -262,45 +284,43 @@ distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__
     words[row * k + j] = first ? c : -1;
     weights[row * k + j] = q;
   }
-  if (lane == 0) rows[row] = make_float2(dl[row] * tau, some ? 1.f : 0.f);
+  if (lane == 0) {
+    const double shift = (double)lse[row] * (1.0 / L_LN2);
+    const float hi = (float)shift;
+    rows[row] = make_float4(dl[row] * tau, some ? 1.f : 0.f, hi, exp2f((float)((double)hi - shift)));
+  }
 }
 
-// One part of one row: the student's softmax, then the words of the teacher that lie in it once more.
-template <typename T, int PER>
-__global__ void __launch_bounds__(D_THREADS, 4)
-distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, int parts, int tpr, float scale, int k, const int32_t *__restrict__ words,
-                    const float *__restrict__ weights, const float2 *__restrict__ rows, const float *__restrict__ lse, T *__restrict__ ds) {
+// Every chunk: the student's softmax, then the words of the teacher that lie in it once more.
+template <typename T>
+__global__ void __launch_bounds__(D_THREADS, D_CTAS)
+distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, int chunks, int groups, float scale, int k, const int32_t *__restrict__ words,
+                    const float *__restrict__ weights, const float4 *__restrict__ rows, T *__restrict__ ds) {
   constexpr int W = 16 / (int)sizeof(T);
-  const int t = threadIdx.x & (tpr - 1), rpc = D_THREADS / tpr;
-  const int64_t items = n * parts;
-  for (int64_t b0 = (int64_t)blockIdx.x * rpc; b0 < items; b0 += (int64_t)gridDim.x * rpc) {
-    const int64_t b = b0 + threadIdx.x / tpr;
-    const bool active = b < items;
-    const int64_t row = active ? b / parts : 0;
-    const DistillRow<T> r(s, row, v);
-    T *out = ds + row * v;
-    const int p0 = (int)(b - row * parts) * (tpr * PER), g0 = p0 + t;
-    // exp(S / tau - lse) = 2^(S scale - hi) 2^-lo, hi + lo the exponent's constant term to more than 32 bits
-    float hi = 0.f, f = 0.f, c = 0.f;
-    bool some = false;
-    if (active) {
-      int4 x[PER];
+  const int lane = threadIdx.x & 31;
+  const int64_t items = n * chunks, step = (int64_t)gridDim.x * D_WARPS;
+  const bool small = items < (1ll << 31);
+  int64_t b = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
+  if (b >= items) return;
+  DistillChunk<T> next;
+  next.load(s, v, chunks, groups, b, small, lane);
+  for (; b < items; b += step) {
+    const DistillChunk<T> c = next;
+    const float4 rc = rows[c.row];
+    int word = lane < k ? words[c.row * k + lane] : -1;
+    if (b + step < items) next.load(s, v, chunks, groups, b + step, small, lane);
+    const DistillRow<T> r(s, c.row, v);
+    T *out = ds + c.row * v;
+    const bool some = rc.y != 0.f;
+    const float fc = rc.w * rc.x;
 #pragma unroll
-      for (int i = 0; i < PER; i++) x[i] = load_group<T>(r, g0 + i * tpr);
-      const float2 rc = rows[row];
-      const double shift = (double)lse[row] / L_LN2;
-      c = rc.x;
-      some = rc.y != 0.f;
-      hi = (float)shift;
-      f = exp2f((float)((double)hi - shift));
-      const float fc = f * c;
-#pragma unroll
-      for (int i = 0; i < PER; i++) {
-        const int g = g0 + i * tpr, col = r.first(g);
+    for (int i = 0; i < D_PER; i++)
+      if (lane + 32 * i < groups) {
+        const int g = c.first + 32 * i, col = r.first(g);
         float y[W];
-        unpack(x[i], y);
+        unpack(c.x[i], y);
 #pragma unroll
-        for (int j = 0; j < W; j++) y[j] = some ? ex2_approx(fmaf(y[j], scale, -hi)) * fc : 0.f;
+        for (int j = 0; j < W; j++) y[j] = some ? ex2_approx(fmaf(y[j], scale, -rc.z)) * fc : 0.f;
         if (r.whole(g) && ((uintptr_t)(out + col) & 15) == 0) {
           st_stream_v4(out + col, pack(y));
         } else {
@@ -308,15 +328,14 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, int parts, in
           for (int j = 0; j < W; j++) if (col + j >= 0 && col + j < r.v) out[col + j] = from_f32<T>(y[j]);
         }
       }
-    }
-    __syncthreads();                                 // the words' places have been written
-    if (active && some) {
-      const int c0 = r.first(p0), c1 = r.first(p0 + tpr * PER);
-      for (int j = t; j < k; j += tpr) {
-        const int w = words[row * k + j];
-        if (w >= 0 && w >= c0 && w < c1) {
-          const float p = ex2_approx(fmaf(to_f32<T>(r.base[w]), scale, -hi)) * f;
-          out[w] = from_f32<T>((p - weights[row * k + j]) * c);
+    __syncwarp();                                    // the words' places have been written
+    if (some) {
+      const int c0 = r.first(c.first - lane), c1 = r.first(c.first - lane + groups);
+      for (int j = lane; j < k; j += 32) {
+        if (j >= 32) word = words[c.row * k + j];
+        if (word >= 0 && word >= c0 && word < c1) {
+          const float p = ex2_approx(fmaf(to_f32<T>(r.base[word]), scale, -rc.z)) * rc.w;
+          out[word] = from_f32<T>((p - weights[c.row * k + j]) * rc.x);
         }
       }
     }
@@ -324,88 +343,103 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, int parts, in
 }
 
 static inline size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
-static inline unsigned part_grid(int64_t items, int per_cta) {
-  const int64_t g = (items + per_cta - 1) / per_cta;
-  return (unsigned)(g < (1ll << 30) ? g : (1ll << 30));
+static unsigned chunk_grid(int64_t items, int num_sms) {
+  const int64_t g = (items + D_WARPS - 1) / D_WARPS, most = (int64_t)num_sms * D_CTAS;
+  return (unsigned)(g < most ? g : most);
 }
+// Warps of a CTA that has a row per warp: few rows are spread over more SMs.
+static int row_warps(int64_t n, int num_sms) { return n >= (int64_t)num_sms * 8 ? 8 : 2; }
 
-size_t distill_workspace_bytes(int64_t n, int64_t v, int64_t k, int elem, bool grad) {
-  if (!grad) return up256((size_t)n * distill_shape(v, elem).parts * sizeof(float2));
-  return up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float2));
+size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad) {
+  if (!grad) return up256((size_t)n * distill_shape(s, v, elem).chunks * sizeof(float2));
+  return up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float4));
 }
-
-#define FB_DISTILL_PER(PER_, CALL)                    \
-  switch (PER_) {                                     \
-    case 1: { constexpr int PER = 1; CALL; break; }   \
-    case 2: { constexpr int PER = 2; CALL; break; }   \
-    case 4: { constexpr int PER = 4; CALL; break; }   \
-    default: { constexpr int PER = 8; CALL; break; }  \
-  }
 
 template <typename T>
 static cudaError_t distill(void *workspace, const T *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k, float *loss,
-                           float *lse, cudaStream_t stream) {
+                           float *lse, int num_sms, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
-  const DistillShape sh = distill_shape(v, sizeof(T));
+  const DistillShape d = distill_shape(s, v, sizeof(T));
   float2 *part = reinterpret_cast<float2 *>(workspace);
   const float scale = (float)(1.0 / (L_LN2 * (double)tau));
-  const unsigned grid = part_grid(n * sh.parts, D_THREADS / sh.tpr);
-  FB_DISTILL_PER(sh.per, (distill_part_kernel<T, PER><<<grid, D_THREADS, 0, stream>>>(s, n, v, sh.parts, sh.tpr, scale, part)))
+  distill_part_kernel<T><<<chunk_grid(n * d.chunks, num_sms), D_THREADS, 0, stream>>>(s, n, v, d.chunks, d.groups, scale, part);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  distill_loss_kernel<T><<<(unsigned)((n + 7) / 8), 256, 0, stream>>>(s, is, t, part, sh.parts, n, v, (int)k, tau, loss, lse);
+  const int rw = row_warps(n, num_sms);
+  err = cudaFuncSetAttribute(distill_loss_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * 2 * DISTILL_MAX_K * 4);
+  if (err != cudaSuccess) return err;
+  distill_loss_kernel<T><<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream>>>(s, is, t, part, d.chunks, n, v, (int)k, tau, loss, lse);
   return cudaGetLastError();
 }
 
 template <typename T>
 static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, const float *t, float tau, const float *lse, const float *dl, int64_t n,
-                                int64_t v, int64_t k, T *ds, cudaStream_t stream) {
+                                int64_t v, int64_t k, T *ds, int num_sms, cudaStream_t stream) {
   if (n <= 0 || v <= 0) return cudaSuccess;
-  const DistillShape sh = distill_shape(v, sizeof(T));
+  const DistillShape d = distill_shape(s, v, sizeof(T));
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   int32_t *words = reinterpret_cast<int32_t *>(ws);
   float *weights = reinterpret_cast<float *>(ws + up256((size_t)(n * k) * 4));
-  float2 *rows = reinterpret_cast<float2 *>(ws + 2 * up256((size_t)(n * k) * 4));
+  float4 *rows = reinterpret_cast<float4 *>(ws + 2 * up256((size_t)(n * k) * 4));
   const float scale = (float)(1.0 / (L_LN2 * (double)tau));
   int table = 32;
   while (table < 2 * k) table *= 2;
+  const int rw = row_warps(n, num_sms);
   cudaError_t err = cudaFuncSetAttribute(distill_teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (2 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4);
   if (err != cudaSuccess) return err;
-  distill_teacher_kernel<<<(unsigned)((n + 7) / 8), 256, (size_t)8 * (2 * k + table) * 4, stream>>>(is, t, n, v, (int)k, table, tau, dl, words, weights, rows);
+  distill_teacher_kernel<<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (2 * k + table) * 4, stream>>>(is, t, n, v, (int)k, table, tau, dl, lse, words,
+                                                                                                            weights, rows);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  const unsigned grid = part_grid(n * sh.parts, D_THREADS / sh.tpr);
-  FB_DISTILL_PER(sh.per, (distill_grad_kernel<T, PER><<<grid, D_THREADS, 0, stream>>>(s, n, v, sh.parts, sh.tpr, scale, (int)k, words, weights, rows, lse, ds)))
+  distill_grad_kernel<T><<<chunk_grid(n * d.chunks, num_sms), D_THREADS, 0, stream>>>(s, n, v, d.chunks, d.groups, scale, (int)k, words, weights, rows, ds);
   return cudaGetLastError();
 }
 
 cudaError_t launch_topk_distill(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
-                                float *loss, float *lse, cudaStream_t stream) {
-  if (elem == 2) return distill<__half>(workspace, reinterpret_cast<const __half *>(s), is, t, tau, n, v, k, loss, lse, stream);
-  return distill<float>(workspace, reinterpret_cast<const float *>(s), is, t, tau, n, v, k, loss, lse, stream);
+                                float *loss, float *lse, int num_sms, cudaStream_t stream) {
+  if (elem == 2) return distill<__half>(workspace, reinterpret_cast<const __half *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
+  return distill<float>(workspace, reinterpret_cast<const float *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
 }
 cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,
-                                     const float *dl, int64_t n, int64_t v, int64_t k, void *ds, cudaStream_t stream) {
+                                     const float *dl, int64_t n, int64_t v, int64_t k, void *ds, int num_sms, cudaStream_t stream) {
   if (elem == 2)
-    return distill_grad<__half>(workspace, reinterpret_cast<const __half *>(s), is, t, tau, lse, dl, n, v, k, reinterpret_cast<__half *>(ds), stream);
-  return distill_grad<float>(workspace, reinterpret_cast<const float *>(s), is, t, tau, lse, dl, n, v, k, reinterpret_cast<float *>(ds), stream);
+    return distill_grad<__half>(workspace, reinterpret_cast<const __half *>(s), is, t, tau, lse, dl, n, v, k, reinterpret_cast<__half *>(ds), num_sms, stream);
+  return distill_grad<float>(workspace, reinterpret_cast<const float *>(s), is, t, tau, lse, dl, n, v, k, reinterpret_cast<float *>(ds), num_sms, stream);
 }
 
 // ---- router balance ----------------------------------------------------------------------------------------
 // A row belongs to G lanes of a warp (a power of two, at most 32), each of which has J groups of W consecutive columns
-// (W = 4 where rows are made of whole aligned groups, 1 otherwise).  The lanes keep their columns' sums in
-// registers over all rows of the CTA, so that nothing but the row maxima and sums crosses lanes, and the column sums
-// add in an order that does not depend on timing.  The next row is loaded before this one is worked on: a warp's
-// rows are short chains of dependent steps, and two rows in flight per warp are what hides them.
-constexpr int R_THREADS = 256;
+// (W = 4 where rows are made of whole aligned groups, 1 otherwise).  Sixteen columns per lane where there are as many: a warp
+// per row of 100 columns spent 250 instructions on it, most of them on crossing lanes, and was bound by them.  The lanes
+// keep their columns' sums in registers over all rows of the CTA, so that nothing but the row maxima and sums crosses
+// lanes, and the column sums add in an order that does not depend on timing.  The next row is loaded before this one is worked on.
+constexpr int R_THREADS = 512, R_WARPS = R_THREADS / 32, R_CTAS = 2;
 
 struct RouterShape { int w, g, j; };
 static RouterShape router_shape(const void *r, int64_t e, int elem) {
   RouterShape s = {e % 4 == 0 && ((uintptr_t)r & (4 * elem - 1)) == 0 ? 4 : 1, 1, 1};
-  while (s.g < 32 && s.g * s.w < e) s.g *= 2;
+  while (s.g < 32 && s.g * 16 < e) s.g *= 2;
   while ((int64_t)s.g * s.w * s.j < e) s.j *= 2;
   return s;
 }
+// lanes of a row known at compile time unroll their exchanges
+template <typename F>
+__device__ __forceinline__ float over_lanes(float x, int g, F f) {
+  if (g == 32) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = f(x, __shfl_xor_sync(kFull, x, o));
+  } else if (g == 16) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) x = f(x, __shfl_xor_sync(kFull, x, o));
+  } else if (g > 1) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+      if (o < g) x = f(x, __shfl_xor_sync(kFull, x, o));
+  }
+  return x;
+}
+__device__ __forceinline__ float lanes_max(float x, int g) { return over_lanes(x, g, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float lanes_sum(float x, int g) { return over_lanes(x, g, [](float a, float b) { return a + b; }); }
 
 template <typename T, int W> struct RouterGroup;
 template <> struct RouterGroup<float, 4> { using type = float4; };
@@ -432,12 +466,12 @@ template <typename T, int W, int J> struct RouterRow {
         m = fmaxf(m, p[j * W + i]);
       }
     }
-    for (int o = g / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+    m = lanes_max(m, g);
     const float ref = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < J * W; j++) { p[j] = ex2_approx((p[j] - ref) * L_LOG2E); sum += p[j]; }
-    for (int o = g / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    sum = lanes_sum(sum, g);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int j = 0; j < J * W; j++) p[j] *= inv;
@@ -446,36 +480,50 @@ template <typename T, int W, int J> struct RouterRow {
 
 // Partial results of a CTA: column sums of p [e], counts [e] and the number of rows kept.
 template <typename T, int W, int J>
-__global__ void __launch_bounds__(R_THREADS)
+__global__ void __launch_bounds__(R_THREADS, J * W <= 16 ? R_CTAS : 1)
 router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ is, int64_t n, int e, int k, int g,
                    float *__restrict__ psum, int *__restrict__ pcount, int *__restrict__ ticket) {
-  extern __shared__ float rsh[];                     // [8][g * J * W] column sums of the warps, then [e + 1] counts
+  extern __shared__ float rsh[];                     // [R_WARPS][g * J * W] column sums of the warps, then [e + 1] counts
   const int span = g * J * W;
-  int *cnt = reinterpret_cast<int *>(rsh + (R_THREADS / 32) * span);
+  int *cnt = reinterpret_cast<int *>(rsh + R_WARPS * span);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (g - 1), sub = lane / g, per_warp = 32 / g;
+  const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;
+  int64_t i = ((int64_t)blockIdx.x * R_WARPS + warp) * per_warp + sub;
+  RouterRow<T, W, J> next;
+  bool use = i < n && keep[i] != 0;
+  int sent = -1;                                     // the lane's first expert of the row
+  if (use) {
+    next.load(r + i * e, e, g, l);
+    if (l < k) sent = is[i * k + l];
+  }
   for (int c = threadIdx.x; c <= e; c += R_THREADS) cnt[c] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;              // of the next kernel
   __syncthreads();
   float acc[J * W];
 #pragma unroll
   for (int j = 0; j < J * W; j++) acc[j] = 0.f;
-  const int64_t step = (int64_t)gridDim.x * (R_THREADS / 32) * per_warp;
-  int64_t i = ((int64_t)blockIdx.x * (R_THREADS / 32) + warp) * per_warp + sub;
   int kept = 0;
-  RouterRow<T, W, J> next;
-  bool use = i < n && keep[i] != 0;
-  if (use) next.load(r + i * e, e, g, l);
   for (; i - sub < n; i += step) {                   // uniform over the warp: every lane takes part in the shuffles
     const RouterRow<T, W, J> row = next;
     const bool mine = use;
+    const int to = sent;
     use = i + step < n && keep[i + step] != 0;
-    if (use) next.load(r + (i + step) * e, e, g, l);
+    sent = -1;
+    if (use) {
+      next.load(r + (i + step) * e, e, g, l);
+      if (l < k) sent = is[(i + step) * k + l];
+    }
     float p[J * W];
     row.softmax(e, g, l, p);
     if (mine) {
 #pragma unroll
       for (int j = 0; j < J * W; j++) acc[j] += p[j];
       if (l == 0) kept++;
+      if (to >= 0 && to < e) atomicAdd(&cnt[to], 1);
+      for (int j = l + g; j < k; j += g) {
+        const int c = is[i * k + j];
+        if (c >= 0 && c < e) atomicAdd(&cnt[c], 1);
+      }
     }
   }
 #pragma unroll
@@ -488,14 +536,11 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
       for (int x = 0; x < W; x++) rsh[warp * span + (lane + g * j) * W + x] = acc[j * W + x];
   kept = warp_sum(kept);
   if (lane == 0 && kept) atomicAdd(&cnt[e], kept);
-  for (int64_t o = (int64_t)blockIdx.x * R_THREADS + threadIdx.x; o < n * k; o += (int64_t)gridDim.x * R_THREADS) {
-    const int c = is[o];
-    if (c >= 0 && c < e && keep[(uint32_t)o / (uint32_t)k] != 0) atomicAdd(&cnt[c], 1);      // n k is below 2^31
-  }
   __syncthreads();
   for (int c = threadIdx.x; c < e; c += R_THREADS) {
     float t = 0.f;
-    for (int w = 0; w < R_THREADS / 32; w++) t += rsh[w * span + c];
+#pragma unroll
+    for (int w = 0; w < R_WARPS; w++) t += rsh[w * span + c];
     psum[(int64_t)blockIdx.x * e + c] = t;
   }
   for (int c = threadIdx.x; c <= e; c += R_THREADS) pcount[(int64_t)blockIdx.x * (e + 1) + c] = cnt[c];
@@ -522,9 +567,11 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
   sp[warp][lane] = p;
   sc[warp][lane] = q;
   __syncthreads();
-  if (warp == 0 && c <= e) {
-    for (int w = 1; w < 32; w++) { p += sp[w][lane]; q += sc[w][lane]; }
-    if (c < e) { sums[c] = p; counts[c] = q; } else *kept = q;
+  p = warp_sum(sp[lane][warp]);                      // the warp's column of the 32
+  q = warp_sum(sc[lane][warp]);
+  const int mine = blockIdx.x * 32 + warp;
+  if (lane == 0 && mine <= e) {
+    if (mine < e) { sums[mine] = p; counts[mine] = q; } else *kept = q;
     __threadfence();
   }
   __syncthreads();
@@ -552,12 +599,12 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
 // Counts are taken around their mean (in integers): where they are nearly equal the gradient is what is left of a
 // difference, and sum_f p_if = 1 makes the shift cancel.
 template <typename T, int W, int J>
-__global__ void __launch_bounds__(R_THREADS)
+__global__ void __launch_bounds__(R_THREADS, J * W <= 16 ? R_CTAS : 1)
 router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ counts, const float *__restrict__ norm,
                    const float *__restrict__ dl, int64_t n, int e, int g, T *__restrict__ dr) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (g - 1), sub = lane / g, per_warp = 32 / g;
-  const int64_t step = (int64_t)gridDim.x * (R_THREADS / 32) * per_warp;
-  int64_t i = ((int64_t)blockIdx.x * (R_THREADS / 32) + warp) * per_warp + sub;
+  const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;
+  int64_t i = ((int64_t)blockIdx.x * R_WARPS + warp) * per_warp + sub;
   RouterRow<T, W, J> next;
   bool use = i < n && keep[i] != 0;
   if (use) next.load(r + i * e, e, g, l);
@@ -582,7 +629,7 @@ router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < J * W; j++) dot = fmaf(p[j], cf[j], dot);
-    for (int o = g / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
+    dot = lanes_sum(dot, g);
     if (i < n) {
 #pragma unroll
       for (int j = 0; j < J; j++)
@@ -598,8 +645,8 @@ router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
 }
 
 static int64_t router_grid(int64_t n, const RouterShape &s, int num_sms) {
-  const int64_t rows = (int64_t)(R_THREADS / 32) * (32 / s.g);
-  const int64_t want = (n + rows - 1) / rows, most = (int64_t)num_sms * 4;
+  const int64_t rows = (int64_t)R_WARPS * (32 / s.g);
+  const int64_t want = (n + rows - 1) / rows, most = (int64_t)num_sms * (s.w * s.j <= 16 ? R_CTAS : 1);
   return want < 1 ? 1 : want < most ? want : most;
 }
 
@@ -627,8 +674,10 @@ static cudaError_t router(void *workspace, const T *r, const uint8_t *keep, cons
   double *sums = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(pcount) + up256((size_t)grid * (e + 1) * 4));
   int *kept = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(sums) + up256((size_t)e * 8));
   int *ticket = kept + 1;
-  const size_t smem = (size_t)(R_THREADS / 32) * s.g * s.j * s.w * 4 + (size_t)(e + 1) * 4;
-#define FB_PART(W, J) router_part_kernel<T, W, J><<<grid, R_THREADS, smem, stream>>>(r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket)
+  const size_t smem = (size_t)R_WARPS * s.g * s.j * s.w * 4 + (size_t)(e + 1) * 4;
+#define FB_PART(W, J)                                                                                                      \
+  if (cudaFuncSetAttribute(router_part_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 << 10) == cudaSuccess) \
+    router_part_kernel<T, W, J><<<grid, R_THREADS, smem, stream>>>(r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket)
   FB_ROUTER_SHAPE(s, FB_PART)
 #undef FB_PART
   const cudaError_t err = cudaGetLastError();
