@@ -287,38 +287,42 @@ class _TypeFns:
         self.shape, self.raw = getattr(L, "futhark_shape_" + tname), getattr(L, "futhark_values_raw_" + tname)
 
 
-_type_fns = {}
+class _TypeTable(dict):
+    def __missing__(self, tname):
+        self[tname] = f = _TypeFns(load(), tname)
+        return f
 
 
-def _fns(tname):
-    f = _type_fns.get(tname)
-    if f is None:
-        f = _type_fns[tname] = _TypeFns(load(), tname)
-    return f
+_type_fns = _TypeTable()
 
 
 class Array:
     """A device array owned by a context (struct futhark_<t>_<n>d *)."""
 
+    __slots__ = ("ctx", "tname", "ptr", "_interface", "_keepalive", "__weakref__")
+
     def __init__(self, ctx, tname, ptr):
-        self.ctx, self.tname, self.ptr = ctx, tname, ptr
+        self.ctx = ctx
+        self.tname = tname
+        self.ptr = ptr
         self._interface = None
 
     @property
     def shape(self):
-        f = _fns(self.tname)
+        f = _type_fns[self.tname]
         return tuple(f.shape(self.ctx.ptr, self.ptr)[:f.rank])
 
     @property
     def raw(self):
         """Device address (futhark_values_raw_*)."""
-        return _fns(self.tname).raw(self.ctx.ptr, self.ptr)
+        return _type_fns[self.tname].raw(self.ctx.ptr, self.ptr)
 
     @property
     def __cuda_array_interface__(self):
         d = self._interface                  # neither the shape nor the address of an array ever changes
         if d is None or self.ptr is None:
-            d = self._interface = {"shape": self.shape, "typestr": _fns(self.tname).typestr, "data": (self.raw, False), "version": 2}
+            f, c, p = _type_fns[self.tname], self.ctx.ptr, self.ptr
+            d = self._interface = {"shape": tuple(f.shape(c, p)[:f.rank]), "typestr": f.typestr, "data": (f.raw(c, p), False), "version": 2}
         return d
 
     def values_into(self, out):
@@ -342,7 +346,7 @@ class Array:
 
     def free(self):
         if self.ptr:
-            _fns(self.tname).free(self.ctx.ptr, self.ptr)
+            _type_fns[self.tname].free(self.ctx.ptr, self.ptr)
             self.ptr = None
 
 
@@ -482,7 +486,7 @@ class Context:
         return arr
 
     def new_raw(self, tname, devptr, *shape):
-        p = _fns(tname).new_raw(self.ptr, int(devptr), *shape)
+        p = _type_fns[tname].new_raw(self.ptr, devptr, *shape)
         if not p:
             raise FutharkError(1, self.get_error() or "futhark_new_raw_%s failed" % tname)
         return Array(self, tname, p)
@@ -668,17 +672,20 @@ class Context:
 
     def _fields(self, rec, types, obj):
         """The fields of an opaque record as arrays; the record is freed."""
-        parts = []
-        for project, t in zip(_record_fns(rec, len(types))[1:], types):
-            out = ctypes.c_void_p()
-            self._check(project(self.ptr, ctypes.byref(out), obj))
+        fns, ptr, out, parts = _record_fns(rec, len(types)), self.ptr, ctypes.c_void_p(), []
+        ref = ctypes.byref(out)
+        for i, t in enumerate(types):
+            if fns[i + 1](ptr, ref, obj):
+                self._check(1)
             parts.append(Array(self, t, out.value))
-        self._check(_record_fns(rec, len(types))[0](self.ptr, obj))
+        fns[0](ptr, obj)
         return tuple(parts)
 
     def _entry_rec(self, name, rec, types, *args):
         obj = ctypes.c_void_p()
-        self._check(getattr(self.lib, "futhark_entry_" + name)(self.ptr, ctypes.byref(obj), *args))
+        rc = getattr(self.lib, "futhark_entry_" + name)(self.ptr, ctypes.byref(obj), *args)
+        if rc:
+            self._check(rc)
         return self._fields(rec, types, obj)
 
     def entry_vocab_xent_f16(self, X, W, ts):

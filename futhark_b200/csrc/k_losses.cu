@@ -413,9 +413,13 @@ cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, c
 // per row of 100 columns spent 250 instructions on it, most of them on crossing lanes, and was bound by them.  The lanes
 // keep their columns' sums in registers over all rows of the CTA, so that nothing but the row maxima and sums crosses
 // lanes, and the column sums add in an order that does not depend on timing.  The next row is loaded before this one is worked on.
-constexpr int R_THREADS = 512, R_WARPS = R_THREADS / 32, R_CTAS = 2;
-
-struct RouterShape { int w, g, j; };
+//
+// One CTA per SM, so that there are few partial results to add up.
+struct RouterShape {
+  int w, g, j;
+  int cols() const { return w * j; }                 // columns of a lane
+  int warps() const { return cols() <= 16 ? 32 : 16; }
+};
 static RouterShape router_shape(const void *r, int64_t e, int elem) {
   RouterShape s = {e % 4 == 0 && ((uintptr_t)r & (4 * elem - 1)) == 0 ? 4 : 1, 1, 1};
   while (s.g < 32 && s.g * 16 < e) s.g *= 2;
@@ -448,41 +452,53 @@ template <> struct RouterGroup<__half, 4> { using type = uint2; };
 template <> struct RouterGroup<__half, 1> { using type = __half; };
 
 template <typename T, int W, int J> struct RouterRow {
+  static constexpr int COLS = W * J, WARPS = COLS <= 16 ? 32 : 16, THREADS = 32 * WARPS;
   typename RouterGroup<T, W>::type x[J];
+  // columns behind the last one are -inf and stay so: nothing is loaded over them
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      T *t = reinterpret_cast<T *>(&x[j]);
+#pragma unroll
+      for (int i = 0; i < W; i++) t[i] = from_f32<T>(-INFINITY);
+    }
+  }
   __device__ __forceinline__ void load(const T *row, int e, int g, int l) {
 #pragma unroll
     for (int j = 0; j < J; j++)
       if ((l + g * j) * W < e) x[j] = *reinterpret_cast<const typename RouterGroup<T, W>::type *>(row + (l + g * j) * W);
   }
-  // p of the lane's columns; 0 in a row that is all -inf
-  __device__ __forceinline__ void softmax(int e, int g, int l, float (&p)[J * W]) const {
-    float m = -INFINITY;
+  __device__ __forceinline__ void unpack(float (&p)[COLS]) const {
 #pragma unroll
     for (int j = 0; j < J; j++) {
       const T *t = reinterpret_cast<const T *>(&x[j]);
 #pragma unroll
-      for (int i = 0; i < W; i++) {
-        p[j * W + i] = (l + g * j) * W < e ? to_f32<T>(t[i]) : -INFINITY;
-        m = fmaxf(m, p[j * W + i]);
-      }
+      for (int i = 0; i < W; i++) p[j * W + i] = to_f32<T>(t[i]);
     }
-    m = lanes_max(m, g);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < J * W; j++) { p[j] = ex2_approx((p[j] - ref) * L_LOG2E); sum += p[j]; }
-    sum = lanes_sum(sum, g);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int j = 0; j < J * W; j++) p[j] *= inv;
   }
 };
+// Logits to exp(logit - maximum), in place; returns the factor that makes them add up to 1 (0 in a row that is all -inf).
+// The maximum's product with log2 e is rounded, which the factor takes back.
+template <int COLS>
+__device__ __forceinline__ float router_exp(float (&p)[COLS], int g) {
+  float m = p[0];
+#pragma unroll
+  for (int j = 1; j < COLS; j++) m = fmaxf(m, p[j]);
+  m = lanes_max(m, g);
+  const float ref = m == -INFINITY ? 0.f : m * L_LOG2E;
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < COLS; j++) { p[j] = ex2_approx(fmaf(p[j], L_LOG2E, -ref)); sum += p[j]; }
+  sum = lanes_sum(sum, g);
+  return sum == 0.f ? 0.f : 1.f / sum;
+}
 
 // Partial results of a CTA: column sums of p [e], counts [e] and the number of rows kept.
 template <typename T, int W, int J>
-__global__ void __launch_bounds__(R_THREADS, J * W <= 16 ? R_CTAS : 1)
+__global__ void __launch_bounds__(RouterRow<T, W, J>::THREADS)
 router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ is, int64_t n, int e, int k, int g,
                    float *__restrict__ psum, int *__restrict__ pcount, int *__restrict__ ticket) {
+  constexpr int R_WARPS = RouterRow<T, W, J>::WARPS, R_THREADS = RouterRow<T, W, J>::THREADS;
   extern __shared__ float rsh[];                     // [R_WARPS][g * J * W] column sums of the warps, then [e + 1] counts
   const int span = g * J * W;
   int *cnt = reinterpret_cast<int *>(rsh + R_WARPS * span);
@@ -490,10 +506,12 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
   const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;
   int64_t i = ((int64_t)blockIdx.x * R_WARPS + warp) * per_warp + sub;
   RouterRow<T, W, J> next;
-  bool use = i < n && keep[i] != 0;
+  uint8_t use = 0;                                   // whether the row counts: loaded beside it, not before it
   int sent = -1;                                     // the lane's first expert of the row
-  if (use) {
+  next.clear();
+  if (i < n) {
     next.load(r + i * e, e, g, l);
+    use = keep[i];
     if (l < k) sent = is[i * k + l];
   }
   for (int c = threadIdx.x; c <= e; c += R_THREADS) cnt[c] = 0;
@@ -504,20 +522,20 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
   for (int j = 0; j < J * W; j++) acc[j] = 0.f;
   int kept = 0;
   for (; i - sub < n; i += step) {                   // uniform over the warp: every lane takes part in the shuffles
-    const RouterRow<T, W, J> row = next;
-    const bool mine = use;
+    float p[J * W];
+    next.unpack(p);
+    const bool mine = use != 0;
     const int to = sent;
-    use = i + step < n && keep[i + step] != 0;
-    sent = -1;
-    if (use) {
+    use = 0;
+    if (i + step < n) {
       next.load(r + (i + step) * e, e, g, l);
+      use = keep[i + step];
       if (l < k) sent = is[(i + step) * k + l];
     }
-    float p[J * W];
-    row.softmax(e, g, l, p);
+    const float inv = router_exp(p, g);
     if (mine) {
 #pragma unroll
-      for (int j = 0; j < J * W; j++) acc[j] += p[j];
+      for (int j = 0; j < J * W; j++) acc[j] = fmaf(p[j], inv, acc[j]);
       if (l == 0) kept++;
       if (to >= 0 && to < e) atomicAdd(&cnt[to], 1);
       for (int j = l + g; j < k; j += g) {
@@ -556,13 +574,14 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   double p = 0;
   int q = 0;
-  if (c < e) {
-#pragma unroll 8
-    for (int b = warp; b < parts; b += 32) p += (double)psum[(int64_t)b * e + c];
-  }
   if (c <= e) {
-#pragma unroll 8
-    for (int b = warp; b < parts; b += 32) q += pcount[(int64_t)b * (e + 1) + c];
+    const int cp = min(c, e - 1);                    // the number of rows kept has no sum of p
+#pragma unroll 5
+    for (int b = warp; b < parts; b += 32) {
+      const float x = e > 0 ? psum[(int64_t)b * e + cp] : 0.f;
+      q += pcount[(int64_t)b * (e + 1) + c];
+      p += (double)x;
+    }
   }
   sp[warp][lane] = p;
   sc[warp][lane] = q;
@@ -599,15 +618,17 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
 // Counts are taken around their mean (in integers): where they are nearly equal the gradient is what is left of a
 // difference, and sum_f p_if = 1 makes the shift cancel.
 template <typename T, int W, int J>
-__global__ void __launch_bounds__(R_THREADS, J * W <= 16 ? R_CTAS : 1)
+__global__ void __launch_bounds__(RouterRow<T, W, J>::THREADS)
 router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ counts, const float *__restrict__ norm,
                    const float *__restrict__ dl, int64_t n, int e, int g, T *__restrict__ dr) {
+  constexpr int R_WARPS = RouterRow<T, W, J>::WARPS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (g - 1), sub = lane / g, per_warp = 32 / g;
   const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;
   int64_t i = ((int64_t)blockIdx.x * R_WARPS + warp) * per_warp + sub;
   RouterRow<T, W, J> next;
-  bool use = i < n && keep[i] != 0;
-  if (use) next.load(r + i * e, e, g, l);
+  uint8_t use = 0;
+  next.clear();
+  if (i < n) { next.load(r + i * e, e, g, l); use = keep[i]; }
   long long all = 0;
   for (int x = lane; x < e; x += 32) all += counts[x];
 #pragma unroll
@@ -620,16 +641,16 @@ router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
     for (int x = 0; x < W; x++) cf[j * W + x] = (l + g * j) * W < e ? (float)(counts[(l + g * j) * W + x] - mean) : 0.f;
   const float f = (float)((double)*norm * (double)*dl);
   for (; i - sub < n; i += step) {
-    const RouterRow<T, W, J> row = next;
-    const bool mine = use;
-    use = i + step < n && keep[i + step] != 0;
-    if (use) next.load(r + (i + step) * e, e, g, l);
     float p[J * W];
-    row.softmax(e, g, l, p);
+    next.unpack(p);
+    const bool mine = use != 0;
+    if (i + step < n) { next.load(r + (i + step) * e, e, g, l); use = keep[i + step]; }
+    const float inv = router_exp(p, g);
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < J * W; j++) dot = fmaf(p[j], cf[j], dot);
-    dot = lanes_sum(dot, g);
+    dot = lanes_sum(dot, g) * inv;
+    const float s = inv * f;
     if (i < n) {
 #pragma unroll
       for (int j = 0; j < J; j++)
@@ -637,7 +658,7 @@ router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
           typename RouterGroup<T, W>::type y;
           T *t = reinterpret_cast<T *>(&y);
 #pragma unroll
-          for (int x = 0; x < W; x++) t[x] = from_f32<T>(mine ? p[j * W + x] * (cf[j * W + x] - dot) * f : 0.f);
+          for (int x = 0; x < W; x++) t[x] = from_f32<T>(mine ? p[j * W + x] * s * (cf[j * W + x] - dot) : 0.f);
           *reinterpret_cast<typename RouterGroup<T, W>::type *>(dr + i * e + (l + g * j) * W) = y;
         }
     }
@@ -645,8 +666,8 @@ router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
 }
 
 static int64_t router_grid(int64_t n, const RouterShape &s, int num_sms) {
-  const int64_t rows = (int64_t)R_WARPS * (32 / s.g);
-  const int64_t want = (n + rows - 1) / rows, most = (int64_t)num_sms * (s.w * s.j <= 16 ? R_CTAS : 1);
+  const int64_t rows = (int64_t)s.warps() * (32 / s.g);
+  const int64_t want = (n + rows - 1) / rows, most = num_sms;
   return want < 1 ? 1 : want < most ? want : most;
 }
 
@@ -674,10 +695,10 @@ static cudaError_t router(void *workspace, const T *r, const uint8_t *keep, cons
   double *sums = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(pcount) + up256((size_t)grid * (e + 1) * 4));
   int *kept = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(sums) + up256((size_t)e * 8));
   int *ticket = kept + 1;
-  const size_t smem = (size_t)R_WARPS * s.g * s.j * s.w * 4 + (size_t)(e + 1) * 4;
+  const size_t smem = (size_t)s.warps() * s.g * s.cols() * 4 + (size_t)(e + 1) * 4;
 #define FB_PART(W, J)                                                                                                      \
-  if (cudaFuncSetAttribute(router_part_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 << 10) == cudaSuccess) \
-    router_part_kernel<T, W, J><<<grid, R_THREADS, smem, stream>>>(r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket)
+  if (cudaFuncSetAttribute(router_part_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10) == cudaSuccess) \
+    router_part_kernel<T, W, J><<<grid, 32 * s.warps(), smem, stream>>>(r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket)
   FB_ROUTER_SHAPE(s, FB_PART)
 #undef FB_PART
   const cudaError_t err = cudaGetLastError();
@@ -692,7 +713,7 @@ static cudaError_t router_grad(const T *r, const uint8_t *keep, const int32_t *c
   if (n <= 0 || e <= 0) return cudaSuccess;
   const RouterShape s = router_shape(r, e, sizeof(T));               // the result starts on a 256-byte boundary
   const int grid = (int)router_grid(n, s, num_sms);
-#define FB_GRAD(W, J) router_grad_kernel<T, W, J><<<grid, R_THREADS, 0, stream>>>(r, keep, counts, norm, dl, n, (int)e, s.g, dr)
+#define FB_GRAD(W, J) router_grad_kernel<T, W, J><<<grid, 32 * s.warps(), 0, stream>>>(r, keep, counts, norm, dl, n, (int)e, s.g, dr)
   FB_ROUTER_SHAPE(s, FB_GRAD)
 #undef FB_GRAD
   return cudaGetLastError();
