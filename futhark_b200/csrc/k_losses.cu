@@ -39,20 +39,26 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return
 
 // ---- distillation -----------------------------------------------------------------------------------------
 // A row is read in aligned 16-byte groups; what of the first and last group lies outside the row is not read.  It is cut
-// into chunks of at most 32 x 4 groups, one for a warp at a time: a lane has up to 4 groups in registers and the 4 of the
-// warp's next chunk in flight.  Nothing is shared between warps, so rows of any length and start keep every SM busy, a
-// single one included.
+// into chunks of 32 x 4 groups, and those into runs that a warp works off one after the other: a lane has up to 4 groups
+// in registers and the 4 of its next chunk (of whatever row) in flight.  Nothing is shared between warps, so rows of any
+// length and start keep every SM busy, a single one included; lanes meet only at the end of a run, since with one chunk per
+// meeting the steps around a chunk's elements took as many instructions as the elements (10.7 per element in all, issue-bound).
 constexpr int D_THREADS = 256, D_WARPS = D_THREADS / 32, D_PER = 4, D_CTAS = 4;
 struct DistillShape {
   int chunks, groups;                // chunks of a row, groups of a chunk
+  int run, runs;                     // chunks of a run, runs of a row
 };
-static DistillShape distill_shape(const void *s, int64_t v, int elem) {
+static DistillShape distill_shape(const void *s, int64_t n, int64_t v, int elem, int num_sms, int longest) {
   const int64_t w = 16 / elem, slack = ((uintptr_t)s & 15) == 0 && v % w == 0 ? 0 : 1;      // rows may start inside a group
-  const int64_t groups = (v + w - 1) / w + slack;
+  const int64_t groups = (v + w - 1) / w + slack, most = 32 * D_PER;
   DistillShape d;
-  d.chunks = (int)((groups + 32 * D_PER - 1) / (32 * D_PER));
-  if (d.chunks < 1) d.chunks = 1;
-  d.groups = (int)((groups + d.chunks - 1) / d.chunks);
+  d.chunks = groups <= most ? 1 : (int)((groups + most - 1) / most);
+  d.groups = (int)(groups < most ? groups : most);
+  // as long as there are four runs for every warp that is resident
+  const int64_t warps = (int64_t)num_sms * D_CTAS * D_WARPS;
+  d.run = 1;
+  while (d.run < longest && d.run < d.chunks && n * ((d.chunks + 2 * d.run - 1) / (2 * d.run)) >= 4 * warps) d.run *= 2;
+  d.runs = (d.chunks + d.run - 1) / d.run;
   return d;
 }
 
@@ -113,56 +119,107 @@ __device__ __forceinline__ void fold_pair(float &m, float &s, float om, float os
   m = mn;
 }
 
-// A warp's chunk: its row, its groups, and their contents.
-template <typename T> struct DistillChunk {
-  int64_t row;
-  int first;                                         // the lane's first group
-  int4 x[D_PER];
-  __device__ __forceinline__ void load(const T *s, int64_t v, int chunks, int groups, int64_t item, bool small, int lane) {
-    row = small ? (int64_t)((uint32_t)item / (uint32_t)chunks) : item / chunks;
-    const int at = (int)(item - row * chunks) * groups, end = at + groups;
-    const DistillRow<T> r(s, row, v);
-    first = at + lane;
-#pragma unroll
-    for (int i = 0; i < D_PER; i++)
-      if (first + 32 * i < end) x[i] = load_group<T>(r, first + 32 * i);
+// Where a warp is: run `item` of all rows, at one of its chunks.
+struct DistillAt {
+  int64_t item, row;
+  int chunk, last;                                   // the chunk, and the one behind the run's last
+  __device__ __forceinline__ void start(int64_t items, const DistillShape &d, bool small) {
+    if (item >= items) return;
+    row = small ? (int64_t)((uint32_t)item / (uint32_t)d.runs) : item / d.runs;
+    chunk = (int)(item - row * d.runs) * d.run;
+    last = min(chunk + d.run, d.chunks);
+  }
+  __device__ __forceinline__ void next(int64_t items, int64_t step, const DistillShape &d, bool small) {
+    if (++chunk == last) { item += step; start(items, d, small); }
   }
 };
+// The lane's groups of a chunk.  Away from the ends of the row every group is whole.
+template <typename T>
+__device__ __forceinline__ void load_chunk(const DistillRow<T> &r, int chunk, int groups, int lane, int4 (&x)[D_PER]) {
+  const int g0 = chunk * groups;
+  if (r.first(g0) >= 0 && groups == 32 * D_PER && r.first(g0 + groups) <= r.v) {
+    const T *p = r.base + r.first(g0 + lane);
+#pragma unroll
+    for (int i = 0; i < D_PER; i++) x[i] = ld_stream_v4(p + i * 32 * DistillRow<T>::W);
+  } else {
+#pragma unroll
+    for (int i = 0; i < D_PER; i++)
+      if (lane + 32 * i < groups) x[i] = load_group<T>(r, g0 + lane + 32 * i);
+  }
+}
 
-// (maximum, sum) of every chunk.
+// two f32 products and sums in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t x, y, z;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(y), "l"(z));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+  return a;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+  return a;
+}
+
+// (maximum, sum) of every run.
 template <typename T>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
-distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, int chunks, int groups, float scale, float2 *__restrict__ part) {
+distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, float2 *__restrict__ part) {
   constexpr int W = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
-  const int64_t items = n * chunks, step = (int64_t)gridDim.x * D_WARPS;
+  const int64_t items = n * d.runs, step = (int64_t)gridDim.x * D_WARPS;
   const bool small = items < (1ll << 31);
-  int64_t b = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
-  if (b >= items) return;
-  DistillChunk<T> next;
-  next.load(s, v, chunks, groups, b, small, lane);
-  for (; b < items; b += step) {
-    const DistillChunk<T> c = next;
-    if (b + step < items) next.load(s, v, chunks, groups, b + step, small, lane);
-    float m = -INFINITY;
+  DistillAt at;
+  at.item = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
+  at.start(items, d, small);
+  int4 next[D_PER];
+  if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
+  float m = -INFINITY, sum = 0.f;
+  while (at.item < items) {
+    int4 x[D_PER];
+#pragma unroll
+    for (int i = 0; i < D_PER; i++) x[i] = next[i];
+    const DistillAt here = at;
+    at.next(items, step, d, small);
+    if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
+    float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
-      if (lane + 32 * i < groups) m = fmaxf(m, group_max(c.x[i], (const T *)nullptr));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-    m *= scale;
-    const float ref = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, sum1 = 0.f;
+      if (lane + 32 * i < d.groups) mx = fmaxf(mx, group_max(x[i], (const T *)nullptr));
+    mx = fmaxf(m, mx * scale);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float2 sc = make_float2(scale, scale), nr = make_float2(-ref, -ref);
+    float2 a = make_float2(sum * ex2_approx(m - ref), 0.f), b = make_float2(0.f, 0.f);
+    m = mx;
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
-      if (lane + 32 * i < groups) {
+      if (lane + 32 * i < d.groups) {
         float f[W];
-        unpack(c.x[i], f);
+        unpack(x[i], f);
 #pragma unroll
-        for (int j = 0; j < W; j += 2) { sum += ex2_approx(fmaf(f[j], scale, -ref)); sum1 += ex2_approx(fmaf(f[j + 1], scale, -ref)); }
+        for (int j = 0; j < W; j += 4) {
+          const float2 e = fma2(make_float2(f[j], f[j + 1]), sc, nr), g = fma2(make_float2(f[j + 2], f[j + 3]), sc, nr);
+          a = add2(a, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
+          b = add2(b, make_float2(ex2_approx(g.x), ex2_approx(g.y)));
+        }
       }
-    sum = warp_sum(sum + sum1);
-    if (lane == 0) part[b] = make_float2(m, sum);
+    sum = (a.x + a.y) + (b.x + b.y);
+    if (here.chunk + 1 == here.last) {               // the lanes meet
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float om = __shfl_xor_sync(kFull, m, o), os = __shfl_xor_sync(kFull, sum, o);
+        fold_pair(m, sum, om, os);
+      }
+      if (lane == 0) part[here.item] = make_float2(m, sum);
+      m = -INFINITY;
+      sum = 0.f;
+    }
   }
 }
 
@@ -200,10 +257,10 @@ __device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, i
   return __any_sync(kFull, some);
 }
 
-// One warp per row: fold of the chunks, and the loss over the teacher's words (in f64: its terms cancel).
+// One warp per row: fold of the runs, and the loss over the teacher's words (in f64: its terms cancel).
 template <typename T>
 __global__ void __launch_bounds__(256)
-distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, const float *__restrict__ t, const float2 *__restrict__ part, int chunks,
+distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, const float *__restrict__ t, const float2 *__restrict__ part, int runs,
                     int64_t n, int64_t v, int k, float tau, float *__restrict__ loss, float *__restrict__ lse) {
   extern __shared__ float sh[];                      // per warp: words [k], log q [k]
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -214,8 +271,8 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
   is += row * k; t += row * k; s += row * v;
   const bool some = teacher_row<true>(is, t, k, v, 1.f / tau, lane, wi, wq);
   float m = -INFINITY, sum = 0.f;
-  for (int p = lane; p < chunks; p += 32) {
-    const float2 q = part[row * chunks + p];
+  for (int p = lane; p < runs; p += 32) {
+    const float2 q = part[row * runs + p];
     fold_pair(m, sum, q.x, q.y);
   }
 #pragma unroll
@@ -242,47 +299,59 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
   }
 }
 
-// One warp per row, before the gradient: per word of the teacher its weight, those of a word that stands there
-// more than once added up (in the order of j) at the first place, -1 at the others.  Whether one does is seen by a hash
-// table of the words; only then are they compared with one another.
+// One warp per row, before the gradient: per word of the teacher its weight; of places with the same word one has the sum of
+// their weights and the others -1.  Which places those are is found without comparing all with all: in a round every
+// place that has not met its word yet writes itself into the word's slot of a hash table, and who then finds a place with its
+// own word there has met it (all places of a word do so in the same round, and in every slot someone does).
 // Per row: dl tau, whether there is a word, and exp(S / tau - lse) = 2^(S scale - hi) f, with hi + log f to more than 32 bits.
 __global__ void __launch_bounds__(256)
 distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__ t, int64_t n, int64_t v, int k, int table, float tau,
                        const float *__restrict__ dl, const float *__restrict__ lse, int32_t *__restrict__ words, float *__restrict__ weights,
                        float4 *__restrict__ rows) {
-  extern __shared__ float sh[];                      // per warp: words [k], weights [k], places [table]
+  extern __shared__ float sh[];                      // per warp: words [k], weights [k], the place met [k], slots [table]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
   if (row >= n) return;
   is += row * k; t += row * k;
-  int *wi = reinterpret_cast<int *>(sh) + warp * (2 * k + table);
+  int *wi = reinterpret_cast<int *>(sh) + warp * (3 * k + table);
   float *wq = reinterpret_cast<float *>(wi + k);
-  int *place = wi + 2 * k;
-  for (int h = lane; h < table; h += 32) place[h] = -1;
+  int *met = wi + 2 * k, *slot = wi + 3 * k;
   const bool some = teacher_row<false>(is, t, k, v, 1.f / tau, lane, wi, wq);
-  __syncwarp();
-  bool twice = false;
-  for (int j = lane; j < k; j += 32) {
-    const int c = wi[j];
-    if (c < 0) continue;
-    for (int h = (int)(((uint32_t)c * 2654435761u) >> 16) & (table - 1);; h = (h + 1) & (table - 1)) {   // at least half of the table is free
-      const int at = atomicCAS(place + h, -1, c);
-      if (at == -1) break;
-      if (at == c) { twice = true; break; }
+  for (int j = lane; j < k; j += 32) met[j] = wi[j] < 0 ? j : -1;
+  uint32_t mul = 2654435761u;
+  for (bool left = true; left; mul = mul * 1664525u + 1013904224u | 1u) {
+    for (int j = lane; j < k; j += 32)
+      if (met[j] < 0) slot[(((uint32_t)wi[j] * mul) >> 16) & (table - 1)] = j;
+    __syncwarp();
+    left = false;
+    for (int j = lane; j < k; j += 32)
+      if (met[j] < 0) {
+        const int w = slot[(((uint32_t)wi[j] * mul) >> 16) & (table - 1)];
+        if (wi[w] == wi[j]) met[j] = w; else left = true;
+      }
+    left = __any_sync(kFull, left);
+    __syncwarp();
+  }
+  for (int j0 = 0; j0 < k; j0 += 32) {
+    const int j = j0 + lane;
+    for (;;) {                                       // one word that stands more than once, the whole warp
+      const unsigned more = __ballot_sync(kFull, j < k && met[j] != j);
+      if (more == 0) break;
+      const int w = __shfl_sync(kFull, j < k ? met[j] : 0, __ffs(more) - 1);
+      float q = 0.f;
+      for (int o = lane; o < k; o += 32)
+        if (met[o] == w && wi[o] >= 0) {
+          q += wq[o];
+          if (o != w) { wi[o] = -1; met[o] = o; }
+        }
+      q = warp_sum(q);
+      if (lane == 0) wq[w] = q;
+      __syncwarp();
     }
   }
-  twice = __any_sync(kFull, twice);
   for (int j = lane; j < k; j += 32) {
-    const int c = wi[j];
-    float q = wq[j];
-    bool first = c >= 0;
-    if (twice && c >= 0) {
-      q = 0.f;
-      for (int o = 0; o < k; o++)
-        if (wi[o] == c) { if (o < j) first = false; q += wq[o]; }
-    }
-    words[row * k + j] = first ? c : -1;
-    weights[row * k + j] = q;
+    words[row * k + j] = wi[j];
+    weights[row * k + j] = wq[j];
   }
   if (lane == 0) {
     const double shift = (double)lse[row] * (1.0 / L_LN2);
@@ -291,51 +360,76 @@ distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__
   }
 }
 
-// Every chunk: the student's softmax, then the words of the teacher that lie in it once more.
+// The gradient is read and written by neighbouring warps at neighbouring places, which HBM likes better than long runs: with runs
+// of 1, 2, 4 and 16 chunks 131.5, 138, 142 and 147 us (f32, 2049 x 50001) and 377, 352, 362 and 388 us (binary16, 4096 x 131072,
+// where a chunk is twice the elements per instruction around them).
+template <typename T> constexpr int D_GRAD_RUN = sizeof(T) == 2 ? 2 : 1;
+
+// Every chunk: the student's softmax; after a run the words of the teacher that lie in it once more.
 template <typename T>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
-distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, int chunks, int groups, float scale, int k, const int32_t *__restrict__ words,
+distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, int k, const int32_t *__restrict__ words,
                     const float *__restrict__ weights, const float4 *__restrict__ rows, T *__restrict__ ds) {
   constexpr int W = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
-  const int64_t items = n * chunks, step = (int64_t)gridDim.x * D_WARPS;
+  const int64_t items = n * d.runs, step = (int64_t)gridDim.x * D_WARPS;
   const bool small = items < (1ll << 31);
-  int64_t b = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
-  if (b >= items) return;
-  DistillChunk<T> next;
-  next.load(s, v, chunks, groups, b, small, lane);
-  for (; b < items; b += step) {
-    const DistillChunk<T> c = next;
-    const float4 rc = rows[c.row];
-    int word = lane < k ? words[c.row * k + lane] : -1;
-    if (b + step < items) next.load(s, v, chunks, groups, b + step, small, lane);
-    const DistillRow<T> r(s, c.row, v);
-    T *out = ds + c.row * v;
-    const bool some = rc.y != 0.f;
+  DistillAt at;
+  at.item = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
+  at.start(items, d, small);
+  int4 next[D_PER];
+  if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
+  float4 rc = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool fresh = true;
+  while (at.item < items) {
+    int4 x[D_PER];
+#pragma unroll
+    for (int i = 0; i < D_PER; i++) x[i] = next[i];
+    const DistillAt here = at;
+    if (fresh) rc = rows[here.row];
+    at.next(items, step, d, small);
+    if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
+    const DistillRow<T> r(s, here.row, v);
+    T *out = ds + here.row * v;
+    const bool some = rc.y != 0.f;                   // uniform over the warp
+    const int g0 = here.chunk * d.groups;
+    const float2 sc = make_float2(scale, scale), nr = make_float2(-rc.z, -rc.z);
     const float fc = rc.w * rc.x;
+    const bool inner = r.first(g0) >= 0 && d.groups == 32 * D_PER && r.first(g0 + d.groups) <= r.v && ((uintptr_t)(out + r.first(g0)) & 15) == 0;
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
-      if (lane + 32 * i < groups) {
-        const int g = c.first + 32 * i, col = r.first(g);
+      if (lane + 32 * i < d.groups) {
         float y[W];
-        unpack(c.x[i], y);
+        unpack(x[i], y);
 #pragma unroll
-        for (int j = 0; j < W; j++) y[j] = some ? ex2_approx(fmaf(y[j], scale, -rc.z)) * fc : 0.f;
-        if (r.whole(g) && ((uintptr_t)(out + col) & 15) == 0) {
+        for (int j = 0; j < W; j += 2) {
+          const float2 e = fma2(make_float2(y[j], y[j + 1]), sc, nr);
+          y[j] = ex2_approx(e.x) * fc;
+          y[j + 1] = ex2_approx(e.y) * fc;
+        }
+        if (!some) {
+#pragma unroll
+          for (int j = 0; j < W; j++) y[j] = 0.f;
+        }
+        const int col = r.first(g0 + lane + 32 * i);
+        if (inner) {
           st_stream_v4(out + col, pack(y));
         } else {
 #pragma unroll
           for (int j = 0; j < W; j++) if (col + j >= 0 && col + j < r.v) out[col + j] = from_f32<T>(y[j]);
         }
       }
-    __syncwarp();                                    // the words' places have been written
-    if (some) {
-      const int c0 = r.first(c.first - lane), c1 = r.first(c.first - lane + groups);
-      for (int j = lane; j < k; j += 32) {
-        if (j >= 32) word = words[c.row * k + j];
-        if (word >= 0 && word >= c0 && word < c1) {
-          const float p = ex2_approx(fmaf(to_f32<T>(r.base[word]), scale, -rc.z)) * rc.w;
-          out[word] = from_f32<T>((p - weights[c.row * k + j]) * rc.x);
+    fresh = here.chunk + 1 == here.last;
+    if (fresh) {
+      __syncwarp();                                  // the words' places have been written
+      if (some) {
+        const int c0 = r.first((here.last - 1) / d.run * d.run * d.groups), c1 = r.first(here.last * d.groups);
+        for (int j = lane; j < k; j += 32) {
+          const int word = words[here.row * k + j];
+          if (word >= 0 && word >= c0 && word < c1) {
+            const float p = ex2_approx(fmaf(to_f32<T>(r.base[word]), scale, -rc.z)) * rc.w;
+            out[word] = from_f32<T>((p - weights[here.row * k + j]) * rc.x);
+          }
         }
       }
     }
@@ -350,8 +444,8 @@ static unsigned chunk_grid(int64_t items, int num_sms) {
 // Warps of a CTA that has a row per warp: few rows are spread over more SMs.
 static int row_warps(int64_t n, int num_sms) { return n >= (int64_t)num_sms * 8 ? 8 : 2; }
 
-size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad) {
-  if (!grad) return up256((size_t)n * distill_shape(s, v, elem).chunks * sizeof(float2));
+size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms) {
+  if (!grad) return up256((size_t)n * distill_shape(s, n, v, elem, num_sms, 16).runs * sizeof(float2));
   return up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float4));
 }
 
@@ -359,16 +453,16 @@ template <typename T>
 static cudaError_t distill(void *workspace, const T *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k, float *loss,
                            float *lse, int num_sms, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
-  const DistillShape d = distill_shape(s, v, sizeof(T));
+  const DistillShape d = distill_shape(s, n, v, sizeof(T), num_sms, 16);
   float2 *part = reinterpret_cast<float2 *>(workspace);
   const float scale = (float)(1.0 / (L_LN2 * (double)tau));
-  distill_part_kernel<T><<<chunk_grid(n * d.chunks, num_sms), D_THREADS, 0, stream>>>(s, n, v, d.chunks, d.groups, scale, part);
+  distill_part_kernel<T><<<chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream>>>(s, n, v, d, scale, part);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   const int rw = row_warps(n, num_sms);
   err = cudaFuncSetAttribute(distill_loss_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * 2 * DISTILL_MAX_K * 4);
   if (err != cudaSuccess) return err;
-  distill_loss_kernel<T><<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream>>>(s, is, t, part, d.chunks, n, v, (int)k, tau, loss, lse);
+  distill_loss_kernel<T><<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream>>>(s, is, t, part, d.runs, n, v, (int)k, tau, loss, lse);
   return cudaGetLastError();
 }
 
@@ -376,7 +470,7 @@ template <typename T>
 static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, const float *t, float tau, const float *lse, const float *dl, int64_t n,
                                 int64_t v, int64_t k, T *ds, int num_sms, cudaStream_t stream) {
   if (n <= 0 || v <= 0) return cudaSuccess;
-  const DistillShape d = distill_shape(s, v, sizeof(T));
+  const DistillShape d = distill_shape(s, n, v, sizeof(T), num_sms, D_GRAD_RUN<T>);
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   int32_t *words = reinterpret_cast<int32_t *>(ws);
   float *weights = reinterpret_cast<float *>(ws + up256((size_t)(n * k) * 4));
@@ -385,13 +479,13 @@ static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, 
   int table = 32;
   while (table < 2 * k) table *= 2;
   const int rw = row_warps(n, num_sms);
-  cudaError_t err = cudaFuncSetAttribute(distill_teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (2 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4);
+  cudaError_t err = cudaFuncSetAttribute(distill_teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (3 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4);
   if (err != cudaSuccess) return err;
-  distill_teacher_kernel<<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (2 * k + table) * 4, stream>>>(is, t, n, v, (int)k, table, tau, dl, lse, words,
+  distill_teacher_kernel<<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (3 * k + table) * 4, stream>>>(is, t, n, v, (int)k, table, tau, dl, lse, words,
                                                                                                             weights, rows);
   err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  distill_grad_kernel<T><<<chunk_grid(n * d.chunks, num_sms), D_THREADS, 0, stream>>>(s, n, v, d.chunks, d.groups, scale, (int)k, words, weights, rows, ds);
+  distill_grad_kernel<T><<<chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream>>>(s, n, v, d, scale, (int)k, words, weights, rows, ds);
   return cudaGetLastError();
 }
 
