@@ -265,6 +265,21 @@ def load():
     return L
 
 
+_mirror_module = None
+
+
+def _native():
+    """The native callables (futhark_b200/mirror.c), built beside the library."""
+    global _mirror_module
+    if _mirror_module is None:
+        try:
+            from . import _mirror
+        except ImportError as e:
+            raise ImportError("the native part of the mirror is missing: run `python -m futhark_b200.build` (%s)" % e)
+        _mirror_module = _mirror
+    return _mirror_module
+
+
 _libc = ctypes.CDLL(None)
 _libc.free.argtypes = [ctypes.c_void_p]
 
@@ -277,14 +292,20 @@ def _take_string(ptr):
     return s
 
 
+def _addr(name):
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+
+
 class _TypeFns:
     """The functions of one array type, looked up once."""
 
     def __init__(self, L, tname):
-        self.dtype, self.rank, _ = ARRAY_TYPES[tname]
-        self.typestr = np.dtype(self.dtype).str
-        self.new_raw, self.free = getattr(L, "futhark_new_raw_" + tname), getattr(L, "futhark_free_" + tname)
+        dtype, self.rank, _ = ARRAY_TYPES[tname]
         self.shape, self.raw = getattr(L, "futhark_shape_" + tname), getattr(L, "futhark_values_raw_" + tname)
+        Fn = _native().Fn
+        self.new_raw = Fn("new_raw", _addr("futhark_new_raw_" + tname), self.rank)
+        self.free = Fn("free", _addr("futhark_free_" + tname))
+        self.interface = Fn("interface", _addr("futhark_shape_" + tname), _addr("futhark_values_raw_" + tname), self.rank, np.dtype(dtype).str)
 
 
 class _TypeTable(dict):
@@ -321,8 +342,7 @@ class Array:
     def __cuda_array_interface__(self):
         d = self._interface                  # neither the shape nor the address of an array ever changes
         if d is None or self.ptr is None:
-            f, c, p = _type_fns[self.tname], self.ctx.ptr, self.ptr
-            d = self._interface = {"shape": tuple(f.shape(c, p)[:f.rank]), "typestr": f.typestr, "data": (f.raw(c, p), False), "version": 2}
+            d = self._interface = _type_fns[self.tname].interface(self.ctx.ptr, self.ptr)
         return d
 
     def values_into(self, out):
@@ -350,16 +370,21 @@ class Array:
             self.ptr = None
 
 
-_record_fn_cache = {}
+class _EntryTable(dict):
+    """Entry points as native callables, by (name, whether a float comes first, the opaque record returned or "", its fields)."""
+
+    def __missing__(self, key):
+        name, float_first, rec, fields = key
+        Fn, entry = _native().Fn, _addr("futhark_entry_" + name)
+        if rec:
+            f = Fn("record", entry, float_first, _addr("futhark_free_" + rec), *[_addr("futhark_project_%s_%d" % (rec, i)) for i in range(fields)])
+        else:
+            f = Fn("array", entry, float_first)
+        self[key] = f
+        return f
 
 
-def _record_fns(rec, k):
-    """(free, project_0, ...) of an opaque record type, looked up once."""
-    f = _record_fn_cache.get(rec)
-    if f is None:
-        L = load()
-        f = _record_fn_cache[rec] = tuple([getattr(L, "futhark_free_" + rec)] + [getattr(L, "futhark_project_%s_%d" % (rec, i)) for i in range(k)])
-    return f
+_entries = _EntryTable()
 
 
 class Pair:
@@ -670,23 +695,18 @@ class Context:
         self._check(getattr(self.lib, "futhark_free_" + SEXTUPLE)(self.ptr, obj))
         return parts
 
-    def _fields(self, rec, types, obj):
-        """The fields of an opaque record as arrays; the record is freed."""
-        fns, ptr, out, parts = _record_fns(rec, len(types)), self.ptr, ctypes.c_void_p(), []
-        ref = ctypes.byref(out)
-        for i, t in enumerate(types):
-            if fns[i + 1](ptr, ref, obj):
-                self._check(1)
-            parts.append(Array(self, t, out.value))
-        fns[0](ptr, obj)
-        return tuple(parts)
+    def _entry_rec(self, name, rec, types, *args, float_first=False):
+        """The fields of the record that an entry point returns, as arrays; the record is freed."""
+        r = _entries[name, float_first, rec, len(types)](self.ptr, *args)
+        if r.__class__ is int:
+            self._check(-r)
+        return tuple([Array(self, t, p) for t, p in zip(types, r)])
 
-    def _entry_rec(self, name, rec, types, *args):
-        obj = ctypes.c_void_p()
-        rc = getattr(self.lib, "futhark_entry_" + name)(self.ptr, ctypes.byref(obj), *args)
-        if rc:
-            self._check(rc)
-        return self._fields(rec, types, obj)
+    def _entry_one(self, name, out_t, *args, float_first=False):
+        p = _entries[name, float_first, "", 0](self.ptr, *args)
+        if p < 0:
+            self._check(-p)
+        return Array(self, out_t, p)
 
     def entry_vocab_xent_f16(self, X, W, ts):
         """Cross entropy of hidden states X against the vocabulary W: (losses, lses)."""
@@ -698,17 +718,17 @@ class Context:
 
     def entry_topk_distill(self, t, tau, S, iss, T):
         """Distillation of a student's logits S (t: "f32" or "f16") from a teacher's top logits T at words iss: (losses, lses)."""
-        return self._entry_rec("topk_distill_" + t, LOSSES, ("f32_1d", "f32_1d"), tau, S.ptr, iss.ptr, T.ptr)
+        return self._entry_rec("topk_distill_" + t, LOSSES, ("f32_1d", "f32_1d"), tau, S.ptr, iss.ptr, T.ptr, float_first=True)
 
     def entry_topk_distill_grad(self, t, tau, S, iss, T, lses, dls):
-        return self._entry_arr("topk_distill_grad_" + t, t + "_2d", tau, S.ptr, iss.ptr, T.ptr, lses.ptr, dls.ptr)
+        return self._entry_one("topk_distill_grad_" + t, t + "_2d", tau, S.ptr, iss.ptr, T.ptr, lses.ptr, dls.ptr, float_first=True)
 
     def entry_router_balance(self, t, R, keep, iss):
         """The balance loss of a router's logits R (t: "f32" or "f16"): (loss, counts, norm)."""
         return self._entry_rec("router_balance_" + t, BALANCE, ("f32_1d", "i32_1d", "f32_1d"), R.ptr, keep.ptr, iss.ptr)
 
     def entry_router_balance_grad(self, t, R, keep, counts, norm, dl):
-        return self._entry_arr("router_balance_grad_" + t, t + "_2d", R.ptr, keep.ptr, counts.ptr, norm.ptr, dl.ptr)
+        return self._entry_one("router_balance_grad_" + t, t + "_2d", R.ptr, keep.ptr, counts.ptr, norm.ptr, dl.ptr)
 
     def entry_mss_i32(self, xs):
         out = ctypes.c_int32()

@@ -9,6 +9,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -63,6 +64,7 @@ def build(force=False, verbose=False, ptxas_v=False):
     if ptxas_v and log:
         print(log)
     build_cli(force, verbose)
+    build_mirror(force, verbose)
     return LIB
 
 
@@ -86,6 +88,21 @@ def build_cli(force=False, verbose=False):
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
     return CLI_BIN
+
+
+MIRROR_SRC = os.path.join(HERE, "mirror.c")
+MIRROR = os.path.join(HERE, "_mirror" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_mirror(force=False, verbose=False):
+    """The native callables of the Python mirror (CPython extension, plain C)."""
+    if not force and os.path.exists(MIRROR) and os.path.getmtime(MIRROR) >= os.path.getmtime(MIRROR_SRC):
+        return MIRROR
+    cmd = [os.environ.get("CC", "gcc"), "-std=gnu11", "-O2", "-Wall", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"], MIRROR_SRC, "-o", MIRROR]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return MIRROR
 
 
 if __name__ == "__main__":

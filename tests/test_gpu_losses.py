@@ -414,6 +414,10 @@ def test_records_share_their_fields(ctx, rec, types):
     assert getattr(ctx.lib, "futhark_new_" + rec)(ctx.ptr, ctypes.byref(obj), *[a.ptr for a in arrs]) == 0
     for a in arrs:
         a.free()
-    for got, want in zip(ctx._fields(rec, types, obj), data):
+    for i, (t, want) in enumerate(zip(types, data)):
+        p = ctypes.c_void_p()
+        assert getattr(ctx.lib, "futhark_project_%s_%d" % (rec, i))(ctx.ptr, ctypes.byref(p), obj) == 0
+        got = fb.Array(ctx, t, p.value)
         assert np.array_equal(got.values(), want)
         got.free()
+    assert getattr(ctx.lib, "futhark_free_" + rec)(ctx.ptr, obj) == 0
