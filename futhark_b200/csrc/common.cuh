@@ -185,4 +185,38 @@ __device__ __forceinline__ uint32_t status_state(uint64_t w, uint32_t epoch) {
 __device__ __forceinline__ uint32_t status_flag(uint64_t w) { return ((uint32_t)(w >> 32) >> 2) & 1u; }
 __device__ __forceinline__ uint32_t status_value(uint64_t w) { return (uint32_t)w; }
 
+// ---- chains of kernels ------------------------------------------------------------------------
+// A kernel launched by launch_after may start while the one before it in the stream is still running: it sets itself up
+// and then waits, before its first access to global memory, until that one has ended and its writes are
+// visible.  Every kernel of a chain waits, so the end of one is the end of all before it.
+__device__ __forceinline__ void chain_wait() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... KARGS, typename... ARGS>
+static inline cudaError_t launch_after(void (*kernel)(KARGS...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, ARGS... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KARGS>(args)...);
+}
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the driver once per kernel and device.
+static inline cudaError_t allow_smem(const void *kernel, int bytes, unsigned long long &devices) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (__atomic_load_n(&devices, __ATOMIC_ACQUIRE) & bit) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) __atomic_fetch_or(&devices, bit, __ATOMIC_RELEASE);
+  return err;
+}
+
 }  // namespace fb

@@ -178,6 +178,7 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
   DistillAt at;
   at.item = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
   at.start(items, d, small);
+  chain_wait();
   int4 next[D_PER];
   if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
   float m = -INFINITY, sum = 0.f;
@@ -265,6 +266,7 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
   extern __shared__ float sh[];                      // per warp: words [k], log q [k]
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  chain_wait();
   if (row >= n) return;
   int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * k;
   float *wq = reinterpret_cast<float *>(wi + k);
@@ -311,6 +313,7 @@ distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__
   extern __shared__ float sh[];                      // per warp: words [k], weights [k], the place met [k], slots [table]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
+  chain_wait();
   if (row >= n) return;
   is += row * k; t += row * k;
   int *wi = reinterpret_cast<int *>(sh) + warp * (3 * k + table);
@@ -377,6 +380,7 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
   DistillAt at;
   at.item = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
   at.start(items, d, small);
+  chain_wait();
   int4 next[D_PER];
   if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
   float4 rc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -456,14 +460,14 @@ static cudaError_t distill(void *workspace, const T *s, const int32_t *is, const
   const DistillShape d = distill_shape(s, n, v, sizeof(T), num_sms, 16);
   float2 *part = reinterpret_cast<float2 *>(workspace);
   const float scale = (float)(1.0 / (L_LN2 * (double)tau));
-  distill_part_kernel<T><<<chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream>>>(s, n, v, d, scale, part);
-  cudaError_t err = cudaGetLastError();
+  cudaError_t err = launch_after(distill_part_kernel<T>, chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream, s, n, v, d, scale, part);
   if (err != cudaSuccess) return err;
   const int rw = row_warps(n, num_sms);
-  err = cudaFuncSetAttribute(distill_loss_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * 2 * DISTILL_MAX_K * 4);
+  static unsigned long long allowed = 0;
+  err = allow_smem(reinterpret_cast<const void *>(distill_loss_kernel<T>), 8 * 2 * DISTILL_MAX_K * 4, allowed);
   if (err != cudaSuccess) return err;
-  distill_loss_kernel<T><<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream>>>(s, is, t, part, d.runs, n, v, (int)k, tau, loss, lse);
-  return cudaGetLastError();
+  return launch_after(distill_loss_kernel<T>, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream, s, is, t, part, d.runs, n, v, (int)k, tau,
+                      loss, lse);
 }
 
 template <typename T>
@@ -479,14 +483,13 @@ static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, 
   int table = 32;
   while (table < 2 * k) table *= 2;
   const int rw = row_warps(n, num_sms);
-  cudaError_t err = cudaFuncSetAttribute(distill_teacher_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (3 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4);
+  static unsigned long long allowed = 0;
+  cudaError_t err = allow_smem(reinterpret_cast<const void *>(distill_teacher_kernel), 8 * (3 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4, allowed);
   if (err != cudaSuccess) return err;
-  distill_teacher_kernel<<<(unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (3 * k + table) * 4, stream>>>(is, t, n, v, (int)k, table, tau, dl, lse, words,
-                                                                                                            weights, rows);
-  err = cudaGetLastError();
+  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (3 * k + table) * 4, stream, is, t, n, v, (int)k, table, tau, dl,
+                     lse, words, weights, rows);
   if (err != cudaSuccess) return err;
-  distill_grad_kernel<T><<<chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream>>>(s, n, v, d, scale, (int)k, words, weights, rows, ds);
-  return cudaGetLastError();
+  return launch_after(distill_grad_kernel<T>, chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream, s, n, v, d, scale, (int)k, words, weights, rows, ds);
 }
 
 cudaError_t launch_topk_distill(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
@@ -600,6 +603,7 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
   const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;
   int64_t i = ((int64_t)blockIdx.x * R_WARPS + warp) * per_warp + sub;
   RouterRow<T, W, J> next;
+  chain_wait();
   uint8_t use = 0;                                   // whether the row counts: loaded beside it, not before it
   int sent = -1;                                     // the lane's first expert of the row
   next.clear();
@@ -668,6 +672,7 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   double p = 0;
   int q = 0;
+  chain_wait();
   if (c <= e) {
     const int cp = min(c, e - 1);                    // the number of rows kept has no sum of p
 #pragma unroll 5
@@ -720,6 +725,7 @@ router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
   const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;
   int64_t i = ((int64_t)blockIdx.x * R_WARPS + warp) * per_warp + sub;
   RouterRow<T, W, J> next;
+  chain_wait();
   uint8_t use = 0;
   next.clear();
   if (i < n) { next.load(r + i * e, e, g, l); use = keep[i]; }
@@ -790,15 +796,18 @@ static cudaError_t router(void *workspace, const T *r, const uint8_t *keep, cons
   int *kept = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(sums) + up256((size_t)e * 8));
   int *ticket = kept + 1;
   const size_t smem = (size_t)s.warps() * s.g * s.cols() * 4 + (size_t)(e + 1) * 4;
-#define FB_PART(W, J)                                                                                                      \
-  if (cudaFuncSetAttribute(router_part_kernel<T, W, J>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10) == cudaSuccess) \
-    router_part_kernel<T, W, J><<<grid, 32 * s.warps(), smem, stream>>>(r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket)
+  cudaError_t err = cudaSuccess;
+#define FB_PART(W, J)                                                                                                     \
+  {                                                                                                                       \
+    static unsigned long long allowed = 0;                                                                                \
+    err = allow_smem(reinterpret_cast<const void *>(router_part_kernel<T, W, J>), 160 << 10, allowed);                    \
+    if (err == cudaSuccess)                                                                                               \
+      err = launch_after(router_part_kernel<T, W, J>, grid, 32 * s.warps(), smem, stream, r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket); \
+  }
   FB_ROUTER_SHAPE(s, FB_PART)
 #undef FB_PART
-  const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
-  router_loss_kernel<<<(unsigned)((e + 1 + 31) / 32), 1024, 0, stream>>>(psum, pcount, grid, (int)e, sums, kept, ticket, counts, loss, norm);
-  return cudaGetLastError();
+  return launch_after(router_loss_kernel, (unsigned)((e + 1 + 31) / 32), 1024, 0, stream, psum, pcount, grid, (int)e, sums, kept, ticket, counts, loss, norm);
 }
 
 template <typename T>
@@ -807,10 +816,10 @@ static cudaError_t router_grad(const T *r, const uint8_t *keep, const int32_t *c
   if (n <= 0 || e <= 0) return cudaSuccess;
   const RouterShape s = router_shape(r, e, sizeof(T));               // the result starts on a 256-byte boundary
   const int grid = (int)router_grid(n, s, num_sms);
-#define FB_GRAD(W, J) router_grad_kernel<T, W, J><<<grid, 32 * s.warps(), 0, stream>>>(r, keep, counts, norm, dl, n, (int)e, s.g, dr)
+#define FB_GRAD(W, J) return launch_after(router_grad_kernel<T, W, J>, grid, 32 * s.warps(), 0, stream, r, keep, counts, norm, dl, n, (int)e, s.g, dr)
   FB_ROUTER_SHAPE(s, FB_GRAD)
 #undef FB_GRAD
-  return cudaGetLastError();
+  return cudaSuccess;
 }
 
 cudaError_t launch_router_balance(void *workspace, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k,

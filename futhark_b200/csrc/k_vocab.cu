@@ -48,6 +48,7 @@ enum VocabEpilogue : int {
   VE_GRAD = 1,         // G in binary16
   VE_SLAB = 2,         // f32 partial products, one slab per part of the summed axis
   VE_HALF = 3,         // binary16, times a factor from device memory
+  VE_ROWS = 4,         // binary16, times 2^-13 and the row's weight: dX where the sum is in one part
 };
 
 // Sixteen epilogue warps, four per SM partition, each with a row and 64 of the tile's columns per thread.  One warp
@@ -72,6 +73,7 @@ struct VocabArgs {
   float *ztarget;
   const float *cexp;            // VE_GRAD: per row the exponent's constant term
   const float *factor;          // VE_HALF
+  const float *w;               // VE_ROWS
   int add;                      // VE_SLAB: add to the slab instead of writing it
   int *failure;
 };
@@ -136,6 +138,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   cluster_sync_all();                                  // both CTAs' barriers exist before either signals the other's
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  chain_wait();
   const bool poisoned = ld_failure(a.failure) != FAIL_NONE;
 
   if (!poisoned) {
@@ -220,13 +223,15 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       // what a tile needs of its row is fetched while the tile before it is worked on
       int tm = 0, tn = 0, split = 0, next_target = -1;
       float next_c = 0.f;
+      constexpr bool PER_ROW = EPI == VE_SOFTMAX || EPI == VE_GRAD || EPI == VE_ROWS;
       auto fetch = [&](uint32_t t, int &sp, int &m, int &n) {
         if (t >= num_tiles) return;
         vocab_tile(a, t, sp, m, n);
         const int r = m * VT + (int)rank * 128 + quarter * 32 + lane;
-        if ((EPI == VE_SOFTMAX || EPI == VE_GRAD) && r < a.M) {
+        if (PER_ROW && r < a.M) {
           next_target = a.targets[r];
           if (EPI == VE_GRAD) next_c = a.cexp[r];
+          if (EPI == VE_ROWS) next_c = a.w[r];
         }
       };
       fetch(pair, split, tm, tn);
@@ -285,6 +290,8 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (EPI == VE_GRAD) {
               const float e = ex2(fmaf(__uint_as_float(v[j]), V_LOG2E, c));
               f[j] = e > 65504.f ? 65504.f : e;            // NaN stays
+            } else if (EPI == VE_ROWS) {
+              f[j] = __uint_as_float(v[j]) * (1.f / V_GSCALE) * c;
             } else {
               f[j] = __uint_as_float(v[j]) * factor;
             }
@@ -299,7 +306,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
           for (int j = 0; j < 16; j++) {
             const __half2 p = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-            h[j] = (EPI == VE_GRAD && !counts) ? 0u : *reinterpret_cast<const uint32_t *>(&p);
+            h[j] = ((EPI == VE_GRAD || EPI == VE_ROWS) && !counts) ? 0u : *reinterpret_cast<const uint32_t *>(&p);
           }
         };
         // 128 bytes of a row are staged as the 128-byte swizzle wants them (16-byte piece q of row r at q ^ (r & 7))
@@ -392,6 +399,7 @@ vocab_loss_kernel(const float2 *__restrict__ part, int tiles, const float *__res
                   float *__restrict__ loss, float *__restrict__ lse, int64_t n, int64_t v) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  chain_wait();
   if (row >= n) return;
   float m = -INFINITY, s = 0.f;
   for (int t = lane; t < tiles; t += 32) {
@@ -415,55 +423,57 @@ vocab_loss_kernel(const float2 *__restrict__ part, int tiles, const float *__res
   }
 }
 
-// One CTA: per row w_i = dl_i q_i and the constant term of G's exponent, and over the rows the largest exponent E.
-// factors[0] = 2^-(E+1) as an exponent for ldexp, factors[1] = 2^(E+1-13) as a float.
-__global__ void __launch_bounds__(1024)
-vocab_prep_kernel(const int32_t *__restrict__ targets, const float *__restrict__ loss, const float *__restrict__ lse,
-                  const float *__restrict__ dl, float *__restrict__ w, float *__restrict__ cexp, int *__restrict__ exponent,
-                  float *__restrict__ factor, int64_t n, int64_t v) {
-  __shared__ int top;
-  if (threadIdx.x == 0) top = -200;
-  __syncthreads();
-  int mine = -200;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    const int64_t t = targets[i];
-    float wi = 0.f, ci = 0.f;
-    if (t >= 0 && t < v) {
-      const float l = lse[i];
-      // losses are off by a few units in the last place of lse: q below that is as good as that
-      const float least = 0x1p-22f * fmaxf(1.f, fabsf(l)), q0 = -expm1f(-loss[i]), q = q0 < least ? least : q0;
-      wi = dl[i] * q;
-      ci = 13.f - log2f(q) - l * V_LOG2E;
-      if (wi != 0.f && isfinite(wi)) mine = max(mine, ilogbf(wi));
-    }
-    w[i] = wi;
-    cexp[i] = ci;
-  }
-  atomicMax(&top, mine);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int e = top == -200 ? 0 : top;
-    *exponent = -(e + 1);
-    *factor = ldexpf(1.f, e + 1 - 13);
-  }
+// w_i = dl_i q_i and the constant term of G's exponent; false for a token without a target
+__device__ __forceinline__ bool row_weight(const int32_t *targets, const float *loss, const float *lse, const float *dl, int64_t i, int64_t v, float &w,
+                                           float &c) {
+  const int64_t t = targets[i];
+  const float ls = loss[i], l = lse[i], d = dl[i];
+  // losses are off by a few units in the last place of lse: q below that is as good as that
+  const float least = 0x1p-22f * fmaxf(1.f, fabsf(l)), q0 = -expm1f(-ls), q = q0 < least ? least : q0;
+  const bool counts = t >= 0 && t < v;
+  w = counts ? d * q : 0.f;
+  c = counts ? 13.f - log2f(q) - l * V_LOG2E : 0.f;
+  return counts;
 }
 
-// X_i w_i 2^-(E+1) in binary16, rows without a target 0.
-__global__ void __launch_bounds__(256)
-vocab_scale_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const int32_t *__restrict__ targets, int64_t v, const float *__restrict__ w, const int *__restrict__ exponent, __half *__restrict__ out) {
-  const int64_t per = dp / 8, total = n * per;
-  const int ex = *exponent;
-  for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
-    const int64_t i = o / per, c = (o - i * per) * 8;
-    const int64_t t = targets[i];
-    __align__(16) __half h[8] = {};
-    if (t >= 0 && t < v) {
-      const float f = ldexpf(w[i], ex);
-      *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(x + i * dp + c);
+// Per row w_i and the exponent's constant, and X_i w_i 2^-(E+1) in binary16 (0 without a target).  E is over all rows: every CTA
+// finds it for itself, which costs it n / 1024 steps and saves a kernel.  *factor = 2^(E+1-13).
+__global__ void __launch_bounds__(1024)
+vocab_prep_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const int32_t *__restrict__ targets, int64_t v, const float *__restrict__ loss,
+                  const float *__restrict__ lse, const float *__restrict__ dl, float *__restrict__ w, float *__restrict__ cexp,
+                  float *__restrict__ factor, __half *__restrict__ out) {
+  __shared__ int tops[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  chain_wait();
+  int top = -200;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    float wi, ci;
+    row_weight(targets, loss, lse, dl, i, v, wi, ci);
+    if (wi != 0.f && isfinite(wi)) top = max(top, ilogbf(wi));
+  }
+  top = __reduce_max_sync(kFull, top);
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  top = __reduce_max_sync(kFull, tops[lane]);
+  const int e = top == -200 ? 0 : top;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *factor = ldexpf(1.f, e + 1 - 13);
+  const int64_t per = dp / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 32 + warp; i < n; i += (int64_t)gridDim.x * 32) {
+    float wi, ci;
+    const bool counts = row_weight(targets, loss, lse, dl, i, v, wi, ci);
+    if (lane == 0) { w[i] = wi; cexp[i] = ci; }
+    const float f = ldexpf(wi, -(e + 1));
+#pragma unroll 4
+    for (int64_t c = lane; c < per; c += 32) {
+      __align__(16) __half h[8] = {};
+      if (counts) {
+        *reinterpret_cast<uint4 *>(h) = reinterpret_cast<const uint4 *>(x + i * dp)[c];
 #pragma unroll
-      for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
+        for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
+      }
+      reinterpret_cast<uint4 *>(out + i * dp)[c] = *reinterpret_cast<const uint4 *>(h);
     }
-    *reinterpret_cast<uint4 *>(out + i * dp + c) = *reinterpret_cast<const uint4 *>(h);
   }
 }
 
@@ -471,6 +481,7 @@ vocab_scale_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const in
 __global__ void __launch_bounds__(256)
 vocab_pitch_kernel(const __half *__restrict__ in, int64_t rows, int64_t in_cols, __half *__restrict__ out, int64_t out_cols) {
   const int64_t total = rows * out_cols;
+  chain_wait();
   for (int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; o < total; o += (int64_t)gridDim.x * 2048) {
     int64_t i = o / out_cols, c = o - i * out_cols;
     __align__(16) __half h[8];
@@ -489,6 +500,7 @@ __global__ void __launch_bounds__(256)
 vocab_dx_kernel(const float *__restrict__ slabs, int splits, int64_t n, int64_t d, int64_t dp, const int32_t *__restrict__ targets, int64_t v,
                 const float *__restrict__ w, __half *__restrict__ dx) {
   const int64_t per = dp / 4, total = n * per;
+  chain_wait();
   for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
     const int64_t i = o / per, c = (o - i * per) * 4;
     const int64_t t = targets[i];
@@ -519,6 +531,7 @@ vocab_dx_kernel(const float *__restrict__ slabs, int splits, int64_t n, int64_t 
 
 __global__ void __launch_bounds__(256)
 vocab_fill_kernel(float *__restrict__ loss, float *__restrict__ lse, int64_t n, float l) {
+  chain_wait();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) { loss[i] = 0.f; lse[i] = l; }
 }
 
@@ -546,7 +559,7 @@ static int tile_columns(int64_t rows, int64_t cols, int64_t parts, int64_t kbloc
 
 // Parts of the summed axis of dX = G W.  A small batch has fewer tiles than there are pairs of SMs, while its sum
 // runs over the vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks, as above, with
-// 3000 per tile for its epilogue where nothing hides it and 3600 bytes of HBM per clock for the slabs.
+// 3000 per tile for its epilogue where nothing hides it, 6000 for the kernel that adds the slabs and 3600 bytes of HBM per clock.
 static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int pairs, int *nt) {
   int best = 1;
   double best_cost = 0;
@@ -555,7 +568,7 @@ static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int pairs, int *nt)
     for (int s = 1; s <= 64 && s <= kblocks; s++) {
       const int64_t kps = ceil_div(kblocks, s);
       if (ceil_div(kblocks, kps) != s) continue;
-      const double cost = (double)ceil_div(tiles * s, pairs) * (kps * (w + 64) * 1.6 + 3000.0) + (double)s * n * dp * 8 / 3600.0;
+      const double cost = (double)ceil_div(tiles * s, pairs) * (kps * (w + 64) * 1.6 + 3000.0) + (s > 1 ? 6000.0 + (double)s * n * dp * 8 / 3600.0 : 0.0);
       if ((s == 1 && w == VT) || cost < best_cost) { best = s; *nt = w; best_cost = cost; }
     }
   }
@@ -587,13 +600,16 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     if (words > want) words = want;
     p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
     p.nt = tile_columns(n, p.piece < v ? p.piece : v, 1, ceil_div(p.dp, VK), 64, pairs);
+    p.pieces = (int)ceil_div(v, p.piece);
     p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), pairs, &p.ntd);
     p.w = take((size_t)n * 4);
     p.cexp = take((size_t)n * 4);
     p.scalars = take(256);
     p.xs = take((size_t)(n * p.dp) * 2);
     p.g = take((size_t)(n * p.piece) * 2);
-    p.slabs = take((size_t)p.splits * (size_t)(n * p.dp) * 4);
+    p.direct = p.splits == 1 && p.pieces == 1;
+    if (p.direct) p.dxp = padded ? take((size_t)(n * p.dp) * 2) : 0;
+    else p.slabs = take((size_t)p.splits * (size_t)(n * p.dp) * 4);
     p.dwp = padded ? take((size_t)((p.piece < v ? p.piece : v) * p.dp) * 2) : 0;
   }
   p.bytes = off;
@@ -604,7 +620,8 @@ template <bool A_MN, bool B_MN, int EPI>
 static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
   constexpr int smem = VocabShape<EPI>::smem;
   auto kernel = vocab_mma_kernel<A_MN, B_MN, EPI>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static unsigned long long allowed = 0;
+  const cudaError_t err = allow_smem(reinterpret_cast<const void *>(kernel), smem, allowed);
   if (err != cudaSuccess) return err;
   a.tiles_m = (int)ceil_div(a.M, VT);
   a.tiles_n = (int)ceil_div(a.N, a.nt);
@@ -612,8 +629,7 @@ static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, co
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   int pairs = num_sms / 2;
   if (tiles < pairs) pairs = (int)tiles;
-  kernel<<<2 * pairs, V_THREADS, smem, stream>>>(tmA, tmB, tmC, a);
-  return cudaGetLastError();
+  return launch_after(kernel, 2 * pairs, V_THREADS, smem, stream, tmA, tmB, tmC, a);
 }
 
 // an operand [rows][cols] of row pitch `pitch`, in boxes of 64 columns and `box` rows: 64 where it is read across the sum
@@ -628,9 +644,8 @@ static void single_tile_rows(VocabArgs &a) {
 }
 
 static cudaError_t repitch(const uint16_t *in, int64_t rows, int64_t in_cols, uint16_t *out, int64_t out_cols, int num_sms, cudaStream_t stream) {
-  vocab_pitch_kernel<<<elementwise_grid((rows * out_cols + 7) / 8, num_sms), 256, 0, stream>>>(reinterpret_cast<const __half *>(in), rows, in_cols,
-                                                                                     reinterpret_cast<__half *>(out), out_cols);
-  return cudaGetLastError();
+  return launch_after(vocab_pitch_kernel, elementwise_grid((rows * out_cols + 7) / 8, num_sms), 256, 0, stream, reinterpret_cast<const __half *>(in), rows,
+                      in_cols, reinterpret_cast<__half *>(out), out_cols);
 }
 
 #define FB_TRY(e) do { const cudaError_t fb_err = (e); if (fb_err != cudaSuccess) return fb_err; } while (0)
@@ -639,8 +654,7 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
                               float *lse, int64_t n, int64_t v, int64_t d, int *failure, int num_sms, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
   if (v <= 0) {                                   // the sum of nothing
-    vocab_fill_kernel<<<elementwise_grid(n, num_sms), 256, 0, stream>>>(loss, lse, n, -INFINITY);
-    return cudaGetLastError();
+    return launch_after(vocab_fill_kernel, elementwise_grid(n, num_sms), 256, 0, stream, loss, lse, n, -INFINITY);
   }
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
@@ -656,8 +670,7 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
   a.ztarget = reinterpret_cast<float *>(ws + p.zt);
   a.failure = failure;
   FB_TRY((launch_mma<false, false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
-  vocab_loss_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, stream>>>(a.part, (int)ceil_div(v, p.nt), a.ztarget, targets, loss, lse, n, v);
-  return cudaGetLastError();
+  return launch_after(vocab_loss_kernel, (unsigned)ceil_div(n, 8), 256, 0, stream, a.part, (int)ceil_div(v, p.nt), a.ztarget, targets, loss, lse, n, v);
 }
 
 cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets,
@@ -670,16 +683,14 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
   }
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   float *rw = reinterpret_cast<float *>(ws + p.w), *cexp = reinterpret_cast<float *>(ws + p.cexp), *slabs = reinterpret_cast<float *>(ws + p.slabs);
-  int *exponent = reinterpret_cast<int *>(ws + p.scalars);
-  float *factor = reinterpret_cast<float *>(ws + p.scalars) + 1;
+  float *factor = reinterpret_cast<float *>(ws + p.scalars);
   uint16_t *xs = reinterpret_cast<uint16_t *>(ws + p.xs), *g = reinterpret_cast<uint16_t *>(ws + p.g);
-  vocab_prep_kernel<<<1, 1024, 0, stream>>>(targets, loss, lse, dl, rw, cexp, exponent, factor, n, v);
-  FB_TRY(cudaGetLastError());
   if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
   if (p.copy_w) { FB_TRY(repitch(w, v, d, reinterpret_cast<uint16_t *>(ws + p.wp), p.dp, num_sms, stream)); w = reinterpret_cast<uint16_t *>(ws + p.wp); }
-  vocab_scale_kernel<<<elementwise_grid(n * p.dp / 8, num_sms), 256, 0, stream>>>(reinterpret_cast<const __half *>(x), n, p.dp, targets, v, rw,
-                                                                                  exponent, reinterpret_cast<__half *>(xs));
-  FB_TRY(cudaGetLastError());
+  const int64_t row_ctas = ceil_div(n, 32);
+  FB_TRY(launch_after(vocab_prep_kernel, (unsigned)(row_ctas < 2 * num_sms ? row_ctas : 2 * num_sms), 1024, 0, stream, reinterpret_cast<const __half *>(x), n,
+                      p.dp, targets, v, loss, lse, dl, rw, cexp, factor, reinterpret_cast<__half *>(xs)));
+  uint16_t *dxo = p.dp == d ? dx : reinterpret_cast<uint16_t *>(ws + p.dxp);
   for (int64_t v0 = 0; v0 < v; v0 += p.piece) {
     const int64_t vw = v - v0 < p.piece ? v - v0 : p.piece;
     CUtensorMap tmX, tmW, tmG, tmGk, tmWn, tmS, tmGm, tmXn, tmD;
@@ -690,7 +701,8 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, a.arows0) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, p.nt / 2) &&
                     make_tensor_map(&tmG, g, (uint64_t)vw, (uint64_t)n, 1, (uint64_t)p.piece, (uint64_t)p.piece * n, 64, 32) &&
                     operand_map(&tmGk, g, n, vw, p.piece, a.arows0) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, 64) &&
-                    make_tensor_map(&tmS, slabs, (uint64_t)p.dp, (uint64_t)n, (uint64_t)p.splits, (uint64_t)p.dp, (uint64_t)(p.dp * n), 32, 32, true) &&
+                    (p.direct ? make_tensor_map(&tmS, dxo, (uint64_t)p.dp, (uint64_t)n, 1, (uint64_t)p.dp, (uint64_t)(p.dp * n), 64, 32)
+                              : make_tensor_map(&tmS, slabs, (uint64_t)p.dp, (uint64_t)n, (uint64_t)p.splits, (uint64_t)p.dp, (uint64_t)(p.dp * n), 32, 32, true)) &&
                     operand_map(&tmGm, g, n, vw, p.piece, 64) && operand_map(&tmXn, xs, n, p.dp, p.dp, 64) &&
                     make_tensor_map(&tmD, dwo, (uint64_t)p.dp, (uint64_t)vw, 1, (uint64_t)p.dp, (uint64_t)(p.dp * vw), 64, 32);
     if (!ok) return cudaErrorInvalidValue;
@@ -703,15 +715,18 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     a.N = (int)p.dp; a.kblocks = (int)ceil_div(vw, VK); a.nt = p.ntd;
     a.splits = (int)ceil_div(a.kblocks, ceil_div(a.kblocks, p.splits < a.kblocks ? p.splits : a.kblocks));
     a.add = v0 > 0;
-    FB_TRY((launch_mma<false, true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
+    a.w = rw;
+    if (p.direct) FB_TRY((launch_mma<false, true, VE_ROWS>(tmGk, tmWn, tmS, a, num_sms, stream)));
+    else FB_TRY((launch_mma<false, true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
     a.M = (int)vw; a.N = (int)p.dp; a.kblocks = (int)ceil_div(n, VK); a.splits = 1; a.add = 0;
     a.nt = tile_columns(vw, p.dp, 1, a.kblocks, 128, num_sms / 2);
     a.arows0 = a.arows1 = 128;
     FB_TRY((launch_mma<true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
     if (p.dp != d) FB_TRY(repitch(dwo, vw, p.dp, dw + v0 * d, d, num_sms, stream));
   }
-  vocab_dx_kernel<<<elementwise_grid(n * p.dp / 4, num_sms), 256, 0, stream>>>(slabs, p.splits, n, d, p.dp, targets, v, rw, reinterpret_cast<__half *>(dx));
-  return cudaGetLastError();
+  if (p.direct) return p.dp == d ? cudaSuccess : repitch(dxo, n, p.dp, dx, d, num_sms, stream);
+  return launch_after(vocab_dx_kernel, elementwise_grid(n * p.dp / 4, num_sms), 256, 0, stream, slabs, p.splits, n, d, p.dp, targets, v, rw,
+                      reinterpret_cast<__half *>(dx));
 }
 
 }  // namespace fb

@@ -189,7 +189,9 @@ struct VocabPlan {
   int64_t piece;               // gradient: words per piece of the vocabulary
   int nt;                      // columns of a tile of logits
   int splits, ntd;             // gradient: parts of the sum over a piece's words, columns of a tile of dX
-  size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dwp, bytes;
+  int pieces;
+  bool direct;                 // gradient: dX leaves the tensor cores finished (one piece, one part)
+  size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dxp, dwp, bytes;
 };
 VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_aligned, bool grad, int num_sms);
 cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
