@@ -21,8 +21,8 @@
 // a unit in the last place of each element, independent of the others, of the size of the result's own rounding.
 // Both products accumulate in f32.
 //
-// All four products run on one kernel (vocab_mma_kernel): pairs of CTAs on 256 x 256 tiles with
-// tcgen05.mma.cta_group::2, operands by bulk tensor copies through a six-stage ring, two accumulators in tensor
+// The products run on one kernel (vocab_mma_kernel): pairs of CTAs on 256 x 256 tiles with
+// tcgen05.mma.cta_group::2 (single CTAs on 128 x 256 for small batches), operands by bulk tensor copies through a ring of stages, two accumulators in tensor
 // memory so that the epilogue of a tile runs under the next tile's instructions.  The operands are taken
 // as they lie in memory, contiguous along the summed axis or across it: no transposition.
 #include <cuda_fp16.h>
@@ -35,13 +35,17 @@ namespace fb {
 
 constexpr int VT = 256;                                // tile edge of a CTA pair
 constexpr int VK = 64;                                 // summed elements per stage
-constexpr int V_OPERAND = 128 * VK * 2;                // a CTA's half of one operand in one stage: 16 KiB
-constexpr int V_STAGE = 2 * V_OPERAND;
+constexpr int V_OPERAND = 128 * VK * 2;                // 128 rows of an operand in one stage: 16 KiB
 constexpr int V_SLAB = VK * 64 * 2;                    // 64 x 64 block of an operand that is contiguous across the sum
 constexpr int V_EPI_BUF = 32 * 128;                    // 32 rows of 128 bytes
 constexpr int V_GROUP = 16;                            // row tiles that share the columns' operand before it moves on
 constexpr float V_LOG2E = 1.4426950408889634f;
 constexpr float V_GSCALE = 8192.f;                     // 2^13, see above
+// Longest sum, in blocks of VK, that a logit is accumulated in at once.  The tensor cores truncate the running sum at every
+// step, so a logit's error grows with the number of steps and has the logit's sign: over 4096 products the logarithm of the sum was
+// 1.4e-6 off relative to itself.  Longer sums run in two accumulators that the epilogue adds, which halves that; both halves of tensor
+// memory then belong to one tile, and the next one begins when they have been read.
+constexpr int V_ONE_SUM = 32;
 
 enum VocabEpilogue : int {
   VE_SOFTMAX = 0,      // (maximum, sum) of the tile's columns per row, and the target's logit
@@ -55,16 +59,19 @@ enum VocabEpilogue : int {
 // per partition cannot hide its own latencies: it issued every 4.5 clocks and took 7400 clocks for a tile of which the
 // exponentials need 2048.  Folding stages nothing and leaves room for another stage of operands.
 constexpr int V_WARPS = 16, V_COLS = VT / (V_WARPS / 4), V_THREADS = 64 + 32 * V_WARPS;
-template <int EPI> struct VocabShape {
-  static constexpr int stages = EPI == VE_SOFTMAX ? 6 : 5;
+template <bool PAIR, int EPI> struct VocabShape {
+  static constexpr int rows = PAIR ? 256 : 128;                     // of a tile
+  static constexpr int stage = PAIR ? 2 * V_OPERAND : 3 * V_OPERAND;
+  static constexpr int stages = PAIR ? (EPI == VE_SOFTMAX ? 6 : 5) : (EPI == VE_SOFTMAX ? 4 : 3);
   static constexpr int staging = EPI == VE_SOFTMAX ? 2 * (V_WARPS / 4) * 128 * (int)sizeof(float2) : V_WARPS * V_EPI_BUF;
-  static constexpr int smem = stages * V_STAGE + 1024 /*alignment*/ + 1024 /*barriers*/ + staging;
+  static constexpr int smem = stages * stage + 1024 /*alignment*/ + 1024 /*barriers*/ + staging;
 };
 
 struct VocabArgs {
   int M, N, kblocks;            // extents; the summed axis in blocks of VK
   int nt;                       // columns of a tile: a multiple of 32 up to 256
-  int arows0, arows1;           // rows of A that the two CTAs bring per stage: 128 unless there is one row tile
+  int arows;                    // rows of A that a CTA brings per stage
+  int halves;                   // VE_SOFTMAX: the sum in two accumulators
   int splits, kps;              // parts of the summed axis and the blocks of each
   int tiles_m, tiles_n;
   const int32_t *targets;       // VE_SOFTMAX, VE_GRAD
@@ -108,34 +115,42 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs &a, uint32_t t, int &
 }
 
 // A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
-template <bool A_MN, bool B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
+// PAIR: two CTAs per tile of 256 rows; otherwise one per tile of 128 rows, for batches of at most 128 tokens.  Of a pair's 256
+// rows those would leave half or more to zeros: 64 tokens against 131072 x 4096 weights took 185 us, which is what the tensor
+// cores need for 256 rows, where the weights can be read in 164.
+template <bool PAIR, bool A_MN, bool B_MN, int EPI>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(V_THREADS, 1)
 vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const VocabArgs a) {
-  constexpr int V_STAGES = VocabShape<EPI>::stages;
+  constexpr int V_STAGES = VocabShape<PAIR, EPI>::stages, V_STAGE = VocabShape<PAIR, EPI>::stage, MT = VocabShape<PAIR, EPI>::rows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   VocabBarriers *bars = reinterpret_cast<VocabBarriers *>(smem + V_STAGES * V_STAGE);
   uint8_t *epi = smem + V_STAGES * V_STAGE + 1024;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = cluster_ctarank();
-  const uint32_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const uint32_t pair = PAIR ? blockIdx.x >> 1 : blockIdx.x, npairs = PAIR ? gridDim.x >> 1 : gridDim.x;
   const uint32_t num_tiles = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n * (uint32_t)a.splits;     // below 2^31
 
   if (tid == 0) {
     for (int s = 0; s < V_STAGES; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], 2 * V_WARPS); }
+    for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], (PAIR ? 2 : 1) * V_WARPS); }
     for (int i = 0; i < 8; i++) mbar_init(&bars->met[i >> 2][i & 3], V_WARPS / 4 - 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(&bars->tmem_base, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();                                  // both CTAs' barriers exist before either signals the other's
+  if (PAIR) cluster_sync_all();                        // both CTAs' barriers exist before either signals the other's
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
   chain_wait();
@@ -150,8 +165,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         for (uint32_t t = pair; t < num_tiles && ok; t += npairs) {
           int split, tm, tn;
           vocab_tile(a, t, split, tm, tn);
-          const int m0 = tm * VT + (int)rank * 128, n0 = tn * a.nt + (int)rank * (a.nt >> 1);
-          const int arows = rank == 0 ? a.arows0 : a.arows1;
+          const int m0 = tm * MT + (int)rank * 128, n0 = tn * a.nt + (int)rank * (a.nt >> 1);
           const int kb1 = min(a.kblocks, (split + 1) * a.kps);
           for (int kb = split * a.kps; kb < kb1; kb++, it++) {
             const int s = it % V_STAGES;
@@ -159,19 +173,24 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (!mbar_wait_bounded(&bars->empty[s], ph ^ 1)) { ok = false; break; }
             uint8_t *sa = smem + s * V_STAGE;
             uint8_t *sb = sa + V_OPERAND;
-            const uint32_t full0 = map_to_cta(smem_u32(&bars->full[s]), 0);
-            if (rank == 0) mbar_expect_tx(&bars->full[s], (a.arows0 + a.arows1 + a.nt) * (VK * 2));   // both CTAs' bytes
+            uint64_t *full = &bars->full[s];
+            const uint32_t full0 = PAIR ? map_to_cta(smem_u32(full), 0) : 0;
+            auto load = [&](void *dst, const CUtensorMap *tm, int x, int y) {
+              if (PAIR) tma_load_3d_pair(dst, tm, x, y, 0, full0);
+              else tma_load_3d(dst, tm, x, y, 0, full);
+            };
+            if (rank == 0) mbar_expect_tx(full, ((PAIR ? 2 : 1) * a.arows + a.nt) * (VK * 2));     // both CTAs' bytes
             if (A_MN) {
-              tma_load_3d_pair(sa, &tmA, m0, kb * VK, 0, full0);
-              tma_load_3d_pair(sa + V_SLAB, &tmA, m0 + 64, kb * VK, 0, full0);
-            } else if (arows > 0) {
-              tma_load_3d_pair(sa, &tmA, kb * VK, m0, 0, full0);
+              load(sa, &tmA, m0, kb * VK);
+              load(sa + V_SLAB, &tmA, m0 + 64, kb * VK);
+            } else {
+              load(sa, &tmA, kb * VK, m0);
             }
             if (B_MN) {
-              tma_load_3d_pair(sb, &tmB, n0, kb * VK, 0, full0);
-              if (a.nt > 128) tma_load_3d_pair(sb + V_SLAB, &tmB, n0 + 64, kb * VK, 0, full0);
+              const int slabs = a.nt / (PAIR ? 128 : 64);
+              for (int j = 0; j < slabs; j++) load(sb + j * V_SLAB, &tmB, n0 + j * 64, kb * VK);
             } else {
-              tma_load_3d_pair(sb, &tmB, kb * VK, n0, 0, full0);
+              load(sb, &tmB, kb * VK, n0);
             }
           }
         }
@@ -180,23 +199,26 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     } else if (warp == 1) {
       // ---------------- MMA issuer: one thread of the first CTA ----------------
       if (lane == 0 && rank == 0) {
-        // D = f32, A = B = f16, M = 256 over the pair, N the tile's columns
-        const uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(a.nt >> 3) << 17) | ((uint32_t)(VT >> 4) << 24);
+        // D = f32, A = B = f16, M the tile's rows, N its columns
+        const uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(a.nt >> 3) << 17) | ((uint32_t)(MT >> 4) << 24);
         uint32_t it = 0, tile_it = 0;
         bool ok = true;
         for (uint32_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
           int split, tm, tn;
           vocab_tile(a, t, split, tm, tn);
-          const uint32_t acc = tile_it & 1, acc_ph = (tile_it >> 1) & 1;
+          const bool halves = EPI == VE_SOFTMAX && a.halves;
+          const uint32_t acc = halves ? 0 : tile_it & 1, acc_ph = (halves ? tile_it : tile_it >> 1) & 1;
           if (!mbar_wait_bounded(&bars->tmem_empty[acc], acc_ph ^ 1)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t d_tmem = tmem_base + acc * VT;
-          const int kb0 = split * a.kps, kb1 = min(a.kblocks, kb0 + a.kps);
+          uint32_t d_tmem = tmem_base + acc * VT;
+          int kb0 = split * a.kps;
+          const int kb1 = min(a.kblocks, kb0 + a.kps), turn = halves ? (kb0 + kb1) / 2 : kb1;
           for (int kb = kb0; kb < kb1; kb++, it++) {
             const int s = it % V_STAGES;
             const uint32_t ph = (it / V_STAGES) & 1;
             if (!mbar_wait_bounded(&bars->full[s], ph)) { ok = false; break; }
             tc_fence_after();
+            if (kb == turn) { d_tmem += VT; kb0 = kb; }      // the second half starts from nothing
             const uint32_t sa = smem_u32(smem + s * V_STAGE);
             const uint32_t sb = sa + V_OPERAND;
             // along the sum: rows of 128 bytes, 8-row groups 1024 bytes apart, a step of 16 is 32 bytes inside the
@@ -204,12 +226,19 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             const uint64_t adesc = A_MN ? make_smem_desc(sa, V_SLAB, 1024) : make_smem_desc(sa, 16, 1024);
             const uint64_t bdesc = B_MN ? make_smem_desc(sb, V_SLAB, 1024) : make_smem_desc(sb, 16, 1024);
 #pragma unroll
-            for (int k = 0; k < VK / 16; k++)
-              tc2_mma_f16(d_tmem, adesc + (uint64_t)(k * (A_MN ? 128 : 2)), bdesc + (uint64_t)(k * (B_MN ? 128 : 2)), idesc,
-                          (kb > kb0 || k > 0) ? 1u : 0u);
-            tc2_commit_both(&bars->empty[s]);
+            for (int k = 0; k < VK / 16; k++) {
+              const uint64_t ad = adesc + (uint64_t)(k * (A_MN ? 128 : 2)), bd = bdesc + (uint64_t)(k * (B_MN ? 128 : 2));
+              const uint32_t more = (kb > kb0 || k > 0) ? 1u : 0u;
+              if (PAIR) tc2_mma_f16(d_tmem, ad, bd, idesc, more);
+              else tc_mma_f16(d_tmem, ad, bd, idesc, more);
+            }
+            if (PAIR) tc2_commit_both(&bars->empty[s]);
+            else tc_commit(&bars->empty[s]);
           }
-          if (ok) tc2_commit_both(&bars->tmem_full[acc]);
+          if (ok) {
+            if (PAIR) tc2_commit_both(&bars->tmem_full[acc]);
+            else tc_commit(&bars->tmem_full[acc]);
+          }
         }
         if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
       }
@@ -227,7 +256,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       auto fetch = [&](uint32_t t, int &sp, int &m, int &n) {
         if (t >= num_tiles) return;
         vocab_tile(a, t, sp, m, n);
-        const int r = m * VT + (int)rank * 128 + quarter * 32 + lane;
+        const int r = m * MT + (int)rank * 128 + quarter * 32 + lane;
         if (PER_ROW && r < a.M) {
           next_target = a.targets[r];
           if (EPI == VE_GRAD) next_c = a.cexp[r];
@@ -236,9 +265,10 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       };
       fetch(pair, split, tm, tn);
       for (uint32_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
-        const int row0 = tm * VT + (int)rank * 128 + quarter * 32, n0 = tn * a.nt;
+        const int row0 = tm * MT + (int)rank * 128 + quarter * 32, n0 = tn * a.nt;
         const int row = row0 + lane;
-        const uint32_t acc = tile_it & 1, acc_ph = (tile_it >> 1) & 1;
+        const bool halves = EPI == VE_SOFTMAX && a.halves;
+        const uint32_t acc = halves ? 0 : tile_it & 1, acc_ph = (halves ? tile_it : tile_it >> 1) & 1;
         const int ncols = min(a.nt, a.N - n0);
         int tcol = -1;                                     // the target's column in this tile, if it has it
         const float c = next_c;
@@ -340,29 +370,54 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           release(c0);
         };
 
-        if (row0 < a.M && cbase < ncols) {                 // uniform over the warp
+        // the accumulator may be written again
+        auto give_back = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) mbar_arrive_pair(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
+            else mbar_arrive(&bars->tmem_empty[acc]);
+          }
+        };
+        const bool mine = row0 < a.M && cbase < ncols;     // uniform over the warp
+        if (halves && !mine) give_back();
+        if (mine) {
           uint32_t va[32], vb[32];
           tmem_ld_32x32(taddr0 + cbase, va);
-          tmem_ld_wait();
-          tmem_ld_32x32(taddr0 + cbase + 32, vb);
-          if (EPI == VE_SOFTMAX) fold(va, cbase);
-          else if (EPI == VE_SLAB) slab(va, cbase);
-          else { uint32_t h[16]; to_half(va, cbase, h); acquire(); half_pieces(h, 0); }
-          tmem_ld_wait();
+          if (halves) {                                    // each 32 columns from both accumulators
+            tmem_ld_32x32(taddr0 + VT + cbase, vb);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j++) va[j] = __float_as_uint(__uint_as_float(va[j]) + __uint_as_float(vb[j]));
+            fold(va, cbase);
+            tmem_ld_32x32(taddr0 + cbase + 32, va);
+            tmem_ld_32x32(taddr0 + VT + cbase + 32, vb);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j++) vb[j] = __float_as_uint(__uint_as_float(va[j]) + __uint_as_float(vb[j]));
+            give_back();
+          } else {
+            tmem_ld_wait();
+            tmem_ld_32x32(taddr0 + cbase + 32, vb);
+            if (EPI == VE_SOFTMAX) fold(va, cbase);
+            else if (EPI == VE_SLAB) slab(va, cbase);
+            else { uint32_t h[16]; to_half(va, cbase, h); acquire(); half_pieces(h, 0); }
+            tmem_ld_wait();
+          }
           if (EPI == VE_SOFTMAX) fold(vb, cbase + 32);
           else if (EPI == VE_SLAB) slab(vb, cbase + 32);
           else { uint32_t h[16]; to_half(vb, cbase + 32, h); half_pieces(h, 4); release(cbase); }
         }
         if (EPI == VE_SOFTMAX) {
-          // the four shares of a row meet in shared memory, at the first one's warp; its arrival below is what lets the
-          // tile after the next one, which uses the same places, begin
+          // the four shares of a row meet in shared memory, at the first one's warp.  The tile after the next one uses the same
+          // places: it begins when this warp has given back the next tile's accumulator, or this one's where there are two
           float2 *meet = reinterpret_cast<float2 *>(epi) + (tile_it & 1) * (V_WARPS / 4) * 128 + quarter * 32 + lane;
           if (share != 0) {
             meet[share * 128] = make_float2(m2, sum);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->met[tile_it & 1][quarter]);
           } else {
-            if (!__all_sync(kFull, mbar_wait_bounded(&bars->met[tile_it & 1][quarter], acc_ph))) { ok = false; break; }
+            if (!__all_sync(kFull, mbar_wait_bounded(&bars->met[tile_it & 1][quarter], (tile_it >> 1) & 1))) { ok = false; break; }
 #pragma unroll
             for (int w = 1; w < V_WARPS / 4; w++) {
               const float2 o = meet[w * 128];
@@ -372,9 +427,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_pair(map_to_cta(smem_u32(&bars->tmem_empty[acc]), 0));
+        if (!halves) give_back();
         if (EPI == VE_SOFTMAX && share == 0 && row < a.M) a.part[(int64_t)row * a.tiles_n + this_tn] = make_float2(m2, sum);
       }
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -385,10 +438,11 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();                                  // nobody signals into a partner that has left
+  if (PAIR) cluster_sync_all();                        // nobody signals into a partner that has left
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    if (!PAIR) tmem_dealloc(tmem_base, 512);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
   }
 }
 
@@ -543,32 +597,40 @@ static inline int elementwise_grid(int64_t items, int num_sms) {
   return (int)(g < 1 ? 1 : g < (int64_t)num_sms * 16 ? g : (int64_t)num_sms * 16);
 }
 
+// Batches of at most 128 tokens go to single CTAs, where the tokens are the rows of the product.
+static inline bool small_batch(int64_t n) { return n <= 128; }
+// Clocks of a block of 64 summed elements of a tile of `cols` columns: on pairs 512 for 256 columns at the tensor cores'
+// rate and a fifth of that for the rows' operand; on single CTAs what 148 of them leave each other of HBM, 24 bytes per clock.
+static inline double block_clocks(bool pair, int cols) { return pair ? (cols + 64) * 1.6 : cols * 5.3; }
+
 // Columns of a tile.  A tile of fewer columns reuses its rows less, but a number of tiles that is just above a multiple of
-// the number of pairs leaves most pairs idle in the last round; the estimate is in clocks, 512 per block of 64
-// summed elements and 256 columns at the tensor cores' rate, a fifth of it for the rows' operand.
-static int tile_columns(int64_t rows, int64_t cols, int64_t parts, int64_t kblocks, int step, int pairs) {
+// the number of CTAs or pairs leaves most of them idle in the last round.
+static int tile_columns(bool pair, int64_t rows, int64_t cols, int64_t kblocks, int step, int num_sms) {
   int best = VT;
   double best_cost = 0;
+  const int64_t workers = pair ? num_sms / 2 : num_sms;
   for (int nt = VT; nt >= 128; nt -= step) {
-    const int64_t tiles = ceil_div(rows, VT) * ceil_div(cols, nt) * parts;
-    const double cost = (double)ceil_div(tiles, pairs) * (kblocks * (nt + 64) * 1.6 + 1500.0);
+    const int64_t tiles = ceil_div(rows, pair ? 256 : 128) * ceil_div(cols, nt);
+    const double cost = (double)ceil_div(tiles, workers) * (kblocks * block_clocks(pair, nt) + 1500.0);
     if (nt == VT || cost < 0.97 * best_cost) { best = nt; best_cost = cost; }
   }
   return best;
 }
 
-// Parts of the summed axis of dX = G W.  A small batch has fewer tiles than there are pairs of SMs, while its sum
-// runs over the vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks, as above, with
+// Parts of the summed axis of dX = G W.  A small batch has fewer tiles than there are SMs, while its sum runs over the
+// vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks, as above, with
 // 3000 per tile for its epilogue where nothing hides it, 6000 for the kernel that adds the slabs and 3600 bytes of HBM per clock.
-static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int pairs, int *nt) {
+static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int num_sms, int *nt) {
   int best = 1;
   double best_cost = 0;
+  const bool pair = !small_batch(n);
+  const int64_t workers = pair ? num_sms / 2 : num_sms;
   for (int w = VT; w >= 128; w -= 128) {
-    const int64_t tiles = ceil_div(n, VT) * ceil_div(dp, w);
-    for (int s = 1; s <= 64 && s <= kblocks; s++) {
+    const int64_t tiles = ceil_div(n, pair ? 256 : 128) * ceil_div(dp, w);
+    for (int s = 1; s <= 128 && s <= kblocks; s++) {
       const int64_t kps = ceil_div(kblocks, s);
       if (ceil_div(kblocks, kps) != s) continue;
-      const double cost = (double)ceil_div(tiles * s, pairs) * (kps * (w + 64) * 1.6 + 3000.0) + (s > 1 ? 6000.0 + (double)s * n * dp * 8 / 3600.0 : 0.0);
+      const double cost = (double)ceil_div(tiles * s, workers) * (kps * block_clocks(pair, w) + 3000.0) + (s > 1 ? 6000.0 + (double)s * n * dp * 8 / 3600.0 : 0.0);
       if ((s == 1 && w == VT) || cost < best_cost) { best = s; *nt = w; best_cost = cost; }
     }
   }
@@ -580,7 +642,7 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   if (n <= 0 || v <= 0 || (grad && d <= 0)) return p;           // nothing will run
   p.dp = d <= 0 ? 8 : (d + 7) & ~(int64_t)7;
   const bool padded = p.dp != d;
-  const int pairs = num_sms / 2;
+  const bool pair = !small_batch(n);
   size_t off = 0;
   auto take = [&](size_t bytes) { const size_t at = off; off += align256(bytes); return at; };
   p.copy_x = padded || !x_aligned;
@@ -588,7 +650,7 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   p.xp = p.copy_x ? take((size_t)(n * p.dp) * 2) : 0;
   p.wp = p.copy_w ? take((size_t)(v * p.dp) * 2) : 0;
   if (!grad) {
-    p.nt = tile_columns(n, v, 1, ceil_div(p.dp, VK), 32, pairs);
+    p.nt = tile_columns(pair, n, v, ceil_div(p.dp, VK), 32, num_sms);
     p.part = take((size_t)(n * ceil_div(v, p.nt)) * sizeof(float2));
     p.zt = take((size_t)n * 4);
   } else {
@@ -599,9 +661,9 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     if (words < VT) words = VT;
     if (words > want) words = want;
     p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
-    p.nt = tile_columns(n, p.piece < v ? p.piece : v, 1, ceil_div(p.dp, VK), 64, pairs);
+    p.nt = tile_columns(pair, n, p.piece < v ? p.piece : v, ceil_div(p.dp, VK), 64, num_sms);
     p.pieces = (int)ceil_div(v, p.piece);
-    p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), pairs, &p.ntd);
+    p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), num_sms, &p.ntd);
     p.w = take((size_t)n * 4);
     p.cexp = take((size_t)n * 4);
     p.scalars = take(256);
@@ -616,32 +678,37 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   return p;
 }
 
-template <bool A_MN, bool B_MN, int EPI>
-static cudaError_t launch_mma(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
-  constexpr int smem = VocabShape<EPI>::smem;
-  auto kernel = vocab_mma_kernel<A_MN, B_MN, EPI>;
+template <bool PAIR, bool A_MN, bool B_MN, int EPI>
+static cudaError_t launch_tiles(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
+  constexpr int smem = VocabShape<PAIR, EPI>::smem;
+  auto kernel = vocab_mma_kernel<PAIR, A_MN, B_MN, EPI>;
   static unsigned long long allowed = 0;
   const cudaError_t err = allow_smem(reinterpret_cast<const void *>(kernel), smem, allowed);
   if (err != cudaSuccess) return err;
-  a.tiles_m = (int)ceil_div(a.M, VT);
+  a.tiles_m = (int)ceil_div(a.M, VocabShape<PAIR, EPI>::rows);
   a.tiles_n = (int)ceil_div(a.N, a.nt);
   a.kps = (int)ceil_div(a.kblocks, a.splits);
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
-  int pairs = num_sms / 2;
-  if (tiles < pairs) pairs = (int)tiles;
-  return launch_after(kernel, 2 * pairs, V_THREADS, smem, stream, tmA, tmB, tmC, a);
+  int64_t workers = PAIR ? num_sms / 2 : num_sms;
+  if (tiles < workers) workers = tiles;
+  return launch_after(kernel, (unsigned)((PAIR ? 2 : 1) * workers), V_THREADS, smem, stream, tmA, tmB, tmC, a);
+}
+// products whose rows are tokens
+template <bool B_MN, int EPI>
+static cudaError_t launch_tokens(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, const VocabArgs &a, int num_sms, cudaStream_t stream) {
+  return small_batch(a.M) ? launch_tiles<false, false, B_MN, EPI>(tmA, tmB, tmC, a, num_sms, stream)
+                          : launch_tiles<true, false, B_MN, EPI>(tmA, tmB, tmC, a, num_sms, stream);
 }
 
 // an operand [rows][cols] of row pitch `pitch`, in boxes of 64 columns and `box` rows: 64 where it is read across the sum
 static bool operand_map(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, int64_t pitch, int box) {
   return make_tensor_map(tm, base, (uint64_t)cols, (uint64_t)rows, 1, (uint64_t)pitch, (uint64_t)pitch * rows, 64, (uint32_t)box);
 }
-// Rows of an operand that the CTAs of a pair bring per stage.  A single row tile brings no more than there are (whole
-// groups of 8, as the swizzle has them): what shared memory holds below is the product of rows that no one reads.
-static void single_tile_rows(VocabArgs &a) {
-  a.arows0 = a.arows1 = 128;
-  if (a.M <= 128) { a.arows0 = (a.M + 7) / 8 * 8; a.arows1 = 0; }
-}
+// Rows of the tokens' operand that a CTA brings per stage.  A small batch brings no more than there are (whole groups
+// of 8, as the swizzle has them): what shared memory holds below is the product of rows that no one reads.
+static int token_rows(int64_t n) { return small_batch(n) ? (int)(n + 7) / 8 * 8 : 128; }
+// Columns of a tile of logits that a CTA brings.
+static int word_rows(int64_t n, int nt) { return small_batch(n) ? nt : nt / 2; }
 
 static cudaError_t repitch(const uint16_t *in, int64_t rows, int64_t in_cols, uint16_t *out, int64_t out_cols, int num_sms, cudaStream_t stream) {
   return launch_after(vocab_pitch_kernel, elementwise_grid((rows * out_cols + 7) / 8, num_sms), 256, 0, stream, reinterpret_cast<const __half *>(in), rows,
@@ -663,13 +730,14 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
   VocabArgs a = {};
   a.M = (int)n; a.N = (int)v; a.kblocks = (int)ceil_div(p.dp, VK); a.splits = 1;
   a.nt = p.nt;
-  single_tile_rows(a);
-  if (!operand_map(&tmX, x, n, p.dp, p.dp, a.arows0) || !operand_map(&tmW, w, v, p.dp, p.dp, a.nt / 2)) return cudaErrorInvalidValue;
+  a.arows = token_rows(n);
+  a.halves = a.kblocks > V_ONE_SUM;
+  if (!operand_map(&tmX, x, n, p.dp, p.dp, a.arows) || !operand_map(&tmW, w, v, p.dp, p.dp, word_rows(n, a.nt))) return cudaErrorInvalidValue;
   a.targets = targets; a.v = (int)v; a.v0 = 0;
   a.part = reinterpret_cast<float2 *>(ws + p.part);
   a.ztarget = reinterpret_cast<float *>(ws + p.zt);
   a.failure = failure;
-  FB_TRY((launch_mma<false, false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
+  FB_TRY((launch_tokens<false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
   return launch_after(vocab_loss_kernel, (unsigned)ceil_div(n, 8), 256, 0, stream, a.part, (int)ceil_div(v, p.nt), a.ztarget, targets, loss, lse, n, v);
 }
 
@@ -697,10 +765,10 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     uint16_t *dwo = p.dp == d ? dw + v0 * d : reinterpret_cast<uint16_t *>(ws + p.dwp);
     VocabArgs a = {};
     a.M = (int)n;
-    single_tile_rows(a);
-    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, a.arows0) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, p.nt / 2) &&
+    a.arows = token_rows(n);
+    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, a.arows) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, word_rows(n, p.nt)) &&
                     make_tensor_map(&tmG, g, (uint64_t)vw, (uint64_t)n, 1, (uint64_t)p.piece, (uint64_t)p.piece * n, 64, 32) &&
-                    operand_map(&tmGk, g, n, vw, p.piece, a.arows0) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, 64) &&
+                    operand_map(&tmGk, g, n, vw, p.piece, a.arows) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, 64) &&
                     (p.direct ? make_tensor_map(&tmS, dxo, (uint64_t)p.dp, (uint64_t)n, 1, (uint64_t)p.dp, (uint64_t)(p.dp * n), 64, 32)
                               : make_tensor_map(&tmS, slabs, (uint64_t)p.dp, (uint64_t)n, (uint64_t)p.splits, (uint64_t)p.dp, (uint64_t)(p.dp * n), 32, 32, true)) &&
                     operand_map(&tmGm, g, n, vw, p.piece, 64) && operand_map(&tmXn, xs, n, p.dp, p.dp, 64) &&
@@ -710,18 +778,18 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     a.targets = targets; a.v = (int)v; a.v0 = (int)v0; a.cexp = cexp; a.factor = factor;
     a.splits = 1;
     a.N = (int)vw; a.kblocks = (int)ceil_div(p.dp, VK); a.nt = p.nt;
-    FB_TRY((launch_mma<false, false, VE_GRAD>(tmX, tmW, tmG, a, num_sms, stream)));
+    FB_TRY((launch_tokens<false, VE_GRAD>(tmX, tmW, tmG, a, num_sms, stream)));
     // every part has its blocks in every piece: the last one may be shorter, and then some slabs get nothing more
     a.N = (int)p.dp; a.kblocks = (int)ceil_div(vw, VK); a.nt = p.ntd;
     a.splits = (int)ceil_div(a.kblocks, ceil_div(a.kblocks, p.splits < a.kblocks ? p.splits : a.kblocks));
     a.add = v0 > 0;
     a.w = rw;
-    if (p.direct) FB_TRY((launch_mma<false, true, VE_ROWS>(tmGk, tmWn, tmS, a, num_sms, stream)));
-    else FB_TRY((launch_mma<false, true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
+    if (p.direct) FB_TRY((launch_tokens<true, VE_ROWS>(tmGk, tmWn, tmS, a, num_sms, stream)));
+    else FB_TRY((launch_tokens<true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
     a.M = (int)vw; a.N = (int)p.dp; a.kblocks = (int)ceil_div(n, VK); a.splits = 1; a.add = 0;
-    a.nt = tile_columns(vw, p.dp, 1, a.kblocks, 128, num_sms / 2);
-    a.arows0 = a.arows1 = 128;
-    FB_TRY((launch_mma<true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
+    a.nt = tile_columns(true, vw, p.dp, a.kblocks, 128, num_sms);
+    a.arows = 128;
+    FB_TRY((launch_tiles<true, true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
     if (p.dp != d) FB_TRY(repitch(dwo, vw, p.dp, dw + v0 * d, d, num_sms, stream));
   }
   if (p.direct) return p.dp == d ? cudaSuccess : repitch(dxo, n, p.dp, dx, d, num_sms, stream);

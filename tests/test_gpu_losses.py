@@ -46,7 +46,8 @@ def check_xent(ctx, X, W, ts, dl):
 
 @pytest.mark.parametrize("n,v,d", [
     (1, 256, 64), (256, 256, 64), (1, 1, 1), (2, 3, 5), (1, 1000, 64), (31, 257, 8), (129, 255, 72), (128, 513, 136), (257, 1000, 100),
-    (300, 700, 129), (5, 4097, 64), (1000, 300, 512), (64, 3001, 1000), (7, 20001, 64), (700, 1234, 63)])
+    (300, 700, 129), (5, 4097, 64), (1000, 300, 512), (64, 3001, 1000), (7, 20001, 64), (700, 1234, 63),
+    (128, 300, 2048), (40, 600, 2056), (300, 1000, 4100), (1, 40000, 2500), (130, 2100, 2112)])
 def test_vocab_xent_and_gradient(ctx, n, v, d):
     check_xent(ctx, *xent_inputs(n, v, d, n * 7 + v + d))
 
