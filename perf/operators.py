@@ -121,16 +121,23 @@ def _wrap(ctx, t):
     return ctx.new_raw("%s_%dd" % (name, t.dim()), t.data_ptr(), *t.shape)
 
 
+class _Result:
+    """An array of the context that goes back to it with the last tensor on its memory."""
+
+    def __init__(self, a):
+        self.array, self.__cuda_array_interface__ = a, a.__cuda_array_interface__
+
+    def __del__(self):
+        self.array.free()
+
+
 def _tensor(a):
-    """An array of the context as a tensor; the memory stays the array's."""
-    t = torch.as_tensor(a, device="cuda")
+    t = torch.as_tensor(_Result(a), device="cuda")
     return t.view(torch.float16) if t.dtype == torch.uint16 else t
 
 
 def _run_own(s):
     ctx = _context()
-    for a in s.pop("held", ()):          # the last step's results go back to the context
-        a.free()
     ins = []
 
     def arr(t):
@@ -152,7 +159,6 @@ def _run_own(s):
         out = out + (ctx.entry_router_balance_grad(s["t"], r, keep, out[1], out[2], arr(s["dl"])),)
     for a in ins:
         a.free()
-    s["held"] = out
     return tuple(_tensor(a) for a in out)
 
 
