@@ -112,10 +112,23 @@ __device__ __forceinline__ float group_max(const int4 &b, const __half *) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
-// (maximum in units of log 2, exactly what was subtracted; sum): the fold of two
-__device__ __forceinline__ void fold_pair(float &m, float &s, float om, float os) {
+// Maxima are kept in units in which what was subtracted from the logits is known exactly.  For binary16 that is log 2, the unit
+// of the exponents: x scale - m in one step.  For f32 it is the logit's own, (x - m) scale, since a logit of the type's lowest
+// value (a mask) times the scale would be no finite number.
+template <typename T> struct LogitUnit;
+template <> struct LogitUnit<__half> {
+  static __device__ __forceinline__ float of(float x, float scale) { return x * scale; }             // of a logit
+  static __device__ __forceinline__ float log2(float d, float) { return d; }                         // of a difference
+};
+template <> struct LogitUnit<float> {
+  static __device__ __forceinline__ float of(float x, float) { return x; }
+  static __device__ __forceinline__ float log2(float d, float scale) { return d * scale; }
+};
+// (maximum, sum): the fold of two
+template <typename T>
+__device__ __forceinline__ void fold_pair(float &m, float &s, float om, float os, float scale) {
   const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
-  s = s * exp2f(m - ref) + os * exp2f(om - ref);
+  s = s * exp2f(LogitUnit<T>::log2(m - ref, scale)) + os * exp2f(LogitUnit<T>::log2(om - ref, scale));
   m = mn;
 }
 
@@ -167,6 +180,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return a;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t x, y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
+  return a;
+}
+// exponents of 2 of two logits, relative to the reference whose negative is nr
+template <typename T> __device__ __forceinline__ float2 exponents(float2 x, float2 scale, float2 nr);
+template <> __device__ __forceinline__ float2 exponents<__half>(float2 x, float2 scale, float2 nr) { return fma2(x, scale, nr); }
+template <> __device__ __forceinline__ float2 exponents<float>(float2 x, float2 scale, float2 nr) { return mul2(add2(x, nr), scale); }
+
 // (maximum, sum) of every run.
 template <typename T>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
@@ -193,10 +219,10 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
       if (lane + 32 * i < d.groups) mx = fmaxf(mx, group_max(x[i], (const T *)nullptr));
-    mx = fmaxf(m, mx * scale);
+    mx = fmaxf(m, LogitUnit<T>::of(mx, scale));
     const float ref = mx == -INFINITY ? 0.f : mx;
     const float2 sc = make_float2(scale, scale), nr = make_float2(-ref, -ref);
-    float2 a = make_float2(sum * ex2_approx(m - ref), 0.f), b = make_float2(0.f, 0.f);
+    float2 a = make_float2(sum * ex2_approx(LogitUnit<T>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
     m = mx;
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
@@ -205,7 +231,7 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
         unpack(x[i], f);
 #pragma unroll
         for (int j = 0; j < W; j += 4) {
-          const float2 e = fma2(make_float2(f[j], f[j + 1]), sc, nr), g = fma2(make_float2(f[j + 2], f[j + 3]), sc, nr);
+          const float2 e = exponents<T>(make_float2(f[j], f[j + 1]), sc, nr), g = exponents<T>(make_float2(f[j + 2], f[j + 3]), sc, nr);
           a = add2(a, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
           b = add2(b, make_float2(ex2_approx(g.x), ex2_approx(g.y)));
         }
@@ -215,7 +241,7 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const float om = __shfl_xor_sync(kFull, m, o), os = __shfl_xor_sync(kFull, sum, o);
-        fold_pair(m, sum, om, os);
+        fold_pair<T>(m, sum, om, os, scale);
       }
       if (lane == 0) part[here.item] = make_float2(m, sum);
       m = -INFINITY;
@@ -237,8 +263,8 @@ __device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, i
     const float x = t[j];
     const bool in = is_word(c, x, v);
     wi[j] = in ? c : -1;
-    wq[j] = x * inv_tau;
-    if (in) m = fmaxf(m, x * inv_tau);
+    wq[j] = x;
+    if (in) m = fmaxf(m, x);
   }
   bool some = false;
 #pragma unroll
@@ -247,7 +273,7 @@ __device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, i
   for (int j = lane; j < k; j += 32)
     if (wi[j] >= 0) {
       some = true;
-      const float x = wq[j] - m, e = expf(x);
+      const float x = (wq[j] - m) * inv_tau, e = expf(x);
       wq[j] = LOG ? x : e;
       sum += e;
     }
@@ -262,7 +288,7 @@ __device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, i
 template <typename T>
 __global__ void __launch_bounds__(256)
 distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, const float *__restrict__ t, const float2 *__restrict__ part, int runs,
-                    int64_t n, int64_t v, int k, float tau, float *__restrict__ loss, float *__restrict__ lse) {
+                    int64_t n, int64_t v, int k, float tau, float scale, float *__restrict__ loss, float *__restrict__ lse) {
   extern __shared__ float sh[];                      // per warp: words [k], log q [k]
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -275,14 +301,14 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
   float m = -INFINITY, sum = 0.f;
   for (int p = lane; p < runs; p += 32) {
     const float2 q = part[row * runs + p];
-    fold_pair(m, sum, q.x, q.y);
+    fold_pair<T>(m, sum, q.x, q.y, scale);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, sum, o);
-    fold_pair(m, sum, pm, ps);
+    fold_pair<T>(m, sum, pm, ps, scale);
   }
-  const double l = ((double)m + log2((double)sum)) * L_LN2, inv_tau = 1.0 / (double)tau;
+  const double inv_tau = 1.0 / (double)tau, l = (double)m * (sizeof(T) == 2 ? L_LN2 : inv_tau) + log((double)sum);
   double total = 0;
   if (some) {
 #pragma unroll 4
@@ -305,9 +331,10 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
 // their weights and the others -1.  Which places those are is found without comparing all with all: in a round every
 // place that has not met its word yet writes itself into the word's slot of a hash table, and who then finds a place with its
 // own word there has met it (all places of a word do so in the same round, and in every slot someone does).
-// Per row: dl tau, whether there is a word, and exp(S / tau - lse) = 2^(S scale - hi) f, with hi + log f to more than 32 bits.
+// Per row: dl tau, whether there is a word, and the reference of its exponents with the factor that makes it exact: for binary16
+// exp(S / tau - lse) = 2^(S scale - hi) f, with hi + log f to more than 32 bits; for f32 lse itself, exp(S / tau - lse).
 __global__ void __launch_bounds__(256)
-distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__ t, int64_t n, int64_t v, int k, int table, float tau,
+distill_teacher_kernel(bool wide, const int32_t *__restrict__ is, const float *__restrict__ t, int64_t n, int64_t v, int k, int table, float tau,
                        const float *__restrict__ dl, const float *__restrict__ lse, int32_t *__restrict__ words, float *__restrict__ weights,
                        float4 *__restrict__ rows) {
   extern __shared__ float sh[];                      // per warp: words [k], weights [k], the place met [k], slots [table]
@@ -359,7 +386,7 @@ distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__
   if (lane == 0) {
     const double shift = (double)lse[row] * (1.0 / L_LN2);
     const float hi = (float)shift;
-    rows[row] = make_float4(dl[row] * tau, some ? 1.f : 0.f, hi, exp2f((float)((double)hi - shift)));
+    rows[row] = make_float4(dl[row] * tau, some ? 1.f : 0.f, wide ? lse[row] : hi, wide ? 1.f : exp2f((float)((double)hi - shift)));
   }
 }
 
@@ -367,6 +394,13 @@ distill_teacher_kernel(const int32_t *__restrict__ is, const float *__restrict__
 // of 1, 2, 4 and 16 chunks 131.5, 138, 142 and 147 us (f32, 2049 x 50001) and 377, 352, 362 and 388 us (binary16, 4096 x 131072,
 // where a chunk is twice the elements per instruction around them).
 template <typename T> constexpr int D_GRAD_RUN = sizeof(T) == 2 ? 2 : 1;
+
+// exponents of 2 of two logits less the row's reference, whose negative is nr: scale is log2 e / tau (binary16) or 1 / tau (f32)
+template <typename T> __device__ __forceinline__ float2 row_exponents(float2 x, float2 scale, float2 nr);
+template <> __device__ __forceinline__ float2 row_exponents<__half>(float2 x, float2 scale, float2 nr) { return fma2(x, scale, nr); }
+template <> __device__ __forceinline__ float2 row_exponents<float>(float2 x, float2 scale, float2 nr) {
+  return mul2(fma2(x, scale, nr), make_float2(L_LOG2E, L_LOG2E));
+}
 
 // Every chunk: the student's softmax; after a run the words of the teacher that lie in it once more.
 template <typename T>
@@ -407,7 +441,7 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
         unpack(x[i], y);
 #pragma unroll
         for (int j = 0; j < W; j += 2) {
-          const float2 e = fma2(make_float2(y[j], y[j + 1]), sc, nr);
+          const float2 e = row_exponents<T>(make_float2(y[j], y[j + 1]), sc, nr);
           y[j] = ex2_approx(e.x) * fc;
           y[j + 1] = ex2_approx(e.y) * fc;
         }
@@ -431,7 +465,7 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
         for (int j = lane; j < k; j += 32) {
           const int word = words[here.row * k + j];
           if (word >= 0 && word >= c0 && word < c1) {
-            const float p = ex2_approx(fmaf(to_f32<T>(r.base[word]), scale, -rc.z)) * rc.w;
+            const float xw = to_f32<T>(r.base[word]), p = ex2_approx(row_exponents<T>(make_float2(xw, xw), sc, nr).x) * rc.w;
             out[word] = from_f32<T>((p - weights[here.row * k + j]) * rc.x);
           }
         }
@@ -467,7 +501,7 @@ static cudaError_t distill(void *workspace, const T *s, const int32_t *is, const
   err = allow_smem(reinterpret_cast<const void *>(distill_loss_kernel<T>), 8 * 2 * DISTILL_MAX_K * 4, allowed);
   if (err != cudaSuccess) return err;
   return launch_after(distill_loss_kernel<T>, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream, s, is, t, part, d.runs, n, v, (int)k, tau,
-                      loss, lse);
+                      scale, loss, lse);
 }
 
 template <typename T>
@@ -479,14 +513,14 @@ static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, 
   int32_t *words = reinterpret_cast<int32_t *>(ws);
   float *weights = reinterpret_cast<float *>(ws + up256((size_t)(n * k) * 4));
   float4 *rows = reinterpret_cast<float4 *>(ws + 2 * up256((size_t)(n * k) * 4));
-  const float scale = (float)(1.0 / (L_LN2 * (double)tau));
+  const float scale = (float)(1.0 / ((sizeof(T) == 2 ? L_LN2 : 1.0) * (double)tau));
   int table = 32;
   while (table < 2 * k) table *= 2;
   const int rw = row_warps(n, num_sms);
   static unsigned long long allowed = 0;
   cudaError_t err = allow_smem(reinterpret_cast<const void *>(distill_teacher_kernel), 8 * (3 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4, allowed);
   if (err != cudaSuccess) return err;
-  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (3 * k + table) * 4, stream, is, t, n, v, (int)k, table, tau, dl,
+  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (3 * k + table) * 4, stream, sizeof(T) == 4, is, t, n, v, (int)k, table, tau, dl,
                      lse, words, weights, rows);
   if (err != cudaSuccess) return err;
   return launch_after(distill_grad_kernel<T>, chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream, s, n, v, d, scale, (int)k, words, weights, rows, ds);
@@ -575,17 +609,17 @@ template <typename T, int W, int J> struct RouterRow {
   }
 };
 // Logits to exp(logit - maximum), in place; returns the factor that makes them add up to 1 (0 in a row that is all -inf).
-// The maximum's product with log2 e is rounded, which the factor takes back.
+// The difference is taken first: a logit of the type's lowest value (a mask) times log2 e would be no finite number.
 template <int COLS>
 __device__ __forceinline__ float router_exp(float (&p)[COLS], int g) {
   float m = p[0];
 #pragma unroll
   for (int j = 1; j < COLS; j++) m = fmaxf(m, p[j]);
   m = lanes_max(m, g);
-  const float ref = m == -INFINITY ? 0.f : m * L_LOG2E;
+  const float ref = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < COLS; j++) { p[j] = ex2_approx(fmaf(p[j], L_LOG2E, -ref)); sum += p[j]; }
+  for (int j = 0; j < COLS; j++) { p[j] = ex2_approx((p[j] - ref) * L_LOG2E); sum += p[j]; }
   sum = lanes_sum(sum, g);
   return sum == 0.f ? 0.f : 1.f / sum;
 }

@@ -191,7 +191,7 @@ def check_distill(ctx, t, tau, S, iss, T, dl):
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("n,v,k,tau", [
     (1, 1, 1, 1.0), (3, 5, 2, 2.0), (17, 64, 8, 1.0), (9, 1001, 33, 0.5), (5, 8191, 64, 2.0), (4, 16385, 7, 4.0), (3, 50003, 128, 1.5),
-    (300, 257, 20, 3.0), (2, 70000, 1024, 1.0)])
+    (300, 257, 20, 3.0), (2, 70000, 1024, 1.0), (6, 70, 1024, 2.0), (20, 1500, 300, 1.0), (600, 3000, 9, 1.0), (1300, 4100, 5, 2.0)])
 def test_topk_distill_and_gradient(ctx, t, n, v, k, tau):
     check_distill(ctx, t, tau, *distill_inputs(t, n, v, k, n + v + k))
 
@@ -208,6 +208,10 @@ def test_topk_distill_rows_of_every_kind(ctx, t):
     iss[5] = [0, 1, 99, 5, 6, -1]
     S[6] = 0                                           # flat
     T[7] = [60000, 0, 0, -60000, 1, 2]                 # all of the weight on one word
+    iss[5, 5], T[5, 5] = 4099, np.nan                  # padding that holds anything
+    S[3, 50:] = np.finfo(S.dtype).min                  # words ruled out by the type's lowest value, in the student
+    iss[3] = [3, 4, 5, 6, 7, 8]
+    T[0, 4:] = np.finfo(np.float32).min                # and in the teacher
     S[7, iss[7, 3]] = -np.inf if iss[7, 3] not in (iss[7, 0], iss[7, 4], iss[7, 5]) else 0
     check_distill_special(ctx, t, 1.5, S, iss, T, dl)
 
@@ -222,6 +226,21 @@ def check_distill_special(ctx, t, tau, S, iss, T, dl):
     got = half(g) if t == "f16" else np.asarray(g, np.float64)
     within(got, wg, 1e-5 * mag + (ref.H * np.abs(wg) + ref.HMIN if t == "f16" else 1e-37), "dS")
     assert loss[1] == 0 and loss[2] == 0 and not got[1].any() and not got[2].any()
+
+
+def test_topk_distill_of_lowest_values_only(ctx):
+    """A teacher that gives every word the lowest value prefers none; a student's row of them has a finite lse (in f32, whose
+    steps there are far larger than the logarithm of the number of words)."""
+    S, iss, T, dl = distill_inputs("f32", 3, 300, 4, 8)
+    iss[:] = [1, 2, 3, 4]
+    T[:] = np.finfo(np.float32).min
+    S[1] = np.finfo(np.float32).min
+    loss, lse = fb.topk_distill(ctx, "f32", 1.0, S, iss, T)
+    assert np.isfinite(loss[[0, 2]]).all() and np.isfinite(lse).all() and lse[1] == np.finfo(np.float32).min
+    g = fb.topk_distill_grad(ctx, "f32", 1.0, S, iss, T, lse, dl)
+    want, mag = ref.topk_distill_grad(S, iss, T, 1.0, dl)
+    assert np.isfinite(g).all()
+    within(g[[0, 2]], want[[0, 2]], 1e-5 * mag[[0, 2]] + 1e-37, "dS")
 
 
 @pytest.mark.parametrize("t", ["f32", "f16"])
@@ -290,7 +309,8 @@ def test_router_balance_rows_of_every_kind(ctx, t):
     R, keep, iss = router_inputs(t, 40, 20, 3, 9)
     R[keep.nonzero()[0][0]] = -np.inf                  # every expert ruled out: no probability at all
     R[5, 3:] = -np.inf
-    R[6] = -60000
+    R[6] = np.finfo(R.dtype).min                       # ruled out by the type's lowest value: all alike
+    R[7, 1:] = np.finfo(R.dtype).min
     out = (~keep).nonzero()[0]
     R[out], iss[out] = np.nan, 1                       # padding does not count, whatever it holds
     iss[8] = [4, 4, 4]
@@ -355,15 +375,109 @@ def test_a_step_with_all_three_losses(ctx):
     assert np.array_equal(want[5], ref.router_balance(R, keep, ri)[1])
 
 
+def sampled(n, rows, seed):
+    import torch
+    return torch.randint(0, n, (rows,), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def borrowed(ctx, t):
+    import torch
+    name = {torch.float16: "f16", torch.float32: "f32", torch.int32: "i32", torch.bool: "bool"}[t.dtype]
+    return ctx.new_raw("%s_%dd" % (name, t.dim()), t.data_ptr(), *t.shape)
+
+
+def tensor(a):
+    import torch
+    t = torch.as_tensor(a, device="cuda")
+    return t.view(torch.float16) if t.dtype == torch.uint16 else t
+
+
+def test_topk_distill_beyond_32_bit_offsets(ctx):
+    """More than 2^32 logits: rows at both ends and between against 64 bits."""
+    import torch
+    n, v, k = 33000, 131100, 6
+    g = torch.Generator(device="cuda").manual_seed(3)
+    S = torch.empty(n, v, dtype=torch.float16, device="cuda")
+    for a in range(0, n, 1000):
+        S[a:a + 1000] = torch.randn(min(1000, n - a), v, device="cuda", generator=g).mul_(3)
+    iss = torch.randint(0, v, (n, k), device="cuda", generator=g).int()
+    T = torch.randn(n, k, device="cuda", generator=g)
+    dl = torch.full((n,), 64.0, device="cuda")
+    torch.cuda.synchronize()
+    ins = [borrowed(ctx, x) for x in (S, iss, T, dl)]
+    loss, lse = ctx.entry_topk_distill("f16", 2.0, *ins[:3])
+    grad = ctx.entry_topk_distill_grad("f16", 2.0, *ins[:3], lse, ins[3])
+    ctx.sync()
+    at = torch.cat([torch.tensor([0, 1, 16383, 16384, 32767, 32768, n - 2, n - 1]).cuda(), sampled(n, 30, 1)])
+    Sn, In, Tn, Dn = (x[at].cpu().numpy() for x in (S, iss, T, dl))
+    want, wantl, mag = ref.topk_distill(Sn, In, Tn, 2.0)
+    within(tensor(lse)[at].cpu().numpy(), wantl, 1e-5, "lse")
+    within(tensor(loss)[at].cpu().numpy(), want, 1e-5 * (1 + mag), "loss")
+    wg, mag = ref.topk_distill_grad(Sn, In, Tn, 2.0, Dn)
+    within(tensor(grad)[at].cpu().numpy(), wg, 1e-5 * mag + ref.H * np.abs(wg) + ref.HMIN, "dS")
+    for a in [loss, lse, grad] + ins:
+        a.free()
+    ctx.clear_caches()
+
+
+@pytest.mark.parametrize("n,v,d", [(9, 600000, 4096), (600000, 250, 4096)])
+def test_vocab_xent_beyond_32_bit_offsets(ctx, n, v, d):
+    """More than 2^31 weights, or hidden values: rows at both ends and between against 64 bits."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(4)
+
+    def half(rows, scale):
+        t = torch.empty(rows, d, dtype=torch.float16, device="cuda")
+        for a in range(0, rows, 20000):
+            t[a:a + 20000] = torch.randn(min(20000, rows - a), d, device="cuda", generator=gen).mul_(scale)
+        return t
+
+    X, W = half(n, 1.0), half(v, 2 / d ** 0.5)
+    ts = torch.randint(0, v, (n,), device="cuda", generator=gen).int()
+    ts[-1] = v - 1
+    few = sampled(n, 8, 2) if n > 100 else torch.arange(n).cuda()
+    few = torch.unique(torch.cat([few, torch.tensor([0, n - 1]).cuda()]))
+    dl = torch.zeros(n, device="cuda")
+    dl[few] = 64.0                                     # dW sums over all rows: all but these weigh nothing
+    torch.cuda.synchronize()
+    ins = [borrowed(ctx, x) for x in (X, W, ts, dl)]
+    loss, lse = ctx.entry_vocab_xent_f16(*ins[:3])
+    gx, gw = ctx.entry_vocab_xent_grad_f16(*ins[:3], loss, lse, ins[3])
+    ctx.sync()
+    x = X[few].double()
+    z = torch.cat([x @ W[a:a + 20000].double().T for a in range(0, v, 20000)], dim=1)
+    want = torch.logsumexp(z, dim=1)
+    p = torch.softmax(z, dim=1)
+    p[torch.arange(len(few)), ts[few].long()] -= 1
+    p *= 64
+    top = float(torch.cat([x.abs() @ W[a:a + 20000].abs().double().T for a in range(0, v, 20000)], dim=1).max())
+    err = 2 * (d / 16 + 2) * 2.0 ** -23 * top + 2.0 ** -20 * (1 + top)
+    within(tensor(lse)[few].cpu().numpy(), want.cpu().numpy(), err, "lse")
+    rows = torch.unique(torch.cat([torch.tensor([0, v // 2, v - 1]).cuda(), sampled(v, 40, 5), ts[few].long()]))
+    wx = sum(p[:, a:a + 20000] @ W[a:a + 20000].double() for a in range(0, v, 20000)).cpu().numpy()
+    ax = sum(p[:, a:a + 20000].abs() @ W[a:a + 20000].abs().double() for a in range(0, v, 20000)).cpu().numpy()
+    rel = 2 * ref.H + 4 * err + (n + v) / 16 * 2.0 ** -22        # roundings of G and of the result, the loss's error, the sums
+    within(tensor(gx)[few].cpu().numpy(), wx, rel * ax + ref.HMIN, "dX")
+    ww, aw = (p[:, rows].T @ x).cpu().numpy(), (p[:, rows].abs().T @ x.abs()).cpu().numpy()
+    within(tensor(gw)[rows].cpu().numpy(), ww, 2 * rel * aw + 64 * ref.HMIN, "dW")
+    for a in [loss, lse, gx, gw] + ins:
+        a.free()
+    ctx.clear_caches()
+
+
 def test_two_contexts_at_once(ctx):
     X, W, ts, dl = xent_inputs(600, 3000, 128, 41)
     want = fb.vocab_xent_f16(ctx, X, W, ts)
     with fb.Context() as other:
         a = [[c.new("f16_2d", X.view(np.uint16)), c.new("f16_2d", W.view(np.uint16)), c.new("i32_1d", ts)] for c in (ctx, other)]
-        outs = [c.entry_vocab_xent_f16(*b) for _ in range(4) for c, b in zip((ctx, other), a)]
+        g = [c.new("f32_1d", dl) for c in (ctx, other)]
+        outs = [(lambda o: o + c.entry_vocab_xent_grad_f16(*b, *o, d))(c.entry_vocab_xent_f16(*b)) for _ in range(4) for c, b, d in zip((ctx, other), a, g)]
+        want += fb.vocab_xent_grad_f16(ctx, X, W, ts, *want, dl)
         for o in outs:
-            assert np.array_equal(o[0].values(), want[0]) and np.array_equal(o[1].values(), want[1])
-            o[0].free(); o[1].free()
+            assert all(np.array_equal(x.values(), y) for x, y in zip(o, want))
+            for x in o:
+                x.free()
+        g[0].free(); g[1].free()
         for b in a:
             for x in b:
                 x.free()
