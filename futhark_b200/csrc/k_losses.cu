@@ -24,12 +24,6 @@ namespace fb {
 constexpr float L_LOG2E = 1.4426950408889634f;
 constexpr double L_LN2 = 0.69314718055994530942;
 
-__device__ __forceinline__ float ex2_approx(float x) {   // 2^x: at most 2 units in the last place off, 0 below 2^-126
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <typename T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
@@ -161,33 +155,6 @@ __device__ __forceinline__ void load_chunk(const DistillRow<T> &r, int chunk, in
   }
 }
 
-// two f32 products and sums in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t x, y, z;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(z) : "f"(c.x), "f"(c.y));
-  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(x) : "l"(y), "l"(z));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
-  return a;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t x, y;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
-  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
-  return a;
-}
-
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t x, y;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
-  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(x));
-  return a;
-}
 // exponents of 2 of two logits, relative to the reference whose negative is nr
 template <typename T> __device__ __forceinline__ float2 exponents(float2 x, float2 scale, float2 nr);
 template <> __device__ __forceinline__ float2 exponents<__half>(float2 x, float2 scale, float2 nr) { return fma2(x, scale, nr); }
@@ -222,7 +189,7 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
     mx = fmaxf(m, LogitUnit<T>::of(mx, scale));
     const float ref = mx == -INFINITY ? 0.f : mx;
     const float2 sc = make_float2(scale, scale), nr = make_float2(-ref, -ref);
-    float2 a = make_float2(sum * ex2_approx(LogitUnit<T>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
+    float2 a = make_float2(sum * ex2(LogitUnit<T>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
     m = mx;
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
@@ -232,8 +199,8 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
 #pragma unroll
         for (int j = 0; j < W; j += 4) {
           const float2 e = exponents<T>(make_float2(f[j], f[j + 1]), sc, nr), g = exponents<T>(make_float2(f[j + 2], f[j + 3]), sc, nr);
-          a = add2(a, make_float2(ex2_approx(e.x), ex2_approx(e.y)));
-          b = add2(b, make_float2(ex2_approx(g.x), ex2_approx(g.y)));
+          a = add2(a, make_float2(ex2(e.x), ex2(e.y)));
+          b = add2(b, make_float2(ex2(g.x), ex2(g.y)));
         }
       }
     sum = (a.x + a.y) + (b.x + b.y);
@@ -442,8 +409,8 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
 #pragma unroll
         for (int j = 0; j < W; j += 2) {
           const float2 e = row_exponents<T>(make_float2(y[j], y[j + 1]), sc, nr);
-          y[j] = ex2_approx(e.x) * fc;
-          y[j + 1] = ex2_approx(e.y) * fc;
+          y[j] = ex2(e.x) * fc;
+          y[j + 1] = ex2(e.y) * fc;
         }
         if (!some) {
 #pragma unroll
@@ -465,7 +432,7 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
         for (int j = lane; j < k; j += 32) {
           const int word = words[here.row * k + j];
           if (word >= 0 && word >= c0 && word < c1) {
-            const float xw = to_f32<T>(r.base[word]), p = ex2_approx(row_exponents<T>(make_float2(xw, xw), sc, nr).x) * rc.w;
+            const float xw = to_f32<T>(r.base[word]), p = ex2(row_exponents<T>(make_float2(xw, xw), sc, nr).x) * rc.w;
             out[word] = from_f32<T>((p - weights[here.row * k + j]) * rc.x);
           }
         }
@@ -619,7 +586,7 @@ __device__ __forceinline__ float router_exp(float (&p)[COLS], int g) {
   const float ref = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < COLS; j++) { p[j] = ex2_approx((p[j] - ref) * L_LOG2E); sum += p[j]; }
+  for (int j = 0; j < COLS; j++) { p[j] = ex2((p[j] - ref) * L_LOG2E); sum += p[j]; }
   sum = lanes_sum(sum, g);
   return sum == 0.f ? 0.f : 1.f / sum;
 }

@@ -85,12 +85,6 @@ struct VocabArgs {
   int *failure;
 };
 
-__device__ __forceinline__ float ex2(float x) {        // 2^x: at most 2 units in the last place off, 0 below 2^-126
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 constexpr int V_MAX_STAGES = 8;
 struct VocabBarriers {
   uint64_t full[V_MAX_STAGES];   // used in the pair's first CTA only
@@ -134,6 +128,9 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const uint32_t num_tiles = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n * (uint32_t)a.splits;     // below 2^31
 
   if (tid == 0) {
+    prefetch_map(&tmA);
+    prefetch_map(&tmB);
+    if (EPI != VE_SOFTMAX) prefetch_map(&tmC);
     for (int s = 0; s < V_STAGES; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
     for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], (PAIR ? 2 : 1) * V_WARPS); }
     for (int i = 0; i < 8; i++) mbar_init(&bars->met[i >> 2][i & 3], V_WARPS / 4 - 1);
@@ -299,10 +296,16 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * V_LOG2E;
           const float mn = fmaxf(m2, cm);
           const float ref = mn == -INFINITY ? 0.f : mn;    // a row of -inf so far: the sum stays 0
-          float s4[4] = {sum * ex2(m2 - ref), 0.f, 0.f, 0.f};
+          const float2 scale = make_float2(V_LOG2E, V_LOG2E), nr = make_float2(-ref, -ref);
+          float2 s0 = make_float2(sum * ex2(m2 - ref), 0.f), s1 = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int j = 0; j < 32; j++) s4[j & 3] += ex2(fmaf(__uint_as_float(v[j]), V_LOG2E, -ref));
-          sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          for (int j = 0; j < 32; j += 4) {
+            const float2 e = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale, nr);
+            const float2 f = fma2(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), scale, nr);
+            s0 = add2(s0, make_float2(ex2(e.x), ex2(e.y)));
+            s1 = add2(s1, make_float2(ex2(f.x), ex2(f.y)));
+          }
+          sum = (s0.x + s0.y) + (s1.x + s1.y);
           m2 = mn;
           const int tj = tcol - c0;
           if (tj >= 0 && tj < 32) {
@@ -314,29 +317,33 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         };
         // 32 columns of G (or of the scaled product) as 16 pairs of binary16
         auto to_half = [&](const uint32_t (&v)[32], int c0, uint32_t (&h)[16]) {
-          float f[32];
+          const bool none = (EPI == VE_GRAD || EPI == VE_ROWS) && !counts;
+          const float2 by = EPI == VE_GRAD ? make_float2(V_LOG2E, V_LOG2E) : EPI == VE_ROWS ? make_float2(c, c) : make_float2(factor, factor);
+          const __half2 most = __float2half2_rn(65504.f);
 #pragma unroll
-          for (int j = 0; j < 32; j++) {
+          for (int j = 0; j < 16; j++) {
+            float2 f = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+            __half2 p;
             if (EPI == VE_GRAD) {
-              const float e = ex2(fmaf(__uint_as_float(v[j]), V_LOG2E, c));
-              f[j] = e > 65504.f ? 65504.f : e;            // NaN stays
-            } else if (EPI == VE_ROWS) {
-              f[j] = __uint_as_float(v[j]) * (1.f / V_GSCALE) * c;
+              f = fma2(f, by, make_float2(c, c));
+              p = __hmin2_nan(__floats2half2_rn(ex2(f.x), ex2(f.y)), most);        // NaN stays
             } else {
-              f[j] = __uint_as_float(v[j]) * factor;
+              if (EPI == VE_ROWS) f = mul2(f, make_float2(1.f / V_GSCALE, 1.f / V_GSCALE));
+              f = mul2(f, by);
+              p = __floats2half2_rn(f.x, f.y);
             }
+            h[j] = none ? 0u : *reinterpret_cast<const uint32_t *>(&p);
           }
           if (EPI == VE_GRAD) {
             const int tj = tcol - c0;
-            if (tj >= 0 && tj < 32) {
+            if (tj >= 0 && tj < 32) {                      // the target's, exactly
+              const uint32_t g = __half_as_ushort(__float2half_rn(-V_GSCALE));
 #pragma unroll
-              for (int j = 0; j < 32; j++) if (j == tj) f[j] = -V_GSCALE;
+              for (int j = 0; j < 16; j++) {
+                if (tj == 2 * j) h[j] = (h[j] & 0xffff0000u) | g;
+                if (tj == 2 * j + 1) h[j] = (h[j] & 0x0000ffffu) | (g << 16);
+              }
             }
-          }
-#pragma unroll
-          for (int j = 0; j < 16; j++) {
-            const __half2 p = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-            h[j] = ((EPI == VE_GRAD || EPI == VE_ROWS) && !counts) ? 0u : *reinterpret_cast<const uint32_t *>(&p);
           }
         };
         // 128 bytes of a row are staged as the 128-byte swizzle wants them (16-byte piece q of row r at q ^ (r & 7))

@@ -20,6 +20,9 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *tm, const void *
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                ::"l"(tm), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *tm) {      // the descriptor, before the first copy needs it
+  asm volatile("prefetch.tensormap [%0];" ::"l"(tm) : "memory");
+}
 __device__ __forceinline__ void tmem_alloc(uint32_t *smem_slot, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                ::"r"(smem_u32(smem_slot)), "r"(ncols) : "memory");
