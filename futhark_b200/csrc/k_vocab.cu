@@ -445,7 +445,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (PAIR) cluster_sync_all();                        // nobody signals into a partner that has left
+  if (PAIR) cluster_meet();                            // nobody signals into a partner that has left
   if (warp == 1) {
     tc_fence_after();
     if (!PAIR) tmem_dealloc(tmem_base, 512);

@@ -90,6 +90,11 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same where nothing but arrival matters: no memory access is ordered by it.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 // bulk tensor copy into this CTA's shared memory whose completion is counted by a barrier given by
 // its cluster address (it may be the partner's)
 __device__ __forceinline__ void tma_load_3d_pair(void *smem_dst, const CUtensorMap *tm, int x, int y, int z, uint32_t bar_cluster_addr) {

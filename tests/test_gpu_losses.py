@@ -299,7 +299,7 @@ def check_router(ctx, t, R, keep, iss, dl):
 @pytest.mark.parametrize("t", ["f32", "f16"])
 @pytest.mark.parametrize("n,e,k", [
     (1, 1, 1), (1, 2, 1), (5, 3, 2), (16, 8, 2), (100, 31, 4), (333, 32, 4), (333, 33, 6), (1000, 60, 4), (777, 64, 8), (500, 100, 3),
-    (2000, 256, 8), (300, 300, 16), (100, 513, 8), (64, 1024, 32), (20000, 5, 5), (9000, 160, 6)])
+    (2000, 256, 8), (300, 300, 16), (100, 513, 8), (64, 1024, 32), (20000, 5, 5), (9000, 160, 6), (70001, 8, 2), (30011, 100, 12), (20003, 256, 40)])
 def test_router_balance_and_gradient(ctx, t, n, e, k):
     check_router(ctx, t, *router_inputs(t, n, e, k, n + e + k), 100.0 if t == "f16" else 0.01)
 
@@ -316,6 +316,29 @@ def test_router_balance_rows_of_every_kind(ctx, t):
     iss[8] = [4, 4, 4]
     iss[9] = [-1, 20, 2**31 - 1]
     check_router(ctx, t, R, keep, iss, 3.0)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("n,e,shift", [(3000, 64, 1), (3000, 64, 2), (700, 63, 3), (2500, 256, 4), (999, 1000, 1), (4001, 12, 2)])
+def test_router_balance_rows_at_any_address(ctx, t, n, e, shift):
+    R, keep, iss = router_inputs(t, n, e, min(4, e), n + e)
+    loss, counts, norm = fb.router_balance(ctx, t, R, keep, iss)
+    want = fb.router_balance_grad(ctx, t, R, keep, counts, norm, np.ones(1, np.float32))
+    raw = fb._bits(R).ravel()
+    base = ctx.new(t + "_1d", np.concatenate([np.zeros(shift, raw.dtype), raw]))
+    r = ctx.new_raw(t + "_2d", base.raw + shift * raw.itemsize, n, e)
+    k, i, d = ctx.new("bool_1d", keep), ctx.new("i32_2d", iss), ctx.new("f32_1d", np.ones(1, np.float32))
+    l, c, m = ctx.entry_router_balance(t, r, k, i)
+    g = ctx.entry_router_balance_grad(t, r, k, c, m, d)
+    assert np.array_equal(c.values(), counts) and np.array_equal(m.values(), norm)
+    assert np.allclose(l.values(), loss, rtol=1e-6)
+    # rows are shared out differently among lanes: sums associate differently
+    if t == "f32":
+        assert np.allclose(g.values(), want, rtol=1e-5, atol=1e-6 * np.abs(want).max())
+    else:
+        assert np.allclose(half(g.values()), half(want), rtol=2.0 ** -9, atol=2.0 ** -24)
+    for a in (g, l, c, m, d, i, k, r, base):
+        a.free()
 
 
 @pytest.mark.parametrize("keep,expert", [(False, 0), (True, -1)])
