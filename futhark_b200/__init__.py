@@ -320,8 +320,6 @@ _type_fns = _TypeTable()
 class Array:
     """A device array owned by a context (struct futhark_<t>_<n>d *)."""
 
-    __slots__ = ("ctx", "tname", "ptr", "_interface", "_keepalive", "__weakref__")
-
     def __init__(self, ctx, tname, ptr):
         self.ctx = ctx
         self.tname = tname
@@ -511,7 +509,7 @@ class Context:
         return arr
 
     def new_raw(self, tname, devptr, *shape):
-        p = _type_fns[tname].new_raw(self.ptr, devptr, *shape)
+        p = _type_fns[tname].new_raw(self.ptr, int(devptr), *shape)
         if not p:
             raise FutharkError(1, self.get_error() or "futhark_new_raw_%s failed" % tname)
         return Array(self, tname, p)

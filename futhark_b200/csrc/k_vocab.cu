@@ -270,9 +270,9 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         int tcol = -1;                                     // the target's column in this tile, if it has it
         const float c = next_c;
         const bool counts = next_target >= 0 && next_target < a.v && row < a.M;
-        if (EPI == VE_SOFTMAX || EPI == VE_GRAD) {
+        if ((EPI == VE_SOFTMAX || EPI == VE_GRAD) && counts) {
           const int tl = next_target - a.v0 - n0;
-          if (counts && tl >= 0 && tl < ncols) tcol = tl;
+          if (tl >= 0 && tl < ncols) tcol = tl;
         }
         const int this_split = split, this_tn = tn;
         if (!__all_sync(kFull, mbar_wait_bounded(&bars->tmem_full[acc], acc_ph))) { ok = false; break; }
