@@ -538,21 +538,43 @@ vocab_prep_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const int
   }
 }
 
-// Rows of another pitch, what is behind the narrower of the two 0 or left out; 8 elements of the result per thread.
+// Rows of up to two matrices in another pitch, what is behind the narrower of the two 0 or left out; 8 elements of a result per thread.
+struct PitchJob {
+  const __half *in;
+  __half *out;
+  int64_t rows;
+};
 __global__ void __launch_bounds__(256)
-vocab_pitch_kernel(const __half *__restrict__ in, int64_t rows, int64_t in_cols, __half *__restrict__ out, int64_t out_cols) {
-  const int64_t total = rows * out_cols;
+vocab_pitch_kernel(const PitchJob a, const PitchJob b, int64_t in_cols, int64_t out_cols) {
+  const int64_t first = (a.rows * out_cols + 7) / 8, groups = first + (b.rows * out_cols + 7) / 8;
   chain_wait();
-  for (int64_t o = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; o < total; o += (int64_t)gridDim.x * 2048) {
-    int64_t i = o / out_cols, c = o - i * out_cols;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < groups; at += (int64_t)gridDim.x * 256) {
+    const PitchJob &job = at < first ? a : b;
+    const int64_t o = (at < first ? at : at - first) * 8, total = job.rows * out_cols;
+    int64_t i = total < (1ll << 32) ? (int64_t)((uint32_t)o / (uint32_t)out_cols) : o / out_cols, c = o - i * out_cols;
     __align__(16) __half h[8];
+    const int64_t src = i * in_cols + c;
+    if (c + 8 <= in_cols && c + 8 <= out_cols && src > 0 && src + 9 <= job.rows * in_cols) {
+      // 8 neighbours from any place: the words they lie in, shifted by half a word where they start in the middle of one
+      const uint32_t *w = reinterpret_cast<const uint32_t *>((uintptr_t)(job.in + src) & ~(uintptr_t)3);
+      const bool odd = ((uintptr_t)(job.in + src) & 2) != 0;
+      uint32_t *hw = reinterpret_cast<uint32_t *>(h);
+      uint32_t lo = w[0];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      h[j] = c < in_cols && o + j < total ? in[i * in_cols + c] : __half(0.f);
-      if (++c == out_cols) { c = 0; i++; }
+      for (int j = 0; j < 4; j++) {
+        const uint32_t next = j < 3 || odd ? w[j + 1] : 0u;
+        hw[j] = odd ? __funnelshift_r(lo, next, 16) : lo;
+        lo = next;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        h[j] = c < in_cols && o + j < total ? job.in[i * in_cols + c] : __half(0.f);
+        if (++c == out_cols) { c = 0; i++; }
+      }
     }
-    if (o + 8 <= total && ((uintptr_t)(out + o) & 15) == 0) *reinterpret_cast<uint4 *>(out + o) = *reinterpret_cast<const uint4 *>(h);
-    else for (int j = 0; j < 8 && o + j < total; j++) out[o + j] = h[j];
+    if (o + 8 <= total && ((uintptr_t)(job.out + o) & 15) == 0) *reinterpret_cast<uint4 *>(job.out + o) = *reinterpret_cast<const uint4 *>(h);
+    else for (int j = 0; j < 8 && o + j < total; j++) job.out[o + j] = h[j];
   }
 }
 
@@ -634,11 +656,11 @@ static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int num_sms, int *n
   const int64_t workers = pair ? num_sms / 2 : num_sms;
   for (int w = VT; w >= 128; w -= 128) {
     const int64_t tiles = ceil_div(n, pair ? 256 : 128) * ceil_div(dp, w);
-    for (int s = 1; s <= 128 && s <= kblocks; s++) {
-      const int64_t kps = ceil_div(kblocks, s);
-      if (ceil_div(kblocks, kps) != s) continue;
+    const int most = (int)(kblocks < 128 ? kblocks : 128);
+    for (int want = 1; want <= most && (want == 1 || tiles * want < 4 * workers); want += 1 + want / 8) {
+      const int64_t kps = ceil_div(kblocks, want), s = ceil_div(kblocks, kps);      // parts that all have something to add
       const double cost = (double)ceil_div(tiles * s, workers) * (kps * block_clocks(pair, w) + 3000.0) + (s > 1 ? 6000.0 + (double)s * n * dp * 8 / 3600.0 : 0.0);
-      if ((s == 1 && w == VT) || cost < best_cost) { best = s; *nt = w; best_cost = cost; }
+      if ((want == 1 && w == VT) || cost < best_cost) { best = (int)s; *nt = w; best_cost = cost; }
     }
   }
   return best;
@@ -717,9 +739,22 @@ static int token_rows(int64_t n) { return small_batch(n) ? (int)(n + 7) / 8 * 8 
 // Columns of a tile of logits that a CTA brings.
 static int word_rows(int64_t n, int nt) { return small_batch(n) ? nt : nt / 2; }
 
-static cudaError_t repitch(const uint16_t *in, int64_t rows, int64_t in_cols, uint16_t *out, int64_t out_cols, int num_sms, cudaStream_t stream) {
-  return launch_after(vocab_pitch_kernel, elementwise_grid((rows * out_cols + 7) / 8, num_sms), 256, 0, stream, reinterpret_cast<const __half *>(in), rows,
-                      in_cols, reinterpret_cast<__half *>(out), out_cols);
+static PitchJob pitch_job(const uint16_t *in, uint16_t *out, int64_t rows) {
+  return {reinterpret_cast<const __half *>(in), reinterpret_cast<__half *>(out), rows};
+}
+static cudaError_t repitch(const PitchJob &a, const PitchJob &b, int64_t in_cols, int64_t out_cols, int num_sms, cudaStream_t stream) {
+  const int64_t groups = ((a.rows + b.rows) * out_cols + 7) / 8;
+  if (groups <= 0) return cudaSuccess;
+  return launch_after(vocab_pitch_kernel, elementwise_grid(groups, num_sms), 256, 0, stream, a, b, in_cols, out_cols);
+}
+// The operands where the tensor cores can read them.
+static cudaError_t operands(const VocabPlan &p, uint8_t *ws, const uint16_t *&x, const uint16_t *&w, int64_t n, int64_t v, int64_t d, int num_sms,
+                            cudaStream_t stream) {
+  uint16_t *xp = reinterpret_cast<uint16_t *>(ws + p.xp), *wp = reinterpret_cast<uint16_t *>(ws + p.wp);
+  const cudaError_t err = repitch(pitch_job(x, xp, p.copy_x ? n : 0), pitch_job(w, wp, p.copy_w ? v : 0), d, p.dp, num_sms, stream);
+  if (p.copy_x) x = xp;
+  if (p.copy_w) w = wp;
+  return err;
 }
 
 #define FB_TRY(e) do { const cudaError_t fb_err = (e); if (fb_err != cudaSuccess) return fb_err; } while (0)
@@ -731,8 +766,7 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
     return launch_after(vocab_fill_kernel, elementwise_grid(n, num_sms), 256, 0, stream, loss, lse, n, -INFINITY);
   }
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
-  if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
-  if (p.copy_w) { FB_TRY(repitch(w, v, d, reinterpret_cast<uint16_t *>(ws + p.wp), p.dp, num_sms, stream)); w = reinterpret_cast<uint16_t *>(ws + p.wp); }
+  FB_TRY(operands(p, ws, x, w, n, v, d, num_sms, stream));
   CUtensorMap tmX, tmW;
   VocabArgs a = {};
   a.M = (int)n; a.N = (int)v; a.kblocks = (int)ceil_div(p.dp, VK); a.splits = 1;
@@ -760,8 +794,7 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
   float *rw = reinterpret_cast<float *>(ws + p.w), *cexp = reinterpret_cast<float *>(ws + p.cexp), *slabs = reinterpret_cast<float *>(ws + p.slabs);
   float *factor = reinterpret_cast<float *>(ws + p.scalars);
   uint16_t *xs = reinterpret_cast<uint16_t *>(ws + p.xs), *g = reinterpret_cast<uint16_t *>(ws + p.g);
-  if (p.copy_x) { FB_TRY(repitch(x, n, d, reinterpret_cast<uint16_t *>(ws + p.xp), p.dp, num_sms, stream)); x = reinterpret_cast<uint16_t *>(ws + p.xp); }
-  if (p.copy_w) { FB_TRY(repitch(w, v, d, reinterpret_cast<uint16_t *>(ws + p.wp), p.dp, num_sms, stream)); w = reinterpret_cast<uint16_t *>(ws + p.wp); }
+  FB_TRY(operands(p, ws, x, w, n, v, d, num_sms, stream));
   const int64_t row_ctas = ceil_div(n, 32);
   FB_TRY(launch_after(vocab_prep_kernel, (unsigned)(row_ctas < 2 * num_sms ? row_ctas : 2 * num_sms), 1024, 0, stream, reinterpret_cast<const __half *>(x), n,
                       p.dp, targets, v, loss, lse, dl, rw, cexp, factor, reinterpret_cast<__half *>(xs)));
@@ -797,9 +830,12 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     a.nt = tile_columns(true, vw, p.dp, a.kblocks, 128, num_sms);
     a.arows = 128;
     FB_TRY((launch_tiles<true, true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
-    if (p.dp != d) FB_TRY(repitch(dwo, vw, p.dp, dw + v0 * d, d, num_sms, stream));
+    if (p.dp != d) {                               // and with the last piece's a finished dX
+      const bool both = p.direct && v0 + vw == v;
+      FB_TRY(repitch(pitch_job(dwo, dw + v0 * d, vw), pitch_job(dxo, dx, both ? n : 0), p.dp, d, num_sms, stream));
+    }
   }
-  if (p.direct) return p.dp == d ? cudaSuccess : repitch(dxo, n, p.dp, dx, d, num_sms, stream);
+  if (p.direct) return cudaSuccess;
   return launch_after(vocab_dx_kernel, elementwise_grid(n * p.dp / 4, num_sms), 256, 0, stream, slabs, p.splits, n, d, p.dp, targets, v, rw,
                       reinterpret_cast<__half *>(dx));
 }
