@@ -559,3 +559,47 @@ def test_records_share_their_fields(ctx, rec, types):
         assert np.array_equal(got.values(), want)
         got.free()
     assert getattr(ctx.lib, "futhark_free_" + rec)(ctx.ptr, obj) == 0
+
+
+def test_server_session_through_all_losses(tmp_path):
+    """The server front-end: values of the new types from a file, every loss with its gradient, fields of the records stored."""
+    from futhark_b200 import build
+    from test_cli import ServerProc
+    X, W, ts, dl = xent_inputs(20, 60, 16, 51)
+    S, si, T, ddl = distill_inputs("f16", 20, 50, 3, 52)
+    R, keep, ri = router_inputs("f32", 20, 6, 2, 53)
+    values = [("x", "f16", X.view(np.uint16)), ("w", "f16", W.view(np.uint16)), ("t", "i32", ts), ("g", "f32", dl),
+              ("s", "f16", S.view(np.uint16)), ("i", "i32", si), ("q", "f32", T), ("sg", "f32", ddl), ("tau", "f32", np.float32(2)),
+              ("r", "f32", R), ("k", "bool", keep), ("e", "i32", ri), ("rg", "f32", np.ones(1, np.float32))]
+    f = tmp_path / "in.dat"
+    f.write_bytes(b"\n".join(fb.value_to_bytes(v, t, True) for _, t, v in values))
+    srv = ServerProc(build.SERVER_BIN)
+    srv.ok("restore %s %s" % (f, " ".join("%s %s%s" % (n, "[]" * np.ndim(v), t) for n, t, v in values)))
+    srv.ok("call vocab_xent_f16 a x w t")
+    for i in range(2):
+        srv.ok("project a%d a %d" % (i, i))
+    srv.ok("call vocab_xent_grad_f16 b x w t a0 a1 g")
+    srv.ok("project b0 b 0")
+    srv.ok("call topk_distill_f16 c tau s i q")
+    srv.ok("project c1 c 1")
+    srv.ok("call topk_distill_grad_f16 d tau s i q c1 sg")
+    srv.ok("call router_balance_f32 h r k e")
+    for i in range(3):
+        srv.ok("project h%d h %d" % (i, i))
+    srv.ok("call router_balance_grad_f32 m r k h1 h2 rg")
+    assert srv.ok('fields "([]f32, []i32, []f32)"') == ["0 []f32", "1 []i32", "2 []f32"]
+    o = tmp_path / "out.dat"
+    srv.ok("store %s a0 b0 d h1 m" % o)
+    srv.close()
+    raw, got = o.read_bytes(), []
+    for t, rank in (("f32", 1), ("f16", 2), ("f16", 2), ("i32", 1), ("f32", 2)):
+        v, used = fb.value_from_bytes(raw, t, rank)
+        got.append(v)
+        raw = raw[used:]
+    within(got[0], ref.vocab_xent(X, W, ts)[0], 2 * ref.vocab_xent_error(X, W, ts), "loss")
+    within(half(got[1]), ref.vocab_xent_grad(X, W, ts, dl)[0], ref.vocab_xent_grad_error(X, W, ts, dl)[0], "dX")
+    wg, mag = ref.topk_distill_grad(S, si, T, 2.0, ddl)
+    within(half(got[2]), wg, 1e-5 * mag + ref.H * np.abs(wg) + ref.HMIN, "dS")
+    assert np.array_equal(got[3], ref.router_balance(R, keep, ri)[1])
+    wg, mag = ref.router_balance_grad(R, keep, ri, 1.0)
+    within(got[4], wg, 2.0 ** -19 * mag + 1e-37, "dR")
