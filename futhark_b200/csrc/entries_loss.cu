@@ -102,7 +102,7 @@ int futhark_entry_vocab_xent_f16(struct futhark_context *ctx, losses_t **out0, c
   void *ws = call.workspace(plan.bytes, "vocab_xent_f16.workspace");
   call.launch("vocab_xent_f16.segred", "map2 (\\x t -> log (sum (map exp (map (dot x) W))) - dot x W[t]) X ts", [&] { return vocab_details(n, v, d); }, [&] {
     ctx->failure_is_an_option = true;
-    return fb::launch_vocab_xent(plan, ws, dptr<uint16_t>(in0->mem), dptr<uint16_t>(in1->mem), dptr<int32_t>(in2->mem), dptr<float>(loss->mem),
+    return fb::launch_vocab_xent(plan, ws, ctx->reduce_scratch, dptr<uint16_t>(in0->mem), dptr<uint16_t>(in1->mem), dptr<int32_t>(in2->mem), dptr<float>(loss->mem),
                                  dptr<float>(lse->mem), n, v, d, ctx->d_failure, ctx->num_sms, ctx->stream);
   });
   if (call.rc != FUTHARK_SUCCESS) return call.rc;
@@ -160,7 +160,7 @@ static int topk_distill(futhark_context *ctx, const char *name, int elem, losses
   auto *rec = call.record<losses_t>();
   void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), n, v, k, elem, false, ctx->num_sms), "topk_distill.workspace");
   call.launch(name, "map3 (\\s is t -> tau**2 * sum (map2 (\\q i -> q * (log q - s[i]/tau + lse s)) (softmax t) is)) S iss T", [&] { return distill_details(n, v, k); }, [&] {
-    return fb::launch_topk_distill(ws, elem, dptr<void>(s->mem), dptr<int32_t>(is->mem), dptr<float>(t->mem), tau, n, v, k, dptr<float>(loss->mem),
+    return fb::launch_topk_distill(ws, ctx->reduce_scratch, elem, dptr<void>(s->mem), dptr<int32_t>(is->mem), dptr<float>(t->mem), tau, n, v, k, dptr<float>(loss->mem),
                                    dptr<float>(lse->mem), ctx->num_sms, ctx->stream);
   });
   if (call.rc != FUTHARK_SUCCESS) return call.rc;
@@ -230,7 +230,7 @@ static int router_balance(futhark_context *ctx, const char *name, int elem, bala
   void *ws = call.workspace(fb::router_workspace_bytes(dptr<void>(r->mem), elem, n, e, ctx->num_sms), "router_balance.workspace");
   call.launch(name, "(norm * sum (map2 (*) counts (reduce (map2 (+)) (map softmax R))), hist (+) 0 e is, norm)",
               [&] { return "{" + kv("n", n) + "," + kv("e", e) + "," + kv("k", k) + "}"; }, [&] {
-    return fb::launch_router_balance(ws, elem, dptr<void>(r->mem), dptr<uint8_t>(keep->mem), dptr<int32_t>(is->mem), n, e, k, dptr<float>(loss->mem),
+    return fb::launch_router_balance(ws, ctx->reduce_scratch, elem, dptr<void>(r->mem), dptr<uint8_t>(keep->mem), dptr<int32_t>(is->mem), n, e, k, dptr<float>(loss->mem),
                                      dptr<int32_t>(counts->mem), dptr<float>(norm->mem), ctx->num_sms, ctx->stream);
   });
   if (call.rc != FUTHARK_SUCCESS) return call.rc;

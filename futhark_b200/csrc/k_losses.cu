@@ -160,63 +160,6 @@ template <typename T> __device__ __forceinline__ float2 exponents(float2 x, floa
 template <> __device__ __forceinline__ float2 exponents<__half>(float2 x, float2 scale, float2 nr) { return fma2(x, scale, nr); }
 template <> __device__ __forceinline__ float2 exponents<float>(float2 x, float2 scale, float2 nr) { return mul2(add2(x, nr), scale); }
 
-// (maximum, sum) of every run.
-template <typename T>
-__global__ void __launch_bounds__(D_THREADS, D_CTAS)
-distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, float2 *__restrict__ part) {
-  constexpr int W = 16 / (int)sizeof(T);
-  const int lane = threadIdx.x & 31;
-  const int64_t items = n * d.runs, step = (int64_t)gridDim.x * D_WARPS;
-  const bool small = items < (1ll << 31);
-  DistillAt at;
-  at.item = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
-  at.start(items, d, small);
-  chain_wait();
-  int4 next[D_PER];
-  if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
-  float m = -INFINITY, sum = 0.f;
-  while (at.item < items) {
-    int4 x[D_PER];
-#pragma unroll
-    for (int i = 0; i < D_PER; i++) x[i] = next[i];
-    const DistillAt here = at;
-    at.next(items, step, d, small);
-    if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < D_PER; i++)
-      if (lane + 32 * i < d.groups) mx = fmaxf(mx, group_max(x[i], (const T *)nullptr));
-    mx = fmaxf(m, LogitUnit<T>::of(mx, scale));
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    const float2 sc = make_float2(scale, scale), nr = make_float2(-ref, -ref);
-    float2 a = make_float2(sum * ex2(LogitUnit<T>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
-    m = mx;
-#pragma unroll
-    for (int i = 0; i < D_PER; i++)
-      if (lane + 32 * i < d.groups) {
-        float f[W];
-        unpack(x[i], f);
-#pragma unroll
-        for (int j = 0; j < W; j += 4) {
-          const float2 e = exponents<T>(make_float2(f[j], f[j + 1]), sc, nr), g = exponents<T>(make_float2(f[j + 2], f[j + 3]), sc, nr);
-          a = add2(a, make_float2(ex2(e.x), ex2(e.y)));
-          b = add2(b, make_float2(ex2(g.x), ex2(g.y)));
-        }
-      }
-    sum = (a.x + a.y) + (b.x + b.y);
-    if (here.chunk + 1 == here.last) {               // the lanes meet
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(kFull, m, o), os = __shfl_xor_sync(kFull, sum, o);
-        fold_pair<T>(m, sum, om, os, scale);
-      }
-      if (lane == 0) part[here.item] = make_float2(m, sum);
-      m = -INFINITY;
-      sum = 0.f;
-    }
-  }
-}
-
 __device__ __forceinline__ bool is_word(int32_t c, float t, int64_t v) { return c >= 0 && c < v && t != -INFINITY; }
 
 // The teacher's softmax of a row over its words, by one warp in shared memory: its words (-1: padding), and log q or q.  The lanes
@@ -251,31 +194,33 @@ __device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, i
   return __any_sync(kFull, some);
 }
 
-// One warp per row: fold of the runs, and the loss over the teacher's words (in f64: its terms cancel).
+// The loss of a row by one warp, over the teacher's words (in f64: its terms cancel), after the fold of the row's runs, eight per lane in flight.
+struct DistillLoss {
+  const int32_t *is;
+  const float *t;
+  int k;
+  float tau;
+  float *loss, *lse;
+};
 template <typename T>
-__global__ void __launch_bounds__(256)
-distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, const float *__restrict__ t, const float2 *__restrict__ part, int runs,
-                    int64_t n, int64_t v, int k, float tau, float scale, float *__restrict__ loss, float *__restrict__ lse) {
-  extern __shared__ float sh[];                      // per warp: words [k], log q [k]
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  chain_wait();
-  if (row >= n) return;
-  int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * k;
-  float *wq = reinterpret_cast<float *>(wi + k);
-  is += row * k; t += row * k; s += row * v;
-  const bool some = teacher_row<true>(is, t, k, v, 1.f / tau, lane, wi, wq);
+__device__ __forceinline__ void distill_row(const DistillLoss &a, const T *s, int64_t v, const float2 *part, int runs, float scale, int64_t row, int lane, int *wi,
+                                            float *wq) {
+  const int k = a.k;
+  const bool some = teacher_row<true>(a.is + row * k, a.t + row * k, k, v, 1.f / a.tau, lane, wi, wq);
   float m = -INFINITY, sum = 0.f;
-  for (int p = lane; p < runs; p += 32) {
-    const float2 q = part[row * runs + p];
-    fold_pair<T>(m, sum, q.x, q.y, scale);
+  for (int p0 = lane; p0 < runs; p0 += 256) {
+    float2 q[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = p0 + 32 * j < runs ? __ldcg(part + row * runs + p0 + 32 * j) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int j = 0; j < 8; j++) fold_pair<T>(m, sum, q[j].x, q[j].y, scale);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, sum, o);
     fold_pair<T>(m, sum, pm, ps, scale);
   }
-  const double inv_tau = 1.0 / (double)tau, l = (double)m * (sizeof(T) == 2 ? L_LN2 : inv_tau) + log((double)sum);
+  const double inv_tau = 1.0 / (double)a.tau, l = (double)m * (sizeof(T) == 2 ? L_LN2 : inv_tau) + log((double)sum);
   double total = 0;
   if (some) {
 #pragma unroll 4
@@ -283,37 +228,117 @@ distill_loss_kernel(const T *__restrict__ s, const int32_t *__restrict__ is, con
       const int c = wi[j];
       const float lq = wq[j], q = c >= 0 ? expf(lq) : 0.f;
       // a teacher's weight of exactly 0 adds nothing, whatever the student says
-      if (q != 0.f) total += (double)q * ((double)lq - (double)to_f32<T>(s[c]) * inv_tau + l);
+      if (q != 0.f) total += (double)q * ((double)lq - (double)to_f32<T>(s[row * v + c]) * inv_tau + l);
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
   if (lane == 0) {
-    lse[row] = (float)l;
-    loss[row] = (float)((double)tau * (double)tau * total);
+    a.lse[row] = (float)l;
+    a.loss[row] = (float)((double)a.tau * (double)a.tau * total);
   }
 }
 
-// One warp per row, before the gradient: per word of the teacher its weight; of places with the same word one has the sum of
-// their weights and the others -1.  Which places those are is found without comparing all with all: in a round every
-// place that has not met its word yet writes itself into the word's slot of a hash table, and who then finds a place with its
-// own word there has met it (all places of a word do so in the same round, and in every slot someone does).
-// Per row: dl tau, whether there is a word, and the reference of its exponents with the factor that makes it exact: for binary16
-// exp(S / tau - lse) = 2^(S scale - hi) f, with hi + log f to more than 32 bits; for f32 lse itself, exp(S / tau - lse).
-__global__ void __launch_bounds__(256)
-distill_teacher_kernel(bool wide, const int32_t *__restrict__ is, const float *__restrict__ t, int64_t n, int64_t v, int k, int table, float tau,
-                       const float *__restrict__ dl, const float *__restrict__ lse, int32_t *__restrict__ words, float *__restrict__ weights,
-                       float4 *__restrict__ rows) {
-  extern __shared__ float sh[];                      // per warp: words [k], weights [k], the place met [k], slots [table]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
+// (maximum, sum) of every run.  JOIN: of few rows, whose losses the CTA that ends last then makes; `ticket` is 0 between launches.
+template <typename T, bool JOIN>
+__global__ void __launch_bounds__(D_THREADS, D_CTAS)
+distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, float2 *__restrict__ part,
+                    uint32_t *__restrict__ ticket, const DistillLoss a) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const int64_t items = n * d.runs, step = (int64_t)gridDim.x * D_WARPS;
+  const bool small = items < (1ll << 31);
+  DistillAt at;
+  at.item = (int64_t)blockIdx.x * D_WARPS + (threadIdx.x >> 5);
+  at.start(items, d, small);
   chain_wait();
-  if (row >= n) return;
-  is += row * k; t += row * k;
-  int *wi = reinterpret_cast<int *>(sh) + warp * (3 * k + table);
-  float *wq = reinterpret_cast<float *>(wi + k);
-  int *met = wi + 2 * k, *slot = wi + 3 * k;
-  const bool some = teacher_row<false>(is, t, k, v, 1.f / tau, lane, wi, wq);
+  int4 next[D_PER];
+  if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
+  float m = -INFINITY, sum = 0.f;
+  while (at.item < items) {
+    int4 x[D_PER];
+#pragma unroll
+    for (int i = 0; i < D_PER; i++) x[i] = next[i];
+    const DistillAt here = at;
+    at.next(items, step, d, small);
+    if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < D_PER; i++)
+      if (lane + 32 * i < d.groups) mx = fmaxf(mx, group_max(x[i], (const T *)nullptr));
+    mx = fmaxf(m, LogitUnit<T>::of(mx, scale));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float2 sc = make_float2(scale, scale), nr = make_float2(-ref, -ref);
+    float2 u = make_float2(sum * ex2(LogitUnit<T>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
+    m = mx;
+#pragma unroll
+    for (int i = 0; i < D_PER; i++)
+      if (lane + 32 * i < d.groups) {
+        float f[W];
+        unpack(x[i], f);
+#pragma unroll
+        for (int j = 0; j < W; j += 4) {
+          const float2 e = exponents<T>(make_float2(f[j], f[j + 1]), sc, nr), g = exponents<T>(make_float2(f[j + 2], f[j + 3]), sc, nr);
+          u = add2(u, make_float2(ex2(e.x), ex2(e.y)));
+          b = add2(b, make_float2(ex2(g.x), ex2(g.y)));
+        }
+      }
+    sum = (u.x + u.y) + (b.x + b.y);
+    if (here.chunk + 1 == here.last) {               // the lanes meet
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float om = __shfl_xor_sync(kFull, m, o), os = __shfl_xor_sync(kFull, sum, o);
+        fold_pair<T>(m, sum, om, os, scale);
+      }
+      if (lane == 0) part[here.item] = make_float2(m, sum);
+      m = -INFINITY;
+      sum = 0.f;
+    }
+  }
+  if (JOIN) {
+    extern __shared__ float sh[];                    // per warp: words [k], log q [k]
+    __shared__ bool last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * a.k;
+    for (int64_t row = threadIdx.x >> 5; row < n; row += D_WARPS)
+      distill_row<T>(a, s, v, part, d.runs, scale, row, lane, wi, reinterpret_cast<float *>(wi + a.k));
+    if (threadIdx.x == 0) *ticket = 0;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+distill_loss_kernel(const T *__restrict__ s, const float2 *__restrict__ part, int runs, int64_t n, int64_t v, float scale, const DistillLoss a) {
+  extern __shared__ float sh[];                      // per warp: words [k], log q [k]
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  chain_wait();
+  int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * a.k;
+  if (row < n) distill_row<T>(a, s, v, part, runs, scale, row, threadIdx.x & 31, wi, reinterpret_cast<float *>(wi + a.k));
+}
+
+// What the gradient needs of a row's teacher, by one warp in shared memory: per word its weight; of places with the same word one has
+// the sum of their weights and the others -1.  Which places those are is found without comparing all with all: in a round every
+// place that has not met its word yet writes itself into the word's slot of a hash table, and who then finds a place with its
+// own word there has met it (all places of a word do so in the same round, and in every slot someone does).  False if the row has no word.
+struct DistillTeacher {
+  const int32_t *is;
+  const float *t;
+  int k, table;                                      // slots of the hash table: a power of two, at least 2 k
+  float tau;
+  const float *dl, *lse;
+  __host__ __device__ __forceinline__ int shared() const { return 3 * k + table; }       // 32-bit words a warp needs
+};
+__device__ __forceinline__ bool teacher_weights(const DistillTeacher &a, int64_t row, int64_t v, int lane, int *wi, float *wq) {
+  const int k = a.k, table = a.table;
+  int *met = wi + 2 * k, *slot = wi + 3 * k;         // the place met, and the table
+  const bool some = teacher_row<false>(a.is + row * k, a.t + row * k, k, v, 1.f / a.tau, lane, wi, wq);
   for (int j = lane; j < k; j += 32) met[j] = wi[j] < 0 ? j : -1;
   uint32_t mul = 2654435761u;
   for (bool left = true; left; mul = mul * 1664525u + 1013904224u | 1u) {
@@ -346,15 +371,33 @@ distill_teacher_kernel(bool wide, const int32_t *__restrict__ is, const float *_
       __syncwarp();
     }
   }
-  for (int j = lane; j < k; j += 32) {
-    words[row * k + j] = wi[j];
-    weights[row * k + j] = wq[j];
+  return some;
+}
+// Per row: dl tau, whether there is a word, and the reference of its exponents with the factor that makes it exact: for binary16
+// exp(S / tau - lse) = 2^(S scale - hi) f, with hi + log f to more than 32 bits; for f32 lse itself, exp(S / tau - lse).
+__device__ __forceinline__ float4 teacher_record(const DistillTeacher &a, int64_t row, bool some, bool wide) {
+  const float lse = a.lse[row];
+  const double shift = (double)lse * (1.0 / L_LN2);
+  const float hi = (float)shift;
+  return make_float4(a.dl[row] * a.tau, some ? 1.f : 0.f, wide ? lse : hi, wide ? 1.f : exp2f((float)((double)hi - shift)));
+}
+// Both for every row, one warp per row.
+__global__ void __launch_bounds__(256)
+distill_teacher_kernel(bool wide, const DistillTeacher a, int64_t n, int64_t v, int32_t *__restrict__ words, float *__restrict__ weights,
+                       float4 *__restrict__ rows) {
+  extern __shared__ float sh[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
+  chain_wait();
+  if (row >= n) return;
+  int *wi = reinterpret_cast<int *>(sh) + warp * a.shared();
+  float *wq = reinterpret_cast<float *>(wi + a.k);
+  const bool some = teacher_weights(a, row, v, lane, wi, wq);
+  for (int j = lane; j < a.k; j += 32) {
+    words[row * a.k + j] = wi[j];
+    weights[row * a.k + j] = wq[j];
   }
-  if (lane == 0) {
-    const double shift = (double)lse[row] * (1.0 / L_LN2);
-    const float hi = (float)shift;
-    rows[row] = make_float4(dl[row] * tau, some ? 1.f : 0.f, wide ? lse[row] : hi, wide ? 1.f : exp2f((float)((double)hi - shift)));
-  }
+  if (lane == 0) rows[row] = teacher_record(a, row, some, wide);
 }
 
 // The gradient is read and written by neighbouring warps at neighbouring places, which HBM likes better than long runs: with runs
@@ -370,10 +413,12 @@ template <> __device__ __forceinline__ float2 row_exponents<float>(float2 x, flo
 }
 
 // Every chunk: the student's softmax; after a run the words of the teacher that lie in it once more.
-template <typename T>
+// OWN: every warp has one run at most, and finds what it needs of its row's teacher for itself.
+template <typename T, bool OWN>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
-distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, int k, const int32_t *__restrict__ words,
-                    const float *__restrict__ weights, const float4 *__restrict__ rows, T *__restrict__ ds) {
+distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, const DistillTeacher a,
+                    const int32_t *__restrict__ words, const float *__restrict__ weights, const float4 *__restrict__ rows, T *__restrict__ ds) {
+  extern __shared__ float sh[];
   constexpr int W = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
   const int64_t items = n * d.runs, step = (int64_t)gridDim.x * D_WARPS;
@@ -386,12 +431,18 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
   if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
   float4 rc = make_float4(0.f, 0.f, 0.f, 0.f);
   bool fresh = true;
+  int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * a.shared();
+  float *wq = reinterpret_cast<float *>(wi + a.k);
+  if (OWN && at.item < items) {
+    rc = teacher_record(a, at.row, teacher_weights(a, at.row, v, lane, wi, wq), sizeof(T) == 4);
+    __syncwarp();
+  }
   while (at.item < items) {
     int4 x[D_PER];
 #pragma unroll
     for (int i = 0; i < D_PER; i++) x[i] = next[i];
     const DistillAt here = at;
-    if (fresh) rc = rows[here.row];
+    if (!OWN && fresh) rc = rows[here.row];
     at.next(items, step, d, small);
     if (at.item < items) load_chunk<T>(DistillRow<T>(s, at.row, v), at.chunk, d.groups, lane, next);
     const DistillRow<T> r(s, here.row, v);
@@ -429,11 +480,11 @@ distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
       __syncwarp();                                  // the words' places have been written
       if (some) {
         const int c0 = r.first((here.last - 1) / d.run * d.run * d.groups), c1 = r.first(here.last * d.groups);
-        for (int j = lane; j < k; j += 32) {
-          const int word = words[here.row * k + j];
+        for (int j = lane; j < a.k; j += 32) {
+          const int word = OWN ? wi[j] : words[here.row * a.k + j];
           if (word >= 0 && word >= c0 && word < c1) {
             const float xw = to_f32<T>(r.base[word]), p = ex2(row_exponents<T>(make_float2(xw, xw), sc, nr).x) * rc.w;
-            out[word] = from_f32<T>((p - weights[here.row * k + j]) * rc.x);
+            out[word] = from_f32<T>((p - (OWN ? wq[j] : weights[here.row * a.k + j])) * rc.x);
           }
         }
       }
@@ -449,26 +500,40 @@ static unsigned chunk_grid(int64_t items, int num_sms) {
 // Warps of a CTA that has a row per warp: few rows are spread over more SMs.
 static int row_warps(int64_t n, int num_sms) { return n >= (int64_t)num_sms * 8 ? 8 : 2; }
 
+// Small calls, where a kernel less is 4 us on the GPU and 2 on the host: what the runs leave of a row is then done by the kernel that works them
+// off.  Of the forward the last CTA makes the losses, at most two rows of 256 runs per warp; in the gradient, where a warp has a run at most, it
+// finds the weights of its row's teacher itself, in what shared memory leaves each of four CTAs.  One row of 32000 f32 with 8 words of its
+// teacher, both directions: 25 us instead of 28.5; 16 rows of 2000000 binary16, 1954 runs, would be 64 instead of 58.5.
+constexpr int D_OWN_K = 256;
+static bool own_loss(const DistillShape &d, int64_t n, int64_t k) { return n <= 2 * D_WARPS && d.runs <= 256 && k <= D_OWN_K; }
+static bool own_teacher(const DistillShape &d, int64_t n, int64_t k, int num_sms) {
+  return n * d.runs <= (int64_t)num_sms * D_CTAS * D_WARPS && k <= D_OWN_K;
+}
+
 size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms) {
-  if (!grad) return up256((size_t)n * distill_shape(s, n, v, elem, num_sms, 16).runs * sizeof(float2));
-  return up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float4));
+  const DistillShape d = distill_shape(s, n, v, elem, num_sms, !grad ? 16 : elem == 2 ? D_GRAD_RUN<__half> : D_GRAD_RUN<float>);
+  if (!grad) return up256((size_t)n * d.runs * sizeof(float2));
+  return own_teacher(d, n, k, num_sms) ? 0 : up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float4));
 }
 
 template <typename T>
-static cudaError_t distill(void *workspace, const T *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k, float *loss,
-                           float *lse, int num_sms, cudaStream_t stream) {
+static cudaError_t distill(void *workspace, uint32_t *ticket, const T *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
+                           float *loss, float *lse, int num_sms, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
   const DistillShape d = distill_shape(s, n, v, sizeof(T), num_sms, 16);
   float2 *part = reinterpret_cast<float2 *>(workspace);
   const float scale = (float)(1.0 / (L_LN2 * (double)tau));
-  cudaError_t err = launch_after(distill_part_kernel<T>, chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream, s, n, v, d, scale, part);
+  const DistillLoss a = {is, t, (int)k, tau, loss, lse};
+  const unsigned grid = chunk_grid(n * d.runs, num_sms);
+  if (own_loss(d, n, k))
+    return launch_after(distill_part_kernel<T, true>, grid, D_THREADS, (size_t)D_WARPS * 2 * k * 4, stream, s, n, v, d, scale, part, ticket, a);
+  cudaError_t err = launch_after(distill_part_kernel<T, false>, grid, D_THREADS, 0, stream, s, n, v, d, scale, part, ticket, a);
   if (err != cudaSuccess) return err;
   const int rw = row_warps(n, num_sms);
   static unsigned long long allowed = 0;
   err = allow_smem(reinterpret_cast<const void *>(distill_loss_kernel<T>), 8 * 2 * DISTILL_MAX_K * 4, allowed);
   if (err != cudaSuccess) return err;
-  return launch_after(distill_loss_kernel<T>, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream, s, is, t, part, d.runs, n, v, (int)k, tau,
-                      scale, loss, lse);
+  return launch_after(distill_loss_kernel<T>, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream, s, part, d.runs, n, v, scale, a);
 }
 
 template <typename T>
@@ -481,22 +546,26 @@ static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, 
   float *weights = reinterpret_cast<float *>(ws + up256((size_t)(n * k) * 4));
   float4 *rows = reinterpret_cast<float4 *>(ws + 2 * up256((size_t)(n * k) * 4));
   const float scale = (float)(1.0 / ((sizeof(T) == 2 ? L_LN2 : 1.0) * (double)tau));
-  int table = 32;
-  while (table < 2 * k) table *= 2;
+  DistillTeacher a = {is, t, (int)k, 32, tau, dl, lse};
+  while (a.table < 2 * k) a.table *= 2;
+  const unsigned grid = chunk_grid(n * d.runs, num_sms);
+  if (own_teacher(d, n, k, num_sms))
+    return launch_after(distill_grad_kernel<T, true>, grid, D_THREADS, (size_t)D_WARPS * a.shared() * 4, stream, s, n, v, d, scale, a, words, weights, rows, ds);
   const int rw = row_warps(n, num_sms);
   static unsigned long long allowed = 0;
   cudaError_t err = allow_smem(reinterpret_cast<const void *>(distill_teacher_kernel), 8 * (3 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4, allowed);
   if (err != cudaSuccess) return err;
-  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * (3 * k + table) * 4, stream, sizeof(T) == 4, is, t, n, v, (int)k, table, tau, dl,
-                     lse, words, weights, rows);
+  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * a.shared() * 4, stream, sizeof(T) == 4, a, n, v, words, weights,
+                     rows);
   if (err != cudaSuccess) return err;
-  return launch_after(distill_grad_kernel<T>, chunk_grid(n * d.runs, num_sms), D_THREADS, 0, stream, s, n, v, d, scale, (int)k, words, weights, rows, ds);
+  return launch_after(distill_grad_kernel<T, false>, grid, D_THREADS, 0, stream, s, n, v, d, scale, a, words, weights, rows, ds);
 }
 
-cudaError_t launch_topk_distill(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
-                                float *loss, float *lse, int num_sms, cudaStream_t stream) {
-  if (elem == 2) return distill<__half>(workspace, reinterpret_cast<const __half *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
-  return distill<float>(workspace, reinterpret_cast<const float *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
+cudaError_t launch_topk_distill(void *workspace, void *ticket, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v,
+                                int64_t k, float *loss, float *lse, int num_sms, cudaStream_t stream) {
+  uint32_t *tk = reinterpret_cast<uint32_t *>(ticket);
+  if (elem == 2) return distill<__half>(workspace, tk, reinterpret_cast<const __half *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
+  return distill<float>(workspace, tk, reinterpret_cast<const float *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
 }
 cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,
                                      const float *dl, int64_t n, int64_t v, int64_t k, void *ds, int num_sms, cudaStream_t stream) {
@@ -608,13 +677,23 @@ __device__ __forceinline__ float router_exp(float (&p)[COLS], int g) {
   return sum == 0.f ? 0.f : __fdividef(1.f, sum);       // at most 2 units in the last place off; sum is at most 1024
 }
 
-// Partial results of a CTA: column sums of p [e], counts [e] and the number of rows kept.
+// Partial results that a thread of the last CTA adds up at most.  More are left to a kernel of their own: 148 of 256 experts took one SM
+// 2.4 us longer than that kernel, and 148 of 1024 experts 37 us.  It costs small calls 2 us.
+constexpr int R_JOIN = 4;
+// Columns of the CTAs' partial results: the experts and the number of rows kept, in whole groups of 4.
+static __host__ __device__ __forceinline__ int router_groups(int e) { return e / 4 + 1; }
+// Slices of the CTAs that the last one adds up side by side.
+static __host__ __device__ __forceinline__ int router_slices(int threads, int e) { const int s = threads / router_groups(e); return s < 16 ? s : 16; }
+
+// Partial results of a CTA: column sums of p, counts and, behind them, the number of rows kept.  `ticket`, which is 0 between
+// launches: where there are few partial results the CTA that ends last adds them all up, in f64 and in the order of the CTAs, and makes the loss.
 template <typename T, int W, int J>
 __global__ void __launch_bounds__(RouterRow<T, W, J>::THREADS)
 router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ is, int64_t n, int e, int k, int g,
-                   float *__restrict__ psum, int *__restrict__ pcount, int *__restrict__ ticket) {
+                   float *__restrict__ psum, int *__restrict__ pcount, uint32_t *__restrict__ ticket, int32_t *__restrict__ counts,
+                   float *__restrict__ loss, float *__restrict__ norm) {
   constexpr int R_WARPS = RouterRow<T, W, J>::WARPS, R_THREADS = RouterRow<T, W, J>::THREADS;
-  extern __shared__ float rsh[];                     // [R_WARPS][g * J * W] column sums of the warps, then [e + 1] counts
+  extern __shared__ __align__(16) float rsh[];       // [R_WARPS][g * J * W] column sums of the warps, then [e + 1] counts
   const int span = g * J * W;
   int *cnt = reinterpret_cast<int *>(rsh + R_WARPS * span);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (g - 1), sub = lane / g, per_warp = 32 / g;
@@ -634,7 +713,6 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
     if (l < k) sent = *ex;
   }
   for (int c = threadIdx.x; c <= e; c += R_THREADS) cnt[c] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;              // of the next kernel
   __syncthreads();
   float acc[J * W];
 #pragma unroll
@@ -686,33 +764,95 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
   kept = warp_sum(kept);
   if (lane == 0 && kept) atomicAdd(&cnt[e], kept);
   __syncthreads();
-  for (int c = threadIdx.x; c < e; c += R_THREADS) {
+  const int groups = router_groups(e), span4 = 4 * groups, parts = (int)gridDim.x;
+  for (int c = threadIdx.x; c < span4; c += R_THREADS) {
     float t = 0.f;
+    if (c < e) {
 #pragma unroll
-    for (int w = 0; w < R_WARPS; w++) t += rsh[w * span + c];
-    psum[(int64_t)blockIdx.x * e + c] = t;
+      for (int w = 0; w < R_WARPS; w++) t += rsh[w * span + c];
+    }
+    psum[(int64_t)blockIdx.x * span4 + c] = t;
+    pcount[(int64_t)blockIdx.x * span4 + c] = c <= e ? cnt[c] : 0;
   }
-  for (int c = threadIdx.x; c <= e; c += R_THREADS) pcount[(int64_t)blockIdx.x * (e + 1) + c] = cnt[c];
+  if (ticket == nullptr) return;
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  // a slice of the CTAs and a group of 4 columns per thread
+  const int slices = router_slices(R_THREADS, e);
+  double *dsum = reinterpret_cast<double *>(rsh);    // [slices][span4]
+  int *dcnt = reinterpret_cast<int *>(dsum + slices * span4);
+  if ((int)threadIdx.x < slices * groups) {
+    const int sl = threadIdx.x / groups, c = 4 * (threadIdx.x - sl * groups);
+    double p0 = 0, p1 = 0, p2 = 0, p3 = 0;
+    int4 q = make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < R_JOIN; j++) {
+      const int b = sl + j * slices;
+      if (b >= parts) break;
+      const float4 x = __ldcg(reinterpret_cast<const float4 *>(psum + (int64_t)b * span4 + c));
+      const int4 y = __ldcg(reinterpret_cast<const int4 *>(pcount + (int64_t)b * span4 + c));
+      p0 += (double)x.x; p1 += (double)x.y; p2 += (double)x.z; p3 += (double)x.w;
+      q.x += y.x; q.y += y.y; q.z += y.z; q.w += y.w;
+    }
+    double *dp = dsum + sl * span4 + c;
+    dp[0] = p0; dp[1] = p1; dp[2] = p2; dp[3] = p3;
+    *reinterpret_cast<int4 *>(dcnt + sl * span4 + c) = q;
+  }
+  __syncthreads();
+  __shared__ double stotal[32];
+  __shared__ long long sall[32];
+  __shared__ int skept;
+  double total = 0;
+  long long all = 0;
+  for (int c = threadIdx.x; c <= e; c += R_THREADS) {
+    double p = 0;
+    int q = 0;
+    for (int sl = 0; sl < slices; sl++) { p += dsum[sl * span4 + c]; q += dcnt[sl * span4 + c]; }
+    if (c == e) { skept = q; break; }
+    counts[c] = q;
+    total += (double)q * p;
+    all += q;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { total += __shfl_xor_sync(kFull, total, o); all += __shfl_xor_sync(kFull, all, o); }
+  if (lane == 0) { stotal[warp] = total; sall[warp] = all; }
+  __syncthreads();
+  if (warp != 0) return;
+  total = lane < R_WARPS ? stotal[lane] : 0;
+  all = lane < R_WARPS ? sall[lane] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { total += __shfl_xor_sync(kFull, total, o); all += __shfl_xor_sync(kFull, all, o); }
+  if (lane == 0) {
+    const double m = (double)skept, f = all > 0 && m > 0 ? (double)e / ((double)all * m) : 0.0;
+    *norm = (float)f;
+    *loss = all > 0 ? (float)(total * f) : 0.f;
+    *ticket = 0;
+  }
 }
 
 // 32 columns per CTA, the partial results of the CTAs over the warps, in f64; the CTA that ends last makes the loss.
 __global__ void __launch_bounds__(1024)
 router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcount, int parts, int e, double *__restrict__ sums, int *__restrict__ kept,
-                   int *__restrict__ ticket, int32_t *__restrict__ counts, float *__restrict__ loss, float *__restrict__ norm) {
+                   uint32_t *__restrict__ ticket, int32_t *__restrict__ counts, float *__restrict__ loss, float *__restrict__ norm) {
   __shared__ double sp[32][33];
   __shared__ int sc[32][33];
   __shared__ bool last;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, span4 = 4 * router_groups(e);
   double p = 0;
   int q = 0;
   chain_wait();
   if (c <= e) {
-    const int cp = min(c, e - 1);                    // the number of rows kept has no sum of p
 #pragma unroll 5
     for (int b = warp; b < parts; b += 32) {
-      const float x = e > 0 ? psum[(int64_t)b * e + cp] : 0.f;
-      q += pcount[(int64_t)b * (e + 1) + c];
-      p += (double)x;
+      q += pcount[(int64_t)b * span4 + c];
+      p += (double)psum[(int64_t)b * span4 + c];
     }
   }
   sp[warp][lane] = p;
@@ -726,7 +866,7 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
     __threadfence();
   }
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
+  if (threadIdx.x == 0) last = atomicAdd(ticket, 1u) == gridDim.x - 1;
   __syncthreads();
   if (!last || warp != 0) return;
   __threadfence();
@@ -744,6 +884,7 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
     const double f = all > 0 && m > 0 ? (double)e / ((double)all * m) : 0.0;
     *norm = (float)f;
     *loss = all > 0 ? (float)(total * f) : 0.f;
+    *ticket = 0;
   }
 }
 
@@ -811,7 +952,7 @@ static int64_t router_grid(int64_t n, const RouterShape &s, int num_sms) {
 
 size_t router_workspace_bytes(const void *r, int elem, int64_t n, int64_t e, int num_sms) {
   const int64_t grid = router_grid(n, router_shape(r, e, elem), num_sms);
-  return up256((size_t)(grid * e) * 4) + up256((size_t)(grid * (e + 1)) * 4) + up256((size_t)e * 8) + 256;
+  return 2 * up256((size_t)grid * 16 * router_groups((int)e)) + up256((size_t)e * 8) + 256;
 }
 
 // F is instantiated for the row's shape: W = 4 has up to 8 groups per lane, W = 1 up to 32
@@ -823,28 +964,30 @@ size_t router_workspace_bytes(const void *r, int elem, int64_t n, int64_t e, int
   }
 
 template <typename T>
-static cudaError_t router(void *workspace, const T *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k, float *loss,
-                          int32_t *counts, float *norm, int num_sms, cudaStream_t stream) {
+static cudaError_t router(void *workspace, uint32_t *ticket, const T *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k,
+                          float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream) {
   const RouterShape s = router_shape(r, e, sizeof(T));
-  const int grid = (int)router_grid(n, s, num_sms);
+  const int grid = (int)router_grid(n, s, num_sms), threads = 32 * s.warps(), span4 = 4 * router_groups((int)e);
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
   float *psum = reinterpret_cast<float *>(ws);
-  int *pcount = reinterpret_cast<int *>(ws + up256((size_t)grid * e * 4));
-  double *sums = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(pcount) + up256((size_t)grid * (e + 1) * 4));
+  int *pcount = reinterpret_cast<int *>(ws + up256((size_t)grid * span4 * 4));
+  double *sums = reinterpret_cast<double *>(reinterpret_cast<uint8_t *>(pcount) + up256((size_t)grid * span4 * 4));
   int *kept = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(sums) + up256((size_t)e * 8));
-  int *ticket = kept + 1;
-  const size_t smem = (size_t)s.warps() * s.g * s.cols() * 4 + (size_t)(e + 1) * 4;
+  const bool join = grid <= R_JOIN * router_slices(threads, (int)e);
+  const size_t rows = (size_t)s.warps() * s.g * s.cols() * 4 + (size_t)(e + 1) * 4, joined = join ? (size_t)router_slices(threads, (int)e) * span4 * 12 : 0;
+  const size_t smem = rows > joined ? rows : joined;
   cudaError_t err = cudaSuccess;
 #define FB_PART(W, J)                                                                                                     \
   {                                                                                                                       \
     static unsigned long long allowed = 0;                                                                                \
     err = allow_smem(reinterpret_cast<const void *>(router_part_kernel<T, W, J>), 160 << 10, allowed);                    \
     if (err == cudaSuccess)                                                                                               \
-      err = launch_after(router_part_kernel<T, W, J>, grid, 32 * s.warps(), smem, stream, r, keep, is, n, (int)e, (int)k, s.g, psum, pcount, ticket); \
+      err = launch_after(router_part_kernel<T, W, J>, grid, threads, smem, stream, r, keep, is, n, (int)e, (int)k, s.g, psum, pcount,   \
+                         join ? ticket : nullptr, counts, loss, norm);                                                    \
   }
   FB_ROUTER_SHAPE(s, FB_PART)
 #undef FB_PART
-  if (err != cudaSuccess) return err;
+  if (err != cudaSuccess || join) return err;
   return launch_after(router_loss_kernel, (unsigned)((e + 1 + 31) / 32), 1024, 0, stream, psum, pcount, grid, (int)e, sums, kept, ticket, counts, loss, norm);
 }
 
@@ -860,10 +1003,11 @@ static cudaError_t router_grad(const T *r, const uint8_t *keep, const int32_t *c
   return cudaSuccess;
 }
 
-cudaError_t launch_router_balance(void *workspace, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k,
-                                  float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream) {
-  if (elem == 2) return router<__half>(workspace, reinterpret_cast<const __half *>(r), keep, is, n, e, k, loss, counts, norm, num_sms, stream);
-  return router<float>(workspace, reinterpret_cast<const float *>(r), keep, is, n, e, k, loss, counts, norm, num_sms, stream);
+cudaError_t launch_router_balance(void *workspace, void *ticket, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e,
+                                  int64_t k, float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream) {
+  uint32_t *tk = reinterpret_cast<uint32_t *>(ticket);
+  if (elem == 2) return router<__half>(workspace, tk, reinterpret_cast<const __half *>(r), keep, is, n, e, k, loss, counts, norm, num_sms, stream);
+  return router<float>(workspace, tk, reinterpret_cast<const float *>(r), keep, is, n, e, k, loss, counts, norm, num_sms, stream);
 }
 
 cudaError_t launch_router_balance_grad(int elem, const void *r, const uint8_t *keep, const int32_t *counts, const float *norm, const float *dl, int64_t n,

@@ -78,6 +78,8 @@ struct VocabArgs {
   int v, v0;                    // size of the vocabulary, first word of the piece
   float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum in units of log 2, sum)
   float *ztarget;
+  float *loss, *lse;            // and the results, where the kernel finishes them itself:
+  uint32_t *ticket;             // then a word that is 0 between launches
   const float *cexp;            // VE_GRAD: per row the exponent's constant term
   const float *factor;          // VE_HALF
   const float *w;               // VE_ROWS
@@ -93,6 +95,7 @@ struct VocabBarriers {
   uint64_t tmem_empty[2];        // used in the pair's first CTA only
   uint64_t met[2][4];            // VE_SOFTMAX: three shares of 32 rows are in shared memory
   uint32_t tmem_base;
+  uint32_t last;                 // whether this CTA is the one that ends last
 };
 
 // Tiles in the order the pairs take them: V_GROUP row tiles by all column tiles, the rows first.  74 pairs then
@@ -106,6 +109,39 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs &a, uint32_t t, int &
   split = (int)sp;
   tn = (int)n;
   tm = (int)(g * V_GROUP + in - n * rows);
+}
+
+// A row's loss by one warp: fold of its (maximum, sum) pairs, eight per lane in flight; the last step in f64, where a loss near 0 is
+// a difference.
+__device__ __forceinline__ void row_loss(const float2 *part, int tiles, const float *ztarget, const int32_t *targets, float *loss, float *lse, int64_t row,
+                                         int64_t v, int lane) {
+  float m = -INFINITY, s = 0.f;
+  for (int t0 = lane; t0 < tiles; t0 += 256) {
+    float2 p[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) p[j] = t0 + 32 * j < tiles ? __ldcg(part + row * tiles + t0 + 32 * j) : make_float2(-INFINITY, 0.f);
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < 8; j++) mn = fmaxf(mn, p[j].x);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    s *= exp2f(m - ref);
+#pragma unroll
+    for (int j = 0; j < 8; j++) s += p[j].y * exp2f(p[j].x - ref);
+    m = mn;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, s, o);
+    const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.f : mn;
+    s = s * exp2f(m - ref) + ps * exp2f(pm - ref);
+    m = mn;
+  }
+  if (lane == 0) {
+    const double l = ((double)m + log2((double)s)) * 0.69314718055994530942;
+    const int64_t t = targets[row];
+    lse[row] = (float)l;
+    loss[row] = t >= 0 && t < v ? (float)(l - (double)__ldcg(ztarget + row)) : 0.f;
+  }
 }
 
 // A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
@@ -446,6 +482,19 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   if (PAIR) cluster_meet();                            // nobody signals into a partner that has left
+  if (EPI == VE_SOFTMAX && !PAIR && a.ticket != nullptr) {
+    // the CTA that ends last makes the losses, a row per warp
+    if (tid == 0) {
+      __threadfence();
+      bars->last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (bars->last) {
+      __threadfence();
+      if (warp < a.M) row_loss(a.part, a.tiles_n, a.ztarget, a.targets, a.loss, a.lse, warp, a.v, lane);
+      if (tid == 0) *a.ticket = 0;
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     if (!PAIR) tmem_dealloc(tmem_base, 512);
@@ -454,34 +503,12 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 }
 
 // ---- the small kernels around it ------------------------------------------------------------------
-// One warp per row: fold of the row's (maximum, sum) pairs; the last step in f64, where a loss near 0 is a difference.
 __global__ void __launch_bounds__(256)
 vocab_loss_kernel(const float2 *__restrict__ part, int tiles, const float *__restrict__ ztarget, const int32_t *__restrict__ targets,
                   float *__restrict__ loss, float *__restrict__ lse, int64_t n, int64_t v) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
   chain_wait();
-  if (row >= n) return;
-  float m = -INFINITY, s = 0.f;
-  for (int t = lane; t < tiles; t += 32) {
-    const float2 p = part[row * tiles + t];
-    const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.f : mn;
-    s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
-    m = mn;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, s, o);
-    const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.f : mn;
-    s = s * exp2f(m - ref) + ps * exp2f(pm - ref);
-    m = mn;
-  }
-  if (lane == 0) {
-    const double l = ((double)m + log2((double)s)) * 0.69314718055994530942;
-    const int64_t t = targets[row];
-    lse[row] = (float)l;
-    loss[row] = t >= 0 && t < v ? (float)(l - (double)ztarget[row]) : 0.f;
-  }
+  if (row < n) row_loss(part, tiles, ztarget, targets, loss, lse, row, v, threadIdx.x & 31);
 }
 
 // w_i = dl_i q_i and the constant term of G's exponent; false for a token without a target
@@ -628,6 +655,8 @@ static inline int elementwise_grid(int64_t items, int num_sms) {
 
 // Batches of at most 128 tokens go to single CTAs, where the tokens are the rows of the product.
 static inline bool small_batch(int64_t n) { return n <= 128; }
+// Batches whose losses the contraction's last CTA makes, a row per warp.  A kernel for them costs a launch.
+static inline bool tiny_batch(int64_t n) { return n <= V_THREADS / 32; }
 // Clocks of a block of 64 summed elements of a tile of `cols` columns: on pairs 512 for 256 columns at the tensor cores'
 // rate and a fifth of that for the rows' operand; on single CTAs what 148 of them leave each other of HBM, 24 bytes per clock.
 static inline double block_clocks(bool pair, int cols) { return pair ? (cols + 64) * 1.6 : cols * 5.3; }
@@ -759,7 +788,7 @@ static cudaError_t operands(const VocabPlan &p, uint8_t *ws, const uint16_t *&x,
 
 #define FB_TRY(e) do { const cudaError_t fb_err = (e); if (fb_err != cudaSuccess) return fb_err; } while (0)
 
-cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
+cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, void *ticket, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
                               float *lse, int64_t n, int64_t v, int64_t d, int *failure, int num_sms, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
   if (v <= 0) {                                   // the sum of nothing
@@ -778,7 +807,11 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_
   a.part = reinterpret_cast<float2 *>(ws + p.part);
   a.ztarget = reinterpret_cast<float *>(ws + p.zt);
   a.failure = failure;
+  if (tiny_batch(n)) {
+    a.loss = loss; a.lse = lse; a.ticket = reinterpret_cast<uint32_t *>(ticket);
+  }
   FB_TRY((launch_tokens<false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
+  if (tiny_batch(n)) return cudaSuccess;
   return launch_after(vocab_loss_kernel, (unsigned)ceil_div(n, 8), 256, 0, stream, a.part, (int)ceil_div(v, p.nt), a.ztarget, targets, loss, lse, n, v);
 }
 

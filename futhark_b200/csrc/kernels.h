@@ -194,7 +194,7 @@ struct VocabPlan {
   size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dxp, dwp, bytes;
 };
 VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_aligned, bool grad, int num_sms);
-cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
+cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, void *ticket, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,
                               float *lse, int64_t n, int64_t v, int64_t d, int *failure, int num_sms, cudaStream_t stream);
 cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const uint16_t *x, const uint16_t *w, const int32_t *targets,
                                    const float *loss, const float *lse, const float *dl, uint16_t *dx, uint16_t *dw, int64_t n, int64_t v,
@@ -203,13 +203,13 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
 // ---- losses on logits (k_losses.cu); elem is the size of a logit: 2 (binary16) or 4 ---------------
 constexpr int DISTILL_MAX_K = 1024, ROUTER_MAX_E = 1024;
 size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms);
-cudaError_t launch_topk_distill(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
-                                float *loss, float *lse, int num_sms, cudaStream_t stream);
+cudaError_t launch_topk_distill(void *workspace, void *ticket, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v,
+                                int64_t k, float *loss, float *lse, int num_sms, cudaStream_t stream);
 cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,
                                      const float *dl, int64_t n, int64_t v, int64_t k, void *ds, int num_sms, cudaStream_t stream);
 size_t router_workspace_bytes(const void *r, int elem, int64_t n, int64_t e, int num_sms);
-cudaError_t launch_router_balance(void *workspace, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e, int64_t k,
-                                  float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream);
+cudaError_t launch_router_balance(void *workspace, void *ticket, int elem, const void *r, const uint8_t *keep, const int32_t *is, int64_t n, int64_t e,
+                                  int64_t k, float *loss, int32_t *counts, float *norm, int num_sms, cudaStream_t stream);
 cudaError_t launch_router_balance_grad(int elem, const void *r, const uint8_t *keep, const int32_t *counts, const float *norm, const float *dl, int64_t n,
                                        int64_t e, void *dr, int num_sms, cudaStream_t stream);
 
