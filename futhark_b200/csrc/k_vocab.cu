@@ -172,6 +172,15 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     for (int i = 0; i < 8; i++) mbar_init(&bars->met[i >> 2][i & 3], V_WARPS / 4 - 1);
     fence_mbar_init();
   }
+  if (!PAIR && !A_MN) {
+    // rows of the tile that no token has are 0, in every stage and from now on
+    const int per = (128 - a.arows) * 8;
+    for (int i = tid; i < V_STAGES * per; i += V_THREADS) {
+      const int st = i / per;
+      *reinterpret_cast<uint4 *>(smem + st * V_STAGE + a.arows * 128 + (i - st * per) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+  }
   if (warp == 1) {
     if (PAIR) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)), "r"(512) : "memory");
