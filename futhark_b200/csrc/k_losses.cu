@@ -12,7 +12,10 @@
 //   loss = norm sum_e counts_e sum_{i kept} p_ie
 //   dR_ie = dl norm p_ie (counts_e - sum_f counts_f p_if);                     0 for padding
 //
-// All four are bound by memory: each direction reads its logits once and the gradients are written once.
+// All four are bound by memory: each direction reads its logits once and the gradients are written once.  One at a time, 4096 x 131072
+// binary16: distill_part 171 us (6.3 TB/s), distill_grad 346 us (6.2 TB/s), and 12 and 8 us for losses and teachers; 2049 x 50001 f32: 64 us (6.4),
+// 125 us (6.6), 6 and 6 us; 131072 x 256 f32: router_part 25 us (5.3 TB/s), router_loss 10 us, router_grad 38 us (7.0 TB/s, some of the writes
+// still in L2).
 #include <cuda_fp16.h>
 #include <math.h>
 
