@@ -385,6 +385,11 @@ class _EntryTable(dict):
 _entries = _EntryTable()
 
 
+def _wrong_types(arrays, *wanted):
+    """An entry point would read memory that an array of another type does not have."""
+    raise TypeError("arrays of types (%s) are wanted, got (%s)" % (", ".join(wanted), ", ".join(a.tname for a in arrays)))
+
+
 class Pair:
     """The opaque (selected, rejected) record returned by partition."""
 
@@ -708,24 +713,36 @@ class Context:
 
     def entry_vocab_xent_f16(self, X, W, ts):
         """Cross entropy of hidden states X against the vocabulary W: (losses, lses)."""
+        if X.tname != "f16_2d" or W.tname != "f16_2d" or ts.tname != "i32_1d":
+            _wrong_types((X, W, ts), "f16_2d", "f16_2d", "i32_1d")
         return self._entry_rec("vocab_xent_f16", LOSSES, ("f32_1d", "f32_1d"), X.ptr, W.ptr, ts.ptr)
 
     def entry_vocab_xent_grad_f16(self, X, W, ts, losses, lses, dls):
         """Its gradients (dX, dW); losses and lses as entry_vocab_xent_f16 returned them."""
+        if X.tname != "f16_2d" or W.tname != "f16_2d" or ts.tname != "i32_1d" or not losses.tname == lses.tname == dls.tname == "f32_1d":
+            _wrong_types((X, W, ts, losses, lses, dls), "f16_2d", "f16_2d", "i32_1d", "f32_1d", "f32_1d", "f32_1d")
         return self._entry_rec("vocab_xent_grad_f16", GRADS_F16, ("f16_2d", "f16_2d"), X.ptr, W.ptr, ts.ptr, losses.ptr, lses.ptr, dls.ptr)
 
     def entry_topk_distill(self, t, tau, S, iss, T):
         """Distillation of a student's logits S (t: "f32" or "f16") from a teacher's top logits T at words iss: (losses, lses)."""
+        if S.tname != t + "_2d" or iss.tname != "i32_2d" or T.tname != "f32_2d":
+            _wrong_types((S, iss, T), t + "_2d", "i32_2d", "f32_2d")
         return self._entry_rec("topk_distill_" + t, LOSSES, ("f32_1d", "f32_1d"), tau, S.ptr, iss.ptr, T.ptr, float_first=True)
 
     def entry_topk_distill_grad(self, t, tau, S, iss, T, lses, dls):
+        if S.tname != t + "_2d" or iss.tname != "i32_2d" or T.tname != "f32_2d" or not lses.tname == dls.tname == "f32_1d":
+            _wrong_types((S, iss, T, lses, dls), t + "_2d", "i32_2d", "f32_2d", "f32_1d", "f32_1d")
         return self._entry_one("topk_distill_grad_" + t, t + "_2d", tau, S.ptr, iss.ptr, T.ptr, lses.ptr, dls.ptr, float_first=True)
 
     def entry_router_balance(self, t, R, keep, iss):
         """The balance loss of a router's logits R (t: "f32" or "f16"): (loss, counts, norm)."""
+        if R.tname != t + "_2d" or keep.tname != "bool_1d" or iss.tname != "i32_2d":
+            _wrong_types((R, keep, iss), t + "_2d", "bool_1d", "i32_2d")
         return self._entry_rec("router_balance_" + t, BALANCE, ("f32_1d", "i32_1d", "f32_1d"), R.ptr, keep.ptr, iss.ptr)
 
     def entry_router_balance_grad(self, t, R, keep, counts, norm, dl):
+        if R.tname != t + "_2d" or keep.tname != "bool_1d" or counts.tname != "i32_1d" or not norm.tname == dl.tname == "f32_1d":
+            _wrong_types((R, keep, counts, norm, dl), t + "_2d", "bool_1d", "i32_1d", "f32_1d", "f32_1d")
         return self._entry_one("router_balance_grad_" + t, t + "_2d", R.ptr, keep.ptr, counts.ptr, norm.ptr, dl.ptr)
 
     def entry_mss_i32(self, xs):

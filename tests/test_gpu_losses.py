@@ -123,6 +123,12 @@ def test_vocab_xent_nan_and_infinity_stay(ctx):
     assert np.isnan(half(dx)[7]).all() and np.isfinite(np.delete(half(dx), 7, axis=0)).all() and np.isnan(half(dw)).all()
 
 
+@pytest.mark.parametrize("n,v,d", [(2, 70000, 8), (17, 9000, 40), (18, 9000, 40), (19, 9000, 40), (18, 1, 8)])
+def test_vocab_xent_of_few_tokens(ctx, n, v, d):
+    # losses of up to 18 tokens are made by the last CTA of the contraction
+    check_xent(ctx, *xent_inputs(n, v, d, n + v))
+
+
 @pytest.mark.parametrize("n,v,d", [(0, 5, 8), (5, 0, 8), (5, 7, 0), (0, 0, 0)])
 def test_vocab_xent_of_nothing(ctx, n, v, d):
     X, W, ts, dl = xent_inputs(n, v, d, 1)
@@ -265,6 +271,18 @@ def test_topk_distill_rows_at_any_address(ctx, t, shift):
         a.free()
 
 
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("n,v,k", [
+    (16, 3000, 40), (17, 3000, 40), (16, 3000, 256), (16, 3000, 257), (1, 261888, 9), (1, 263000, 9), (3, 300000, 200), (592, 5000, 33), (600, 9000, 256)])
+def test_topk_distill_of_few_rows(ctx, t, n, v, k):
+    # few rows, words and runs are finished by the kernels that read the logits: both sides of each limit
+    S, iss, T, dl = distill_inputs(t, n, v, k, n + v + k)
+    iss[:, k // 2:] = iss[:, :k - k // 2][:, ::-1]                # every word twice, most of them far apart
+    if n > 2:
+        iss[1] = -1
+    check_distill(ctx, t, 1.7, S, iss, T, dl)
+
+
 @pytest.mark.parametrize("n,v,k", [(0, 5, 2), (4, 0, 2), (4, 5, 0)])
 def test_topk_distill_of_nothing(ctx, n, v, k):
     S, iss, T, dl = distill_inputs("f32", n, v, k, 1)
@@ -349,6 +367,14 @@ def test_router_balance_with_nothing_to_count(ctx, keep, expert):
     assert loss[0] == 0 and norm[0] == 0 and not counts.any()
     g = fb.router_balance_grad(ctx, "f32", R, np.full(30, keep), counts, norm, np.ones(1, np.float32))
     assert not g.any()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("e", [1, 3, 8, 60, 64, 255, 256, 1000, 1024])
+def test_router_balance_partial_results_joined_either_way(ctx, t, e):
+    # by the last CTA where there are few of them, by a kernel of their own where there are many
+    for n in (1, 33, 1500, 9000):
+        check_router(ctx, t, *router_inputs(t, n, e, min(3, e), n + e), 0.7)
 
 
 @pytest.mark.parametrize("n,e,k", [(0, 4, 2), (4, 0, 2), (4, 4, 0)])
@@ -486,6 +512,23 @@ def test_vocab_xent_beyond_32_bit_offsets(ctx, n, v, d):
     for a in [loss, lse, gx, gw] + ins:
         a.free()
     ctx.clear_caches()
+
+
+def test_losses_between_other_reductions(ctx):
+    # they share the context's scratch words, each of which is 0 again when a kernel ends
+    S, iss, T, dl = distill_inputs("f16", 3, 2000, 5, 1)
+    X, W, ts, dls = xent_inputs(4, 900, 24, 2)
+    R, keep, ie = router_inputs("f32", 50, 12, 2, 3)
+    xs = np.arange(50000, dtype=np.int32)
+    first = None
+    for _ in range(3):
+        out = [*fb.topk_distill(ctx, "f16", 2.0, S, iss, T), *fb.vocab_xent_f16(ctx, X, W, ts), *fb.router_balance(ctx, "f32", R, keep, ie)]
+        assert fb.reduce_i32(ctx, xs) == xs.sum()
+        dot = fb.dotprod_f32(ctx, xs.astype(np.float32), np.full(len(xs), 2.0 ** -10, np.float32))
+        assert abs(dot - xs.sum() / 1024) <= len(xs) * 2.0 ** -24 * xs.sum() / 1024       # positive terms, whatever their order
+        first = first or out
+        for a, b in zip(first, out):
+            assert np.array_equal(np.asarray(a), np.asarray(b))
 
 
 def test_two_contexts_at_once(ctx):

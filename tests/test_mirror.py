@@ -70,3 +70,28 @@ def test_a_context_that_did_not_come_up_refuses(bare):
         fb._entries["topk_distill_grad_f32", True, "", 0](bare, "one", s, i, s, t, t)
     for name, x in (("f16_2d", a), ("i32_1d", t), ("f32_2d", s), ("i32_2d", i)):
         assert fb._type_fns[name].free(bare, x) == 0
+
+
+def test_loss_entry_points_check_the_types_of_arrays():
+    ctx = fb.Context.__new__(fb.Context)
+    ctx.ptr = None                           # a closed one: whatever passes the check of types is refused there
+    wanted = {
+        "entry_vocab_xent_f16": ((), ("f16_2d", "f16_2d", "i32_1d")),
+        "entry_vocab_xent_grad_f16": ((), ("f16_2d", "f16_2d", "i32_1d", "f32_1d", "f32_1d", "f32_1d")),
+        "entry_topk_distill": (("f16", 1.0), ("f16_2d", "i32_2d", "f32_2d")),
+        "entry_topk_distill_grad": (("f32", 1.0), ("f32_2d", "i32_2d", "f32_2d", "f32_1d", "f32_1d")),
+        "entry_router_balance": (("f32",), ("f32_2d", "bool_1d", "i32_2d")),
+        "entry_router_balance_grad": (("f16",), ("f16_2d", "bool_1d", "i32_1d", "f32_1d", "f32_1d")),
+    }
+
+    def arrays(types):
+        return [fb.Array(ctx, t, None) for t in types]
+
+    for name, (head, types) in wanted.items():
+        for i in range(len(types)):
+            for other in ("f32_2d", "f16_2d", "i32_1d", "f32_1d", "f64_2d"):
+                if other != types[i]:
+                    with pytest.raises(TypeError, match="arrays of types"):
+                        getattr(ctx, name)(*head, *arrays(types[:i] + (other,) + types[i + 1:]))
+        with pytest.raises((TypeError, ValueError), match="(?!arrays of types)"):
+            getattr(ctx, name)(*head, *arrays(types))
