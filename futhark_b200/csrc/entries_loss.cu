@@ -30,7 +30,12 @@ struct Call {
   struct Made { void *obj; memblock_device *mem; };
   Made made[4];
   int count = 0;
-  explicit Call(futhark_context *c) : ctx(c) {}
+  // A captured call would write, at every replay, blocks that the pool has meanwhile given to others.
+  explicit Call(futhark_context *c) : ctx(c) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c->stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone)
+      rc = refuse(c, "Error: entry points that allocate their results cannot be captured.\n");
+  }
 
   template <typename ARR>
   ARR *array(std::initializer_list<int64_t> shape, size_t elem, const char *desc) {

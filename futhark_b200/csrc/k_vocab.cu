@@ -492,6 +492,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     }
   }
   // ---------------- teardown: every thread of both CTAs arrives here, whatever happened ----------------
+  // A role that gave up has waited its whole limit after the last copy it issued; stores are waited for above.
   __syncwarp();
   tc_fence_before();
   __syncthreads();

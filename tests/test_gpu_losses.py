@@ -555,6 +555,32 @@ def refused(ctx, call, text):
     assert text in str(e.value)
 
 
+def test_captured_calls_are_refused(ctx):
+    import torch
+    X, W, ts, dl = xent_inputs(4, 100, 16, 1)
+    S, iss, T, dls = distill_inputs("f32", 3, 50, 4, 2)
+    R, keep, ie = router_inputs("f16", 9, 8, 2, 3)
+    x, w, t = ctx.new("f16_2d", X.view(np.uint16)), ctx.new("f16_2d", W.view(np.uint16)), ctx.new("i32_1d", ts)
+    l, d = ctx.new("f32_1d", dl), ctx.new("f32_1d", dls)
+    s, i, q = ctx.new("f32_2d", S), ctx.new("i32_2d", iss), ctx.new("f32_2d", T)
+    r, k, j = ctx.new("f16_2d", R.view(np.uint16)), ctx.new("bool_1d", keep), ctx.new("i32_2d", ie)
+    c, one = ctx.new("i32_1d", np.zeros(8, np.int32)), ctx.new("f32_1d", np.ones(1, np.float32))
+    ctx.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream)):
+        graph.capture_begin(capture_error_mode="relaxed")
+        try:
+            for call in (lambda: ctx.entry_vocab_xent_f16(x, w, t), lambda: ctx.entry_vocab_xent_grad_f16(x, w, t, l, l, l),
+                         lambda: ctx.entry_topk_distill("f32", 1.0, s, i, q), lambda: ctx.entry_topk_distill_grad("f32", 1.0, s, i, q, d, d),
+                         lambda: ctx.entry_router_balance("f16", r, k, j), lambda: ctx.entry_router_balance_grad("f16", r, k, c, one, one)):
+                refused(ctx, call, "cannot be captured")
+        finally:
+            graph.capture_end()
+    for a in (x, w, t, l, d, s, i, q, r, k, j, c, one):
+        a.free()
+    check_xent(ctx, X, W, ts, dl)
+
+
 def test_refusals(ctx):
     X, W, ts, dl = xent_inputs(4, 6, 8, 1)
     f = np.zeros(4, np.float32)
