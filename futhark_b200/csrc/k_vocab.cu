@@ -7,7 +7,7 @@
 //
 // A map-map-reduce contraction whose result is consumed by a (maximum, sum) reduction.  The logits stay in
 // tensor memory: the contraction's epilogue folds each 256 x 256 tile to one (maximum, sum) pair per
-// row, and a small kernel (for at most 18 tokens the last CTA) folds the v/256 pairs of a row.  The gradient works the vocabulary off in pieces: a
+// row, and a small kernel (in small calls the last CTA) folds the v/256 pairs of a row.  The gradient works the vocabulary off in pieces: a
 // piece's logits are computed again (the same instructions in the same order, so the same bits), turned into g in
 // binary16 in the epilogue, and that piece of g meets W (summed over the pieces in f32) and X.
 //
@@ -82,9 +82,10 @@ struct VocabArgs {
   int v, v0;                    // size of the vocabulary, first word of the piece
   float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum in units of log 2, sum)
   float *ztarget;
-  float *loss, *lse;            // and the results, where the kernel finishes them itself:
-  uint32_t *ticket;             // then a word that is 0 between launches
-  const float *cexp;            // VE_GRAD: per row the exponent's constant term
+  float *loss, *lse;            // and the results, where small calls finish them,
+  uint32_t *ticket;             // with a word that is 0 between launches
+  const float *cexp;            // VE_GRAD: per row the exponent's constant term, or, in small calls, what it comes from
+  const float *losses, *lses;
   const float *factor;          // VE_HALF
   const float *w;               // VE_ROWS
   int add;                      // VE_SLAB: add to the slab instead of writing it
@@ -115,15 +116,16 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs &a, uint32_t t, int &
   tm = (int)(g * V_GROUP + in - n * rows);
 }
 
-// A row's loss by one warp: fold of its (maximum, sum) pairs, eight per lane in flight; the last step in f64, where a loss near 0 is
-// a difference.
+// A row's loss by L neighbouring lanes: fold of its (maximum, sum) pairs, eight per lane in flight; the last step in f64, where a loss near 0 is
+// a difference.  All lanes of the warp come here, those of rows that do not exist with valid = false.
 __device__ __forceinline__ void row_loss(const float2 *part, int tiles, const float *ztarget, const int32_t *targets, float *loss, float *lse, int64_t row,
-                                         int64_t v, int lane) {
+                                         bool valid, int64_t v, int L) {
+  const int lane = threadIdx.x & (L - 1);
   float m = -INFINITY, s = 0.f;
-  for (int t0 = lane; t0 < tiles; t0 += 256) {
+  for (int t0 = lane; t0 < tiles; t0 += 8 * L) {
     float2 p[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) p[j] = t0 + 32 * j < tiles ? __ldcg(part + row * tiles + t0 + 32 * j) : make_float2(-INFINITY, 0.f);
+    for (int j = 0; j < 8; j++) p[j] = valid && t0 + L * j < tiles ? __ldcg(part + row * tiles + t0 + L * j) : make_float2(-INFINITY, 0.f);
     float mn = m;
 #pragma unroll
     for (int j = 0; j < 8; j++) mn = fmaxf(mn, p[j].x);
@@ -133,29 +135,43 @@ __device__ __forceinline__ void row_loss(const float2 *part, int tiles, const fl
     for (int j = 0; j < 8; j++) s += p[j].y * exp2f(p[j].x - ref);
     m = mn;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = L >> 1; o > 0; o >>= 1) {
     const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, s, o);
     const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.f : mn;
     s = s * exp2f(m - ref) + ps * exp2f(pm - ref);
     m = mn;
   }
-  if (lane == 0) {
+  if (lane == 0 && valid) {
     const double l = ((double)m + log2((double)s)) * 0.69314718055994530942;
     const int64_t t = targets[row];
     lse[row] = (float)l;
     loss[row] = t >= 0 && t < v ? (float)(l - (double)__ldcg(ztarget + row)) : 0.f;
   }
 }
+// Lanes of a row where one CTA makes all losses.
+static __host__ __device__ __forceinline__ int join_lanes(int64_t n) {
+  int L = 32;
+  while (L > 1 && n * L > V_THREADS) L >>= 1;
+  return L;
+}
+
+// q_i and the constant term of G's exponent
+__device__ __forceinline__ float row_q(float loss, float lse) {
+  // losses are off by a few units in the last place of lse: q below that is as good as that
+  const float least = 0x1p-22f * fmaxf(1.f, fabsf(lse)), q = -expm1f(-loss);
+  return q < least ? least : q;
+}
+__device__ __forceinline__ float row_exponent(float loss, float lse) { return 13.f - log2f(row_q(loss, lse)) - lse * V_LOG2E; }
 
 // A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
 // PAIR: two CTAs per tile of 256 rows; otherwise one per tile of 128 rows, for batches of at most 128 tokens.  Of a pair's 256
 // rows those would leave half or more to zeros: 64 tokens against 131072 x 4096 weights took 185 us, which is what the tensor
 // cores need for 256 rows, where the weights can be read in 164.
-template <bool PAIR, bool A_MN, bool B_MN, int EPI>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(V_THREADS, 1)
-vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmC, const VocabArgs a) {
+// SMALL: folding also makes the losses, G's exponents come from the losses and not from a kernel before it.  Either in every call
+// made the loops 2 to 3 % slower, by other registers alone (2048 x 50000 x 256: G 59.7 -> 61.7 us).
+template <bool PAIR, bool A_MN, bool B_MN, int EPI, bool SMALL>
+__device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, const VocabArgs &a, uint32_t block,
+                                               uint32_t blocks) {
   constexpr int V_STAGES = VocabShape<PAIR, EPI>::stages, V_STAGE = VocabShape<PAIR, EPI>::stage, MT = VocabShape<PAIR, EPI>::rows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -164,7 +180,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
-  const uint32_t pair = PAIR ? blockIdx.x >> 1 : blockIdx.x, npairs = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const uint32_t pair = PAIR ? block >> 1 : block, npairs = PAIR ? blocks >> 1 : blocks;
   const uint32_t num_tiles = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n * (uint32_t)a.splits;     // below 2^31
 
   if (tid == 0) {
@@ -306,7 +322,7 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int r = m * MT + (int)rank * 128 + quarter * 32 + lane;
         if (PER_ROW && r < a.M) {
           next_target = a.targets[r];
-          if (EPI == VE_GRAD) next_c = a.cexp[r];
+          if (EPI == VE_GRAD) next_c = SMALL ? row_exponent(a.losses[r], a.lses[r]) : a.cexp[r];
           if (EPI == VE_ROWS) next_c = a.w[r];
         }
       };
@@ -497,16 +513,18 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   if (PAIR) cluster_meet();                            // nobody signals into a partner that has left
-  if (EPI == VE_SOFTMAX && !PAIR && a.ticket != nullptr) {
-    // the CTA that ends last makes the losses, a row per warp
+  if (EPI == VE_SOFTMAX && SMALL) {
+    // the CTA that ends last makes the losses
     if (tid == 0) {
       __threadfence();
-      bars->last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+      bars->last = atomicAdd(a.ticket, 1u) == blocks - 1;
     }
     __syncthreads();
     if (bars->last) {
       __threadfence();
-      if (warp < a.M) row_loss(a.part, a.tiles_n, a.ztarget, a.targets, a.loss, a.lse, warp, a.v, lane);
+      const int L = join_lanes(a.M), row = tid / L;      // in one turn
+      if (L == 32) row_loss(a.part, a.tiles_n, a.ztarget, a.targets, a.loss, a.lse, row, row < a.M, a.v, 32);
+      else row_loss(a.part, a.tiles_n, a.ztarget, a.targets, a.loss, a.lse, row, row < a.M, a.v, L);
       if (tid == 0) *a.ticket = 0;
     }
   }
@@ -517,67 +535,101 @@ vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   }
 }
 
+struct VocabRows {
+  const __half *x;
+  int64_t n, dp, v;
+  const int32_t *targets;
+  const float *loss, *lse, *dl;
+  float *w, *factor;
+  float *cexp;                                       // or nullptr
+  __half *out;
+};
+// w_i = dl_i q_i and the constant term of G's exponent; false for a token without a target
+__device__ __forceinline__ bool row_weight(const VocabRows &a, int64_t i, float &w, float &c) {
+  const int64_t t = __ldg(a.targets + i);
+  const float ls = __ldg(a.loss + i), l = __ldg(a.lse + i), d = __ldg(a.dl + i);
+  const bool counts = t >= 0 && t < a.v;
+  w = counts ? d * row_q(ls, l) : 0.f;
+  c = counts ? row_exponent(ls, l) : 0.f;
+  return counts;
+}
+// Per row w_i, the exponent's constant, and X_i w_i 2^-(E+1) in binary16 (0 without a target), a warp per row.  E is over all rows: every CTA
+// finds it for itself, which costs it a step per n / threads rows and saves a kernel.  *factor = 2^(E+1-13).
+template <int THREADS>
+__device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, uint32_t blocks) {
+  __shared__ int tops[32];
+  constexpr int warps = THREADS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  chain_wait();
+  int top = -200;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < a.n; i += THREADS) {
+    float wi, ci;
+    row_weight(a, i, wi, ci);
+    if (wi != 0.f && isfinite(wi)) top = max(top, ilogbf(wi));
+  }
+  top = __reduce_max_sync(kFull, top);
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  top = __reduce_max_sync(kFull, lane < warps ? tops[lane] : -200);
+  const int e = top == -200 ? 0 : top;
+  if (block == 0 && threadIdx.x == 0) *a.factor = ldexpf(1.f, e + 1 - 13);
+  const int64_t per = a.dp / 8;
+  for (int64_t i = (int64_t)block * warps + warp; i < a.n; i += (int64_t)blocks * warps) {
+    float wi, ci;
+    const bool counts = row_weight(a, i, wi, ci);
+    if (lane == 0) {
+      a.w[i] = wi;
+      if (a.cexp != nullptr) a.cexp[i] = ci;
+    }
+    const float f = ldexpf(wi, -(e + 1));
+#pragma unroll 4
+    for (int64_t c = lane; c < per; c += 32) {
+      __align__(16) __half h[8] = {};
+      if (counts) {
+        *reinterpret_cast<uint4 *>(h) = __ldg(reinterpret_cast<const uint4 *>(a.x + i * a.dp) + c);
+#pragma unroll
+        for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
+      }
+      reinterpret_cast<uint4 *>(a.out + i * a.dp)[c] = *reinterpret_cast<const uint4 *>(h);
+    }
+  }
+}
+__global__ void __launch_bounds__(1024) vocab_rows_kernel(const VocabRows a) { vocab_rows<1024>(a, blockIdx.x, gridDim.x); }
+
+template <bool PAIR, bool A_MN, bool B_MN, int EPI, bool SMALL = false>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(V_THREADS, 1)
+vocab_mma_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmC, const VocabArgs a) {
+  vocab_mma_body<PAIR, A_MN, B_MN, EPI, SMALL>(tmA, tmB, tmC, a, blockIdx.x, gridDim.x);
+}
+
+// G of a small call, and in the CTAs behind the first `blocks`, which it leaves idle, the rows' weights and the scaled X that the products need.
+template <bool PAIR>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(V_THREADS, 1)
+vocab_grad_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmG,
+                  const VocabArgs a, const uint32_t blocks, const VocabRows r) {
+  if (blockIdx.x < blocks) vocab_mma_body<PAIR, false, false, VE_GRAD, true>(tmX, tmW, tmG, a, blockIdx.x, blocks);
+  else vocab_rows<V_THREADS>(r, blockIdx.x - blocks, gridDim.x - blocks);
+}
+
+// Both products of a small call side by side: dX in the first `blocks` CTAs, dW in the others.
+template <int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(V_THREADS, 1)
+vocab_products_kernel(const __grid_constant__ CUtensorMap tmGk, const __grid_constant__ CUtensorMap tmWn, const __grid_constant__ CUtensorMap tmX,
+                      const VocabArgs ax, const uint32_t blocks, const __grid_constant__ CUtensorMap tmGm, const __grid_constant__ CUtensorMap tmXn,
+                      const __grid_constant__ CUtensorMap tmD, const VocabArgs aw) {
+  if (blockIdx.x < blocks) vocab_mma_body<true, false, true, EPI, true>(tmGk, tmWn, tmX, ax, blockIdx.x, blocks);
+  else vocab_mma_body<true, true, true, VE_HALF, true>(tmGm, tmXn, tmD, aw, blockIdx.x - blocks, gridDim.x - blocks);
+}
+
 // ---- the small kernels around it ------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
 vocab_loss_kernel(const float2 *__restrict__ part, int tiles, const float *__restrict__ ztarget, const int32_t *__restrict__ targets,
                   float *__restrict__ loss, float *__restrict__ lse, int64_t n, int64_t v) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   chain_wait();
-  if (row < n) row_loss(part, tiles, ztarget, targets, loss, lse, row, v, threadIdx.x & 31);
-}
-
-// w_i = dl_i q_i and the constant term of G's exponent; false for a token without a target
-__device__ __forceinline__ bool row_weight(const int32_t *targets, const float *loss, const float *lse, const float *dl, int64_t i, int64_t v, float &w,
-                                           float &c) {
-  const int64_t t = targets[i];
-  const float ls = loss[i], l = lse[i], d = dl[i];
-  // losses are off by a few units in the last place of lse: q below that is as good as that
-  const float least = 0x1p-22f * fmaxf(1.f, fabsf(l)), q0 = -expm1f(-ls), q = q0 < least ? least : q0;
-  const bool counts = t >= 0 && t < v;
-  w = counts ? d * q : 0.f;
-  c = counts ? 13.f - log2f(q) - l * V_LOG2E : 0.f;
-  return counts;
-}
-
-// Per row w_i and the exponent's constant, and X_i w_i 2^-(E+1) in binary16 (0 without a target).  E is over all rows: every CTA
-// finds it for itself, which costs it n / 1024 steps and saves a kernel.  *factor = 2^(E+1-13).
-__global__ void __launch_bounds__(1024)
-vocab_prep_kernel(const __half *__restrict__ x, int64_t n, int64_t dp, const int32_t *__restrict__ targets, int64_t v, const float *__restrict__ loss,
-                  const float *__restrict__ lse, const float *__restrict__ dl, float *__restrict__ w, float *__restrict__ cexp,
-                  float *__restrict__ factor, __half *__restrict__ out) {
-  __shared__ int tops[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  chain_wait();
-  int top = -200;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    float wi, ci;
-    row_weight(targets, loss, lse, dl, i, v, wi, ci);
-    if (wi != 0.f && isfinite(wi)) top = max(top, ilogbf(wi));
-  }
-  top = __reduce_max_sync(kFull, top);
-  if (lane == 0) tops[warp] = top;
-  __syncthreads();
-  top = __reduce_max_sync(kFull, tops[lane]);
-  const int e = top == -200 ? 0 : top;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *factor = ldexpf(1.f, e + 1 - 13);
-  const int64_t per = dp / 8;
-  for (int64_t i = (int64_t)blockIdx.x * 32 + warp; i < n; i += (int64_t)gridDim.x * 32) {
-    float wi, ci;
-    const bool counts = row_weight(targets, loss, lse, dl, i, v, wi, ci);
-    if (lane == 0) { w[i] = wi; cexp[i] = ci; }
-    const float f = ldexpf(wi, -(e + 1));
-#pragma unroll 4
-    for (int64_t c = lane; c < per; c += 32) {
-      __align__(16) __half h[8] = {};
-      if (counts) {
-        *reinterpret_cast<uint4 *>(h) = reinterpret_cast<const uint4 *>(x + i * dp)[c];
-#pragma unroll
-        for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
-      }
-      reinterpret_cast<uint4 *>(out + i * dp)[c] = *reinterpret_cast<const uint4 *>(h);
-    }
-  }
+  row_loss(part, tiles, ztarget, targets, loss, lse, row, row < n, v, 32);
 }
 
 // Rows of up to two matrices in another pitch, what is behind the narrower of the two 0 or left out; 8 elements of a result per thread.
@@ -670,9 +722,12 @@ static inline int elementwise_grid(int64_t items, int num_sms) {
 
 // Batches of at most 128 tokens go to single CTAs, where the tokens are the rows of the product.
 static inline bool small_batch(int64_t n) { return n <= 128; }
-// Batches whose losses the contraction's last CTA makes, a row per warp.  A kernel for them costs a launch: 1 x 32000 x 1024 takes 18.3 us per
-// call instead of 19, 16 x 131072 x 2048 the same either way.
-static inline bool tiny_batch(int64_t n) { return n <= V_THREADS / 32; }
+// Whether the contraction's last CTA makes the losses: in one turn, which costs
+// less than a kernel's launch (200 x 2000 x 512 forward: 17.1 us instead of 19.2).  Two turns cost more: 1000 x 2000 x 512, 20.4 to 21.9 us instead of 19.5.
+static bool last_makes_losses(int64_t n, int64_t tiles_n) {
+  const int64_t L = join_lanes(n);
+  return ceil_div(n, V_THREADS / L) * ceil_div(tiles_n, 8 * L) <= 1;
+}
 // Clocks of a block of 64 summed elements of a tile of `cols` columns: on pairs 512 for 256 columns at the tensor cores'
 // rate and a fifth of that for the rows' operand; on single CTAs what 148 of them leave each other of HBM, 24 bytes per clock.
 static inline double block_clocks(bool pair, int cols) { return pair ? (cols + 64) * 1.6 : cols * 5.3; }
@@ -694,11 +749,9 @@ static int tile_columns(bool pair, int64_t rows, int64_t cols, int64_t kblocks, 
 // Parts of the summed axis of dX = G W.  A small batch has fewer tiles than there are SMs, while its sum runs over the
 // vocabulary; each part costs a slab of f32 written and read again.  The estimate is in clocks, as above, with
 // 3000 per tile for its epilogue where nothing hides it, 6000 for the kernel that adds the slabs and 3600 bytes of HBM per clock.
-static int dx_splits(int64_t n, int64_t dp, int64_t kblocks, int num_sms, int *nt) {
+static int dx_splits(bool pair, int64_t workers, int64_t n, int64_t dp, int64_t kblocks, int *nt) {
   int best = 1;
   double best_cost = 0;
-  const bool pair = !small_batch(n);
-  const int64_t workers = pair ? num_sms / 2 : num_sms;
   for (int w = VT; w >= 128; w -= 128) {
     const int64_t tiles = ceil_div(n, pair ? 256 : 128) * ceil_div(dp, w);
     const int most = (int)(kblocks < 128 ? kblocks : 128);
@@ -737,7 +790,17 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
     p.nt = tile_columns(pair, n, p.piece < v ? p.piece : v, ceil_div(p.dp, VK), 64, num_sms);
     p.pieces = (int)ceil_div(v, p.piece);
-    p.splits = dx_splits(n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), num_sms, &p.ntd);
+    p.ntw = tile_columns(true, p.piece < v ? p.piece : v, p.dp, ceil_div(n, VK), 128, num_sms);
+    // Small calls: what the products need besides G is made beside it, and the products side by side, on CTAs that have nothing else
+    // to do.  Both products are then pairs' work, since all tensor-core instructions of a kernel are of one kind.  Both directions of 16 x 500
+    // x 64 take 34 us instead of 38.5, 1000 x 1000 x 200 36.5 instead of 40.5, 500 x 8000 x 1024 60.5 instead of 65.5.
+    const int64_t gtiles = ceil_div(n, pair ? 256 : 128) * ceil_div(v, p.nt), gctas = pair ? 2 * gtiles : gtiles;
+    const int64_t rctas = ceil_div(n, V_THREADS / 32), idle = pair ? (num_sms - gctas) / 2 * 2 : num_sms - gctas, wtiles = ceil_div(v, VT) * ceil_div(p.dp, p.ntw), pairs = num_sms / 2;
+    const int64_t want_rows = pair ? (rctas + 1) / 2 * 2 : rctas;
+    p.row_ctas = p.pieces == 1 && rctas <= 4 * idle ? (int)(want_rows < idle ? want_rows : idle) : 0;
+    p.together = p.pieces == 1 && wtiles + ceil_div(n, VT) * ceil_div(p.dp, VT) <= pairs;
+    const int64_t free = p.together ? pairs - wtiles : pair ? pairs : num_sms;
+    p.splits = dx_splits(pair || p.together, free, n, p.dp, ceil_div(p.piece < v ? p.piece : v, VK), &p.ntd);
     p.w = take((size_t)n * 4);
     p.cexp = take((size_t)n * 4);
     p.scalars = take(256);
@@ -752,26 +815,49 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   return p;
 }
 
-template <bool PAIR, bool A_MN, bool B_MN, int EPI>
+// Fills in the tiles of a product; the CTAs that work on them, of at most `most`.
+static int tile_ctas(bool pair, VocabArgs &a, int most) {
+  a.tiles_m = (int)ceil_div(a.M, pair ? 256 : 128);
+  a.tiles_n = (int)ceil_div(a.N, a.nt);
+  a.kps = (int)ceil_div(a.kblocks, a.splits);
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits, workers = pair ? most / 2 : most;
+  return (int)(tiles < workers ? tiles : workers) * (pair ? 2 : 1);
+}
+template <bool PAIR, bool A_MN, bool B_MN, int EPI, bool SMALL = false>
 static cudaError_t launch_tiles(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, VocabArgs a, int num_sms, cudaStream_t stream) {
   constexpr int smem = VocabShape<PAIR, EPI>::smem;
-  auto kernel = vocab_mma_kernel<PAIR, A_MN, B_MN, EPI>;
+  auto kernel = vocab_mma_kernel<PAIR, A_MN, B_MN, EPI, SMALL>;
   static unsigned long long allowed = 0;
   const cudaError_t err = allow_smem(reinterpret_cast<const void *>(kernel), smem, allowed);
   if (err != cudaSuccess) return err;
-  a.tiles_m = (int)ceil_div(a.M, VocabShape<PAIR, EPI>::rows);
-  a.tiles_n = (int)ceil_div(a.N, a.nt);
-  a.kps = (int)ceil_div(a.kblocks, a.splits);
-  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
-  int64_t workers = PAIR ? num_sms / 2 : num_sms;
-  if (tiles < workers) workers = tiles;
-  return launch_after(kernel, (unsigned)((PAIR ? 2 : 1) * workers), V_THREADS, smem, stream, tmA, tmB, tmC, a);
+  const int ctas = tile_ctas(PAIR, a, num_sms);
+  return launch_after(kernel, (unsigned)ctas, V_THREADS, smem, stream, tmA, tmB, tmC, a);
+}
+template <bool PAIR>
+static cudaError_t launch_grad(const CUtensorMap &tmX, const CUtensorMap &tmW, const CUtensorMap &tmG, VocabArgs a, const VocabRows &rows, int row_ctas,
+                               int num_sms, cudaStream_t stream) {
+  constexpr int smem = VocabShape<PAIR, VE_GRAD>::smem;
+  static unsigned long long allowed = 0;
+  const cudaError_t err = allow_smem(reinterpret_cast<const void *>(vocab_grad_kernel<PAIR>), smem, allowed);
+  if (err != cudaSuccess) return err;
+  const int ctas = tile_ctas(PAIR, a, num_sms);
+  return launch_after(vocab_grad_kernel<PAIR>, (unsigned)(ctas + row_ctas), V_THREADS, smem, stream, tmX, tmW, tmG, a, (uint32_t)ctas, rows);
+}
+template <int EPI>
+static cudaError_t launch_products(const CUtensorMap &tmGk, const CUtensorMap &tmWn, const CUtensorMap &tmX, VocabArgs ax, const CUtensorMap &tmGm,
+                                   const CUtensorMap &tmXn, const CUtensorMap &tmD, VocabArgs aw, int num_sms, cudaStream_t stream) {
+  constexpr int sx = VocabShape<true, EPI>::smem, sw = VocabShape<true, VE_HALF>::smem, smem = sx > sw ? sx : sw;
+  static unsigned long long allowed = 0;
+  const cudaError_t err = allow_smem(reinterpret_cast<const void *>(vocab_products_kernel<EPI>), smem, allowed);
+  if (err != cudaSuccess) return err;
+  const int wctas = tile_ctas(true, aw, num_sms), xctas = tile_ctas(true, ax, num_sms - wctas);
+  return launch_after(vocab_products_kernel<EPI>, (unsigned)(xctas + wctas), V_THREADS, smem, stream, tmGk, tmWn, tmX, ax, (uint32_t)xctas, tmGm, tmXn, tmD, aw);
 }
 // products whose rows are tokens
-template <bool B_MN, int EPI>
+template <bool B_MN, int EPI, bool SMALL = false>
 static cudaError_t launch_tokens(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, const VocabArgs &a, int num_sms, cudaStream_t stream) {
-  return small_batch(a.M) ? launch_tiles<false, false, B_MN, EPI>(tmA, tmB, tmC, a, num_sms, stream)
-                          : launch_tiles<true, false, B_MN, EPI>(tmA, tmB, tmC, a, num_sms, stream);
+  return small_batch(a.M) ? launch_tiles<false, false, B_MN, EPI, SMALL>(tmA, tmB, tmC, a, num_sms, stream)
+                          : launch_tiles<true, false, B_MN, EPI, SMALL>(tmA, tmB, tmC, a, num_sms, stream);
 }
 
 // an operand [rows][cols] of row pitch `pitch`, in boxes of 64 columns and `box` rows: 64 where it is read across the sum
@@ -823,11 +909,9 @@ cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, void *ticket,
   a.part = reinterpret_cast<float2 *>(ws + p.part);
   a.ztarget = reinterpret_cast<float *>(ws + p.zt);
   a.failure = failure;
-  if (tiny_batch(n)) {
-    a.loss = loss; a.lse = lse; a.ticket = reinterpret_cast<uint32_t *>(ticket);
-  }
+  a.loss = loss; a.lse = lse; a.ticket = reinterpret_cast<uint32_t *>(ticket);
+  if (last_makes_losses(n, ceil_div(v, p.nt))) return launch_tokens<false, VE_SOFTMAX, true>(tmX, tmW, tmX, a, num_sms, stream);
   FB_TRY((launch_tokens<false, VE_SOFTMAX>(tmX, tmW, tmX, a, num_sms, stream)));
-  if (tiny_batch(n)) return cudaSuccess;
   return launch_after(vocab_loss_kernel, (unsigned)ceil_div(n, 8), 256, 0, stream, a.part, (int)ceil_div(v, p.nt), a.ztarget, targets, loss, lse, n, v);
 }
 
@@ -840,45 +924,53 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
     return cudaSuccess;
   }
   uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
-  float *rw = reinterpret_cast<float *>(ws + p.w), *cexp = reinterpret_cast<float *>(ws + p.cexp), *slabs = reinterpret_cast<float *>(ws + p.slabs);
-  float *factor = reinterpret_cast<float *>(ws + p.scalars);
+  float *rw = reinterpret_cast<float *>(ws + p.w), *slabs = reinterpret_cast<float *>(ws + p.slabs), *factor = reinterpret_cast<float *>(ws + p.scalars);
+  float *cexp = p.row_ctas == 0 ? reinterpret_cast<float *>(ws + p.cexp) : nullptr;
   uint16_t *xs = reinterpret_cast<uint16_t *>(ws + p.xs), *g = reinterpret_cast<uint16_t *>(ws + p.g);
   FB_TRY(operands(p, ws, x, w, n, v, d, num_sms, stream));
-  const int64_t row_ctas = ceil_div(n, 32);
-  FB_TRY(launch_after(vocab_prep_kernel, (unsigned)(row_ctas < 2 * num_sms ? row_ctas : 2 * num_sms), 1024, 0, stream, reinterpret_cast<const __half *>(x), n,
-                      p.dp, targets, v, loss, lse, dl, rw, cexp, factor, reinterpret_cast<__half *>(xs)));
+  const VocabRows rows = {reinterpret_cast<const __half *>(x), n, p.dp, v, targets, loss, lse, dl, rw, factor, cexp, reinterpret_cast<__half *>(xs)};
+  if (p.row_ctas == 0) {
+    const int64_t row_ctas = ceil_div(n, 32);
+    FB_TRY(launch_after(vocab_rows_kernel, (unsigned)(row_ctas < 2 * num_sms ? row_ctas : 2 * num_sms), 1024, 0, stream, rows));
+  }
   uint16_t *dxo = p.dp == d ? dx : reinterpret_cast<uint16_t *>(ws + p.dxp);
+  const bool small = small_batch(n);
+  const int xrows = small && !p.together ? token_rows(n) : 128;      // of dX's first operand
   for (int64_t v0 = 0; v0 < v; v0 += p.piece) {
     const int64_t vw = v - v0 < p.piece ? v - v0 : p.piece;
     CUtensorMap tmX, tmW, tmG, tmGk, tmWn, tmS, tmGm, tmXn, tmD;
     uint16_t *dwo = p.dp == d ? dw + v0 * d : reinterpret_cast<uint16_t *>(ws + p.dwp);
     VocabArgs a = {};
-    a.M = (int)n;
-    a.arows = token_rows(n);
-    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, a.arows) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, word_rows(n, p.nt)) &&
+    const bool ok = operand_map(&tmX, x, n, p.dp, p.dp, token_rows(n)) && operand_map(&tmW, w + v0 * p.dp, vw, p.dp, p.dp, word_rows(n, p.nt)) &&
                     make_tensor_map(&tmG, g, (uint64_t)vw, (uint64_t)n, 1, (uint64_t)p.piece, (uint64_t)p.piece * n, 64, 32) &&
-                    operand_map(&tmGk, g, n, vw, p.piece, a.arows) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, 64) &&
+                    operand_map(&tmGk, g, n, vw, p.piece, xrows) && operand_map(&tmWn, w + v0 * p.dp, vw, p.dp, p.dp, 64) &&
                     (p.direct ? make_tensor_map(&tmS, dxo, (uint64_t)p.dp, (uint64_t)n, 1, (uint64_t)p.dp, (uint64_t)(p.dp * n), 64, 32)
                               : make_tensor_map(&tmS, slabs, (uint64_t)p.dp, (uint64_t)n, (uint64_t)p.splits, (uint64_t)p.dp, (uint64_t)(p.dp * n), 32, 32, true)) &&
                     operand_map(&tmGm, g, n, vw, p.piece, 64) && operand_map(&tmXn, xs, n, p.dp, p.dp, 64) &&
                     make_tensor_map(&tmD, dwo, (uint64_t)p.dp, (uint64_t)vw, 1, (uint64_t)p.dp, (uint64_t)(p.dp * vw), 64, 32);
     if (!ok) return cudaErrorInvalidValue;
     a.failure = failure;
-    a.targets = targets; a.v = (int)v; a.v0 = (int)v0; a.cexp = cexp; a.factor = factor;
+    a.targets = targets; a.v = (int)v; a.v0 = (int)v0; a.cexp = cexp; a.losses = loss; a.lses = lse; a.factor = factor; a.w = rw;
     a.splits = 1;
-    a.N = (int)vw; a.kblocks = (int)ceil_div(p.dp, VK); a.nt = p.nt;
-    FB_TRY((launch_tokens<false, VE_GRAD>(tmX, tmW, tmG, a, num_sms, stream)));
+    a.M = (int)n; a.N = (int)vw; a.kblocks = (int)ceil_div(p.dp, VK); a.nt = p.nt; a.arows = token_rows(n);
+    if (p.row_ctas == 0) FB_TRY((launch_tokens<false, VE_GRAD>(tmX, tmW, tmG, a, num_sms, stream)));
+    else if (small) FB_TRY(launch_grad<false>(tmX, tmW, tmG, a, rows, p.row_ctas, num_sms, stream));
+    else FB_TRY(launch_grad<true>(tmX, tmW, tmG, a, rows, p.row_ctas, num_sms, stream));
+    VocabArgs ax = a, aw = a;
     // every part has its blocks in every piece: the last one may be shorter, and then some slabs get nothing more
-    a.N = (int)p.dp; a.kblocks = (int)ceil_div(vw, VK); a.nt = p.ntd;
-    a.splits = (int)ceil_div(a.kblocks, ceil_div(a.kblocks, p.splits < a.kblocks ? p.splits : a.kblocks));
-    a.add = v0 > 0;
-    a.w = rw;
-    if (p.direct) FB_TRY((launch_tokens<true, VE_ROWS>(tmGk, tmWn, tmS, a, num_sms, stream)));
-    else FB_TRY((launch_tokens<true, VE_SLAB>(tmGk, tmWn, tmS, a, num_sms, stream)));
-    a.M = (int)vw; a.N = (int)p.dp; a.kblocks = (int)ceil_div(n, VK); a.splits = 1; a.add = 0;
-    a.nt = tile_columns(true, vw, p.dp, a.kblocks, 128, num_sms);
-    a.arows = 128;
-    FB_TRY((launch_tiles<true, true, true, VE_HALF>(tmGm, tmXn, tmD, a, num_sms, stream)));
+    ax.N = (int)p.dp; ax.kblocks = (int)ceil_div(vw, VK); ax.nt = p.ntd; ax.arows = xrows;
+    ax.splits = (int)ceil_div(ax.kblocks, ceil_div(ax.kblocks, p.splits < ax.kblocks ? p.splits : ax.kblocks));
+    ax.add = v0 > 0;
+    aw.M = (int)vw; aw.N = (int)p.dp; aw.kblocks = (int)ceil_div(n, VK); aw.arows = 128;
+    aw.nt = p.ntw;
+    if (p.together) {
+      if (p.direct) FB_TRY((launch_products<VE_ROWS>(tmGk, tmWn, tmS, ax, tmGm, tmXn, tmD, aw, num_sms, stream)));
+      else FB_TRY((launch_products<VE_SLAB>(tmGk, tmWn, tmS, ax, tmGm, tmXn, tmD, aw, num_sms, stream)));
+    } else {
+      if (p.direct) FB_TRY((launch_tokens<true, VE_ROWS>(tmGk, tmWn, tmS, ax, num_sms, stream)));
+      else FB_TRY((launch_tokens<true, VE_SLAB>(tmGk, tmWn, tmS, ax, num_sms, stream)));
+      FB_TRY((launch_tiles<true, true, true, VE_HALF>(tmGm, tmXn, tmD, aw, num_sms, stream)));
+    }
     if (p.dp != d) {                               // and with the last piece's a finished dX
       const bool both = p.direct && v0 + vw == v;
       FB_TRY(repitch(pitch_job(dwo, dw + v0 * d, vw), pitch_job(dxo, dx, both ? n : 0), p.dp, d, num_sms, stream));

@@ -188,8 +188,10 @@ struct VocabPlan {
   bool copy_x, copy_w;         // operands that are copied: another width, or a base that is no multiple of 16 bytes
   int64_t piece;               // gradient: words per piece of the vocabulary
   int nt;                      // columns of a tile of logits
-  int splits, ntd;             // gradient: parts of the sum over a piece's words, columns of a tile of dX
+  int splits, ntd, ntw;        // gradient: parts of the sum over a piece's words, columns of a tile of dX and of dW
   int pieces;
+  int row_ctas;                // gradient: CTAs beside G's that make what the products need; 0: a kernel does
+  bool together;               // gradient: both products in one kernel
   bool direct;                 // gradient: dX leaves the tensor cores finished (one piece, one part)
   size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dxp, dwp, bytes;
 };

@@ -123,9 +123,12 @@ def test_vocab_xent_nan_and_infinity_stay(ctx):
     assert np.isnan(half(dx)[7]).all() and np.isfinite(np.delete(half(dx), 7, axis=0)).all() and np.isnan(half(dw)).all()
 
 
-@pytest.mark.parametrize("n,v,d", [(2, 70000, 8), (17, 9000, 40), (18, 9000, 40), (19, 9000, 40), (18, 1, 8)])
-def test_vocab_xent_of_few_tokens(ctx, n, v, d):
-    # losses of up to 18 tokens are made by the last CTA of the contraction
+@pytest.mark.parametrize("n,v,d", [
+    (2, 70000, 8), (17, 9000, 40), (18, 9000, 40), (19, 9000, 40), (18, 1, 8), (18, 66000, 8), (36, 30000, 16), (37, 30000, 16), (129, 4000, 24),
+    (576, 1020, 16), (577, 1020, 16), (576, 2060, 16), (10, 18688, 64), (10, 18689, 64), (200, 18432, 64), (200, 18433, 64), (5000, 100, 16),
+    (8192, 100, 16), (8192, 300, 16), (300, 9000, 264), (100, 2000, 2050)])
+def test_vocab_xent_small_calls(ctx, n, v, d):
+    # small calls make the losses in the last CTA of the contraction, the rows' weights beside G and both products side by side
     check_xent(ctx, *xent_inputs(n, v, d, n + v))
 
 
