@@ -32,6 +32,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "tcgen.cuh"
 
@@ -65,16 +67,16 @@ enum VocabEpilogue : int {
 constexpr int V_WARPS = 16, V_COLS = VT / (V_WARPS / 4), V_THREADS = 64 + 32 * V_WARPS;
 template <bool PAIR, int EPI> struct VocabShape {
   static constexpr int rows = PAIR ? 256 : 128;                     // of a tile
-  static constexpr int stage = PAIR ? 2 * V_OPERAND : 3 * V_OPERAND;
-  static constexpr int stages = PAIR ? (EPI == VE_SOFTMAX ? 6 : 5) : (EPI == VE_SOFTMAX ? 4 : 3);
+  static constexpr int room = (EPI == VE_SOFTMAX ? 12 : PAIR ? 10 : 9) * V_OPERAND;      // of the ring of stages
   static constexpr int staging = EPI == VE_SOFTMAX ? 2 * (V_WARPS / 4) * 128 * (int)sizeof(float2) : V_WARPS * V_EPI_BUF;
-  static constexpr int smem = stages * stage + 1024 /*alignment*/ + 1024 /*barriers*/ + staging;
+  static constexpr int smem = room + 1024 /*alignment*/ + 1024 /*barriers*/ + staging;
 };
 
 struct VocabArgs {
   int M, N, kblocks;            // extents; the summed axis in blocks of VK
   int nt;                       // columns of a tile: a multiple of 32 up to 256
   int arows;                    // rows of A that a CTA brings per stage
+  int block, sub, stages;       // bytes of a block of the sum, blocks of a stage, stages of the ring
   int halves;                   // VE_SOFTMAX: the sum in two accumulators
   int splits, kps;              // parts of the summed axis and the blocks of each
   int tiles_m, tiles_n;
@@ -92,7 +94,7 @@ struct VocabArgs {
   int *failure;
 };
 
-constexpr int V_MAX_STAGES = 8;
+constexpr int V_MAX_STAGES = 12;
 struct VocabBarriers {
   uint64_t full[V_MAX_STAGES];   // used in the pair's first CTA only
   uint64_t empty[V_MAX_STAGES];
@@ -172,13 +174,13 @@ __device__ __forceinline__ float row_exponent(float loss, float lse) { return 13
 template <bool PAIR, bool A_MN, bool B_MN, int EPI, bool SMALL>
 __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmC, const VocabArgs &a, uint32_t block,
                                                uint32_t blocks) {
-  constexpr int V_STAGES = VocabShape<PAIR, EPI>::stages, V_STAGE = VocabShape<PAIR, EPI>::stage, MT = VocabShape<PAIR, EPI>::rows;
+  constexpr int MT = VocabShape<PAIR, EPI>::rows, ROOM = VocabShape<PAIR, EPI>::room;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  VocabBarriers *bars = reinterpret_cast<VocabBarriers *>(smem + V_STAGES * V_STAGE);
-  uint8_t *epi = smem + V_STAGES * V_STAGE + 1024;
+  VocabBarriers *bars = reinterpret_cast<VocabBarriers *>(smem + ROOM);
+  uint8_t *epi = smem + ROOM + 1024;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
   const uint32_t pair = PAIR ? block >> 1 : block, npairs = PAIR ? blocks >> 1 : blocks;
   const uint32_t num_tiles = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n * (uint32_t)a.splits;     // below 2^31
@@ -187,7 +189,7 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
     prefetch_map(&tmA);
     prefetch_map(&tmB);
     if (EPI != VE_SOFTMAX) prefetch_map(&tmC);
-    for (int s = 0; s < V_STAGES; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+    for (int s = 0; s < a.stages; s++) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
     for (int i = 0; i < 2; i++) { mbar_init(&bars->tmem_full[i], 1); mbar_init(&bars->tmem_empty[i], (PAIR ? 2 : 1) * V_WARPS); }
     for (int i = 0; i < 8; i++) mbar_init(&bars->met[i >> 2][i & 3], V_WARPS / 4 - 1);
     fence_mbar_init();
@@ -196,9 +198,9 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
     // rows of the tile that no token has are 0, in every stage and from now on: the card runs at its power limit even where HBM is the bound, and
     // products of what else lies there cost clocks (64 x 131072 x 4096, call after call: 197 us, with zeros 190)
     const int per = (128 - a.arows) * 8;
-    for (int i = tid; i < V_STAGES * per; i += V_THREADS) {
+    for (int i = tid; i < a.stages * a.sub * per; i += V_THREADS) {
       const int st = i / per;
-      *reinterpret_cast<uint4 *>(smem + st * V_STAGE + a.arows * 128 + (i - st * per) * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4 *>(smem + st * a.block + a.arows * 128 + (i - st * per) * 16) = make_uint4(0, 0, 0, 0);
     }
     fence_proxy_async_smem();
   }
@@ -222,87 +224,105 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
   if (!poisoned) {
     if (warp == 0) {
       // ---------------- producer: this CTA's half of each operand ----------------
-      if (lane == 0) {
-        uint32_t it = 0;
-        bool ok = true;
-        for (uint32_t t = pair; t < num_tiles && ok; t += npairs) {
-          int split, tm, tn;
-          vocab_tile(a, t, split, tm, tn);
-          const int m0 = tm * MT + (int)rank * 128, n0 = tn * a.nt + (int)rank * (a.nt >> 1);
-          const int kb1 = min(a.kblocks, (split + 1) * a.kps);
-          for (int kb = split * a.kps; kb < kb1; kb++, it++) {
-            const int s = it % V_STAGES;
-            const uint32_t ph = (it / V_STAGES) & 1;
-            if (!mbar_wait_bounded(&bars->empty[s], ph ^ 1)) { ok = false; break; }
-            uint8_t *sa = smem + s * V_STAGE;
-            uint8_t *sb = sa + V_OPERAND;
-            uint64_t *full = &bars->full[s];
-            const uint32_t full0 = PAIR ? map_to_cta(smem_u32(full), 0) : 0;
-            auto load = [&](void *dst, const CUtensorMap *tm, int x, int y) {
-              if (PAIR) tma_load_3d_pair(dst, tm, x, y, 0, full0);
-              else tma_load_3d(dst, tm, x, y, 0, full);
-            };
-            if (rank == 0) mbar_expect_tx(full, ((PAIR ? 2 : 1) * a.arows + a.nt) * (VK * 2));     // both CTAs' bytes
-            if (A_MN) {
-              load(sa, &tmA, m0, kb * VK);
-              load(sa + V_SLAB, &tmA, m0 + 64, kb * VK);
-            } else {
-              load(sa, &tmA, kb * VK, m0);
-            }
-            if (B_MN) {
-              const int slabs = a.nt / (PAIR ? 128 : 64);
-              for (int j = 0; j < slabs; j++) load(sb + j * V_SLAB, &tmB, n0 + j * 64, kb * VK);
-            } else {
-              load(sb, &tmB, kb * VK, n0);
+      if (elect_one()) {
+        auto produce = [&](auto blocks_of_stage) {
+          constexpr int SUB = decltype(blocks_of_stage)::value;
+          int s = 0;
+          uint32_t ph = 0;
+          for (uint32_t t = pair; t < num_tiles; t += npairs) {
+            int split, tm, tn;
+            vocab_tile(a, t, split, tm, tn);
+            const int m0 = tm * MT + (int)rank * 128, n0 = tn * a.nt + (int)rank * (a.nt >> 1);
+            const int kb1 = min(a.kblocks, (split + 1) * a.kps);
+            for (int kb = split * a.kps; kb < kb1; kb += SUB) {
+              if (!mbar_wait_bounded(&bars->empty[s], ph ^ 1)) return false;
+              uint64_t *full = &bars->full[s];
+              const uint32_t full0 = PAIR ? map_to_cta(smem_u32(full), 0) : 0;
+              auto load = [&](void *dst, const CUtensorMap *tm, int x, int y) {
+                if (PAIR) tma_load_3d_pair(dst, tm, x, y, 0, full0);
+                else tma_load_3d(dst, tm, x, y, 0, full);
+              };
+              // both CTAs' bytes
+              if (rank == 0) mbar_expect_tx(full, min(SUB, kb1 - kb) * ((PAIR ? 2 : 1) * a.arows + a.nt) * (VK * 2));
+#pragma unroll
+              for (int u = 0; u < SUB; u++) {
+                if (kb + u >= kb1) break;
+                uint8_t *sa = smem + (s * SUB + u) * a.block, *sb = sa + V_OPERAND;
+                const int k0 = (kb + u) * VK;
+                if (A_MN) {
+                  load(sa, &tmA, m0, k0);
+                  load(sa + V_SLAB, &tmA, m0 + 64, k0);
+                } else {
+                  load(sa, &tmA, k0, m0);
+                }
+                if (B_MN) {
+                  const int slabs = a.nt / (PAIR ? 128 : 64);
+                  for (int j = 0; j < slabs; j++) load(sb + j * V_SLAB, &tmB, n0 + j * 64, k0);
+                } else {
+                  load(sb, &tmB, k0, n0);
+                }
+              }
+              if (++s == a.stages) { s = 0; ph ^= 1; }
             }
           }
-        }
+          return true;
+        };
+        const bool ok = a.sub == 2 ? produce(std::integral_constant<int, 2>()) : produce(std::integral_constant<int, 1>());
         if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
       }
     } else if (warp == 1) {
       // ---------------- MMA issuer: one thread of the first CTA ----------------
-      if (lane == 0 && rank == 0) {
+      if (rank == 0 && elect_one()) {
         // D = f32, A = B = f16, M the tile's rows, N its columns
         const uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(a.nt >> 3) << 17) | ((uint32_t)(MT >> 4) << 24);
-        uint32_t it = 0, tile_it = 0;
-        bool ok = true;
-        for (uint32_t t = pair; t < num_tiles && ok; t += npairs, tile_it++) {
-          int split, tm, tn;
-          vocab_tile(a, t, split, tm, tn);
-          const bool halves = EPI == VE_SOFTMAX && a.halves;
-          const uint32_t acc = halves ? 0 : tile_it & 1, acc_ph = (halves ? tile_it : tile_it >> 1) & 1;
-          if (!mbar_wait_bounded(&bars->tmem_empty[acc], acc_ph ^ 1)) { ok = false; break; }
-          tc_fence_after();
-          uint32_t d_tmem = tmem_base + acc * VT;
-          int kb0 = split * a.kps;
-          const int kb1 = min(a.kblocks, kb0 + a.kps), turn = halves ? (kb0 + kb1) / 2 : kb1;
-          for (int kb = kb0; kb < kb1; kb++, it++) {
-            const int s = it % V_STAGES;
-            const uint32_t ph = (it / V_STAGES) & 1;
-            if (!mbar_wait_bounded(&bars->full[s], ph)) { ok = false; break; }
+        // along the sum: rows of 128 bytes, 8-row groups 1024 bytes apart, a step of 16 is 32 bytes inside the
+        // swizzled row; across it: 64-wide slabs (leading), 8-row groups 1024 bytes apart, a step is 16 rows
+        const uint32_t sa = smem_u32(smem), sb = sa + V_OPERAND;
+        const uint64_t adesc0 = A_MN ? make_smem_desc(sa, V_SLAB, 1024) : make_smem_desc(sa, 16, 1024);
+        const uint64_t bdesc0 = B_MN ? make_smem_desc(sb, V_SLAB, 1024) : make_smem_desc(sb, 16, 1024);
+        auto issue = [&](auto blocks_of_stage) {
+          constexpr int SUB = decltype(blocks_of_stage)::value;
+          const uint32_t step = a.block >> 4;              // of a block, in a descriptor
+          int s = 0;
+          uint32_t ph = 0, tile_it = 0;
+          uint64_t adesc = adesc0, bdesc = bdesc0;
+          for (uint32_t t = pair; t < num_tiles; t += npairs, tile_it++) {
+            int split, tm, tn;
+            vocab_tile(a, t, split, tm, tn);
+            const bool halves = EPI == VE_SOFTMAX && a.halves;
+            const uint32_t acc = halves ? 0 : tile_it & 1, acc_ph = (halves ? tile_it : tile_it >> 1) & 1;
+            if (!mbar_wait_bounded(&bars->tmem_empty[acc], acc_ph ^ 1)) return false;
             tc_fence_after();
-            if (kb == turn) { d_tmem += VT; kb0 = kb; }      // the second half starts from nothing
-            const uint32_t sa = smem_u32(smem + s * V_STAGE);
-            const uint32_t sb = sa + V_OPERAND;
-            // along the sum: rows of 128 bytes, 8-row groups 1024 bytes apart, a step of 16 is 32 bytes inside the
-            // swizzled row; across it: 64-wide slabs (leading), 8-row groups 1024 bytes apart, a step is 16 rows
-            const uint64_t adesc = A_MN ? make_smem_desc(sa, V_SLAB, 1024) : make_smem_desc(sa, 16, 1024);
-            const uint64_t bdesc = B_MN ? make_smem_desc(sb, V_SLAB, 1024) : make_smem_desc(sb, 16, 1024);
+            uint32_t d_tmem = tmem_base + acc * VT, more = 0;
+            const int kb0 = split * a.kps, kb1 = min(a.kblocks, kb0 + a.kps), turn = halves ? (kb0 + kb1) / 2 : kb1;
+            for (int kb = kb0; kb < kb1; kb += SUB) {
+              if (!mbar_wait_bounded(&bars->full[s], ph)) return false;
+              tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < VK / 16; k++) {
-              const uint64_t ad = adesc + (uint64_t)(k * (A_MN ? 128 : 2)), bd = bdesc + (uint64_t)(k * (B_MN ? 128 : 2));
-              const uint32_t more = (kb > kb0 || k > 0) ? 1u : 0u;
-              if (PAIR) tc2_mma_f16(d_tmem, ad, bd, idesc, more);
-              else tc_mma_f16(d_tmem, ad, bd, idesc, more);
+              for (int u = 0; u < SUB; u++) {
+                if (kb + u >= kb1) break;
+                if (kb + u == turn) { d_tmem += VT; more = 0; }      // the second half starts from nothing
+                const uint64_t au = adesc + (uint64_t)(u * step), bu = bdesc + (uint64_t)(u * step);
+#pragma unroll
+                for (int k = 0; k < VK / 16; k++) {
+                  const uint64_t ad = au + (uint64_t)(k * (A_MN ? 128 : 2)), bd = bu + (uint64_t)(k * (B_MN ? 128 : 2));
+                  if (PAIR) tc2_mma_f16(d_tmem, ad, bd, idesc, k > 0 ? 1u : more);
+                  else tc_mma_f16(d_tmem, ad, bd, idesc, k > 0 ? 1u : more);
+                }
+                more = 1;
+              }
+              if (PAIR) tc2_commit_both(&bars->empty[s]);
+              else tc_commit(&bars->empty[s]);
+              adesc += SUB * step;
+              bdesc += SUB * step;
+              if (++s == a.stages) { s = 0; ph ^= 1; adesc = adesc0; bdesc = bdesc0; }
             }
-            if (PAIR) tc2_commit_both(&bars->empty[s]);
-            else tc_commit(&bars->empty[s]);
-          }
-          if (ok) {
             if (PAIR) tc2_commit_both(&bars->tmem_full[acc]);
             else tc_commit(&bars->tmem_full[acc]);
           }
-        }
+          return true;
+        };
+        const bool ok = a.sub == 2 ? issue(std::integral_constant<int, 2>()) : issue(std::integral_constant<int, 1>());
         if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);
       }
     } else {
@@ -728,17 +748,27 @@ static bool last_makes_losses(int64_t n, int64_t tiles_n) {
   const int64_t L = join_lanes(n);
   return ceil_div(n, V_THREADS / L) * ceil_div(tiles_n, 8 * L) <= 1;
 }
+// The ring: blocks of 128 rows of the first operand and a CTA's share of the tile's columns, in stages of two blocks where there is room for four of
+// those.  Half as many barriers and commits then: 1000 x 1000 x 8192 forward 28 us instead of 33.  With fewer stages than that they come too
+// late: three of two blocks instead of six took 3.9 ms instead of 3.75 for 4096 x 65536 x 2048.
+static inline int block_bytes(bool pair, int cols) { return V_OPERAND + (pair ? cols / 2 : cols) * VK * 2; }
+static inline int ring_blocks(int room, int block) { return room / block >= 8 ? 2 : 1; }
+static inline int ring_stages(int room, int stage) { return room / stage < V_MAX_STAGES ? room / stage : V_MAX_STAGES; }
 // Clocks of a block of 64 summed elements of a tile of `cols` columns: on pairs 512 for 256 columns at the tensor cores'
 // rate and a fifth of that for the rows' operand; on single CTAs what 148 of them leave each other of HBM, 24 bytes per clock.
-static inline double block_clocks(bool pair, int cols) { return pair ? (cols + 64) * 1.6 : cols * 5.3; }
+// However narrow the tile, a block takes its issuer 330, in stages of two blocks 230.
+static inline double block_clocks(bool pair, int cols) {
+  const double c = pair ? (cols + 64) * 1.6 : cols * 5.3, least = ring_blocks(10 * V_OPERAND, block_bytes(pair, cols)) == 2 ? 230 : 330;
+  return c < least ? least : c;
+}
 
 // Columns of a tile.  A tile of fewer columns reuses its rows less, but a number of tiles that is just above a multiple of
 // the number of CTAs or pairs leaves most of them idle in the last round.
-static int tile_columns(bool pair, int64_t rows, int64_t cols, int64_t kblocks, int step, int num_sms) {
+static int tile_columns(bool pair, int64_t rows, int64_t cols, int64_t kblocks, int step, int least, int num_sms) {
   int best = VT;
   double best_cost = 0;
   const int64_t workers = pair ? num_sms / 2 : num_sms;
-  for (int nt = VT; nt >= 128; nt -= step) {
+  for (int nt = VT; nt >= least; nt -= step) {
     const int64_t tiles = ceil_div(rows, pair ? 256 : 128) * ceil_div(cols, nt);
     const double cost = (double)ceil_div(tiles, workers) * (kblocks * block_clocks(pair, nt) + 1500.0);
     if (nt == VT || cost < 0.97 * best_cost) { best = nt; best_cost = cost; }
@@ -777,7 +807,7 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   p.xp = p.copy_x ? take((size_t)(n * p.dp) * 2) : 0;
   p.wp = p.copy_w ? take((size_t)(v * p.dp) * 2) : 0;
   if (!grad) {
-    p.nt = tile_columns(pair, n, v, ceil_div(p.dp, VK), 32, num_sms);
+    p.nt = tile_columns(pair, n, v, ceil_div(p.dp, VK), 32, 32, num_sms);
     p.part = take((size_t)(n * ceil_div(v, p.nt)) * sizeof(float2));
     p.zt = take((size_t)n * 4);
   } else {
@@ -788,9 +818,9 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     if (words < VT) words = VT;
     if (words > want) words = want;
     p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
-    p.nt = tile_columns(pair, n, p.piece < v ? p.piece : v, ceil_div(p.dp, VK), 64, num_sms);
+    p.nt = tile_columns(pair, n, p.piece < v ? p.piece : v, ceil_div(p.dp, VK), 64, 64, num_sms);
     p.pieces = (int)ceil_div(v, p.piece);
-    p.ntw = tile_columns(true, p.piece < v ? p.piece : v, p.dp, ceil_div(n, VK), 128, num_sms);
+    p.ntw = tile_columns(true, p.piece < v ? p.piece : v, p.dp, ceil_div(n, VK), 128, 128, num_sms);
     // Small calls: what the products need besides G is made beside it, and the products side by side, on CTAs that have nothing else
     // to do.  Both products are then pairs' work, since all tensor-core instructions of a kernel are of one kind.  Both directions of 16 x 500
     // x 64 take 34 us instead of 38.5, 1000 x 1000 x 200 36.5 instead of 40.5, 500 x 8000 x 1024 60.5 instead of 65.5.
@@ -816,7 +846,10 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
 }
 
 // Fills in the tiles of a product; the CTAs that work on them, of at most `most`.
-static int tile_ctas(bool pair, VocabArgs &a, int most) {
+static int tile_ctas(bool pair, int room, VocabArgs &a, int most) {
+  a.block = block_bytes(pair, a.nt);
+  a.sub = ring_blocks(room, a.block);
+  a.stages = ring_stages(room, a.block * a.sub);
   a.tiles_m = (int)ceil_div(a.M, pair ? 256 : 128);
   a.tiles_n = (int)ceil_div(a.N, a.nt);
   a.kps = (int)ceil_div(a.kblocks, a.splits);
@@ -830,7 +863,7 @@ static cudaError_t launch_tiles(const CUtensorMap &tmA, const CUtensorMap &tmB, 
   static unsigned long long allowed = 0;
   const cudaError_t err = allow_smem(reinterpret_cast<const void *>(kernel), smem, allowed);
   if (err != cudaSuccess) return err;
-  const int ctas = tile_ctas(PAIR, a, num_sms);
+  const int ctas = tile_ctas(PAIR, VocabShape<PAIR, EPI>::room, a, num_sms);
   return launch_after(kernel, (unsigned)ctas, V_THREADS, smem, stream, tmA, tmB, tmC, a);
 }
 template <bool PAIR>
@@ -840,7 +873,7 @@ static cudaError_t launch_grad(const CUtensorMap &tmX, const CUtensorMap &tmW, c
   static unsigned long long allowed = 0;
   const cudaError_t err = allow_smem(reinterpret_cast<const void *>(vocab_grad_kernel<PAIR>), smem, allowed);
   if (err != cudaSuccess) return err;
-  const int ctas = tile_ctas(PAIR, a, num_sms);
+  const int ctas = tile_ctas(PAIR, VocabShape<PAIR, VE_GRAD>::room, a, num_sms);
   return launch_after(vocab_grad_kernel<PAIR>, (unsigned)(ctas + row_ctas), V_THREADS, smem, stream, tmX, tmW, tmG, a, (uint32_t)ctas, rows);
 }
 template <int EPI>
@@ -850,7 +883,7 @@ static cudaError_t launch_products(const CUtensorMap &tmGk, const CUtensorMap &t
   static unsigned long long allowed = 0;
   const cudaError_t err = allow_smem(reinterpret_cast<const void *>(vocab_products_kernel<EPI>), smem, allowed);
   if (err != cudaSuccess) return err;
-  const int wctas = tile_ctas(true, aw, num_sms), xctas = tile_ctas(true, ax, num_sms - wctas);
+  const int wctas = tile_ctas(true, VocabShape<true, VE_HALF>::room, aw, num_sms), xctas = tile_ctas(true, VocabShape<true, EPI>::room, ax, num_sms - wctas);
   return launch_after(vocab_products_kernel<EPI>, (unsigned)(xctas + wctas), V_THREADS, smem, stream, tmGk, tmWn, tmX, ax, (uint32_t)xctas, tmGm, tmXn, tmD, aw);
 }
 // products whose rows are tokens
