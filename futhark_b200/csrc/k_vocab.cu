@@ -26,8 +26,8 @@
 // memory so that the epilogue of a tile runs under the next tile's instructions.  The operands are taken
 // as they lie in memory, contiguous along the summed axis or across it: no transposition.
 //
-// 4096 x 65536 x 2048, one at a time: logits folded 706 us (1556 Tflop/s), G 733, dX 749 (128 tiles on 74 pairs: two rounds), dW 745;
-// bound by the tensor cores, and one after the other by the power they draw (3.2 to 3.7 ms for the four).  64 x 131072 x 4096: the
+// 4096 x 65536 x 2048, one at a time: logits folded 707 us (1556 Tflop/s), G 733 to 760, dX 749 to 772 (128 tiles on 74 pairs: two rounds), dW 745 to 757;
+// bound by the tensor cores, and one after the other by the power they draw (3.2 to 3.6 ms for the four).  64 x 131072 x 4096: the
 // weights are read once, in 169 us (6.3 TB/s), bound by HBM.
 #include <cuda_fp16.h>
 #include <math.h>
