@@ -574,13 +574,19 @@ __device__ __forceinline__ bool row_weight(const VocabRows &a, int64_t i, float 
   return counts;
 }
 // Per row w_i, the exponent's constant, and X_i w_i 2^-(E+1) in binary16 (0 without a target), a warp per row.  E is over all rows: every CTA
-// finds it for itself, which costs it a step per n / threads rows and saves a kernel.  *factor = 2^(E+1-13).
+// finds it for itself, which costs it n / threads steps and saves a kernel: 4096 x 2048 takes 12 us in CTAs of 1024 threads, 15 of 512, 29 of
+// 256.  The warp's first row is on its way meanwhile.  *factor = 2^(E+1-13).
 template <int THREADS>
 __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, uint32_t blocks) {
   __shared__ int tops[32];
   constexpr int warps = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per = a.dp / 8, first = (int64_t)block * warps + warp;
   chain_wait();
+  uint4 ahead[4];                                    // of the warp's first row, while E is found
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if (first < a.n && lane + 32 * j < per) ahead[j] = __ldg(reinterpret_cast<const uint4 *>(a.x + first * a.dp) + lane + 32 * j);
   int top = -200;
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < a.n; i += THREADS) {
@@ -594,8 +600,7 @@ __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, u
   top = __reduce_max_sync(kFull, lane < warps ? tops[lane] : -200);
   const int e = top == -200 ? 0 : top;
   if (block == 0 && threadIdx.x == 0) *a.factor = ldexpf(1.f, e + 1 - 13);
-  const int64_t per = a.dp / 8;
-  for (int64_t i = (int64_t)block * warps + warp; i < a.n; i += (int64_t)blocks * warps) {
+  for (int64_t i = first; i < a.n; i += (int64_t)blocks * warps) {
     float wi, ci;
     const bool counts = row_weight(a, i, wi, ci);
     if (lane == 0) {
@@ -603,19 +608,26 @@ __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, u
       if (a.cexp != nullptr) a.cexp[i] = ci;
     }
     const float f = ldexpf(wi, -(e + 1));
-#pragma unroll 4
-    for (int64_t c = lane; c < per; c += 32) {
-      __align__(16) __half h[8] = {};
-      if (counts) {
-        *reinterpret_cast<uint4 *>(h) = __ldg(reinterpret_cast<const uint4 *>(a.x + i * a.dp) + c);
+    const uint4 *x = reinterpret_cast<const uint4 *>(a.x + i * a.dp);
+    uint4 *out = reinterpret_cast<uint4 *>(a.out + i * a.dp);
+    auto scaled = [&](const uint4 &v) {
+      __align__(16) __half h[8];
+      *reinterpret_cast<uint4 *>(h) = v;
 #pragma unroll
-        for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
-      }
-      reinterpret_cast<uint4 *>(a.out + i * a.dp)[c] = *reinterpret_cast<const uint4 *>(h);
+      for (int j = 0; j < 8; j++) h[j] = __float2half_rn(__half2float(h[j]) * f);
+      return counts ? *reinterpret_cast<const uint4 *>(h) : make_uint4(0, 0, 0, 0);
+    };
+    if (i == first) {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (lane + 32 * j < per) out[lane + 32 * j] = scaled(ahead[j]);
     }
+#pragma unroll 4
+    for (int64_t c = lane + (i == first ? 128 : 0); c < per; c += 32) out[c] = scaled(__ldg(x + c));
   }
 }
-__global__ void __launch_bounds__(1024) vocab_rows_kernel(const VocabRows a) { vocab_rows<1024>(a, blockIdx.x, gridDim.x); }
+constexpr int V_ROW_THREADS = 1024;
+__global__ void __launch_bounds__(V_ROW_THREADS) vocab_rows_kernel(const VocabRows a) { vocab_rows<V_ROW_THREADS>(a, blockIdx.x, gridDim.x); }
 
 template <bool PAIR, bool A_MN, bool B_MN, int EPI, bool SMALL = false>
 __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(V_THREADS, 1)
@@ -963,8 +975,8 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
   FB_TRY(operands(p, ws, x, w, n, v, d, num_sms, stream));
   const VocabRows rows = {reinterpret_cast<const __half *>(x), n, p.dp, v, targets, loss, lse, dl, rw, factor, cexp, reinterpret_cast<__half *>(xs)};
   if (p.row_ctas == 0) {
-    const int64_t row_ctas = ceil_div(n, 32);
-    FB_TRY(launch_after(vocab_rows_kernel, (unsigned)(row_ctas < 2 * num_sms ? row_ctas : 2 * num_sms), 1024, 0, stream, rows));
+    const int64_t row_ctas = ceil_div(n, V_ROW_THREADS / 32), most = (int64_t)num_sms * (2048 / V_ROW_THREADS);
+    FB_TRY(launch_after(vocab_rows_kernel, (unsigned)(row_ctas < most ? row_ctas : most), V_ROW_THREADS, 0, stream, rows));
   }
   uint16_t *dxo = p.dp == d ? dx : reinterpret_cast<uint16_t *>(ws + p.dxp);
   const bool small = small_batch(n);

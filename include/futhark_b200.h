@@ -505,7 +505,7 @@ int futhark_entry_bmm_f16(struct futhark_context *ctx, struct futhark_f32_3d **o
  *                        in (if 0 <= t && t < i32.i64 v then lse - zs[t] else 0, lse)) X ts)
  *   Softmax cross entropy of hidden states against a vocabulary, without the [n][v] logits in memory: the losses, and the
  *   logarithms of the sums.  The sums are taken relative to the largest logit.  A target outside [0, v) is a token without one.
- *   Workspace: 8 bytes per token and 128 to 256 words.
+ *   Workspace: 8 bytes per token and 256 words (32 where there are few of both).
  * entry vocab_xent_grad_f16 [n][v][d] (X: [n][d]f16) (W: [v][d]f16) (ts: [n]i32) (losses: [n]f32) (lses: [n]f32) (dls: [n]f32):
  *     ([n][d]f16, [v][d]f16)
  *   The gradients with respect to X and W of sum_i dls[i] losses[i]; losses and lses are what vocab_xent_f16 returned for the
