@@ -775,14 +775,17 @@ static inline double block_clocks(bool pair, int cols) {
 }
 
 // Columns of a tile.  A tile of fewer columns reuses its rows less, but a number of tiles that is just above a multiple of
-// the number of CTAs or pairs leaves most of them idle in the last round.
-static int tile_columns(bool pair, int64_t rows, int64_t cols, int64_t kblocks, int step, int least, int num_sms) {
+// the number of CTAs or pairs leaves most of them idle in the last round; and where there are few tiles, narrow ones put more CTAs to work (down to
+// 32 instead of 128 columns: 8 x 4000 x 8192 forward 25.5 us instead of 33, 1317 x 271 x 2729 in both directions 59 instead of 62).  `losses`: a
+// kernel that folds more partial results than the last CTA does in a turn costs 8000.
+static int tile_columns(bool pair, int64_t rows, int64_t cols, int64_t kblocks, int step, int least, bool losses, int num_sms) {
   int best = VT;
   double best_cost = 0;
   const int64_t workers = pair ? num_sms / 2 : num_sms;
   for (int nt = VT; nt >= least; nt -= step) {
     const int64_t tiles = ceil_div(rows, pair ? 256 : 128) * ceil_div(cols, nt);
-    const double cost = (double)ceil_div(tiles, workers) * (kblocks * block_clocks(pair, nt) + 1500.0);
+    const double cost = (double)ceil_div(tiles, workers) * (kblocks * block_clocks(pair, nt) + 1500.0) +
+                        (losses && !last_makes_losses(rows, ceil_div(cols, nt)) ? 8000.0 : 0.0);
     if (nt == VT || cost < 0.97 * best_cost) { best = nt; best_cost = cost; }
   }
   return best;
@@ -819,7 +822,7 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
   p.xp = p.copy_x ? take((size_t)(n * p.dp) * 2) : 0;
   p.wp = p.copy_w ? take((size_t)(v * p.dp) * 2) : 0;
   if (!grad) {
-    p.nt = tile_columns(pair, n, v, ceil_div(p.dp, VK), 32, 32, num_sms);
+    p.nt = tile_columns(pair, n, v, ceil_div(p.dp, VK), 32, 32, true, num_sms);
     p.part = take((size_t)(n * ceil_div(v, p.nt)) * sizeof(float2));
     p.zt = take((size_t)n * 4);
   } else {
@@ -830,9 +833,9 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     if (words < VT) words = VT;
     if (words > want) words = want;
     p.piece = ceil_div(ceil_div(v, ceil_div(v, words)), VT) * VT;       // equal pieces
-    p.nt = tile_columns(pair, n, p.piece < v ? p.piece : v, ceil_div(p.dp, VK), 64, 64, num_sms);
+    p.nt = tile_columns(pair, n, p.piece < v ? p.piece : v, ceil_div(p.dp, VK), 64, 64, false, num_sms);
     p.pieces = (int)ceil_div(v, p.piece);
-    p.ntw = tile_columns(true, p.piece < v ? p.piece : v, p.dp, ceil_div(n, VK), 128, 128, num_sms);
+    p.ntw = tile_columns(true, p.piece < v ? p.piece : v, p.dp, ceil_div(n, VK), 128, 128, false, num_sms);
     // Small calls: what the products need besides G is made beside it, and the products side by side, on CTAs that have nothing else
     // to do.  Both products are then pairs' work, since all tensor-core instructions of a kernel are of one kind.  Both directions of 16 x 500
     // x 64 take 34 us instead of 38.5, 1000 x 1000 x 200 36.5 instead of 40.5, 500 x 8000 x 1024 60.5 instead of 65.5.
