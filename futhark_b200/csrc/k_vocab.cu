@@ -8,7 +8,8 @@
 // A map-map-reduce contraction whose result is consumed by a (maximum, sum) reduction.  The logits stay in
 // tensor memory: the contraction's epilogue folds each 256 x 256 tile to one (maximum, sum) pair per
 // row, and a small kernel (in small calls the last CTA) folds the v/256 pairs of a row.  The gradient works the vocabulary off in pieces: a
-// piece's logits are computed again (the same instructions in the same order, so the same bits), turned into g in
+// piece's logits are computed again (by the same instructions; sums of more than 2048 products in one
+// accumulator where the losses had two, 1.4e-6 of a logit at most), turned into g in
 // binary16 in the epilogue, and that piece of g meets W (summed over the pieces in f32) and X.
 //
 // Rounding of g to 11 bits.  With q_i = 1 - exp(-loss_i) the row is kept as
@@ -40,8 +41,8 @@
 namespace fb {
 
 constexpr int VT = 256;                                // tile edge of a CTA pair
-constexpr int VK = 64;                                 // summed elements per stage
-constexpr int V_OPERAND = 128 * VK * 2;                // 128 rows of an operand in one stage: 16 KiB
+constexpr int VK = 64;                                 // summed elements of a block
+constexpr int V_OPERAND = 128 * VK * 2;                // 128 rows of an operand in one block: 16 KiB
 constexpr int V_SLAB = VK * 64 * 2;                    // 64 x 64 block of an operand that is contiguous across the sum
 constexpr int V_EPI_BUF = 32 * 128;                    // 32 rows of 128 bytes
 constexpr int V_GROUP = 16;                            // row tiles that share the columns' operand before it moves on
