@@ -222,9 +222,20 @@ __device__ __forceinline__ uint32_t status_value(uint64_t w) { return (uint32_t)
 // A kernel launched by launch_after may start while the one before it in the stream is still running: it sets itself up
 // and then waits, before its first access to global memory, until that one has ended and its writes are
 // visible.  Every kernel of a chain waits, so the end of one is the end of all before it.
+//
+// What a kernel of a chain reads may thus be written while it is already resident, its arguments included: a caller passes
+// on what an earlier call returned.  The read-only path (__ldg, const __restrict__, ld.global.nc) promises memory that nobody
+// writes while the kernel runs, and lets loads move above the wait: kernels of chains do without it.
 __device__ __forceinline__ void chain_wait() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// 16 bytes that this kernel reads once.
+__device__ __forceinline__ int4 ld_chain_v4(const void *p) {
+  int4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 template <typename... KARGS, typename... ARGS>
 static inline cudaError_t launch_after(void (*kernel)(KARGS...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, ARGS... args) {

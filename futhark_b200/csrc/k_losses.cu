@@ -74,7 +74,7 @@ template <typename T>
 __device__ __forceinline__ int4 load_group(const DistillRow<T> &r, int group) {
   constexpr int W = DistillRow<T>::W;
   const int c = r.first(group);
-  if (r.whole(group)) return ld_stream_v4(r.base + c);
+  if (r.whole(group)) return ld_chain_v4(r.base + c);
   __align__(16) T x[W];
 #pragma unroll
   for (int j = 0; j < W; j++) x[j] = c + j >= 0 && c + j < r.v ? r.base[c + j] : from_f32<T>(-INFINITY);
@@ -150,7 +150,7 @@ __device__ __forceinline__ void load_chunk(const DistillRow<T> &r, int chunk, in
   if (r.first(g0) >= 0 && groups == 32 * D_PER && r.first(g0 + groups) <= r.v) {
     const T *p = r.base + r.first(g0 + lane);
 #pragma unroll
-    for (int i = 0; i < D_PER; i++) x[i] = ld_stream_v4(p + i * 32 * DistillRow<T>::W);
+    for (int i = 0; i < D_PER; i++) x[i] = ld_chain_v4(p + i * 32 * DistillRow<T>::W);
   } else {
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
@@ -245,8 +245,8 @@ __device__ __forceinline__ void distill_row(const DistillLoss &a, const T *s, in
 // (maximum, sum) of every run.  JOIN: of few rows, whose losses the CTA that ends last then makes; `ticket` is 0 between launches.
 template <typename T, bool JOIN>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
-distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, float2 *__restrict__ part,
-                    uint32_t *__restrict__ ticket, const DistillLoss a) {
+distill_part_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, float scale, float2 *part,
+                    uint32_t *ticket, const DistillLoss a) {
   constexpr int W = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
   const int64_t items = n * d.runs, step = (int64_t)gridDim.x * D_WARPS;
@@ -318,7 +318,7 @@ distill_part_kernel(const T *__restrict__ s, int64_t n, int64_t v, const Distill
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-distill_loss_kernel(const T *__restrict__ s, const float2 *__restrict__ part, int runs, int64_t n, int64_t v, float scale, const DistillLoss a) {
+distill_loss_kernel(const T *s, const float2 *part, int runs, int64_t n, int64_t v, float scale, const DistillLoss a) {
   extern __shared__ float sh[];                      // per warp: words [k], log q [k]
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   chain_wait();
@@ -386,8 +386,8 @@ __device__ __forceinline__ float4 teacher_record(const DistillTeacher &a, int64_
 }
 // Both for every row, one warp per row.
 __global__ void __launch_bounds__(256)
-distill_teacher_kernel(bool wide, const DistillTeacher a, int64_t n, int64_t v, int32_t *__restrict__ words, float *__restrict__ weights,
-                       float4 *__restrict__ rows) {
+distill_teacher_kernel(bool wide, const DistillTeacher a, int64_t n, int64_t v, int32_t *words, float *weights,
+                       float4 *rows) {
   extern __shared__ float sh[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
@@ -419,8 +419,8 @@ template <> __device__ __forceinline__ float2 row_exponents<float>(float2 x, flo
 // OWN: every warp has one run at most, and finds what it needs of its row's teacher for itself.
 template <typename T, bool OWN>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
-distill_grad_kernel(const T *__restrict__ s, int64_t n, int64_t v, const DistillShape d, float scale, const DistillTeacher a,
-                    const int32_t *__restrict__ words, const float *__restrict__ weights, const float4 *__restrict__ rows, T *__restrict__ ds) {
+distill_grad_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, float scale, const DistillTeacher a,
+                    const int32_t *words, const float *weights, const float4 *rows, T *ds) {
   extern __shared__ float sh[];
   constexpr int W = 16 / (int)sizeof(T);
   const int lane = threadIdx.x & 31;
@@ -692,9 +692,9 @@ static __host__ __device__ __forceinline__ int router_slices(int threads, int e)
 // launches: where there are few partial results the CTA that ends last adds them all up, in f64 and in the order of the CTAs, and makes the loss.
 template <typename T, int W, int J>
 __global__ void __launch_bounds__(RouterRow<T, W, J>::THREADS)
-router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ is, int64_t n, int e, int k, int g,
-                   float *__restrict__ psum, int *__restrict__ pcount, uint32_t *__restrict__ ticket, int32_t *__restrict__ counts,
-                   float *__restrict__ loss, float *__restrict__ norm) {
+router_part_kernel(const T *r, const uint8_t *keep, const int32_t *is, int64_t n, int e, int k, int g,
+                   float *psum, int *pcount, uint32_t *ticket, int32_t *counts,
+                   float *loss, float *norm) {
   constexpr int R_WARPS = RouterRow<T, W, J>::WARPS, R_THREADS = RouterRow<T, W, J>::THREADS;
   extern __shared__ __align__(16) float rsh[];       // [R_WARPS][g * J * W] column sums of the warps, then [e + 1] counts
   const int span = g * J * W;
@@ -842,8 +842,8 @@ router_part_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, co
 
 // 32 columns per CTA, the partial results of the CTAs over the warps, in f64; the CTA that ends last makes the loss.
 __global__ void __launch_bounds__(1024)
-router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcount, int parts, int e, double *__restrict__ sums, int *__restrict__ kept,
-                   uint32_t *__restrict__ ticket, int32_t *__restrict__ counts, float *__restrict__ loss, float *__restrict__ norm) {
+router_loss_kernel(const float *psum, const int *pcount, int parts, int e, double *sums, int *kept,
+                   uint32_t *ticket, int32_t *counts, float *loss, float *norm) {
   __shared__ double sp[32][33];
   __shared__ int sc[32][33];
   __shared__ bool last;
@@ -895,8 +895,8 @@ router_loss_kernel(const float *__restrict__ psum, const int *__restrict__ pcoun
 // difference, and sum_f p_if = 1 makes the shift cancel.
 template <typename T, int W, int J>
 __global__ void __launch_bounds__(RouterRow<T, W, J>::THREADS)
-router_grad_kernel(const T *__restrict__ r, const uint8_t *__restrict__ keep, const int32_t *__restrict__ counts, const float *__restrict__ norm,
-                   const float *__restrict__ dl, int64_t n, int e, int g, T *__restrict__ dr) {
+router_grad_kernel(const T *r, const uint8_t *keep, const int32_t *counts, const float *norm,
+                   const float *dl, int64_t n, int e, int g, T *dr) {
   constexpr int R_WARPS = RouterRow<T, W, J>::WARPS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane & (g - 1), sub = lane / g, per_warp = 32 / g;
   const int64_t step = (int64_t)gridDim.x * R_WARPS * per_warp;

@@ -567,8 +567,8 @@ struct VocabRows {
 };
 // w_i = dl_i q_i and the constant term of G's exponent; false for a token without a target
 __device__ __forceinline__ bool row_weight(const VocabRows &a, int64_t i, float &w, float &c) {
-  const int64_t t = __ldg(a.targets + i);
-  const float ls = __ldg(a.loss + i), l = __ldg(a.lse + i), d = __ldg(a.dl + i);
+  const int64_t t = a.targets[i];
+  const float ls = a.loss[i], l = a.lse[i], d = a.dl[i];
   const bool counts = t >= 0 && t < a.v;
   w = counts ? d * row_q(ls, l) : 0.f;
   c = counts ? row_exponent(ls, l) : 0.f;
@@ -587,7 +587,7 @@ __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, u
   uint4 ahead[4];                                    // of the warp's first row, while E is found
 #pragma unroll
   for (int j = 0; j < 4; j++)
-    if (first < a.n && lane + 32 * j < per) ahead[j] = __ldg(reinterpret_cast<const uint4 *>(a.x + first * a.dp) + lane + 32 * j);
+    if (first < a.n && lane + 32 * j < per) ahead[j] = reinterpret_cast<const uint4 *>(a.x + first * a.dp)[lane + 32 * j];
   int top = -200;
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < a.n; i += THREADS) {
@@ -623,8 +623,15 @@ __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, u
       for (int j = 0; j < 4; j++)
         if (lane + 32 * j < per) out[lane + 32 * j] = scaled(ahead[j]);
     }
-#pragma unroll 4
-    for (int64_t c = lane + (i == first ? 128 : 0); c < per; c += 32) out[c] = scaled(__ldg(x + c));
+    for (int64_t c = lane + (i == first ? 128 : 0); c < per; c += 128) {
+      uint4 some[4];                                 // all in flight before the first is written
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (c + 32 * j < per) some[j] = x[c + 32 * j];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (c + 32 * j < per) out[c + 32 * j] = scaled(some[j]);
+    }
   }
 }
 constexpr int V_ROW_THREADS = 1024;
@@ -658,8 +665,8 @@ vocab_products_kernel(const __grid_constant__ CUtensorMap tmGk, const __grid_con
 
 // ---- the small kernels around it ------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
-vocab_loss_kernel(const float2 *__restrict__ part, int tiles, const float *__restrict__ ztarget, const int32_t *__restrict__ targets,
-                  float *__restrict__ loss, float *__restrict__ lse, int64_t n, int64_t v) {
+vocab_loss_kernel(const float2 *part, int tiles, const float *ztarget, const int32_t *targets,
+                  float *loss, float *lse, int64_t n, int64_t v) {
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   chain_wait();
   row_loss(part, tiles, ztarget, targets, loss, lse, row, row < n, v, 32);
@@ -707,8 +714,8 @@ vocab_pitch_kernel(const PitchJob a, const PitchJob b, int64_t in_cols, int64_t 
 
 // dX_i = 2^-13 w_i times the sum of the slabs, in f32, rounded once.
 __global__ void __launch_bounds__(256)
-vocab_dx_kernel(const float *__restrict__ slabs, int splits, int64_t n, int64_t d, int64_t dp, const int32_t *__restrict__ targets, int64_t v,
-                const float *__restrict__ w, __half *__restrict__ dx) {
+vocab_dx_kernel(const float *slabs, int splits, int64_t n, int64_t d, int64_t dp, const int32_t *targets, int64_t v,
+                const float *w, __half *dx) {
   const int64_t per = dp / 4, total = n * per;
   chain_wait();
   for (int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x; o < total; o += (int64_t)gridDim.x * 256) {
@@ -740,7 +747,7 @@ vocab_dx_kernel(const float *__restrict__ slabs, int splits, int64_t n, int64_t 
 }
 
 __global__ void __launch_bounds__(256)
-vocab_fill_kernel(float *__restrict__ loss, float *__restrict__ lse, int64_t n, float l) {
+vocab_fill_kernel(float *loss, float *lse, int64_t n, float l) {
   chain_wait();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) { loss[i] = 0.f; lse[i] = l; }
 }
