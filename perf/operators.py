@@ -104,15 +104,22 @@ def prepare(case, seed):
 
 
 # ---- the library's calls -----------------------------------------------------------------------------------
-_ctx = None
+_ctx = _stream = _event = None
 
 
 def _context():
-    global _ctx
+    global _ctx, _stream, _event
     if _ctx is None:
         import futhark_b200
         _ctx = futhark_b200.Context(device="#0")
+        _stream, _event = torch.cuda.ExternalStream(_ctx.stream), torch.cuda.Event()
     return _ctx
+
+
+def _after(later, earlier):
+    """What `later` does from now on comes after what `earlier` has been given so far."""
+    _event.record(earlier)
+    later.wait_event(_event)
 
 
 def _wrap(ctx, t):
@@ -122,12 +129,13 @@ def _wrap(ctx, t):
 
 
 class _Result:
-    """An array of the context that goes back to it with the last tensor on its memory."""
+    """An array of the context that goes back to it with the last tensor on its memory, behind what reads that tensor."""
 
     def __init__(self, a):
         self.array, self.__cuda_array_interface__ = a, a.__cuda_array_interface__
 
     def __del__(self):
+        _after(_stream, torch.cuda.current_stream())
         self.array.free()
 
 
@@ -138,6 +146,7 @@ def _tensor(a):
 
 def _run_own(s):
     ctx = _context()
+    _after(_stream, torch.cuda.current_stream())       # the library works on a stream of its own
     ins = []
 
     def arr(t):
@@ -159,6 +168,7 @@ def _run_own(s):
         out = out + (ctx.entry_router_balance_grad(s["t"], r, keep, out[1], out[2], arr(s["dl"])),)
     for a in ins:
         a.free()
+    _after(torch.cuda.current_stream(), _stream)
     return tuple(_tensor(a) for a in out)
 
 
