@@ -105,6 +105,7 @@ def prepare(case, seed):
 
 # ---- the library's calls -----------------------------------------------------------------------------------
 _ctx = _stream = _event = None
+_dropped = []                                          # results whose tensors are gone, with the streams they belong to
 
 
 def _context():
@@ -129,24 +130,30 @@ def _wrap(ctx, t):
 
 
 class _Result:
-    """An array of the context that goes back to it with the last tensor on its memory, behind what reads that tensor."""
+    """An array of the context that belongs to the stream of the call, as torch's own tensors do.  When the last tensor on its memory
+    is gone it goes back with the next call, behind what that stream then holds."""
 
-    def __init__(self, a):
-        self.array, self.__cuda_array_interface__ = a, a.__cuda_array_interface__
+    def __init__(self, a, stream):
+        self.array, self.stream, self.__cuda_array_interface__ = a, stream, a.__cuda_array_interface__
 
     def __del__(self):
-        _after(_stream, torch.cuda.current_stream())
-        self.array.free()
+        _dropped.append((self.array, self.stream))
 
 
-def _tensor(a):
-    t = torch.as_tensor(_Result(a), device="cuda")
+def _tensor(a, stream):
+    t = torch.as_tensor(_Result(a, stream), device="cuda")
     return t.view(torch.float16) if t.dtype == torch.uint16 else t
 
 
 def _run_own(s):
     ctx = _context()
-    _after(_stream, torch.cuda.current_stream())       # the library works on a stream of its own
+    here = torch.cuda.current_stream()
+    _after(_stream, here)                              # the library works on a stream of its own
+    while _dropped:
+        a, reader = _dropped.pop()
+        if reader.cuda_stream != here.cuda_stream:
+            _after(_stream, reader)
+        a.free()
     ins = []
 
     def arr(t):
@@ -168,8 +175,8 @@ def _run_own(s):
         out = out + (ctx.entry_router_balance_grad(s["t"], r, keep, out[1], out[2], arr(s["dl"])),)
     for a in ins:
         a.free()
-    _after(torch.cuda.current_stream(), _stream)
-    return tuple(_tensor(a) for a in out)
+    _after(here, _stream)
+    return tuple(_tensor(a, here) for a in out)
 
 
 # ---- the plain forms: 32 bits, rounded once at the end --------------------------------------------------------
