@@ -15,12 +15,14 @@
 // Rounding of g to 11 bits.  With q_i = 1 - exp(-loss_i) the row is kept as
 //   G_iv = 2^13 (exp(z_iv - lse_i) - [v = t_i]) / q_i,  G_{i,t_i} = -2^13 exactly,  and  w_i = dl_i q_i  aside:
 //   dX_i = 2^-13 w_i sum_v G_iv W_v                 w_i in f32, after the sum
-//   dW_v = 2^(E+1-13) sum_i G_iv (X_i w_i 2^-(E+1))   E the largest exponent of the w_i
+//   dW_v = 2^(E-14-13) sum_i G_iv (X_i w_i 2^(14-E))  E the largest exponent of any |X_ij w_i|
 // The target's term, the largest of its row by far, is thus exact in dX; the others round relative to
 // themselves (2^13 keeps probabilities down to 2^-27 out of binary16's subnormals, and the sum over the others is q_i,
 // so |G| <= 2^13 up to the rounding of the losses).  In dW the scaled X is rounded once more to binary16: half
 // a unit in the last place of each element, independent of the others, of the size of the result's own rounding.
-// Both products accumulate in f32.
+// All of binary16's range is used for it: X_ij w_i keeps its 11 bits down to 2^-28 of the largest, and below that an absolute 2^(E-39),
+// which is no more than what the result itself is rounded to (2^-25) unless the largest is 2^15 or more and the result about
+// to overflow.  Both products accumulate in f32.
 //
 // The products run on one kernel (vocab_mma_kernel): pairs of CTAs on 256 x 256 tiles with
 // tcgen05.mma.cta_group::2 (single CTAs on 128 x 256 for small batches), operands by bulk tensor copies through a ring of stages, two accumulators in tensor
@@ -561,6 +563,8 @@ struct VocabRows {
   int64_t n, dp, v;
   const int32_t *targets;
   const float *loss, *lse, *dl;
+  int *tops;                                         // E of the rows of each of `top_ctas` CTAs of a kernel before
+  int top_ctas;                                      // 0: there was none
   float *w, *factor;
   float *cexp;                                       // or nullptr
   __half *out;
@@ -574,12 +578,55 @@ __device__ __forceinline__ bool row_weight(const VocabRows &a, int64_t i, float 
   c = counts ? row_exponent(ls, l) : 0.f;
   return counts;
 }
-// Per row w_i, the exponent's constant, and X_i w_i 2^-(E+1) in binary16 (0 without a target), a warp per row.  E is over all rows: every CTA
-// finds it for itself, which costs it n / threads steps and saves a kernel: 4096 x 2048 takes 12 us in CTAs of 1024 threads, 15 of 512, 29 of
-// 256.  The warp's first row is on its way meanwhile.  *factor = 2^(E+1-13).
+// E over all rows takes a kernel of its own, since every scaled element waits for it (2.3 us: 777 x 32003 x 1000 gradient 175 instead of 173 us
+// with an E that need not look at X).  Where X is at most this many elements, the CTAs that need E find it for themselves: gradient of
+// 16 x 500 x 64 13 instead of 16 us, 100 x 2000 x 360 19.8 instead of 18.5, 1000 x 1000 x 200 71 instead of 17.
+constexpr int64_t V_OWN_TOPS = 32768;
+constexpr int V_NO_TOP = -1000;                      // below the exponent of any product of an f32 and a binary16 number
+constexpr int V_TOP_THREADS = 256, V_TOP_CTAS = 8;   // CTAs per SM
+// The largest exponent of |X_ij w_i| that `warps` warps find, this one the `warp`-th: 1024 elements of a row at a time, so that few
+// long rows are shared out too.  Elements and weights that are not finite do not count: what they lead to is not finite either.
+__device__ __forceinline__ int rows_top(const VocabRows &a, int64_t warp, int64_t warps) {
+  const int lane = threadIdx.x & 31;
+  const int64_t per = a.dp / 8, chunks = (per + 127) / 128, items = a.n * chunks;
+  int top = V_NO_TOP;
+  for (int64_t at = warp; at < items; at += warps) {
+    const int64_t i = at / chunks, c = (at - i * chunks) * 128 + lane;
+    const uint4 *x = reinterpret_cast<const uint4 *>(a.x + i * a.dp);
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = c + 32 * j < per ? x[c + 32 * j] : make_uint4(0, 0, 0, 0);
+    float w, ci;
+    row_weight(a, i, w, ci);
+    if (w == 0.f || !isfinite(w)) continue;          // uniform over the warp
+    uint32_t m = 0;                                  // bit patterns of sizes order like the sizes
+    auto pair = [&](uint32_t u) { u &= 0x7fff7fffu; m = __vmaxu2(m, u & __vcmpltu2(u, 0x7c007c00u)); };
+#pragma unroll
+    for (int j = 0; j < 4; j++) { pair(v[j].x); pair(v[j].y); pair(v[j].z); pair(v[j].w); }
+    m = __reduce_max_sync(kFull, max(m & 0xffffu, m >> 16));
+    if (m != 0) top = max(top, ilogb((double)fabsf(w) * (double)__half2float(__ushort_as_half((unsigned short)m))));   // the product is exact
+  }
+  return top;
+}
+template <int THREADS>
+__device__ __forceinline__ int cta_max(int x) {
+  __shared__ int of_warp[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  x = __reduce_max_sync(kFull, x);
+  if (lane == 0) of_warp[warp] = x;
+  __syncthreads();
+  return __reduce_max_sync(kFull, of_warp[lane < THREADS / 32 ? lane : 0]);
+}
+__global__ void __launch_bounds__(V_TOP_THREADS) vocab_tops_kernel(const VocabRows a) {
+  constexpr int warps = V_TOP_THREADS / 32;
+  chain_wait();
+  const int top = cta_max<V_TOP_THREADS>(rows_top(a, (int64_t)blockIdx.x * warps + (threadIdx.x >> 5), (int64_t)gridDim.x * warps));
+  if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
+}
+// Per row w_i, the exponent's constant, and X_i w_i 2^(14-E) in binary16 (0 without a target), a warp per row, whose first one is on its way
+// while E is found.  *factor = 2^(E-14-13).
 template <int THREADS>
 __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, uint32_t blocks) {
-  __shared__ int tops[32];
   constexpr int warps = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t per = a.dp / 8, first = (int64_t)block * warps + warp;
@@ -588,19 +635,12 @@ __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, u
 #pragma unroll
   for (int j = 0; j < 4; j++)
     if (first < a.n && lane + 32 * j < per) ahead[j] = reinterpret_cast<const uint4 *>(a.x + first * a.dp)[lane + 32 * j];
-  int top = -200;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < a.n; i += THREADS) {
-    float wi, ci;
-    row_weight(a, i, wi, ci);
-    if (wi != 0.f && isfinite(wi)) top = max(top, ilogbf(wi));
-  }
-  top = __reduce_max_sync(kFull, top);
-  if (lane == 0) tops[warp] = top;
-  __syncthreads();
-  top = __reduce_max_sync(kFull, lane < warps ? tops[lane] : -200);
-  const int e = top == -200 ? 0 : top;
-  if (block == 0 && threadIdx.x == 0) *a.factor = ldexpf(1.f, e + 1 - 13);
+  int top = V_NO_TOP;
+  if (a.top_ctas == 0) top = rows_top(a, warp, warps);
+  else for (int i = threadIdx.x; i < a.top_ctas; i += THREADS) top = max(top, a.tops[i]);
+  top = cta_max<THREADS>(top);
+  const int e = top == V_NO_TOP ? 14 : top;
+  if (block == 0 && threadIdx.x == 0) *a.factor = ldexpf(1.f, e - 14 - 13);
   for (int64_t i = first; i < a.n; i += (int64_t)blocks * warps) {
     float wi, ci;
     const bool counts = row_weight(a, i, wi, ci);
@@ -608,7 +648,8 @@ __device__ __forceinline__ void vocab_rows(const VocabRows &a, uint32_t block, u
       a.w[i] = wi;
       if (a.cexp != nullptr) a.cexp[i] = ci;
     }
-    const float f = ldexpf(wi, -(e + 1));
+    float f = ldexpf(wi, 14 - e);
+    if (isinf(f) && isfinite(wi)) f = copysignf(3.4e38f, wi);        // of a row of zeros, which stay zeros
     const uint4 *x = reinterpret_cast<const uint4 *>(a.x + i * a.dp);
     uint4 *out = reinterpret_cast<uint4 *>(a.out + i * a.dp);
     auto scaled = [&](const uint4 &v) {
@@ -857,6 +898,9 @@ VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_ali
     p.w = take((size_t)n * 4);
     p.cexp = take((size_t)n * 4);
     p.scalars = take(256);
+    const int64_t top_ctas = ceil_div(n * ceil_div(p.dp, 1024), V_TOP_THREADS / 32), most_tops = (int64_t)num_sms * V_TOP_CTAS;
+    p.top_ctas = n * p.dp <= V_OWN_TOPS ? 0 : (int)(top_ctas < most_tops ? top_ctas : most_tops);
+    p.tops = take((size_t)p.top_ctas * 4);
     p.xs = take((size_t)(n * p.dp) * 2);
     p.g = take((size_t)(n * p.piece) * 2);
     p.direct = p.splits == 1 && p.pieces == 1;
@@ -984,7 +1028,9 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
   float *cexp = p.row_ctas == 0 ? reinterpret_cast<float *>(ws + p.cexp) : nullptr;
   uint16_t *xs = reinterpret_cast<uint16_t *>(ws + p.xs), *g = reinterpret_cast<uint16_t *>(ws + p.g);
   FB_TRY(operands(p, ws, x, w, n, v, d, num_sms, stream));
-  const VocabRows rows = {reinterpret_cast<const __half *>(x), n, p.dp, v, targets, loss, lse, dl, rw, factor, cexp, reinterpret_cast<__half *>(xs)};
+  const VocabRows rows = {reinterpret_cast<const __half *>(x), n, p.dp, v, targets, loss, lse, dl, reinterpret_cast<int *>(ws + p.tops), p.top_ctas,
+                          rw, factor, cexp, reinterpret_cast<__half *>(xs)};
+  if (p.top_ctas > 0) FB_TRY(launch_after(vocab_tops_kernel, p.top_ctas, V_TOP_THREADS, 0, stream, rows));
   if (p.row_ctas == 0) {
     const int64_t row_ctas = ceil_div(n, V_ROW_THREADS / 32), most = (int64_t)num_sms * (2048 / V_ROW_THREADS);
     FB_TRY(launch_after(vocab_rows_kernel, (unsigned)(row_ctas < most ? row_ctas : most), V_ROW_THREADS, 0, stream, rows));

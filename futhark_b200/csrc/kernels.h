@@ -191,9 +191,10 @@ struct VocabPlan {
   int splits, ntd, ntw;        // gradient: parts of the sum over a piece's words, columns of a tile of dX and of dW
   int pieces;
   int row_ctas;                // gradient: CTAs beside G's that make what the products need; 0: a kernel does
+  int top_ctas;                // gradient: CTAs that find how large that gets; 0: whoever needs it
   bool together;               // gradient: both products in one kernel
   bool direct;                 // gradient: dX leaves the tensor cores finished (one piece, one part)
-  size_t xp, wp, part, zt, w, cexp, scalars, xs, g, slabs, dxp, dwp, bytes;
+  size_t xp, wp, part, zt, w, cexp, scalars, tops, xs, g, slabs, dxp, dwp, bytes;
 };
 VocabPlan vocab_plan(int64_t n, int64_t v, int64_t d, bool x_aligned, bool w_aligned, bool grad, int num_sms);
 cudaError_t launch_vocab_xent(const VocabPlan &p, void *workspace, void *ticket, const uint16_t *x, const uint16_t *w, const int32_t *targets, float *loss,

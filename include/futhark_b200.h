@@ -510,9 +510,12 @@ int futhark_entry_bmm_f16(struct futhark_context *ctx, struct futhark_f32_3d **o
  *     ([n][d]f16, [v][d]f16)
  *   The gradients with respect to X and W of sum_i dls[i] losses[i]; losses and lses are what vocab_xent_f16 returned for the
  *   same X, W and ts.  The logits are computed again in pieces of the vocabulary (1 GiB of workspace at most, or 512 bytes per
- *   token where that is more; beside it a scaled copy of X and, for small batches, partial sums of the first gradient).  Gradients
- *   are rounded to binary16 once, so dls carries the scale that keeps them in its range.  Rows without a target have gradient
- *   0 and add nothing to that of W, whatever X holds there. */
+ *   token where that is more; beside it a scaled copy of X, sums in f32 of the first gradient where there are several pieces or
+ *   the batch is small, and copies of operands and results whose rows are not whole groups of 16 bytes).  Gradients are rounded to
+ *   binary16, so dls carries the scale that keeps them in its range; the sums are f32, of products of binary16 numbers: the
+ *   logits' gradients, rounded relative to themselves and exact at the target, by W for the first, and by the weighted rows of X for the
+ *   second, rounded relative to themselves down to 2^-28 of the largest.  In both directions that is 1.4 times the error of
+ *   rounding an exact result once.  Rows without a target have gradient 0 and add nothing to that of W, whatever X holds there. */
 int futhark_entry_vocab_xent_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0,
                                  const struct futhark_f16_2d *in0, const struct futhark_f16_2d *in1, const struct futhark_i32_1d *in2);
 int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 **out0,
