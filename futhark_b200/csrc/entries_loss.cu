@@ -163,7 +163,7 @@ static int topk_distill(futhark_context *ctx, const char *name, int elem, losses
   Call call(ctx);
   auto *loss = call.array<futhark_f32_1d>({n}, 4, "topk_distill.loss"), *lse = call.array<futhark_f32_1d>({n}, 4, "topk_distill.lse");
   auto *rec = call.record<losses_t>();
-  void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), n, v, k, elem, false, ctx->num_sms), "topk_distill.workspace");
+  void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), tau, n, v, k, elem, false, ctx->num_sms), "topk_distill.workspace");
   call.launch(name, "map3 (\\s is t -> tau**2 * sum (map2 (\\q i -> q * (log q - s[i]/tau + lse s)) (softmax t) is)) S iss T", [&] { return distill_details(n, v, k); }, [&] {
     return fb::launch_topk_distill(ws, ctx->reduce_scratch, elem, dptr<void>(s->mem), dptr<int32_t>(is->mem), dptr<float>(t->mem), tau, n, v, k, dptr<float>(loss->mem),
                                    dptr<float>(lse->mem), ctx->num_sms, ctx->stream);
@@ -184,7 +184,7 @@ static int topk_distill_grad(futhark_context *ctx, const char *name, int elem, M
   if (distill_refusal(ctx, tau, n, v, k)) return 1;
   Call call(ctx);
   auto *ds = call.array<MAT>({n, v}, elem, "topk_distill_grad.ds");
-  void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), n, v, k, elem, true, ctx->num_sms), "topk_distill_grad.workspace");
+  void *ws = call.workspace(fb::distill_workspace_bytes(dptr<void>(s->mem), tau, n, v, k, elem, true, ctx->num_sms), "topk_distill_grad.workspace");
   call.launch(name, "vjp of topk_distill", [&] { return distill_details(n, v, k); }, [&] {
     return fb::launch_topk_distill_grad(ws, elem, dptr<void>(s->mem), dptr<int32_t>(is->mem), dptr<float>(t->mem), tau, dptr<float>(lse->mem),
                                         dptr<float>(dl->mem), n, v, k, dptr<void>(ds->mem), ctx->num_sms, ctx->stream);

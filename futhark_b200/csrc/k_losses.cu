@@ -109,24 +109,38 @@ __device__ __forceinline__ float group_max(const int4 &b, const __half *) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
-// Maxima are kept in units in which what was subtracted from the logits is known exactly.  For binary16 that is log 2, the unit
-// of the exponents: x scale - m in one step.  For f32 it is the logit's own, (x - m) scale, since a logit of the type's lowest
-// value (a mask) times the scale would be no finite number.
-template <typename T> struct LogitUnit;
-template <> struct LogitUnit<__half> {
-  static __device__ __forceinline__ float of(float x, float scale) { return x * scale; }             // of a logit
-  static __device__ __forceinline__ float log2(float d, float) { return d; }                         // of a difference
-};
-template <> struct LogitUnit<float> {
-  static __device__ __forceinline__ float of(float x, float) { return x; }
-  static __device__ __forceinline__ float log2(float d, float scale) { return d * scale; }
+// Maxima are kept in units in which what was subtracted from the logits is known exactly.  SCALED: log 2, the unit of the
+// exponents: x scale - m in one step, whose rounding of m (|m| 2^-24) goes into the sum as a power of two and out again with m.  Otherwise the
+// logit's own, (x - m) scale.  That is how f32 does it, since a logit of the type's lowest value (a mask) times the scale would be no
+// finite number, and binary16 below the temperature of D_FAR, since there the rounding of m would leave the exponents' range.
+template <bool SCALED> struct LogitUnit {
+  static __device__ __forceinline__ float of(float x, float scale) { return SCALED ? x * scale : x; }             // of a logit
+  static __device__ __forceinline__ float log2(float d, float scale) { return SCALED ? d : d * scale; }           // of a difference
 };
 // (maximum, sum): the fold of two
-template <typename T>
+template <bool SCALED>
 __device__ __forceinline__ void fold_pair(float &m, float &s, float om, float os, float scale) {
   const float mn = fmaxf(m, om), ref = mn == -INFINITY ? 0.f : mn;
-  s = s * exp2f(LogitUnit<T>::log2(m - ref, scale)) + os * exp2f(LogitUnit<T>::log2(om - ref, scale));
+  s = s * exp2f(LogitUnit<SCALED>::log2(m - ref, scale)) + os * exp2f(LogitUnit<SCALED>::log2(om - ref, scale));
   m = mn;
+}
+// of a row's runs, by a warp, eight per lane in flight
+template <bool SCALED>
+__device__ __forceinline__ void fold_runs(const float2 *part, int runs, float scale, int lane, float &m, float &sum) {
+  m = -INFINITY;
+  sum = 0.f;
+  for (int p0 = lane; p0 < runs; p0 += 256) {
+    float2 q[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = p0 + 32 * j < runs ? __ldcg(part + p0 + 32 * j) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int j = 0; j < 8; j++) fold_pair<SCALED>(m, sum, q[j].x, q[j].y, scale);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, sum, o);
+    fold_pair<SCALED>(m, sum, pm, ps, scale);
+  }
 }
 
 // Where a warp is: run `item` of all rows, at one of its chunks.
@@ -159,9 +173,9 @@ __device__ __forceinline__ void load_chunk(const DistillRow<T> &r, int chunk, in
 }
 
 // exponents of 2 of two logits, relative to the reference whose negative is nr
-template <typename T> __device__ __forceinline__ float2 exponents(float2 x, float2 scale, float2 nr);
-template <> __device__ __forceinline__ float2 exponents<__half>(float2 x, float2 scale, float2 nr) { return fma2(x, scale, nr); }
-template <> __device__ __forceinline__ float2 exponents<float>(float2 x, float2 scale, float2 nr) { return mul2(add2(x, nr), scale); }
+template <bool SCALED> __device__ __forceinline__ float2 exponents(float2 x, float2 scale, float2 nr) {
+  return SCALED ? fma2(x, scale, nr) : mul2(add2(x, nr), scale);
+}
 
 __device__ __forceinline__ bool is_word(int32_t c, float t, int64_t v) { return c >= 0 && c < v && t != -INFINITY; }
 
@@ -197,7 +211,7 @@ __device__ __forceinline__ bool teacher_row(const int32_t *is, const float *t, i
   return __any_sync(kFull, some);
 }
 
-// The loss of a row by one warp, over the teacher's words (in f64: its terms cancel), after the fold of the row's runs, eight per lane in flight.
+// The loss of a row by one warp, over the teacher's words (in f64: its terms cancel), after the fold of the row's runs.
 struct DistillLoss {
   const int32_t *is;
   const float *t;
@@ -205,25 +219,14 @@ struct DistillLoss {
   float tau;
   float *loss, *lse;
 };
-template <typename T>
+template <typename T, bool SCALED>
 __device__ __forceinline__ void distill_row(const DistillLoss &a, const T *s, int64_t v, const float2 *part, int runs, float scale, int64_t row, int lane, int *wi,
                                             float *wq) {
   const int k = a.k;
   const bool some = teacher_row<true>(a.is + row * k, a.t + row * k, k, v, 1.f / a.tau, lane, wi, wq);
-  float m = -INFINITY, sum = 0.f;
-  for (int p0 = lane; p0 < runs; p0 += 256) {
-    float2 q[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) q[j] = p0 + 32 * j < runs ? __ldcg(part + row * runs + p0 + 32 * j) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-    for (int j = 0; j < 8; j++) fold_pair<T>(m, sum, q[j].x, q[j].y, scale);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, sum, o);
-    fold_pair<T>(m, sum, pm, ps, scale);
-  }
-  const double inv_tau = 1.0 / (double)a.tau, l = (double)m * (sizeof(T) == 2 ? L_LN2 : inv_tau) + log((double)sum);
+  float m, sum;
+  fold_runs<SCALED>(part + row * runs, runs, scale, lane, m, sum);
+  const double inv_tau = 1.0 / (double)a.tau, l = (double)m * (SCALED ? L_LN2 : inv_tau) + log((double)sum);
   double total = 0;
   if (some) {
 #pragma unroll 4
@@ -243,7 +246,7 @@ __device__ __forceinline__ void distill_row(const DistillLoss &a, const T *s, in
 }
 
 // (maximum, sum) of every run.  JOIN: of few rows, whose losses the CTA that ends last then makes; `ticket` is 0 between launches.
-template <typename T, bool JOIN>
+template <typename T, bool SCALED, bool JOIN>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
 distill_part_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, float scale, float2 *part,
                     uint32_t *ticket, const DistillLoss a) {
@@ -269,10 +272,10 @@ distill_part_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, floa
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
       if (lane + 32 * i < d.groups) mx = fmaxf(mx, group_max(x[i], (const T *)nullptr));
-    mx = fmaxf(m, LogitUnit<T>::of(mx, scale));
+    mx = fmaxf(m, LogitUnit<SCALED>::of(mx, scale));
     const float ref = mx == -INFINITY ? 0.f : mx;
     const float2 sc = make_float2(scale, scale), nr = make_float2(-ref, -ref);
-    float2 u = make_float2(sum * ex2(LogitUnit<T>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
+    float2 u = make_float2(sum * ex2(LogitUnit<SCALED>::log2(m - ref, scale)), 0.f), b = make_float2(0.f, 0.f);
     m = mx;
 #pragma unroll
     for (int i = 0; i < D_PER; i++)
@@ -281,7 +284,7 @@ distill_part_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, floa
         unpack(x[i], f);
 #pragma unroll
         for (int j = 0; j < W; j += 4) {
-          const float2 e = exponents<T>(make_float2(f[j], f[j + 1]), sc, nr), g = exponents<T>(make_float2(f[j + 2], f[j + 3]), sc, nr);
+          const float2 e = exponents<SCALED>(make_float2(f[j], f[j + 1]), sc, nr), g = exponents<SCALED>(make_float2(f[j + 2], f[j + 3]), sc, nr);
           u = add2(u, make_float2(ex2(e.x), ex2(e.y)));
           b = add2(b, make_float2(ex2(g.x), ex2(g.y)));
         }
@@ -291,7 +294,7 @@ distill_part_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, floa
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const float om = __shfl_xor_sync(kFull, m, o), os = __shfl_xor_sync(kFull, sum, o);
-        fold_pair<T>(m, sum, om, os, scale);
+        fold_pair<SCALED>(m, sum, om, os, scale);
       }
       if (lane == 0) part[here.item] = make_float2(m, sum);
       m = -INFINITY;
@@ -311,19 +314,19 @@ distill_part_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, floa
     __threadfence();
     int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * a.k;
     for (int64_t row = threadIdx.x >> 5; row < n; row += D_WARPS)
-      distill_row<T>(a, s, v, part, d.runs, scale, row, lane, wi, reinterpret_cast<float *>(wi + a.k));
+      distill_row<T, SCALED>(a, s, v, part, d.runs, scale, row, lane, wi, reinterpret_cast<float *>(wi + a.k));
     if (threadIdx.x == 0) *ticket = 0;
   }
 }
 
-template <typename T>
+template <typename T, bool SCALED>
 __global__ void __launch_bounds__(256)
 distill_loss_kernel(const T *s, const float2 *part, int runs, int64_t n, int64_t v, float scale, const DistillLoss a) {
   extern __shared__ float sh[];                      // per warp: words [k], log q [k]
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   chain_wait();
   int *wi = reinterpret_cast<int *>(sh) + (threadIdx.x >> 5) * 2 * a.k;
-  if (row < n) distill_row<T>(a, s, v, part, runs, scale, row, threadIdx.x & 31, wi, reinterpret_cast<float *>(wi + a.k));
+  if (row < n) distill_row<T, SCALED>(a, s, v, part, runs, scale, row, threadIdx.x & 31, wi, reinterpret_cast<float *>(wi + a.k));
 }
 
 // What the gradient needs of a row's teacher, by one warp in shared memory: per word its weight; of places with the same word one has
@@ -384,10 +387,16 @@ __device__ __forceinline__ float4 teacher_record(const DistillTeacher &a, int64_
   const float hi = (float)shift;
   return make_float4(a.dl[row] * a.tau, some ? 1.f : 0.f, wide ? lse : hi, wide ? 1.f : exp2f((float)((double)hi - shift)));
 }
+// Below D_FAR an lse in f32 says too little about the row: the record then has the maximum of the row's logits and 1 / the sum of
+// exp((S - maximum) / tau), from runs that distill_part_kernel has worked off again.
+struct DistillFar {
+  const float2 *part;                                // or nullptr
+  int runs;
+  float scale;                                       // log2 e / tau
+};
 // Both for every row, one warp per row.
 __global__ void __launch_bounds__(256)
-distill_teacher_kernel(bool wide, const DistillTeacher a, int64_t n, int64_t v, int32_t *words, float *weights,
-                       float4 *rows) {
+distill_teacher_kernel(bool wide, const DistillTeacher a, const DistillFar far, int64_t n, int64_t v, int32_t *words, float *weights, float4 *rows) {
   extern __shared__ float sh[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
@@ -400,7 +409,14 @@ distill_teacher_kernel(bool wide, const DistillTeacher a, int64_t n, int64_t v, 
     words[row * a.k + j] = wi[j];
     weights[row * a.k + j] = wq[j];
   }
-  if (lane == 0) rows[row] = teacher_record(a, row, some, wide);
+  float4 record = teacher_record(a, row, some, wide);
+  if (far.part != nullptr) {
+    float m, sum;
+    fold_runs<false>(far.part + row * far.runs, far.runs, far.scale, lane, m, sum);
+    record.z = m;
+    record.w = 1.f / sum;
+  }
+  if (lane == 0) rows[row] = record;
 }
 
 // The gradient is read and written by neighbouring warps at neighbouring places, which HBM likes better than long runs: with runs
@@ -408,16 +424,17 @@ distill_teacher_kernel(bool wide, const DistillTeacher a, int64_t n, int64_t v, 
 // where a chunk is twice the elements per instruction around them).
 template <typename T> constexpr int D_GRAD_RUN = sizeof(T) == 2 ? 2 : 1;
 
-// exponents of 2 of two logits less the row's reference, whose negative is nr: scale is log2 e / tau (binary16) or 1 / tau (f32)
-template <typename T> __device__ __forceinline__ float2 row_exponents(float2 x, float2 scale, float2 nr);
-template <> __device__ __forceinline__ float2 row_exponents<__half>(float2 x, float2 scale, float2 nr) { return fma2(x, scale, nr); }
-template <> __device__ __forceinline__ float2 row_exponents<float>(float2 x, float2 scale, float2 nr) {
-  return mul2(fma2(x, scale, nr), make_float2(L_LOG2E, L_LOG2E));
+// exponents of 2 of two logits less the row's reference, whose negative is nr: scale is log2 e / tau (binary16, or far) or 1 / tau (f32)
+template <typename T, bool FAR> __device__ __forceinline__ float2 row_exponents(float2 x, float2 scale, float2 nr) {
+  if (FAR) return exponents<false>(x, scale, nr);
+  const float2 y = fma2(x, scale, nr);
+  return sizeof(T) == 2 ? y : mul2(y, make_float2(L_LOG2E, L_LOG2E));
 }
 
 // Every chunk: the student's softmax; after a run the words of the teacher that lie in it once more.
 // OWN: every warp has one run at most, and finds what it needs of its row's teacher for itself.
-template <typename T, bool OWN>
+// FAR: the rows' records have their own maxima and sums.
+template <typename T, bool OWN, bool FAR>
 __global__ void __launch_bounds__(D_THREADS, D_CTAS)
 distill_grad_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, float scale, const DistillTeacher a,
                     const int32_t *words, const float *weights, const float4 *rows, T *ds) {
@@ -462,7 +479,7 @@ distill_grad_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, floa
         unpack(x[i], y);
 #pragma unroll
         for (int j = 0; j < W; j += 2) {
-          const float2 e = row_exponents<T>(make_float2(y[j], y[j + 1]), sc, nr);
+          const float2 e = row_exponents<T, FAR>(make_float2(y[j], y[j + 1]), sc, nr);
           y[j] = ex2(e.x) * fc;
           y[j + 1] = ex2(e.y) * fc;
         }
@@ -486,7 +503,7 @@ distill_grad_kernel(const T *s, int64_t n, int64_t v, const DistillShape d, floa
         for (int j = lane; j < a.k; j += 32) {
           const int word = OWN ? wi[j] : words[here.row * a.k + j];
           if (word >= 0 && word >= c0 && word < c1) {
-            const float xw = to_f32<T>(r.base[word]), p = ex2(row_exponents<T>(make_float2(xw, xw), sc, nr).x) * rc.w;
+            const float xw = to_f32<T>(r.base[word]), p = ex2(row_exponents<T, FAR>(make_float2(xw, xw), sc, nr).x) * rc.w;
             out[word] = from_f32<T>((p - (OWN ? wq[j] : weights[here.row * a.k + j])) * rc.x);
           }
         }
@@ -513,30 +530,39 @@ static bool own_teacher(const DistillShape &d, int64_t n, int64_t k, int num_sms
   return n * d.runs <= (int64_t)num_sms * D_CTAS * D_WARPS && k <= D_OWN_K;
 }
 
-size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms) {
-  const DistillShape d = distill_shape(s, n, v, elem, num_sms, !grad ? 16 : elem == 2 ? D_GRAD_RUN<__half> : D_GRAD_RUN<float>);
-  if (!grad) return up256((size_t)n * d.runs * sizeof(float2));
-  return own_teacher(d, n, k, num_sms) ? 0 : up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float4));
+// Temperatures below which logits over the temperature need more than the 24 bits of an f32: a logit of 65504 there is 2^22 or more, and
+// neither the rounding of a scaled maximum (at most 0.4 above) nor that of the lse can be left aside.  The gradient then reads the logits
+// once more for statistics of its own (2049 x 50001 f32: 210 us instead of 139).
+constexpr float D_FAR = 0x1p-6f;
+static bool distill_far(float tau) { return tau < D_FAR; }
+constexpr int D_LONGEST = 16;                        // chunks of a run whose elements are only read
+
+size_t distill_workspace_bytes(const void *s, float tau, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms) {
+  const size_t part = up256((size_t)n * distill_shape(s, n, v, elem, num_sms, D_LONGEST).runs * sizeof(float2));
+  if (!grad) return part;
+  const DistillShape d = distill_shape(s, n, v, elem, num_sms, elem == 2 ? D_GRAD_RUN<__half> : D_GRAD_RUN<float>);
+  if (!distill_far(tau) && own_teacher(d, n, k, num_sms)) return 0;
+  return up256((size_t)(n * k) * 4) * 2 + up256((size_t)n * sizeof(float4)) + (distill_far(tau) ? part : 0);
 }
 
-template <typename T>
+template <typename T, bool SCALED>
 static cudaError_t distill(void *workspace, uint32_t *ticket, const T *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v, int64_t k,
                            float *loss, float *lse, int num_sms, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
-  const DistillShape d = distill_shape(s, n, v, sizeof(T), num_sms, 16);
+  const DistillShape d = distill_shape(s, n, v, sizeof(T), num_sms, D_LONGEST);
   float2 *part = reinterpret_cast<float2 *>(workspace);
   const float scale = (float)(1.0 / (L_LN2 * (double)tau));
   const DistillLoss a = {is, t, (int)k, tau, loss, lse};
   const unsigned grid = chunk_grid(n * d.runs, num_sms);
   if (own_loss(d, n, k))
-    return launch_after(distill_part_kernel<T, true>, grid, D_THREADS, (size_t)D_WARPS * 2 * k * 4, stream, s, n, v, d, scale, part, ticket, a);
-  cudaError_t err = launch_after(distill_part_kernel<T, false>, grid, D_THREADS, 0, stream, s, n, v, d, scale, part, ticket, a);
+    return launch_after(distill_part_kernel<T, SCALED, true>, grid, D_THREADS, (size_t)D_WARPS * 2 * k * 4, stream, s, n, v, d, scale, part, ticket, a);
+  cudaError_t err = launch_after(distill_part_kernel<T, SCALED, false>, grid, D_THREADS, 0, stream, s, n, v, d, scale, part, ticket, a);
   if (err != cudaSuccess) return err;
   const int rw = row_warps(n, num_sms);
   static unsigned long long allowed = 0;
-  err = allow_smem(reinterpret_cast<const void *>(distill_loss_kernel<T>), 8 * 2 * DISTILL_MAX_K * 4, allowed);
+  err = allow_smem(reinterpret_cast<const void *>(distill_loss_kernel<T, SCALED>), 8 * 2 * DISTILL_MAX_K * 4, allowed);
   if (err != cudaSuccess) return err;
-  return launch_after(distill_loss_kernel<T>, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream, s, part, d.runs, n, v, scale, a);
+  return launch_after(distill_loss_kernel<T, SCALED>, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * 2 * k * 4, stream, s, part, d.runs, n, v, scale, a);
 }
 
 template <typename T>
@@ -548,27 +574,43 @@ static cudaError_t distill_grad(void *workspace, const T *s, const int32_t *is, 
   int32_t *words = reinterpret_cast<int32_t *>(ws);
   float *weights = reinterpret_cast<float *>(ws + up256((size_t)(n * k) * 4));
   float4 *rows = reinterpret_cast<float4 *>(ws + 2 * up256((size_t)(n * k) * 4));
-  const float scale = (float)(1.0 / ((sizeof(T) == 2 ? L_LN2 : 1.0) * (double)tau));
+  const bool far = distill_far(tau);
+  const float scale = (float)(1.0 / ((sizeof(T) == 2 || far ? L_LN2 : 1.0) * (double)tau));
   DistillTeacher a = {is, t, (int)k, 32, tau, dl, lse};
   while (a.table < 2 * k) a.table *= 2;
   const unsigned grid = chunk_grid(n * d.runs, num_sms);
-  if (own_teacher(d, n, k, num_sms))
-    return launch_after(distill_grad_kernel<T, true>, grid, D_THREADS, (size_t)D_WARPS * a.shared() * 4, stream, s, n, v, d, scale, a, words, weights, rows, ds);
+  if (!far && own_teacher(d, n, k, num_sms))
+    return launch_after(distill_grad_kernel<T, true, false>, grid, D_THREADS, (size_t)D_WARPS * a.shared() * 4, stream, s, n, v, d, scale, a, words, weights, rows,
+                        ds);
+  DistillFar f = {nullptr, 0, scale};
+  if (far) {
+    const DistillShape p = distill_shape(s, n, v, sizeof(T), num_sms, D_LONGEST);
+    float2 *part = reinterpret_cast<float2 *>(reinterpret_cast<uint8_t *>(rows) + up256((size_t)n * sizeof(float4)));
+    const cudaError_t err = launch_after(distill_part_kernel<T, false, false>, chunk_grid(n * p.runs, num_sms), D_THREADS, 0, stream, s, n, v, p, scale, part,
+                                         nullptr, DistillLoss{});
+    if (err != cudaSuccess) return err;
+    f.part = part;
+    f.runs = p.runs;
+  }
   const int rw = row_warps(n, num_sms);
   static unsigned long long allowed = 0;
   cudaError_t err = allow_smem(reinterpret_cast<const void *>(distill_teacher_kernel), 8 * (3 * DISTILL_MAX_K + 2 * DISTILL_MAX_K) * 4, allowed);
   if (err != cudaSuccess) return err;
-  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * a.shared() * 4, stream, sizeof(T) == 4, a, n, v, words, weights,
-                     rows);
+  err = launch_after(distill_teacher_kernel, (unsigned)((n + rw - 1) / rw), 32 * rw, (size_t)rw * a.shared() * 4, stream, sizeof(T) == 4, a, f, n, v, words,
+                     weights, rows);
   if (err != cudaSuccess) return err;
-  return launch_after(distill_grad_kernel<T, false>, grid, D_THREADS, 0, stream, s, n, v, d, scale, a, words, weights, rows, ds);
+  if (far) return launch_after(distill_grad_kernel<T, false, true>, grid, D_THREADS, 0, stream, s, n, v, d, scale, a, words, weights, rows, ds);
+  return launch_after(distill_grad_kernel<T, false, false>, grid, D_THREADS, 0, stream, s, n, v, d, scale, a, words, weights, rows, ds);
 }
 
 cudaError_t launch_topk_distill(void *workspace, void *ticket, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v,
                                 int64_t k, float *loss, float *lse, int num_sms, cudaStream_t stream) {
   uint32_t *tk = reinterpret_cast<uint32_t *>(ticket);
-  if (elem == 2) return distill<__half>(workspace, tk, reinterpret_cast<const __half *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
-  return distill<float>(workspace, tk, reinterpret_cast<const float *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
+  const __half *h = reinterpret_cast<const __half *>(s);
+  if (elem == 2)
+    return distill_far(tau) ? distill<__half, false>(workspace, tk, h, is, t, tau, n, v, k, loss, lse, num_sms, stream)
+                            : distill<__half, true>(workspace, tk, h, is, t, tau, n, v, k, loss, lse, num_sms, stream);
+  return distill<float, false>(workspace, tk, reinterpret_cast<const float *>(s), is, t, tau, n, v, k, loss, lse, num_sms, stream);
 }
 cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,
                                      const float *dl, int64_t n, int64_t v, int64_t k, void *ds, int num_sms, cudaStream_t stream) {

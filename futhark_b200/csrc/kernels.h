@@ -205,7 +205,7 @@ cudaError_t launch_vocab_xent_grad(const VocabPlan &p, void *workspace, const ui
 
 // ---- losses on logits (k_losses.cu); elem is the size of a logit: 2 (binary16) or 4 ---------------
 constexpr int DISTILL_MAX_K = 1024, ROUTER_MAX_E = 1024;
-size_t distill_workspace_bytes(const void *s, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms);
+size_t distill_workspace_bytes(const void *s, float tau, int64_t n, int64_t v, int64_t k, int elem, bool grad, int num_sms);
 cudaError_t launch_topk_distill(void *workspace, void *ticket, int elem, const void *s, const int32_t *is, const float *t, float tau, int64_t n, int64_t v,
                                 int64_t k, float *loss, float *lse, int num_sms, cudaStream_t stream);
 cudaError_t launch_topk_distill_grad(void *workspace, int elem, const void *s, const int32_t *is, const float *t, float tau, const float *lse,

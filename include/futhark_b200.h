@@ -529,7 +529,9 @@ int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, struct futhar
  *   outside [0, v), or whose logit is -inf, is padding; a row without words has loss 0; a word may stand in a row more than once.
  *   tau is in [2^-60, 2^60], k at most 1024.
  * entry topk_distill_grad_{f32,f16} (tau) (S) (iss) (T) (lses: [n]f32) (dls: [n]f32): [n][v]{f32,f16}
- *   The gradient with respect to S of sum_i dls[i] losses[i]; rows without words have gradient 0. */
+ *   The gradient with respect to S of sum_i dls[i] losses[i]; rows without words have gradient 0.  The student's probabilities are
+ *   taken relative to lses, so they are off by |lses[i]| 2^-24 of themselves; below a temperature of 2^-6, where that would be
+ *   too much, S is read once more instead. */
 int futhark_entry_topk_distill_f32(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0, const float in0,
                                    const struct futhark_f32_2d *in1, const struct futhark_i32_2d *in2, const struct futhark_f32_2d *in3);
 int futhark_entry_topk_distill_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0, const float in0,

@@ -4,7 +4,7 @@ import pytest
 
 import futhark_b200 as fb
 import loss_reference as ref
-from test_gpu_losses import half, within, xent_inputs
+from test_gpu_losses import distill_inputs, half, within, xent_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,43 @@ def test_vocab_xent_operands_of_any_size(ctx, scale):
     big = np.abs(want) > 65504                             # rounds to an infinity: both do, or the value is near the border
     within(dw[~big], want[~big], ew[~big], "dW")
     assert np.isinf(dw[np.abs(want) > 65600]).all() and not np.isnan(dw).any()
+
+
+# either side of the temperature below which the gradient takes statistics of its own, and both ends of what is accepted
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("tau", [2.0 ** -60, 1e-9, 4e-5, 2.0 ** -6 * 0.999, 2.0 ** -6, 0.05, 100.0, 2.0 ** 60])
+@pytest.mark.parametrize("n,v,k", [(3, 300, 5), (17, 5001, 40), (300, 2000, 9), (2, 300000, 300)])
+def test_topk_distill_at_any_temperature(ctx, t, tau, n, v, k):
+    """Exponents of 2 below 2^-150 of the row's sum do not count, so one that does is (S - max) log2(e) / tau with three
+    roundings, at most 150 * 3 * 2^-24 ln 2 < 2^-15 of what it stands for; above 2^-6 they come from an lse rounded to f32 as well.
+    The teacher's log q is a difference times 1 / tau, three roundings too: q is off by 3 * 2^-24 |log q| of itself beside the usual
+    2^-19 of a term."""
+    S, iss, T, dl = distill_inputs(t, n, v, k, n + v)
+    S[0, : v // 2] = np.finfo(S.dtype).min                 # a mask
+    S[-1, 7] = S[-1, 11] = S[-1].max()                     # two words alike
+    tau = float(np.float32(tau))
+    dl *= np.float32(min(1, 1 / tau))
+    loss, lse = fb.topk_distill(ctx, t, tau, S, iss, T)
+    want, wantl, _ = ref.topk_distill(S, iss, T, tau)
+    S64 = S.astype(np.float64)
+    top = np.abs(S64.max(axis=1)) / tau
+    within(lse, wantl, 2.0 ** -22 * (top + np.abs(wantl)) + 2.0 ** -20, "lse")
+    ok, q, lq = ref.teacher(iss, T, tau, v)
+    size = np.abs(lq) + np.abs(np.take_along_axis(S64, np.where(ok, iss, 0).astype(np.int64), 1)) / tau + np.abs(wantl)[:, None]
+    err = tau * tau * ((q * size * (2.0 ** -19 + 3 * 2.0 ** -24 * np.abs(lq))).sum(axis=1) + 2.0 ** -21 * top + 2.0 ** -19)
+    over = np.abs(want) > float(np.finfo(np.float32).max)      # a masked word of the teacher's: no f32 number
+    assert np.isposinf(loss[over]).all()
+    within(loss[~over], want[~over], err[~over], "loss")
+    g = fb.topk_distill_grad(ctx, t, tau, S, iss, T, lse, dl)
+    # differences before quotients: even 64 bits lose the logarithm of a sum beside 2^62
+    p = np.exp((S64 - S64.max(axis=1, keepdims=True)) / tau)
+    p = p / p.sum(axis=1, keepdims=True) * ok.any(axis=1)[:, None]
+    wg, mag = p.copy(), p
+    for i in range(n):
+        np.add.at(wg[i], iss[i][ok[i]], -q[i][ok[i]])
+        np.add.at(mag[i], iss[i][ok[i]], q[i][ok[i]])
+    c = dl.astype(np.float64)[:, None] * tau
+    wg, mag = wg * c, mag * c
+    err = 2.0 ** -15 + (0 if tau < 2.0 ** -6 else 2.0 ** -22 * (top + np.abs(wantl)))
+    out = ref.H * np.abs(wg) + ref.HMIN if t == "f16" else 1e-37
+    within(half(g) if t == "f16" else g, wg, mag * (np.zeros(n) + err)[:, None] + out, "dS")
