@@ -269,14 +269,14 @@ _mirror_module = None
 
 
 def _native():
-    """The native callables (futhark_b200/mirror.c), built beside the library."""
+    """The native callables (futhark_b200/mirror.c), built beside the library; the same through ctypes where they were not."""
     global _mirror_module
     if _mirror_module is None:
         try:
-            from . import _mirror
-        except ImportError as e:
-            raise ImportError("the native part of the mirror is missing: run `python -m futhark_b200.build` (%s)" % e)
-        _mirror_module = _mirror
+            from . import _mirror as module
+        except ImportError:
+            from . import mirror as module
+        _mirror_module = module
     return _mirror_module
 
 

@@ -64,7 +64,10 @@ def build(force=False, verbose=False, ptxas_v=False):
     if ptxas_v and log:
         print(log)
     build_cli(force, verbose)
-    build_mirror(force, verbose)
+    try:
+        build_mirror(force, verbose)
+    except (OSError, subprocess.CalledProcessError) as e:      # no compiler or no Python headers
+        print("the mirror's native callables were not built, it will go through ctypes: %s" % e, file=sys.stderr)
     return LIB
 
 
