@@ -341,7 +341,7 @@ class Array:
         d = self._interface                  # neither the shape nor the address of an array ever changes
         if d is None or self.ptr is None:
             d = self._interface = _type_fns[self.tname].interface(self.ctx.ptr, self.ptr)
-        return d
+        return dict(d)                       # the caller's own
 
     def values_into(self, out):
         """Asynchronous copy to a host buffer (futhark_values_*); call ctx.sync() before reading."""

@@ -95,3 +95,15 @@ def test_loss_entry_points_check_the_types_of_arrays():
                         getattr(ctx, name)(*head, *arrays(types[:i] + (other,) + types[i + 1:]))
         with pytest.raises((TypeError, ValueError), match="(?!arrays of types)"):
             getattr(ctx, name)(*head, *arrays(types))
+
+
+def test_a_description_belongs_to_its_caller(bare):
+    ctx = fb.Context.__new__(fb.Context)
+    ctx.ptr = bare
+    a = fb.Array(ctx, "f32_2d", fb._type_fns["f32_2d"].new_raw(bare, 4096, 3, 5))
+    d = a.__cuda_array_interface__
+    want = dict(d)
+    d["version"] = 3
+    d.pop("shape")
+    assert a.__cuda_array_interface__ == want and a.shape == (3, 5)
+    a.free()
