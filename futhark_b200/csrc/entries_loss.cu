@@ -89,7 +89,9 @@ typedef struct futhark_opaque_tup3_arr1d_f32_arr1d_i32_arr1d_f32 balance_t;
 // ---- cross entropy over a vocabulary ------------------------------------------------------------------
 // sizes that are 32-bit numbers in the kernels, tiles among them
 static bool vocab_fits(int64_t n, int64_t v, int64_t d) { return fits(n) && fits(v) && fits(d + 8) && n / 256 * (v / 128) < ((int64_t)1 << 30); }
-static std::string vocab_details(int64_t n, int64_t v, int64_t d) { return "{" + kv("n", n) + "," + kv("v", v) + "," + kv("d", d) + "}"; }
+static std::string vocab_details(int64_t n, int64_t v, int64_t d, const std::string &more = "") {
+  return "{" + kv("n", n) + "," + kv("v", v) + "," + kv("d", d) + more + "}";
+}
 
 extern "C" {
 
@@ -129,7 +131,7 @@ int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, grads_t **out
   auto *rec = call.record<grads_t>();
   const fb::VocabPlan plan = fb::vocab_plan(n, v, d, aligned16(in0->mem), aligned16(in1->mem), true, ctx->num_sms);
   void *ws = call.workspace(plan.bytes, "vocab_xent_grad_f16.workspace");
-  call.launch("vocab_xent_grad_f16.segmap_segred", "vjp of vocab_xent_f16", [&] { return vocab_details(n, v, d); }, [&] {
+  call.launch("vocab_xent_grad_f16.segmap_segred", "vjp of vocab_xent_f16", [&] { return vocab_details(n, v, d, "," + kv("pieces", plan.pieces) + "," + kv("parts", plan.splits)); }, [&] {
     ctx->failure_is_an_option = true;
     return fb::launch_vocab_xent_grad(plan, ws, dptr<uint16_t>(in0->mem), dptr<uint16_t>(in1->mem), dptr<int32_t>(in2->mem), dptr<float>(in3->mem),
                                       dptr<float>(in4->mem), dptr<float>(in5->mem), dptr<uint16_t>(dx->mem), dptr<uint16_t>(dw->mem), n, v, d,
