@@ -9,7 +9,7 @@
 // tensor memory: the contraction's epilogue folds each 256 x 256 tile to one (maximum, sum) pair per
 // row, and a small kernel (in small calls the last CTA) folds the v/256 pairs of a row.  The gradient works the vocabulary off in pieces: a
 // piece's logits are computed again (by the same instructions; sums of more than 2048 products in one
-// accumulator where the losses had two, 1.4e-6 of a logit at most), turned into g in
+// accumulator where the losses had two, which was 1.4e-6 of a logit over 4096 products and grows with their number), turned into g in
 // binary16 in the epilogue, and that piece of g meets W (summed over the pieces in f32) and X.
 //
 // Rounding of g to 11 bits.  With q_i = 1 - exp(-loss_i) the row is kept as
