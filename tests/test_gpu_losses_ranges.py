@@ -95,3 +95,49 @@ def test_topk_distill_at_any_temperature(ctx, t, tau, n, v, k):
     err = 2.0 ** -15 + (0 if tau < 2.0 ** -6 else 2.0 ** -22 * (top + np.abs(wantl)))
     out = ref.H * np.abs(wg) + ref.HMIN if t == "f16" else 1e-37
     within(half(g) if t == "f16" else g, wg, mag * (np.zeros(n) + err)[:, None] + out, "dS")
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("n,v,k,shift", [(5, 2111, 9, 1), (5, 2111, 9, 3), (400, 333, 3, 5), (3, 64, 0, 0), (0, 70, 2, 0), (4, 0, 2, 0), (2, 3, 1024, 1)])
+def test_topk_distill_at_small_temperatures_of_any_shape(ctx, t, n, v, k, shift):
+    S, iss, T, dl = distill_inputs(t, n, v, k, 9)
+    raw = fb._bits(S).ravel()
+    base = ctx.new(t + "_1d", np.concatenate([np.zeros(shift, raw.dtype), raw]))
+    arrs = [ctx.new_raw(t + "_2d", base.raw + shift * raw.itemsize, n, v), ctx.new("i32_2d", iss), ctx.new("f32_2d", T), ctx.new("f32_1d", dl)]
+    tau = float(np.float32(1e-3))
+    loss, lse = ctx.entry_topk_distill(t, tau, *arrs[:3])
+    g = ctx.entry_topk_distill_grad(t, tau, *arrs[:3], lse, arrs[3])
+    want, mag = ref.topk_distill_grad(S, iss, T, tau, dl) if n and v else (np.zeros((n, v)), np.zeros((n, v)))
+    out = ref.H * np.abs(want) + ref.HMIN if t == "f16" else 1e-37
+    got = half(g.values()) if t == "f16" else g.values()
+    assert got.shape == (n, v)
+    within(got, want, 2.0 ** -15 * mag + out, "dS")        # exponents as above
+    for a in [loss, lse, g, base] + arrs:
+        a.free()
+
+
+@pytest.mark.parametrize("n,d", [(20, 64), (300, 400)])
+@pytest.mark.parametrize("weight", [0.0, -0.0, 1e-44, -1e30])
+def test_vocab_xent_weights_all_alike(ctx, n, d, weight):
+    X, W, ts, dl = xent_inputs(n, 200, d, 4)
+    dl[:] = weight
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    dx, dw = (half(x) for x in fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl))
+    if abs(weight) < 1:
+        assert not dx.any() and not dw.any()               # the second one's gradients are below 2^-25
+    else:
+        ok = (ts >= 0) & (ts < 200)
+        assert np.isinf(dx[ok]).mean() > 0.99 and not np.isnan(dx).any() and np.isinf(dw).mean() > 0.99 and not np.isnan(dw).any()
+
+
+def test_losses_in_a_context_with_unified_memory(ctx):
+    X, W, ts, dl = xent_inputs(50, 400, 72, 2)
+    S, iss, T, ddl = distill_inputs("f16", 9, 900, 5, 3)
+    want = None
+    for unified in (False, True):
+        with fb.Context(unified_memory=unified, profiling=unified) as c:
+            l = fb.vocab_xent_f16(c, X, W, ts)
+            s = fb.topk_distill(c, "f16", 2.0, S, iss, T)
+            got = (*l, *fb.vocab_xent_grad_f16(c, X, W, ts, *l, dl), *s, fb.topk_distill_grad(c, "f16", 2.0, S, iss, T, s[1], ddl))
+            want = want or got
+            assert all(np.array_equal(a, b) for a, b in zip(got, want))
