@@ -85,7 +85,7 @@ struct VocabArgs {
   int tiles_m, tiles_n;
   const int32_t *targets;       // VE_SOFTMAX, VE_GRAD
   int v, v0;                    // size of the vocabulary, first word of the piece
-  float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum in units of log 2, sum)
+  float2 *part;                 // VE_SOFTMAX: [M][tiles_n] (maximum, sum of exp(logit - maximum))
   float *ztarget;
   float *loss, *lse;            // and the results, where small calls finish them,
   uint32_t *ticket;             // with a word that is 0 between launches
@@ -135,19 +135,19 @@ __device__ __forceinline__ void row_loss(const float2 *part, int tiles, const fl
 #pragma unroll
     for (int j = 0; j < 8; j++) mn = fmaxf(mn, p[j].x);
     const float ref = mn == -INFINITY ? 0.f : mn;
-    s *= exp2f(m - ref);
+    s *= exp2f((m - ref) * V_LOG2E);
 #pragma unroll
-    for (int j = 0; j < 8; j++) s += p[j].y * exp2f(p[j].x - ref);
+    for (int j = 0; j < 8; j++) s += p[j].y * exp2f((p[j].x - ref) * V_LOG2E);
     m = mn;
   }
   for (int o = L >> 1; o > 0; o >>= 1) {
     const float pm = __shfl_xor_sync(kFull, m, o), ps = __shfl_xor_sync(kFull, s, o);
     const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.f : mn;
-    s = s * exp2f(m - ref) + ps * exp2f(pm - ref);
+    s = s * exp2f((m - ref) * V_LOG2E) + ps * exp2f((pm - ref) * V_LOG2E);
     m = mn;
   }
   if (lane == 0 && valid) {
-    const double l = ((double)m + log2((double)s)) * 0.69314718055994530942;
+    const double l = (double)m + log((double)s);
     const int64_t t = targets[row];
     lse[row] = (float)l;
     loss[row] = t >= 0 && t < v ? (float)(l - (double)__ldcg(ztarget + row)) : 0.f;
@@ -368,9 +368,10 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
         tc_fence_after();
         fetch(t + npairs, split, tm, tn);
         const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * VT;
-        float m2 = -INFINITY, sum = 0.f;
+        float m = -INFINITY, sum = 0.f;
 
-        // 32 columns of a row: running maximum (in units of log 2, so that it is exactly what was subtracted) and sum
+        // 32 columns of a row: running maximum and sum.  The maximum is subtracted before the scaling: scaled first it would be rounded,
+        // by up to |m| 2^-24, which leaves the exponents' range for logits above 2^30
         auto fold = [&](uint32_t (&v)[32], int c0) {
           if (c0 >= ncols) return;
           if (c0 + 32 > ncols) {
@@ -382,20 +383,20 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
           for (int j = 0; j < 4; j++) mx[j] = __uint_as_float(v[j]);
 #pragma unroll
           for (int j = 4; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
-          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * V_LOG2E;
-          const float mn = fmaxf(m2, cm);
+          const float cm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float mn = fmaxf(m, cm);
           const float ref = mn == -INFINITY ? 0.f : mn;    // a row of -inf so far: the sum stays 0
           const float2 scale = make_float2(V_LOG2E, V_LOG2E), nr = make_float2(-ref, -ref);
-          float2 s0 = make_float2(sum * ex2(m2 - ref), 0.f), s1 = make_float2(0.f, 0.f);
+          float2 s0 = make_float2(sum * ex2((m - ref) * V_LOG2E), 0.f), s1 = make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            const float2 e = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale, nr);
-            const float2 f = fma2(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), scale, nr);
+            const float2 e = mul2(add2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), nr), scale);
+            const float2 f = mul2(add2(make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), nr), scale);
             s0 = add2(s0, make_float2(ex2(e.x), ex2(e.y)));
             s1 = add2(s1, make_float2(ex2(f.x), ex2(f.y)));
           }
           sum = (s0.x + s0.y) + (s1.x + s1.y);
-          m2 = mn;
+          m = mn;
           const int tj = tcol - c0;
           if (tj >= 0 && tj < 32) {
             float zt = 0.f;
@@ -509,7 +510,7 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
           // places: it begins when this warp has given back the next tile's accumulator, or this one's where there are two
           float2 *meet = reinterpret_cast<float2 *>(epi) + (tile_it & 1) * (V_WARPS / 4) * 128 + quarter * 32 + lane;
           if (share != 0) {
-            meet[share * 128] = make_float2(m2, sum);
+            meet[share * 128] = make_float2(m, sum);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->met[tile_it & 1][quarter]);
           } else {
@@ -517,14 +518,14 @@ __device__ __forceinline__ void vocab_mma_body(const CUtensorMap &tmA, const CUt
 #pragma unroll
             for (int w = 1; w < V_WARPS / 4; w++) {
               const float2 o = meet[w * 128];
-              const float mn = fmaxf(m2, o.x), ref = mn == -INFINITY ? 0.f : mn;
-              sum = sum * ex2(m2 - ref) + o.y * ex2(o.x - ref);
-              m2 = mn;
+              const float mn = fmaxf(m, o.x), ref = mn == -INFINITY ? 0.f : mn;
+              sum = sum * ex2((m - ref) * V_LOG2E) + o.y * ex2((o.x - ref) * V_LOG2E);
+              m = mn;
             }
           }
         }
         if (!halves) give_back();
-        if (EPI == VE_SOFTMAX && share == 0 && row < a.M) a.part[(int64_t)row * a.tiles_n + this_tn] = make_float2(m2, sum);
+        if (EPI == VE_SOFTMAX && share == 0 && row < a.M) a.part[(int64_t)row * a.tiles_n + this_tn] = make_float2(m, sum);
       }
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       if (!ok) atomicCAS(a.failure, FAIL_NONE, FAIL_MMA_TIMEOUT);

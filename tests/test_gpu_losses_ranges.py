@@ -141,3 +141,18 @@ def test_losses_in_a_context_with_unified_memory(ctx):
             got = (*l, *fb.vocab_xent_grad_f16(c, X, W, ts, *l, dl), *s, fb.topk_distill_grad(c, "f16", 2.0, S, iss, T, s[1], ddl))
             want = want or got
             assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 300, 8), (40, 700, 64), (300, 500, 64), (140, 400, 2500)])
+@pytest.mark.parametrize("size", [1.0, 300.0, 20000.0, 60000.0])
+def test_vocab_xent_logits_of_any_size(ctx, n, v, d, size):
+    """Logits up to 60000^2 d: sums of f32 products, so right to the accumulators' truncations of their terms."""
+    X, W, ts, _ = xent_inputs(n, v, d, 6)
+    X = (np.clip(X.astype(np.float64), -1, 1) * size).astype(np.float16)
+    W = (np.clip(W.astype(np.float64), -1, 1) * size).astype(np.float16)
+    ts[:1] = (X.astype(np.float64) @ W.astype(np.float64).T).argmax(axis=1)[:1]
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    want, wantl = ref.vocab_xent(X, W, ts)
+    err = ref.vocab_xent_error(X, W, ts)
+    within(lse, wantl, err, "lse")
+    within(loss, want, 2 * err, "loss")
