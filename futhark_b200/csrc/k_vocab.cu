@@ -160,13 +160,14 @@ static __host__ __device__ __forceinline__ int join_lanes(int64_t n) {
   return L;
 }
 
-// q_i and the constant term of G's exponent
-__device__ __forceinline__ float row_q(float loss, float lse) {
-  // losses are off by a few units in the last place of lse: q below that is as good as that
-  const float least = 0x1p-22f * fmaxf(1.f, fabsf(lse)), q = -expm1f(-loss);
+// q_i and the constant term of G's exponent.  Near 0 a loss is the logarithm of a sum of f32 numbers that begins with 1 (the target's logit is the
+// maximum, and goes out exactly).  It is off by the roundings of a few dozen additions, 2^-24 each, whatever lse is: a q below 2^-22 is as
+// good as that.
+__device__ __forceinline__ float row_q(float loss) {
+  const float least = 0x1p-22f, q = -expm1f(-loss);
   return q < least ? least : q;
 }
-__device__ __forceinline__ float row_exponent(float loss, float lse) { return 13.f - log2f(row_q(loss, lse)) - lse * V_LOG2E; }
+__device__ __forceinline__ float row_exponent(float loss, float lse) { return 13.f - log2f(row_q(loss)) - lse * V_LOG2E; }
 
 // A_MN / B_MN: the operand is contiguous across the summed axis ([K][M], [K][N]) instead of along it.
 // PAIR: two CTAs per tile of 256 rows; otherwise one per tile of 128 rows, for batches of at most 128 tokens.  Of a pair's 256
@@ -575,7 +576,7 @@ __device__ __forceinline__ bool row_weight(const VocabRows &a, int64_t i, float 
   const int64_t t = a.targets[i];
   const float ls = a.loss[i], l = a.lse[i], d = a.dl[i];
   const bool counts = t >= 0 && t < a.v;
-  w = counts ? d * row_q(ls, l) : 0.f;
+  w = counts ? d * row_q(ls) : 0.f;
   c = counts ? row_exponent(ls, l) : 0.f;
   return counts;
 }

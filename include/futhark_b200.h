@@ -515,7 +515,8 @@ int futhark_entry_bmm_f16(struct futhark_context *ctx, struct futhark_f32_3d **o
  *   binary16, so dls carries the scale that keeps them in its range; the sums are f32, of products of binary16 numbers: the
  *   logits' gradients, rounded relative to themselves and exact at the target, by W for the first, and by the weighted rows of X for the
  *   second, rounded relative to themselves down to 2^-28 of the largest.  In both directions that is 1.4 times the error of
- *   rounding an exact result once.  Rows without a target have gradient 0 and add nothing to that of W, whatever X holds there. */
+ *   rounding an exact result once.  Probabilities are taken relative to lses, an f32: they are off by |lses[i]| 2^-22 of themselves.
+ *   Rows without a target have gradient 0 and add nothing to that of W, whatever X holds there. */
 int futhark_entry_vocab_xent_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr1d_f32_arr1d_f32 **out0,
                                  const struct futhark_f16_2d *in0, const struct futhark_f16_2d *in1, const struct futhark_i32_1d *in2);
 int futhark_entry_vocab_xent_grad_f16(struct futhark_context *ctx, struct futhark_opaque_tup2_arr2d_f16_arr2d_f16 **out0,

@@ -156,3 +156,41 @@ def test_vocab_xent_logits_of_any_size(ctx, n, v, d, size):
     err = ref.vocab_xent_error(X, W, ts)
     within(lse, wantl, err, "lse")
     within(loss, want, 2 * err, "loss")
+
+
+@pytest.mark.parametrize("n", [1, 200])
+def test_vocab_xent_gradient_of_certain_tokens_with_large_logits(ctx, n):
+    """The target's logit is 1.8e7 above all others: q is 0, and the target's term at most dl 2^-22 W_t with a rounding or two."""
+    X = np.full((n, 8), 3000, np.float16)
+    W = np.zeros((300, 8), np.float16)
+    W[:, 0], W[7, 0] = -3000, 3000
+    ts, dl = np.full(n, 7, np.int32), np.full(n, 2, np.float32)
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    assert np.all(loss == 0) and np.all(lse == 9e6)
+    dx, dw = (half(x) for x in fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl))
+    assert np.abs(dx).max() <= 6000 * 2.0 ** -21 and np.abs(dw).max() <= 6000 * 2.0 ** -21 * n
+
+
+@pytest.mark.parametrize("n,v,d", [(50, 500, 64), (300, 2000, 64), (100, 500, 2600)])
+def test_vocab_xent_gradient_of_nearly_certain_tokens(ctx, n, v, d):
+    """q = 1 - exp(-loss) of tokens whose target's logit is 10 to 400 and all others' are smaller, at any size of lse.
+
+    The target's own 1 is in a sum that up to 40 more numbers are added to, each with a rounding of 2^-24: 10 with the other columns of its 32, 10 with
+    the next 32, 3 with the row's other shares, 8 + 5 with other tiles', 4 to put partial sums together.  What is added is q in all, and off by
+    what a logit is off by.  q is at least 2^-22.  The gradient has the other words' terms too, with their roundings: 2^-9 q."""
+    r = np.random.default_rng(n)
+    W = (r.normal(size=(v, d)) / d ** 0.5).astype(np.float16)
+    ts = r.integers(0, v, n).astype(np.int32)
+    to = np.exp(r.uniform(np.log(10), np.log(400), n))
+    X = (W[ts].astype(np.float64) * to[:, None]).astype(np.float16)
+    dl = np.full(n, 4096, np.float32)
+    loss, lse = fb.vocab_xent_f16(ctx, X, W, ts)
+    want = ref.vocab_xent(X, W, ts)[0]
+    q, few = -np.expm1(-want), 40 * 2.0 ** -24
+    off = few + 2 * ref.vocab_xent_error(X, W, ts) * q + 2.0 ** -22 * want
+    within(loss, want, off, "loss")
+    dx = half(fb.vocab_xent_grad_f16(ctx, X, W, ts, loss, lse, dl)[0])
+    wx = ref.vocab_xent_grad(X, W, ts, dl)[0]
+    size = np.abs(W.astype(np.float64)).max()
+    err = 4096 * (off + 2.0 ** -22 + 2.0 ** -9 * q)[:, None] * 2 * size
+    within(dx, wx, err + ref.H * np.abs(wx) + ref.HMIN, "dX")
